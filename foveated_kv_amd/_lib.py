@@ -71,10 +71,32 @@ class BlobInfoC(ctypes.Structure):
     ]
 
 
-# name -> (restype, argtypes); every symbol include/fkv.h declares
 P = ctypes.c_void_p
 I32 = ctypes.c_int32
+I64 = ctypes.c_int64
 F32 = ctypes.c_float
+
+
+class PagesC(ctypes.Structure):
+    _fields_ = [("k", P), ("v", P), ("k_exp", P), ("v_scale", P), ("n_pages", I32), ("page_size", I32),
+                ("H", I32), ("D", I32), ("format", I32)]
+
+
+class RowsC(ctypes.Structure):
+    _fields_ = [("data", P), ("stride_b", I64), ("stride_h", I64), ("stride_l", I64)]
+
+
+class PositionsC(ctypes.Structure):
+    _fields_ = [("data", P), ("stride_b", I64), ("stride_l", I64), ("base", I64), ("is64", I32),
+                ("per_token", I32)]
+
+
+class RopeC(ctypes.Structure):
+    _fields_ = [("table", P), ("n_positions", I32), ("rot_dim", I32), ("interleaved", I32)]
+
+
+# name -> (restype, argtypes); every symbol include/fkv.h declares
+_PAGES, _ROWS, _POS, _ROPE = (ctypes.POINTER(t) for t in (PagesC, RowsC, PositionsC, RopeC))
 SIGNATURES = {
     "fkv_is_available": (ctypes.c_int, []),
     "fkv_last_error": (ctypes.c_char_p, []),
@@ -140,6 +162,13 @@ SIGNATURES = {
     "fkv_promoter_get_stats": (ctypes.c_int, [P, P]),
     "fkv_promoter_near_valid": (ctypes.c_int, [P, I32, P, I32]),
     "fkv_promoter_destroy": (None, [P]),
+    "fkv_rope_apply": (ctypes.c_int, [_ROPE, _ROWS, _ROWS, I32, I32, I32, I32, I32, _POS, P]),
+    "fkv_paged_write": (ctypes.c_int, [_PAGES, _ROWS, _ROWS, I32, I32, I32, P, I32, I64, _POS, P, _ROPE, _ROWS,
+                                       _ROWS, I32, P]),
+    "fkv_paged_read": (ctypes.c_int, [_PAGES, P, I32, I64, P, I32, I32, P, P, I32, P]),
+    "fkv_paged_attn_workspace": (I64, [_PAGES, I32, I32, I64]),
+    "fkv_paged_attn": (ctypes.c_int, [_PAGES, _ROWS, I32, I32, I32, P, I32, I64, P, I32, I64, F32, P, P, P, I64,
+                                      P]),
 }
 
 STATS_FIELDS = ("spikes_detected", "spikes_queued", "spikes_deduplicated", "spikes_cooled_down",

@@ -566,6 +566,115 @@ int fkv_promoter_near_valid(const fkv_promoter* p, int32_t layer, uint32_t* out,
 /* stop() + destructor (promotion_pipeline.cpp:30-38, 243-248). */
 void fkv_promoter_destroy(fkv_promoter* p);
 
+/* ---------------------------------------------------------------------- */
+/* paged KV cache (no counterpart in the reference)                         */
+/* ---------------------------------------------------------------------- */
+
+/* What a layer's pages hold.  16-bit formats: the rows, rounded to nearest
+ * even.  FKV_PAGES_FP8: E4M3 codes of x * 2^-e, round to nearest even, 2^e
+ * the least power of two (e >= -126; e = 0 for a row of zeros) with
+ * amax <= 448 * 2^e over the row's finite elements; infinities and NaN
+ * become NaN codes.  FKV_PAGES_FP8_INT4: keys as FKV_PAGES_FP8; values
+ * min + scale * code with code = round((x - min) / scale) to nearest even in
+ * [0, 15], scale = fp32((max - min) / 15) (a row that is not finite reads
+ * back as NaN). */
+#define FKV_PAGES_F16 0
+#define FKV_PAGES_BF16 1
+#define FKV_PAGES_FP8 2
+#define FKV_PAGES_FP8_INT4 3
+
+/* One layer's pages, device arrays of the caller, contiguous:
+ *   k        (n_pages, H, page_size, D) fp16 / bf16 / E4M3
+ *   v        the same; (n_pages, H, page_size, D/2) u8 for INT4, even dim in
+ *            the low nibble
+ *   k_exp    (n_pages, H, page_size) u8, e + 127 of each key row (0 stands
+ *            for a scale of 0); NULL for the 16-bit formats
+ *   v_scale  FP8: (n_pages, H, page_size) u8 as k_exp; FP8_INT4:
+ *            (n_pages, H, page_size, 2) fp32 (scale, min); else NULL
+ * page_size is a power of two from 16 to 1024, D 64 or 128, H at most 1024;
+ * every array 16-byte aligned. */
+typedef struct fkv_pages {
+    void* k;
+    void* v;
+    uint8_t* k_exp;
+    void* v_scale;
+    int32_t n_pages, page_size, H, D, format;
+} fkv_pages;
+
+/* Activation rows (b, h, l): element d of a row at
+ * data + (b * stride_b + h * stride_h + l * stride_l + d) elements.  Data
+ * 16-byte aligned, strides multiples of 8. */
+typedef struct fkv_rows {
+    void* data;
+    int64_t stride_b, stride_h, stride_l;
+} fkv_rows;
+
+/* Position of token (b, l): base + data[b * stride_b + l * stride_l] (0
+ * without data) + (per_token ? 0 : l); data in device memory, int32, or
+ * int64 with is64. */
+typedef struct fkv_positions {
+    const void* data;
+    int64_t stride_b, stride_l, base;
+    int32_t is64, per_token;
+} fkv_positions;
+
+/* Rotary positions: table (n_positions, 2, rot_dim / 2) fp32, cos then sin
+ * of each pair's angle.  Pair i of a row is elements (i, i + rot_dim / 2), or
+ * (2i, 2i + 1) with interleaved, of its first rot_dim, a multiple of 16;
+ * later elements stay.  (a, b) -> (a cos - b sin, b cos + a sin), computed in
+ * 64 bits from the rows and the table and rounded once to fp32, then to the
+ * result's type.  A position outside the table gives NaN. */
+typedef struct fkv_rope {
+    const float* table;
+    int32_t n_positions, rot_dim, interleaved;
+} fkv_rope;
+
+/* out = rotated x, rows (B, H, L) of D elements (D a multiple of 8, at most
+ * 1024) of dtype; out may be x.  Asynchronous, capturable. */
+int fkv_rope_apply(const fkv_rope* rope, const fkv_rows* x, const fkv_rows* out, int32_t dtype, int32_t B,
+                   int32_t H, int32_t L, int32_t D, const fkv_positions* positions, void* stream);
+
+/* Stores L new tokens of B sequences: rows (B, pages->H, L) of k and v in
+ * dtype, keys rotated first where rope is given, token (b, l) at position
+ * start(b) + l of the sequence's pages, table[b * table_stride + i], i <
+ * n_table, being the page of tokens [i * page_size, (i + 1) * page_size).
+ * n_new (B) int32 in device memory, or NULL: the tokens l < n_new[b] alone.
+ * A token whose position lies outside the table, or whose page id lies
+ * outside the pool, is not stored.  q, q_out (both or neither; rows (B, Hq, L)
+ * of the same dtype, q_out may be q): queries rotated by the same
+ * positions, or copied without rope; those past n_new are not written.  Two
+ * tokens of one call must not name the same row.  Asynchronous, capturable. */
+int fkv_paged_write(const fkv_pages* pages, const fkv_rows* k, const fkv_rows* v, int32_t dtype, int32_t B,
+                    int32_t L, const int32_t* table, int32_t n_table, int64_t table_stride,
+                    const fkv_positions* start, const int32_t* n_new, const fkv_rope* rope, const fkv_rows* q,
+                    const fkv_rows* q_out, int32_t Hq, void* stream);
+
+/* The first S tokens of B sequences out of their pages: out_k, out_v (B, H,
+ * S, D) contiguous in out_dtype, the values that the pages stand for rounded
+ * once.  Rows at or past lens[b] (int32, device), past the table or of a page
+ * id outside the pool are zero.  Asynchronous, capturable. */
+int fkv_paged_read(const fkv_pages* pages, const int32_t* table, int32_t n_table, int64_t table_stride,
+                   const int32_t* lens, int32_t B, int32_t S, void* out_k, void* out_v, int32_t out_dtype,
+                   void* stream);
+
+/* Attention of one new token per sequence over its first lens[b] + lens_add
+ * cached tokens (clamped to [0, n_table * page_size]): query rows (B, Hq) of
+ * q_dtype (fp16 or bf16, the pages' own for the 16-bit formats; stride_l is
+ * not read), out (B, Hq, D) contiguous of the same type, lse (B, Hq) fp32 or
+ * NULL: the natural logarithm of each head's sum of exp(scale * score).  Query
+ * heads [h * Hq/H, (h + 1) * Hq/H) attend to KV head h.  No tokens: out 0,
+ * lse -inf.  Tokens of a page id outside the pool take no part.  max_len: an
+ * upper bound of the lengths that the launch is planned for (longer ones are
+ * attended to all the same).  workspace: device memory of this call alone,
+ * 16-byte aligned, of fkv_paged_attn_workspace bytes for the same sizes, free again once
+ * the call's work is done; calls that share one must be ordered.  The result
+ * does not depend on scheduling.  Asynchronous, capturable. */
+int64_t fkv_paged_attn_workspace(const fkv_pages* pages, int32_t Hq, int32_t B, int64_t max_len);
+int fkv_paged_attn(const fkv_pages* pages, const fkv_rows* query, int32_t q_dtype, int32_t Hq, int32_t B,
+                   const int32_t* table, int32_t n_table, int64_t table_stride, const int32_t* lens,
+                   int32_t lens_add, int64_t max_len, float scale, void* out, float* lse, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
 /* Benchmark utility with no counterpart in the reference: streams `bytes`
  * (a multiple of 16) from device buffer `buf` with 16-byte lane loads,
  * `unroll` (1, 2, 4, 8) loads in flight per lane, optionally non-temporal,
