@@ -40,6 +40,11 @@ HIP graph that is replayed once per token.  The host then issues one launch
 per token instead of the closure's per-layer Python and library calls.  The
 model must accept a device tensor as ``cache.offset`` (its RoPE positions
 computed as ``offset + arange(L)``).
+
+Extension: ``generate_paged`` serves a batch of prompts from a
+``PagedKVCache`` (paged.py): each prompt is prefilled into its own pages, then
+all sequences decode together, every layer's one-token call being answered by
+the cache's paged attention (``install_paged_attention``).
 """
 
 import shutil
@@ -207,6 +212,8 @@ def install_fused_sdpa(fov_cache) -> None:
     missing library raises here instead of on the first decode call."""
     if _fused_state._installed:
         raise RuntimeError("Fused SDPA already installed -- call uninstall_fused_sdpa() first")
+    if _paged_state["original"] is not None:
+        raise RuntimeError("paged attention is installed -- call uninstall_paged_attention() first")
     _lib.load()
 
     s = _fused_state
@@ -305,6 +312,159 @@ def reset_fused_layer_counter() -> None:
     if s._cpp_pipeline_handle is None:
         return
     _drain_into(s._cpp_pipeline_handle, s._fused_wrappers, s._decode_step)
+
+
+# ---------------------------------------------------------------------------
+# paged cache
+# ---------------------------------------------------------------------------
+
+_paged_state = {"original": None, "pending": None}
+
+
+class PagedCacheWrapper:
+    """The cache object that a model sees while a ``PagedKVCache`` serves its
+    sequences ``seqs``: one layer's ``update_and_fetch`` and the position
+    ``offset`` of the batch's first new token (a number, or a (B,) device
+    tensor where the sequences' lengths differ).  A model call's tokens are
+    those of the cache's last ``extend``.
+
+    ``update_and_fetch`` with several tokens (prefill) stores them and hands
+    back every key (rotated, where the cache rotates) and value for the
+    original attention; with one token it leaves the write to the attention
+    call that follows, which rotates the query in the same launch."""
+
+    def __init__(self, cache, layer_idx, seqs=None):
+        self.cache, self.layer_idx, self.seqs = cache, layer_idx, cache.pages._range(seqs)
+        self.rope = cache.rope
+        self._new = None
+
+    @property
+    def offset(self):
+        starts = set(self.cache.pages.starts(self.seqs))
+        return starts.pop() if len(starts) == 1 else self.cache.pages.start[self.seqs]
+
+    def update_and_fetch(self, keys, values):
+        if _paged_state["pending"] is not None:
+            raise RuntimeError("a paged layer's attention call is missing: the model must call "
+                               "F.scaled_dot_product_attention after each update_and_fetch")
+        if _paged_state["original"] is None:
+            raise RuntimeError("paged attention is not installed")
+        _paged_state["pending"] = self
+        if keys.shape[2] == 1:
+            self._new = keys, values
+            return keys, values
+        self.cache.write(self.layer_idx, keys, values, seqs=self.seqs)
+        if self.offset == 0:
+            return (keys if self.rope is None else self.rope(keys, 0)), values
+        return self.cache.read(self.layer_idx, self.seqs, keys.dtype)
+
+    def _answer(self, query, scale):
+        keys, values = self._new
+        self._new = None
+        q = self.cache.write(self.layer_idx, keys, values, q=query.to(keys.dtype), seqs=self.seqs)
+        layer = self.cache.layers[self.layer_idx]
+        want = {"fp16": torch.float16, "bf16": torch.bfloat16}.get(
+            layer.fmt, query.dtype if query.dtype != torch.float32 else torch.float16)
+        return self.cache.attend(self.layer_idx, q.to(want), seqs=self.seqs, scale=scale).to(query.dtype)
+
+
+def _paged_interceptor(query, key, value, attn_mask=None, dropout_p=0.0, is_causal=False, scale=None, **kwargs):
+    w, _paged_state["pending"] = _paged_state["pending"], None
+    if w is not None and query.dim() == 4:
+        if query.shape[2] == 1:
+            return w._answer(query, scale)
+        if w.rope is not None:
+            query = w.rope(query, w.offset)
+    return _paged_state["original"](query, key, value, attn_mask=attn_mask, dropout_p=dropout_p, is_causal=is_causal,
+                                    scale=scale, **kwargs)
+
+
+def install_paged_attention(cache, seqs=None) -> list:
+    """Route one-token attention calls into ``cache``: replaces
+    ``torch.nn.functional.scaled_dot_product_attention`` and returns one
+    ``PagedCacheWrapper`` per layer, to be passed as the model's cache."""
+    if _fused_state._installed or _paged_state["original"] is not None:
+        raise RuntimeError("another decode attention is installed -- uninstall it first")
+    _lib.load()
+    _paged_state["original"], _paged_state["pending"] = F.scaled_dot_product_attention, None
+    F.scaled_dot_product_attention = _paged_interceptor
+    return paged_wrappers(cache, seqs)
+
+
+def paged_wrappers(cache, seqs=None) -> list:
+    """One ``PagedCacheWrapper`` per layer for the sequences ``seqs``."""
+    return [PagedCacheWrapper(cache, i, seqs) for i in range(len(cache.layers))]
+
+
+def uninstall_paged_attention() -> None:
+    if _paged_state["original"] is not None:
+        F.scaled_dot_product_attention = _paged_state["original"]
+        _paged_state["original"] = _paged_state["pending"] = None
+
+
+def generate_paged(model, tokenizer, prompts, cache, max_tokens: int = 100, temp: float = 0.0):
+    """Prefill ``prompts`` (a list, or one string) into sequences 0, 1, ... of
+    the ``PagedKVCache`` ``cache``, which must be free, and decode them
+    together for up to ``max_tokens`` tokens each -> (texts, stats); one text
+    for one string.  The sequences are freed at the end.
+
+    Where ``cache.rope`` is set the model must leave the rotation to the
+    cache, and prompts may have different lengths.  Without it the model
+    rotates by ``cache.offset``, a number for the whole batch: prompts then
+    need one length."""
+    one = isinstance(prompts, str)
+    dev = _model_device(model)
+    ids = [tokenizer.encode(p) for p in ([prompts] if one else prompts)]
+    B = len(ids)
+    if B == 0 or min(len(i) for i in ids) == 0:
+        raise ValueError("generate_paged needs prompts of at least one token")
+    if B > cache.pages.max_seqs or any(cache.pages.lengths(slice(0, B))):
+        raise ValueError(f"sequences 0 to {B - 1} of the cache must be there and free")
+    if cache.rope is None and len({len(i) for i in ids}) > 1:
+        raise ValueError("prompts of different lengths need a cache that rotates (PagedKVCache(rope=...))")
+    batch = slice(0, B)
+    eos = getattr(tokenizer, "eos_token_id", None)
+    out = [[] for _ in range(B)]
+    done = [False] * B
+    install_paged_attention(cache)
+    try:
+        with torch.no_grad():
+            t0 = time.perf_counter()
+            logits = []
+            for b, tok in enumerate(ids):
+                cache.extend(len(tok), slice(b, b + 1))
+                x = torch.tensor([tok], dtype=torch.long, device=dev)
+                logits.append(model(x, cache=paged_wrappers(cache, slice(b, b + 1)))[:, -1, :])
+            logits = torch.cat(logits)
+            torch.cuda.synchronize(dev)
+            t_prefill = time.perf_counter() - t0
+            t0 = time.perf_counter()
+            wrappers = paged_wrappers(cache, batch)
+            steps = 0
+            for _ in range(max_tokens):
+                tok = _next_token(logits, temp)
+                for b, t in enumerate(tok.tolist()):
+                    done[b] = done[b] or t == eos
+                    if not done[b]:
+                        out[b].append(t)
+                if all(done):
+                    break
+                cache.extend(1, batch)
+                logits = model(tok.reshape(B, 1), cache=wrappers)[:, -1, :]
+                steps += 1
+            torch.cuda.synchronize(dev)
+            t_decode = time.perf_counter() - t0
+    finally:
+        uninstall_paged_attention()
+        stored = cache.pages.lengths(batch)
+        for b in range(B):
+            cache.free(b)
+    texts = [tokenizer.decode(o) for o in out]
+    n = sum(len(o) for o in out)
+    stats = {"prompt_tokens": [len(i) for i in ids], "generated_tokens": [len(o) for o in out],
+             "stored_tokens": stored, "model_calls": steps, "prefill_time_s": t_prefill, "decode_time_s": t_decode,
+             "tokens_per_second": n / max(t_decode, 1e-6), "cache_mb": cache.memory_bytes() / 2 ** 20}
+    return (texts[0] if one else texts), stats
 
 
 # ---------------------------------------------------------------------------

@@ -22,7 +22,6 @@ any.  A page, once written by one stream and read by another, is ordered by
 the caller, as any tensor is.
 """
 
-import ctypes
 import math
 
 import torch
@@ -39,58 +38,84 @@ _NEW = {"fp16": torch.float16, "bf16": torch.bfloat16}
 # arguments
 # ---------------------------------------------------------------------------
 
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+def _on(index, name, t):
+    """Refuses what is not a tensor on GPU ``index``."""
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if t.get_device() != index:
+        _require_device(t)
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
 
 
-def _no_grad_needed(**tensors):
-    if torch.is_grad_enabled():
-        for name, t in tensors.items():
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{name} requires grad: this package is for inference and records nothing for "
-                                   "autograd (call it under torch.no_grad())")
+def _no_grad(name, t):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires grad: this package is for inference and records nothing for autograd "
+                           "(call it under torch.no_grad())")
 
 
-def _rows(t):
-    """(B, H, L, D) tensor as C rows, copied only if its last dimension is
-    strided or a row not 16-byte aligned -> (rows, tensor)."""
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(t.shape[i] > 1 and t.stride(i) % 8 for i in range(3)):
-        t = t.clone(memory_format=torch.contiguous_format)
-    s = [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
-    return _lib.RowsC(t.data_ptr(), *s), t
+class _Device:
+    """The GPU's current stream, with that GPU current inside (entering costs
+    nothing where it is already)."""
+
+    def __init__(self, index):
+        self.index, self.guard = index, None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.index:
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
-def _int_tensor(name, t):
-    if t.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
+def _rows(t, shape):
+    """(B, H, L, D) tensor of that shape as C rows, copied only where its last
+    dimension is strided or a row not 16-byte aligned -> (rows, tensor)."""
+    at, (sb, sh, sl, sd) = t.data_ptr(), t.stride()
+    if sd != 1 or at & 15 or (sb | sh | sl) & 7:
+        # (strides of dimensions of one element mean nothing)
+        B, H, L, _ = shape
+        sb, sh, sl = sb if B > 1 else 0, sh if H > 1 else 0, sl if L > 1 else 0
+        if sd != 1 or at & 15 or (sb | sh | sl) & 7:
+            t = t.clone(memory_format=torch.contiguous_format)
+            at, (sb, sh, sl, _) = t.data_ptr(), t.stride()
+    return _lib.RowsC(at, sb, sh, sl), t
 
 
-def _positions(p, B, L, device, per_token_allowed=True):
+def _positions(p, B, L, index, per_token_allowed=True):
     """int | one-element tensor | (B,) tensor: the first token's position of
     each sequence; (B, L) or (1, L): every token's."""
     if not torch.is_tensor(p):
-        return _lib.PositionsC(None, 0, 0, int(p), 0, 0), None
-    _int_tensor("positions", p)
-    _same_device(device, positions=p)
-    is64 = int(p.dtype == torch.int64)
-    if p.dim() == 2 and per_token_allowed:
-        if p.shape[0] not in (1, B) or p.shape[1] != L:
-            raise ValueError(f"positions must be (B, L) = {(B, L)}, (B,) or one number, got {tuple(p.shape)}")
-        return _lib.PositionsC(p.data_ptr(), p.stride(0) if p.shape[0] > 1 else 0, p.stride(1), 0, is64, 1), p
-    if p.dim() == 0 or (p.dim() == 1 and p.shape[0] == 1):
-        return _lib.PositionsC(p.data_ptr(), 0, 0, 0, is64, 0), p
-    if p.dim() != 1 or p.shape[0] != B:
-        raise ValueError(f"positions must hold one number per sequence ({B}), got {tuple(p.shape)}")
-    return _lib.PositionsC(p.data_ptr(), p.stride(0), 0, 0, is64, 0), p
+        return _lib.PositionsC(None, 0, 0, int(p), 0, 0)
+    if p.dtype != torch.int32 and p.dtype != torch.int64:
+        raise TypeError(f"positions must be int32 or int64, got {p.dtype}")
+    _on(index, "positions", p)
+    shape, at, is64 = tuple(p.shape), p.data_ptr(), p.dtype == torch.int64
+    if shape == (B,):
+        return _lib.PositionsC(at, p.stride(0), 0, 0, is64, 0)
+    if shape == () or shape == (1,):
+        return _lib.PositionsC(at, 0, 0, 0, is64, 0)
+    if per_token_allowed and shape in ((B, L), (1, L)):
+        return _lib.PositionsC(at, p.stride(0) if shape[0] > 1 else 0, p.stride(1), 0, is64, 1)
+    raise ValueError(f"positions must be one number, one per sequence ({B},)"
+                     f"{f' or one per token {(B, L)}' if per_token_allowed else ''}, got {shape}")
 
 
-def _lens(name, t, B, device):
-    if not torch.is_tensor(t) or t.dtype != torch.int32 or tuple(t.shape) != (B,):
+def _lens(name, t, B, index):
+    _on(index, name, t)
+    if t.dtype != torch.int32 or tuple(t.shape) != (B,):
         raise TypeError(f"{name} must be an int32 tensor of shape ({B},)")
-    _same_device(device, **{name: t})
-    return t.contiguous()
+    return t if B <= 1 or t.stride(0) == 1 else t.contiguous()
+
+
+def _index_of(device):
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        return torch.device("cuda", torch.cuda.current_device())
+    return device
 
 
 # ---------------------------------------------------------------------------
@@ -170,12 +195,12 @@ class Rope:
             raise ValueError(f"base must be above 1, got {base}")
         if not 1 <= max_positions < 2 ** 31:
             raise ValueError(f"max_positions must be positive and below 2^31, got {max_positions}")
+        if head_dim % 8 or head_dim > 512:
+            raise ValueError(f"the head dim must be a multiple of 8, at most 512, got {head_dim}")
         self.head_dim, self.rot_dim, self.interleaved = int(head_dim), int(rot_dim), bool(interleaved)
         self.base, self.scaling, self.max_positions = float(base), scaling, int(max_positions)
         inv, factor = _frequencies(self.rot_dim, self.base, scaling)
-        device = torch.device(device)
-        if device.type == "cuda" and device.index is None:
-            device = torch.device("cuda", torch.cuda.current_device())
+        device = _index_of(device)
         inv = inv.to(device)
         self.table = torch.empty((self.max_positions, 2, self.rot_dim // 2), dtype=torch.float32, device=device)
         for p in range(0, self.max_positions, 65536):  # (64-bit angles of 64K positions at a time)
@@ -191,25 +216,29 @@ class Rope:
         position), a (B,) tensor (each sequence's first token's) or (B, L) /
         (1, L) (every token's); int32 or int64 tensors on the device, read
         there, so a captured call follows them."""
-        _require_device(x, out)
-        if x.dim() != 4 or x.shape[3] != self.head_dim:
-            raise ValueError(f"x must be (B, H, L, {self.head_dim}), got {tuple(x.shape)}")
-        if self.head_dim % 8 or self.head_dim > 512:
-            raise ValueError("the head dim must be a multiple of 8, at most 512")
-        _no_grad_needed(x=x, out=out)
-        _same_device(self.table.device, x=x, out=out)
-        B, H, L, D = x.shape
+        index = self.table.get_device()
+        if index < 0:
+            _require_device(self.table)
+        _on(index, "x", x)
+        shape = tuple(x.shape)
+        if len(shape) != 4 or shape[3] != self.head_dim:
+            raise ValueError(f"x must be (B, H, L, {self.head_dim}), got {shape}")
+        _no_grad("x", x)
         code = dtype_code(x.dtype)
         if out is None:
             out = torch.empty_like(x)
-        elif out.shape != x.shape or out.dtype != x.dtype:
-            raise ValueError("out must have x's shape and dtype")
-        pos, keep = _positions(positions, B, L, x.device)
-        src, x_held = _rows(x)
-        dst, result = _rows(out)
-        with torch.cuda.device(x.device):
-            check(_lib.load().fkv_rope_apply(ctypes.byref(self._c), ctypes.byref(src), ctypes.byref(dst), code, B, H,
-                                             L, D, ctypes.byref(pos), _lib.stream_ptr(x.device)), "fkv_rope_apply")
+        else:
+            _on(index, "out", out)
+            _no_grad("out", out)
+            if tuple(out.shape) != shape or out.dtype != x.dtype:
+                raise ValueError("out must have x's shape and dtype")
+        B, H, L, D = shape
+        pos = _positions(positions, B, L, index)
+        src, held = _rows(x, shape)
+        dst, result = _rows(out, shape)
+        lib = _lib.load()
+        with _Device(index) as stream:
+            check(lib.fkv_rope_apply(self._c, src, dst, code, B, H, L, D, pos, stream), "fkv_rope_apply")
             if result is not out:
                 out.copy_(result)
         return out
@@ -280,18 +309,26 @@ class PagedLayer:
         for name, (t, shape, dtype) in want.items():
             if t is None or tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous {shape} {dtype} tensor")
-            _same_device(k.device, **{name: t})
+            _on(k.get_device(), name, t)
         self.fmt, self.k, self.v, self.k_exp, self.v_scale = fmt, k, v, k_exp, v_scale
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, H, page, D
-        self.device = k.device
+        self.device, self._index = k.device, k.get_device()
         self._c = _lib.PagesC(k.data_ptr(), v.data_ptr(), ptr(k_exp), ptr(v_scale), n, page, H, D, FORMATS[fmt])
-        check(min(int(_lib.load().fkv_paged_attn_workspace(ctypes.byref(self._c), H, 1, 0)), 0), "PagedLayer")
+        check(min(int(_lib.load().fkv_paged_attn_workspace(self._c, H, 1, 0)), 0), "PagedLayer")
 
-    def _table(self, table):
-        if not torch.is_tensor(table) or table.dtype != torch.int32 or table.dim() != 2:
+    def _table(self, table, B=None):
+        """-> table, its rows, pages per sequence and row stride."""
+        _on(self._index, "table", table)
+        if table.dtype != torch.int32 or table.dim() != 2:
             raise TypeError("table must be a (B, pages per sequence) int32 tensor")
-        _same_device(self.device, table=table)
-        return table if table.shape[1] <= 1 or table.stride(1) == 1 else table.contiguous()
+        rows, P = table.shape
+        if B is not None and rows != B:
+            raise ValueError(f"table must have {B} rows, got {(rows, P)}")
+        stride, step = table.stride()
+        if (P > 1 and step != 1) or (rows > 1 and stride < P):
+            table = table.contiguous()
+            stride = P
+        return table, rows, P, stride if rows > 1 else P
 
     def memory_bytes(self):
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_exp, self.v_scale) if t is not None)
@@ -310,49 +347,54 @@ class PagedLayer:
         its queries come back as ``q_out`` held them (zero in a new tensor).
         Positions outside the table are not stored either.  No two tokens of
         a call may name the same slot."""
-        _require_device(k, v, table, q, q_out, n_new)
-        B, H, L, D = k.shape if k.dim() == 4 else (-1, -1, -1, -1)
-        if (H, D) != (self.n_kv_heads, self.head_dim) or v.shape != k.shape or v.dtype != k.dtype:
+        index, shape = self._index, tuple(k.shape)
+        _on(index, "k", k)
+        _on(index, "v", v)
+        if len(shape) != 4 or shape[1] != self.n_kv_heads or shape[3] != self.head_dim or tuple(v.shape) != shape or \
+                v.dtype != k.dtype:
             raise ValueError(f"k and v must be (B, {self.n_kv_heads}, L, {self.head_dim}) of one dtype, got "
-                             f"{tuple(k.shape)} {k.dtype} / {tuple(v.shape)} {v.dtype}")
+                             f"{shape} {k.dtype} / {tuple(v.shape)} {v.dtype}")
+        B, H, L, D = shape
         code = dtype_code(k.dtype)
-        table = self._table(table)
-        if table.shape[0] != B:
-            raise ValueError(f"table must have {B} rows, got {tuple(table.shape)}")
-        _no_grad_needed(k=k, v=v, q=q, q_out=q_out)
-        _same_device(self.device, k=k, v=v, q=q, q_out=q_out)
+        table, _, P, stride = self._table(table, B)
+        _no_grad("k", k)
+        _no_grad("v", v)
+        rope_c = None
         if rope is not None:
             if rope.head_dim != D:
                 raise ValueError(f"rope is for head dim {rope.head_dim}, not {D}")
-            _same_device(self.device, rope=rope.table)
-        pos, keep = _positions(start, B, L, self.device, per_token_allowed=False)
+            _on(index, "rope", rope.table)
+            rope_c = rope._c
+        pos = _positions(start, B, L, index, per_token_allowed=False)
         if n_new is not None:
-            n_new = _lens("n_new", n_new, B, self.device)
-        rk, k_held = _rows(k)
-        rv, v_held = _rows(v)
-        rq = ro = None
+            n_new = _lens("n_new", n_new, B, index)
+        rk, k_held = _rows(k, shape)
+        rv, v_held = _rows(v, shape)
+        rq = ro = result = None
         Hq = 0
-        if q is None:
-            if q_out is not None:
-                raise ValueError("q_out without q")
-        else:
-            if q.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != (B, L, D) or q.dtype != k.dtype:
-                raise ValueError(f"q must be ({B}, Hq, {L}, {D}) {k.dtype}, got {tuple(q.shape)} {q.dtype}")
+        if q is not None:
+            _on(index, "q", q)
+            _no_grad("q", q)
+            qs = tuple(q.shape)
+            if len(qs) != 4 or (qs[0], qs[2], qs[3]) != (B, L, D) or q.dtype != k.dtype:
+                raise ValueError(f"q must be ({B}, Hq, {L}, {D}) {k.dtype}, got {qs} {q.dtype}")
             if q_out is None:
                 q_out = torch.empty_like(q) if n_new is None else torch.zeros_like(q)
-            elif q_out.shape != q.shape or q_out.dtype != q.dtype:
-                raise ValueError("q_out must have q's shape and dtype")
-            Hq = q.shape[1]
-            rq, q_held = _rows(q)
-            ro, result = _rows(q_out)
-        with torch.cuda.device(self.device):
-            ref = lambda c: None if c is None else ctypes.byref(c)  # noqa: E731
-            check(_lib.load().fkv_paged_write(
-                ctypes.byref(self._c), ref(rk), ref(rv), code, B, L, ptr(table), table.shape[1],
-                table.stride(0) if B > 1 else table.shape[1], ctypes.byref(pos), ptr(n_new),
-                None if rope is None else ctypes.byref(rope._c), ref(rq), ref(ro), Hq,
-                _lib.stream_ptr(self.device)), "fkv_paged_write")
-            if q is not None and result is not q_out:
+            else:
+                _on(index, "q_out", q_out)
+                _no_grad("q_out", q_out)
+                if tuple(q_out.shape) != qs or q_out.dtype != q.dtype:
+                    raise ValueError("q_out must have q's shape and dtype")
+            Hq = qs[1]
+            rq, q_held = _rows(q, qs)
+            ro, result = _rows(q_out, qs)
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        lib = _lib.load()
+        with _Device(index) as stream:
+            check(lib.fkv_paged_write(self._c, rk, rv, code, B, L, table.data_ptr(), P, stride, pos, ptr(n_new),
+                                      rope_c, rq, ro, Hq, stream), "fkv_paged_write")
+            if result is not q_out:
                 q_out.copy_(result)
         return q_out
 
@@ -361,20 +403,20 @@ class PagedLayer:
         ``dtype`` (default: the pages' own, fp16 for quantised ones); rows
         past lens[b] ((B,) int32 on the device) are zero.  ``max_len``
         defaults to the table's width in tokens."""
-        _require_device(table, lens)
-        table = self._table(table)
-        B, P = table.shape
-        lens = _lens("lens", lens, B, self.device)
+        table, B, P, stride = self._table(table)
+        lens = _lens("lens", lens, B, self._index)
         S = P * self.page_size if max_len is None else int(max_len)
         if S < 0:
             raise ValueError("max_len must not be negative")
         dtype = _NEW.get(self.fmt, torch.float16) if dtype is None else dtype
-        out = [torch.empty((B, self.n_kv_heads, S, self.head_dim), dtype=dtype, device=self.device) for _ in range(2)]
-        with torch.cuda.device(self.device):
-            check(_lib.load().fkv_paged_read(
-                ctypes.byref(self._c), ptr(table), P, table.stride(0) if B > 1 else P, ptr(lens), B, S,
-                ptr(out[0]), ptr(out[1]), dtype_code(dtype), _lib.stream_ptr(self.device)), "fkv_paged_read")
-        return tuple(out)
+        code = dtype_code(dtype)
+        k = torch.empty((B, self.n_kv_heads, S, self.head_dim), dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        lib = _lib.load()
+        with _Device(self._index) as stream:
+            check(lib.fkv_paged_read(self._c, table.data_ptr(), P, stride, lens.data_ptr(), B, S, k.data_ptr(),
+                                     v.data_ptr(), code, stream), "fkv_paged_read")
+        return k, v
 
     def attend(self, query, table, lens, max_len=None, lens_add=0, scale=None, out=None, return_lse=False):
         """Attention of one new token per sequence, query (B, Hq, 1, D) fp16
@@ -387,39 +429,224 @@ class PagedLayer:
         ``max_len`` is an upper bound of the lengths if the host knows one
         (default: the table's width); it decides how the work is split, not
         what is attended to.  ``scale`` defaults to D^-1/2."""
-        _require_device(query, table, lens, out)
-        D = self.head_dim
-        if query.dim() != 4 or query.shape[2] != 1 or query.shape[3] != D or query.shape[1] % self.n_kv_heads or \
-                query.shape[1] == 0:
-            raise ValueError(f"query must be (B, a multiple of {self.n_kv_heads}, 1, {D}), got {tuple(query.shape)}")
-        if query.dtype not in (torch.float16, torch.bfloat16) or query.dtype != _NEW.get(self.fmt, query.dtype):
+        index, D, shape, dtype = self._index, self.head_dim, tuple(query.shape), query.dtype
+        _on(index, "query", query)
+        if len(shape) != 4 or shape[2] != 1 or shape[3] != D or shape[1] % self.n_kv_heads or shape[1] == 0:
+            raise ValueError(f"query must be (B, a multiple of {self.n_kv_heads}, 1, {D}), got {shape}")
+        if dtype not in (torch.float16, torch.bfloat16) or dtype != _NEW.get(self.fmt, dtype):
             raise TypeError(f"{self.fmt} pages take {'fp16 or bf16' if self.fmt not in _NEW else self.fmt} queries, "
-                            f"got {query.dtype}")
-        _no_grad_needed(query=query, out=out)
-        table = self._table(table)
-        B, Hq = query.shape[:2]
-        if table.shape[0] != B:
-            raise ValueError(f"table must have {B} rows, got {tuple(table.shape)}")
-        lens = _lens("lens", lens, B, self.device)
-        _same_device(self.device, query=query, out=out)
-        P = table.shape[1]
-        cap = P * self.page_size
-        most = cap if max_len is None else min(int(max_len), cap)
-        rows, held = _rows(query)
+                            f"got {dtype}")
+        _no_grad("query", query)
+        B, Hq = shape[:2]
+        table, _, P, stride = self._table(table, B)
+        lens = _lens("lens", lens, B, index)
+        most = P * self.page_size
+        if max_len is not None and max_len < most:
+            most = int(max_len)
+        rows, held = _rows(query, shape)
         if out is None:
-            out = torch.empty((B, Hq, 1, D), dtype=query.dtype, device=self.device)
-        elif tuple(out.shape) != (B, Hq, 1, D) or out.dtype != query.dtype or not out.is_contiguous() or \
-                out.data_ptr() % 16:
-            raise ValueError(f"out must be a contiguous, 16-byte aligned {(B, Hq, 1, D)} {query.dtype} tensor")
+            out = torch.empty(shape, dtype=dtype, device=self.device)
+        else:
+            _on(index, "out", out)
+            _no_grad("out", out)
+            if tuple(out.shape) != shape or out.dtype != dtype or not out.is_contiguous() or out.data_ptr() % 16:
+                raise ValueError(f"out must be a contiguous, 16-byte aligned {shape} {dtype} tensor")
         lse = torch.empty((B, Hq), dtype=torch.float32, device=self.device) if return_lse else None
         lib = _lib.load()
-        with torch.cuda.device(self.device):
-            n = int(lib.fkv_paged_attn_workspace(ctypes.byref(self._c), Hq, B, most))
-            check(min(n, 0), "fkv_paged_attn_workspace")
-            ws = torch.empty(n, dtype=torch.uint8, device=self.device)
-            check(lib.fkv_paged_attn(
-                ctypes.byref(self._c), ctypes.byref(rows), dtype_code(query.dtype), Hq, B, ptr(table), P,
-                table.stride(0) if B > 1 else P, ptr(lens), int(lens_add), most,
-                D ** -0.5 if scale is None else float(scale), ptr(out), ptr(lse), ptr(ws), n,
-                _lib.stream_ptr(self.device)), "fkv_paged_attn")
+        n = lib.fkv_paged_attn_workspace(self._c, Hq, B, most)
+        if n < 0:
+            check(n, "fkv_paged_attn_workspace")
+        with _Device(index) as stream:
+            ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+            check(lib.fkv_paged_attn(self._c, rows, dtype_code(dtype), Hq, B, table.data_ptr(), P, stride,
+                                     lens.data_ptr(), lens_add, most, D ** -0.5 if scale is None else scale,
+                                     out.data_ptr(), ptr(lse), ptr(ws), n, stream), "fkv_paged_attn")
         return (out, lse) if return_lse else out
+
+
+# ---------------------------------------------------------------------------
+# layers that grow together
+# ---------------------------------------------------------------------------
+
+class PageTable:
+    """Which pages hold which sequence's tokens, for ``max_seqs`` sequences of
+    up to ``max_tokens`` tokens over a pool of ``n_pages`` pages.
+
+    On the device: ``table`` (max_seqs, pages per sequence) int32, -1 where
+    nothing is held, ``lens``, ``start`` and ``new`` (max_seqs,) int32: the
+    tokens of each sequence now, before its last ``extend``, and their
+    difference.  The host keeps its own copy and hands out pages; device
+    updates are work on the current stream."""
+
+    def __init__(self, n_pages, page_size, max_seqs, max_tokens, device="cuda"):
+        n_pages, page_size, max_seqs, max_tokens = (int(x) for x in (n_pages, page_size, max_seqs, max_tokens))
+        if min(n_pages, page_size, max_seqs, max_tokens) < 1:
+            raise ValueError("pages, page size, sequences and tokens must be positive")
+        self.n_pages, self.page_size, self.max_seqs, self.max_tokens = n_pages, page_size, max_seqs, max_tokens
+        width = -(-max_tokens // page_size)
+        self.table = torch.full((max_seqs, width), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(max_seqs, dtype=torch.int32, device=device)
+        self.start = torch.zeros(max_seqs, dtype=torch.int32, device=device)
+        self.new = torch.zeros(max_seqs, dtype=torch.int32, device=device)
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._pages = [[] for _ in range(max_seqs)]
+        self._lens = [0] * max_seqs
+        self._new = [0] * max_seqs
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def lengths(self, seqs=None):
+        """Tokens of the sequences, from the host's copy."""
+        return self._lens[self._range(seqs)]
+
+    def starts(self, seqs=None):
+        """Tokens of the sequences before their last ``extend``, from the
+        host's copy."""
+        sl = self._range(seqs)
+        return [n - t for n, t in zip(self._lens[sl], self._new[sl])]
+
+    def pages(self, seq):
+        """Page ids of one sequence, in order."""
+        return list(self._pages[seq])
+
+    def _range(self, seqs):
+        if seqs is None:
+            return slice(0, self.max_seqs)
+        first, stop, step = seqs.indices(self.max_seqs)
+        if step != 1 or stop < first:
+            raise ValueError(f"seqs must be a slice of neighbouring sequences, got {seqs}")
+        return slice(first, stop)
+
+    def reserve(self, tokens, seqs=None):
+        """Gives each sequence the pages for ``tokens`` tokens (a number, or one
+        per sequence) in all; those it holds stay.  Raises MemoryError, and
+        changes nothing, where the pool or a sequence's row is too small."""
+        sl = self._range(seqs)
+        each = range(sl.start, sl.stop)
+        want = [int(tokens)] * len(each) if isinstance(tokens, int) else [int(t) for t in tokens]
+        if len(want) != len(each):
+            raise ValueError(f"{len(want)} lengths for {len(each)} sequences")
+        if want and max(want) > self.max_tokens:
+            raise MemoryError(f"a sequence of {max(want)} tokens: the table holds {self.max_tokens}")
+        more = [max(0, -(-t // self.page_size) - len(self._pages[b])) for b, t in zip(each, want)]
+        if sum(more) > len(self._free):
+            raise MemoryError(f"{sum(more)} pages needed, {len(self._free)} free")
+        rows, cols, ids = [], [], []
+        for b, n in zip(each, more):
+            for _ in range(n):
+                rows.append(b)
+                cols.append(len(self._pages[b]))
+                ids.append(self._free.pop())
+                self._pages[b].append(ids[-1])
+        if ids:
+            d = self.table.device
+            self.table[torch.tensor(rows, device=d), torch.tensor(cols, device=d)] = \
+                torch.tensor(ids, dtype=torch.int32, device=d)
+
+    def extend(self, n=1, seqs=None):
+        """``n`` more tokens (a number, or one per sequence): reserves their
+        pages and advances start, new and lens."""
+        if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("pages are handed out on the host: extend before the capture, or capture the layer's "
+                               "calls with lengths of your own")
+        sl = self._range(seqs)
+        count = sl.stop - sl.start
+        each = [int(n)] * count if isinstance(n, int) else [int(t) for t in n]
+        if len(each) != count:
+            raise ValueError(f"{len(each)} numbers of tokens for {count} sequences")
+        if each and min(each) < 0:
+            raise ValueError("sequences do not shrink (free them)")
+        self.reserve([a + t for a, t in zip(self._lens[sl], each)], seqs=sl)
+        self.start[sl].copy_(self.lens[sl])
+        if self._new[sl] != each:
+            self.new[sl].copy_(torch.tensor(each, dtype=torch.int32))
+            self._new[sl] = each
+        self.lens[sl].add_(self.new[sl])
+        self._lens[sl] = [a + t for a, t in zip(self._lens[sl], each)]
+
+    def free(self, seq):
+        """Sequence ``seq`` is over: its pages go back to the pool."""
+        if not 0 <= seq < self.max_seqs:
+            raise ValueError(f"no sequence {seq}")
+        self._free.extend(reversed(self._pages[seq]))
+        self._pages[seq] = []
+        self._lens[seq] = self._new[seq] = 0
+        self.table[seq].fill_(-1)
+        for t in (self.lens, self.start, self.new):
+            t[seq].fill_(0)
+
+
+class PagedKVCache:
+    """``n_layers`` layers of pages over one ``PageTable``:
+
+        cache = PagedKVCache(n_layers, n_kv_heads, head_dim, n_pages, max_seqs, max_tokens, fmt="fp8", rope=rope)
+        cache.extend(n)                          # n tokens more per sequence
+        q = cache.write(layer, k, v, q)          # rotated, encoded, stored
+        out = cache.attend(layer, q)             # one-token queries
+        k, v = cache.read(layer)                 # what is stored
+
+    ``seqs`` (a slice, default all sequences) picks the neighbouring
+    sequences that a call's batch stands for.  With ``rope`` the cache rotates
+    what it is handed; without it keys and queries come rotated."""
+
+    def __init__(self, n_layers, n_kv_heads, head_dim, n_pages, max_seqs=1, max_tokens=32768, page_size=64,
+                 fmt="fp16", rope=None, device="cuda"):
+        if rope is not None and rope.head_dim != head_dim:
+            raise ValueError(f"rope is for head dim {rope.head_dim}, not {head_dim}")
+        self.layers = [PagedLayer(n_pages, n_kv_heads, head_dim, page_size, fmt, device) for _ in range(n_layers)]
+        self.pages = PageTable(n_pages, page_size, max_seqs, max_tokens, device)
+        self.rope, self.fmt = rope, fmt
+
+    def extend(self, n=1, seqs=None):
+        """As ``PageTable.extend``; with one number per sequence, a write's
+        batch is padded to the largest of them."""
+        self.pages.extend(n, seqs)
+
+    def free(self, seq):
+        self.pages.free(seq)
+
+    def _batch(self, seqs):
+        sl = self.pages._range(seqs)
+        return sl, self.pages.table[sl]
+
+    def write(self, layer, k, v, q=None, seqs=None, q_out=None):
+        """The new tokens of the last ``extend`` of the same sequences; see
+        ``PagedLayer.write``."""
+        sl, table = self._batch(seqs)
+        new = self.pages._new[sl]
+        if new and max(new) != k.shape[2]:
+            raise ValueError(f"k holds {k.shape[2]} tokens, the last extend made room for {max(new)}")
+        n_new = None if len(set(new)) <= 1 else self.pages.new[sl]
+        return self.layers[layer].write(k, v, table, self.pages.start[sl], n_new=n_new, q=q, rope=self.rope,
+                                        q_out=q_out)
+
+    def attend(self, layer, query, seqs=None, scale=None, out=None):
+        sl, table = self._batch(seqs)
+        return self.layers[layer].attend(query, table, self.pages.lens[sl], max(self.pages._lens[sl], default=0),
+                                         scale=scale, out=out)
+
+    def read(self, layer, seqs=None, dtype=None):
+        """K, V (B, H, longest length, D); rows past a sequence's length are
+        zero."""
+        sl, table = self._batch(seqs)
+        return self.layers[layer].read(table, self.pages.lens[sl], max(self.pages._lens[sl], default=0), dtype)
+
+    def to_foveated(self, cfg=None, seqs=None, importance=None):
+        """A ``FoveatedKVCache`` of the sequences' contexts, compressed into
+        tiers: a prompt prefilled into pages decodes on with the fused
+        two-tier attention.  The sequences must have one length."""
+        from .tier_cache import FoveatedKVCache
+
+        lens = self.pages.lengths(seqs)
+        if not lens or len(set(lens)) != 1 or lens[0] == 0:
+            raise ValueError(f"tiers need sequences of one length, got {lens}")
+        cache = FoveatedKVCache(cfg)
+        for i in range(len(self.layers)):
+            cache.update(*self.read(i, seqs), i)
+        cache.compress(importance=importance)
+        return cache
+
+    def memory_bytes(self):
+        return sum(layer.memory_bytes() for layer in self.layers)
