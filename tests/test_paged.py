@@ -245,7 +245,7 @@ def test_read_refusals(c, word, kw):
     ("aligned", {"out": 0x1008}), ("multiples", {"q": {"stride_h": 60}}), ("workspace", {"ws": None}),
     ("workspace", {"ws_bytes": 16}), ("NULL table", {"table": None})])
 def test_attn_refusals(c, word, kw):
-    a = dict(format=2, q={}, q_dtype=0, Hq=4, B=1, table=c.at, n_table=64, stride=2 ** 27, lens=c.at, max_len=1024,
+    a = dict(format=2, q={}, q_dtype=0, Hq=4, B=1, table=c.at, n_table=64, stride=2 ** 27, lens=c.at, max_len=65536,
              scale=1.0, out=c.at, ws=c.at, ws_bytes=1 << 40)
     a.update(kw)
     rc = c.lib.fkv_paged_attn(R(c.pages(format=a["format"])), None if a["q"] is None else R(c.rows(**a["q"])),
