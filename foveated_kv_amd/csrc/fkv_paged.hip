@@ -2,7 +2,7 @@
 // encoded on the way) and the read-back.  All three stream rows once: eight
 // elements a lane, a row of D elements on D / 8 neighbouring lanes, so the
 // row's reductions (largest magnitude, minimum and maximum) are DPP steps
-// within 8 or 16 lanes and every access is 16 bytes a lane.
+// within 8 or 16 lanes.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -13,25 +13,29 @@
 namespace fkv {
 
 // ---------------------------------------------------------------------------
-// eight elements of an activation row
+// eight elements of a row: four from `lo` and four from `hi` on
 // ---------------------------------------------------------------------------
 
-template <int DT>
-__device__ inline void load8f(const char* row, int64_t elem, float (&x)[8]) {
-    if (DT == FKV_F32) {
-        const float4 a = ((const float4*)((const float*)row + elem))[0];
-        const float4 b = ((const float4*)((const float*)row + elem))[1];
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        return;
-    }
-    const uint4 w = *(const uint4*)((const uint16_t*)row + elem);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        x[2 * i] = DT == FKV_F16 ? h2f((uint16_t)u[i]) : __uint_as_float(u[i] << 16);
-        x[2 * i + 1] = DT == FKV_F16 ? h2f((uint16_t)(u[i] >> 16)) : __uint_as_float(u[i] & 0xFFFF0000u);
-    }
+// In the half layout a lane holds four pairs, elements lo..lo + 3 and their
+// partners hi = lo + rot / 2..; elsewhere eight neighbouring elements.
+struct Place8 {
+    int lo, hi;
+};
+
+// STREAM: results of a large call are stored past the caches: a 64K context
+// out of 8-bit pages 76.8 us, not 85; a 16K prompt into 8-bit keys and 4-bit
+// values 92, not 96.  (Loads past them as well gained nothing.)
+template <bool STREAM, typename T>
+__device__ inline void put(void* p, T v) {
+    if (STREAM) __builtin_nontemporal_store(v, (T*)p);
+    else *(T*)p = v;
 }
+
+// A lane's eight elements as they were loaded.
+template <int DT>
+struct Raw {
+    uint32_t w[DT == FKV_F32 ? 8 : 4];
+};
 
 __device__ inline uint32_t pack_bf16(float a, float b) {
     typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
@@ -41,15 +45,56 @@ __device__ inline uint32_t pack_bf16(float a, float b) {
 __device__ inline uint32_t pack_f16(float a, float b) { return (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16); }
 
 template <int DT>
-__device__ inline void store8f(char* row, int64_t elem, const float (&x)[8]) {
+__device__ inline uint32_t pack16(float a, float b) {
+    return DT == FKV_F16 ? pack_f16(a, b) : pack_bf16(a, b);
+}
+
+template <int DT, bool STREAM>
+__device__ inline void store4f(char* row, int64_t elem, const float* x) {
     if (DT == FKV_F32) {
-        ((float4*)((float*)row + elem))[0] = make_float4(x[0], x[1], x[2], x[3]);
-        ((float4*)((float*)row + elem))[1] = make_float4(x[4], x[5], x[6], x[7]);
+        put<STREAM>((float*)row + elem, fkv_u4{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                                               __float_as_uint(x[3])});
         return;
     }
-    auto two = [](float a, float b) { return DT == FKV_F16 ? pack_f16(a, b) : pack_bf16(a, b); };
-    *(uint4*)((uint16_t*)row + elem) =
-        make_uint4(two(x[0], x[1]), two(x[2], x[3]), two(x[4], x[5]), two(x[6], x[7]));
+    const fkv_u2 w = {pack16<DT>(x[0], x[1]), pack16<DT>(x[2], x[3])};
+    put<STREAM>((uint16_t*)row + elem, w);
+}
+
+// A lane's elements; PAIRS: hi may lie anywhere, else behind lo, and 16 bits an
+// element take one access.
+template <int DT, bool PAIRS>
+__device__ inline Raw<DT> load8(const char* row, Place8 at) {
+    Raw<DT> r;
+    if constexpr (DT == FKV_F32) {
+        const uint4 a = *(const uint4*)(row + 4 * at.lo), b = *(const uint4*)(row + 4 * at.hi);
+        r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w, r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
+    } else if constexpr (PAIRS) {
+        const uint2 a = *(const uint2*)(row + 2 * at.lo), b = *(const uint2*)(row + 2 * at.hi);
+        r.w[0] = a.x, r.w[1] = a.y, r.w[2] = b.x, r.w[3] = b.y;
+    } else {
+        const uint4 a = *(const uint4*)(row + 2 * at.lo);
+        r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
+    }
+    return r;
+}
+template <int DT>
+__device__ inline void unpack8(const Raw<DT>& r, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if (DT == FKV_F32) x[i] = __uint_as_float(r.w[i % (DT == FKV_F32 ? 8 : 4)]);
+        else if (DT == FKV_F16) x[i] = h2f((uint16_t)(r.w[i / 2] >> (16 * (i & 1))));
+        else x[i] = __uint_as_float(i & 1 ? r.w[i / 2] & 0xFFFF0000u : r.w[i / 2] << 16);
+    }
+}
+template <int DT, bool PAIRS, bool STREAM>
+__device__ inline void store8f(char* row, Place8 at, const float (&x)[8]) {
+    if (DT != FKV_F32 && !PAIRS) {
+        const fkv_u4 w = {pack16<DT>(x[0], x[1]), pack16<DT>(x[2], x[3]), pack16<DT>(x[4], x[5]), pack16<DT>(x[6], x[7])};
+        put<STREAM>(row + 2 * at.lo, w);
+    } else {
+        store4f<DT, STREAM>(row, at.lo, x);
+        store4f<DT, STREAM>(row, at.hi, x + 4);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -61,79 +106,88 @@ struct RopeView {
     int32_t n_pos, rot, interleaved;
 };
 
-// Elements [d0, d0 + 8) of a row at `pos`, rotated in place; `partner` holds
-// elements [d0 + rot/2, ..) or [d0 - rot/2, ..) of the row in the half layout.
-// The products of two fp32 numbers are exact in 64 bits, so the only rounding
-// before the result's own is the sum's, in 64 bits, and its rounding to fp32:
-// what a quantised key is decided from does not depend on the order of
-// evaluation.  Memory stays the bound (see the kernels below).
-__device__ inline void rotate8(float (&x)[8], const float (&partner)[8], const RopeView& r, int64_t pos, int d0) {
-    if (d0 >= r.rot) return;
-    const int hd = r.rot >> 1;
+// The elements of lane `lane_in_row`.
+__device__ inline Place8 place8(const RopeView& r, int lane_in_row) {
+    const int d0 = 8 * lane_in_row;
+    if (r.interleaved || d0 >= r.rot) return Place8{d0, d0 + 4};
+    return Place8{d0 >> 1, (d0 >> 1) + (r.rot >> 1)};
+}
+
+// cos and sin of a lane's four pairs at a position (NaN outside the table).
+struct Angles {
+    float c[4], s[4];
+};
+__device__ inline Angles angles_of(const RopeView& r, int64_t pos, int lane_in_row) {
+    Angles a;
     const bool inside = pos >= 0 && pos < r.n_pos;
-    const float* t = r.table + (inside ? pos : 0) * r.rot;
-    if (r.interleaved) {
-        const float4 c4 = *(const float4*)(t + (d0 >> 1)), s4 = *(const float4*)(t + hd + (d0 >> 1));
-        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const double a = x[2 * j], b = x[2 * j + 1], cd = c[j], sd = s[j];
-            x[2 * j] = (float)fma(a, cd, -(b * sd));
-            x[2 * j + 1] = (float)fma(b, cd, a * sd);
-        }
-    } else {
-        const bool second = d0 >= hd;
-        const int i0 = second ? d0 - hd : d0;
-        float c[8], s[8];
-#pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-            const float4 c4 = *(const float4*)(t + i0 + j), s4 = *(const float4*)(t + hd + i0 + j);
-            c[j] = c4.x, c[j + 1] = c4.y, c[j + 2] = c4.z, c[j + 3] = c4.w;
-            s[j] = s4.x, s[j + 1] = s4.y, s[j + 2] = s4.z, s[j + 3] = s4.w;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const double ps = (double)partner[j] * (double)s[j];
-            x[j] = (float)fma((double)x[j], (double)c[j], second ? ps : -ps);
-        }
-    }
-    if (!inside) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = __builtin_nanf("");
-    }
+    const float* t = r.table + (inside ? pos : 0) * r.rot + (8 * lane_in_row < r.rot ? 4 * lane_in_row : 0);
+    const float4 c = *(const float4*)t, s = *(const float4*)(t + (r.rot >> 1));
+    const float nan = __builtin_nanf("");
+    a.c[0] = inside ? c.x : nan, a.c[1] = inside ? c.y : nan, a.c[2] = inside ? c.z : nan, a.c[3] = inside ? c.w : nan;
+    a.s[0] = s.x, a.s[1] = s.y, a.s[2] = s.z, a.s[3] = s.w;
+    return a;
 }
 
-// Where the half layout's partner of elements [d0, d0 + 8) begins (d0 itself
-// where nothing is rotated, so that every lane loads inside its row).
-__device__ inline int partner_of(const RopeView& r, int d0) {
-    const int hd = r.rot >> 1;
-    if (r.interleaved || d0 >= r.rot) return d0;
-    return d0 < hd ? d0 + hd : d0 - hd;
+// a b - c d.  EXACT: the products of two fp32 numbers are exact in 64 bits, so
+// the only roundings are the sum's there and its own to fp32, and what a
+// quantised key is decided from does not depend on the order of evaluation.
+// Else in fp32, with the rounding error of c d taken back out (Kahan's
+// difference of products, within 1.5 units of the last place also where the
+// two cancel), for results that are rounded to 16 bits: in 64 bits those took
+// 127 us for a 16K prompt's 32 + 8 heads, where this takes XXX.
+template <bool EXACT>
+__device__ inline float cross(float a, float b, float c, float d) {
+    if (EXACT) return (float)fma((double)a, (double)b, -((double)c * (double)d));
+    const float cd = c * d;
+    return fmaf(a, b, -cd) - fmaf(c, d, -cd);
 }
 
-// One row of D elements on D / 8 lanes of one wave (rows never straddle
-// waves, and every lane has read its elements and its partner's before any
-// lane writes: out may be x).  A wave takes 64 / (D / 8) rows of consecutive
-// heads, which share the position's table row in the L1.
-template <int DT>
+// `inter`: the lane's elements are (a, b) pairs in turn, else four a, four b.
+template <bool EXACT>
+__device__ inline void rotate8(float (&x)[8], const RopeView& r, const Angles& t, int lane_in_row, bool inter) {
+    if (8 * lane_in_row >= r.rot) return;
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float a = inter ? x[2 * j] : x[j], b = inter ? x[2 * j + 1] : x[4 + j];
+        y[2 * j] = cross<EXACT>(a, t.c[j], b, t.s[j]);
+        y[2 * j + 1] = cross<EXACT>(b, t.c[j], a, -t.s[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = inter ? y[j] : y[2 * (j & 3) + (j >> 2)];
+}
+
+// One row of D elements on D / 8 lanes of one wave (each lane writes the
+// elements that it read: out may be x), the wave's rows and then N times as
+// many being consecutive heads of one token, which share the lane's angles.
+template <int DT, int N, bool PAIRS>
 __global__ void __launch_bounds__(256) rope_kernel(RowsView x, RowsView out, RopeView rope, PositionsView pos,
-                                                   uint32_t n_rows, uint32_t H, uint32_t L, uint32_t lanes,
+                                                   uint32_t n_units, uint32_t H, uint32_t L, uint32_t lanes,
                                                    uint32_t rows_per_wave) {
     constexpr int ES = DT == FKV_F32 ? 4 : 2;
-    const uint32_t lane = threadIdx.x & 63, wave = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const uint32_t in_wave = lane / lanes;
-    const uint64_t row = (uint64_t)wave * rows_per_wave + in_wave;
-    if (in_wave >= rows_per_wave || row >= n_rows) return;
-    const uint32_t r = (uint32_t)row, tok = r / H, h = r - tok * H, b = tok / L, l = tok - b * L;
-    const int d0 = 8 * (lane - in_wave * lanes);
-    const char* src = x.data + (b * x.sb + h * x.sh + l * x.sl) * ES;
-    float v[8], p[8];
-    load8f<DT>(src, d0, v);
-    load8f<DT>(src, partner_of(rope, d0), p);
-    __builtin_amdgcn_wave_barrier();
-    rotate8(v, p, rope, position_of(pos, b, l), d0);
-    __builtin_amdgcn_wave_barrier();
-    store8f<DT>(out.data + (b * out.sb + h * out.sh + l * out.sl) * ES, d0, v);
+    const uint32_t lane = threadIdx.x & 63, unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t sub = lane / lanes, lr = lane - sub * lanes, step = rows_per_wave;
+    if (sub >= step || unit >= n_units) return;
+    const uint32_t chunks = (H + N * step - 1) / (N * step);
+    const uint32_t tok = unit / chunks, h0 = (unit - tok * chunks) * N * step + sub, b = tok / L, l = tok - b * L;
+    if (h0 >= H) return;
+    const Place8 at = place8(rope, lr);
+    const char* src = x.data + (b * x.sb + l * x.sl) * ES;
+    char* dst = out.data + (b * out.sb + l * out.sl) * ES;
+    const Angles t = angles_of(rope, position_of(pos, b, l), lr);
+    Raw<DT> raw[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {  // (past the last head: loaded, not used)
+        const uint32_t h = h0 + i * step < H ? h0 + i * step : h0;
+        raw[i] = load8<DT, PAIRS>(src + h * x.sh * ES, at);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        float v[8];
+        unpack8<DT>(raw[i], v);
+        rotate8<DT == FKV_F32>(v, rope, t, lr, N > 1 ? !PAIRS : rope.interleaved);
+        if (h0 + i * step < H) store8f<DT, PAIRS, (N > 1)>(dst + (h0 + i * step) * out.sh * ES, at, v);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -178,8 +232,10 @@ __device__ inline uint32_t encode_fp8(const float (&x)[8], uint32_t (&codes)[2])
 }
 
 // INT4 codes of the row's eight elements (even dim in the low nibble).  The
-// quotient is decided exactly: floor(d / s) within one unit in 64 bits, then
-// the sign of d - (k + 1/2) s, whose fma rounds once.
+// quotient (x - min) / scale in fp32 is off by less than 4e-6 (four roundings
+// of a number up to 15); where it comes within 1e-4 of the middle between two
+// codes, or is no number, the sign of d - (k + 1/2) scale decides in 64 bits,
+// whose fma rounds once: always the code that the exact quotient rounds to.
 template <int D>
 __device__ inline uint32_t encode_int4(const float (&x)[8], float& scale, float& zero) {
     float lo = x[0], hi = x[0], bad = 0.0f;
@@ -195,45 +251,58 @@ __device__ inline uint32_t encode_int4(const float (&x)[8], float& scale, float&
     const float s = (float)(((double)hi - (double)lo) / 15.0);
     scale = bad == 0.0f ? s : __builtin_nanf("");
     zero = lo;
-    const double sd = s, inv = 1.0 / sd;
+    const float inv = __builtin_amdgcn_rcpf(s);
+    float k[8];
+    bool close = false;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float t = (x[j] - lo) * inv;
+        k[j] = floorf(t);
+        const float past = t - k[j] - 0.5f;
+        close |= !(fabsf(past) > 1e-4f);
+        k[j] += past > 0.0f ? 1.0f : 0.0f;
+    }
+    if (close) {
+        const double sd = s, rcp = 1.0 / sd;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const double d = (double)x[j] - (double)lo, f = floor(d * rcp), r = fma(-(f + 0.5), sd, d);
+            k[j] = (float)f + (r > 0.0 || (r == 0.0 && ((int)f & 1)) ? 1.0f : 0.0f);
+        }
+    }
     uint32_t packed = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const double d = (double)x[j] - (double)lo;
-        double k = floor(d * inv);
-        const double r = fma(-(k + 0.5), sd, d);
-        int c = (int)k;
-        c += r > 0.0 || (r == 0.0 && (c & 1));
-        c = c < 0 ? 0 : c > 15 ? 15 : c;
-        if (!(s > 0.0f)) c = 0;
-        packed |= (uint32_t)c << (4 * j);
+        const uint32_t c = s > 0.0f ? (uint32_t)__builtin_amdgcn_fmed3f(k[j], 0.0f, 15.0f) : 0;
+        packed |= c << (4 * j);
     }
     return packed;
 }
 
-// Eight elements of row `row` of K (or V), stored as the format has them.
-template <int D, int FMT, bool VALUE>
-__device__ inline void store_row(const PageView& pg, int64_t row, int lane_in_row, const float (&x)[8]) {
-    const int64_t at = row * D + 8 * lane_in_row;
+// A lane's elements of row `row` of K (or V), stored as the format has them.
+// (Values lie at neighbouring elements.)  Pages stay in the caches, for the
+// attention or the read that follows: read back at once a 16K prompt takes 16
+// us, not 22.
+template <int D, int FMT, bool VALUE, bool PAIRS>
+__device__ inline void store_row(const PageView& pg, int64_t row, int lane_in_row, Place8 at, const float (&x)[8]) {
     char* base = VALUE ? pg.v : pg.k;
-    if (FMT == FKV_PAGES_F16) {
-        store8f<FKV_F16>(base, at, x);
-    } else if (FMT == FKV_PAGES_BF16) {
-        store8f<FKV_BF16>(base, at, x);
+    if (FMT <= FKV_PAGES_BF16) {
+        store8f<FMT == FKV_PAGES_F16 ? FKV_F16 : FKV_BF16, PAIRS, false>(base + row * (2 * D), at, x);
     } else if (FMT == FKV_PAGES_FP8 || !VALUE) {
         uint32_t codes[2];
         const uint32_t byte = encode_fp8<D>(x, codes);
-        if (row >= 0) {
-            *(uint2*)(base + at) = make_uint2(codes[0], codes[1]);
-            if (lane_in_row == 0) (VALUE ? (uint8_t*)pg.v_scale : pg.k_exp)[row] = (uint8_t)byte;
+        if (PAIRS) {
+            *(uint32_t*)(base + row * D + at.lo) = codes[0];
+            *(uint32_t*)(base + row * D + at.hi) = codes[1];
+        } else {
+            *(uint2*)(base + row * D + at.lo) = make_uint2(codes[0], codes[1]);
         }
+        if (lane_in_row == 0) (VALUE ? (uint8_t*)pg.v_scale : pg.k_exp)[row] = (uint8_t)byte;
     } else {
         float scale, zero;
         const uint32_t codes = encode_int4<D>(x, scale, zero);
-        if (row >= 0) {
-            *(uint32_t*)(base + at / 2) = codes;
-            if (lane_in_row == 0) ((float2*)pg.v_scale)[row] = make_float2(scale, zero);
-        }
+        *(uint32_t*)(base + row * (D / 2) + at.lo / 2) = codes;
+        if (lane_in_row == 0) ((float2*)pg.v_scale)[row] = make_float2(scale, zero);
     }
 }
 
@@ -248,42 +317,64 @@ struct WriteArgs {
     PositionsView start;
     RopeView rope;
     const int32_t* n_new;
-    uint32_t n_rows, B, L, Hq;
+    uint32_t n_units, n_tokens, L, Hq;
 };
 
-// Rows (b, l, head) with the token's queries first, then its keys and its
-// values: one launch for a decode step's rotation and its cache write.
-template <int D, int DT, int FMT>
-__global__ void __launch_bounds__(256) paged_write_kernel(WriteArgs a) {
-    constexpr int LPR = D / 8, ES = DT == FKV_F32 ? 4 : 2;
-    const uint32_t r = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-    if (r >= a.n_rows) return;
-    const uint32_t HT = a.Hq + 2 * a.pg.H;
-    const uint32_t tok = r / HT, hh = r - tok * HT, b = tok / a.L, l = tok - b * a.L;
-    if (a.n_new && (int32_t)l >= a.n_new[b]) return;
-    const int lr = threadIdx.x % LPR, d0 = 8 * lr;
+enum { kQueries, kKeys, kValues };
+
+// N consecutive heads of the wave's tokens.
+template <int D, int DT, int FMT, int N, bool PAIRS, int KIND>
+__device__ inline void write_heads(const WriteArgs& a, uint32_t h0, uint32_t b, uint32_t l, int lr) {
+    constexpr int ES = DT == FKV_F32 ? 4 : 2;
+    constexpr bool kExact = DT == FKV_F32 || (KIND == kKeys && FMT >= FKV_PAGES_FP8);
+    const RowsView& in = KIND == kQueries ? a.q : KIND == kKeys ? a.k : a.v;
+    const uint32_t heads = KIND == kQueries ? a.Hq : a.pg.H;
+    const bool inter = N > 1 ? !PAIRS : a.rope.interleaved;
+    const Place8 at = KIND == kValues ? Place8{8 * lr, 8 * lr + 4} : place8(a.rope, lr);
+    const char* src = in.data + ((int64_t)b * in.sb + (int64_t)l * in.sl) * ES;
+    Raw<DT> raw[N];
+#pragma unroll
+    for (int i = 0; i < N; i++)  // (past the last head: loaded, not used)
+        raw[i] = load8<DT, PAIRS && KIND != kValues>(src + (h0 + i < heads ? h0 + i : heads - 1) * in.sh * ES, at);
     const int64_t pos = position_of(a.start, b, l);
-    const bool is_q = hh < a.Hq, is_v = hh >= a.Hq + a.pg.H;
-    const uint32_t h = is_q ? hh : is_v ? hh - a.Hq - a.pg.H : hh - a.Hq;
-    const RowsView& in = is_q ? a.q : is_v ? a.v : a.k;
-    const char* src = in.data + ((int64_t)b * in.sb + h * in.sh + l * in.sl) * ES;
-    float x[8], p[8];
-    load8f<DT>(src, d0, x);
-    if (!is_v && a.rope.rot) {
-        load8f<DT>(src, partner_of(a.rope, d0), p);
-        __builtin_amdgcn_wave_barrier();
-        rotate8(x, p, a.rope, pos, d0);
+    Angles t = {};
+    if (KIND != kValues && a.rope.rot) t = angles_of(a.rope, pos, lr);
+    int64_t row = 0;
+    if (KIND != kQueries) {
+        row = page_row(a.pg, a.table, b, pos, h0);
+        if (row < 0) return;  // (all lanes of a row agree)
     }
-    __builtin_amdgcn_wave_barrier();
-    if (is_q) {
-        store8f<DT>(a.q_out.data + ((int64_t)b * a.q_out.sb + h * a.q_out.sh + l * a.q_out.sl) * ES, d0, x);
-        return;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (h0 + i >= heads) return;
+        float x[8];
+        unpack8<DT>(raw[i], x);
+        if (KIND != kValues) rotate8<kExact>(x, a.rope, t, lr, inter);
+        if (KIND == kQueries)
+            store8f<DT, PAIRS, (N > 1)>(a.q_out.data + ((int64_t)b * a.q_out.sb + (h0 + i) * a.q_out.sh + (int64_t)l * a.q_out.sl) * ES,
+                                        at, x);
+        else
+            store_row<D, FMT, KIND == kValues, PAIRS && KIND != kValues>(a.pg, row + (int64_t)i * a.pg.page_size, lr, at, x);
     }
-    // (all lanes of a row agree on its place, so they leave together)
-    const int64_t row = page_row(a.pg, a.table, b, pos, h);
-    if (row < 0) return;
-    if (is_v) store_row<D, FMT, true>(a.pg, row, lr, x);
-    else store_row<D, FMT, false>(a.pg, row, lr, x);
+}
+
+// One launch for a step's rotation and its cache write.  A wave takes 64 /
+// (D / 8) neighbouring tokens, a row of each at a time, and N consecutive
+// heads of them, queries, keys or values: its stores of a head are
+// neighbouring rows, and exponents or scales, of a page.
+template <int D, int DT, int FMT, int N, bool PAIRS>
+__global__ void __launch_bounds__(256) paged_write_kernel(WriteArgs a) {
+    constexpr int LPR = D / 8, TOKENS = 64 / LPR;
+    const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    if (unit >= a.n_units) return;
+    const uint32_t cq = (a.Hq + N - 1) / N, ck = (a.pg.H + N - 1) / N, chunks = cq + 2 * ck;
+    const uint32_t group = unit / chunks, chunk = unit - group * chunks;
+    const uint32_t tok = group * TOKENS + lane / LPR, b = tok / a.L, l = tok - b * a.L;
+    if (tok >= a.n_tokens || (a.n_new && (int32_t)l >= a.n_new[b])) return;
+    const int lr = lane % LPR;
+    if (chunk < cq) write_heads<D, DT, FMT, N, PAIRS, kQueries>(a, chunk * N, b, l, lr);
+    else if (chunk < cq + ck) write_heads<D, DT, FMT, N, PAIRS, kKeys>(a, (chunk - cq) * N, b, l, lr);
+    else write_heads<D, DT, FMT, N, PAIRS, kValues>(a, (chunk - cq - ck) * N, b, l, lr);
 }
 
 // ---------------------------------------------------------------------------
@@ -305,10 +396,9 @@ template <int D, int FMT, bool VALUE>
 __device__ inline void load_row(const PageView& pg, int64_t row, int lane_in_row, float (&x)[8]) {
     const int64_t at = row * D + 8 * lane_in_row;
     const char* base = VALUE ? pg.v : pg.k;
-    if (FMT == FKV_PAGES_F16) {
-        load8f<FKV_F16>(base, at, x);
-    } else if (FMT == FKV_PAGES_BF16) {
-        load8f<FKV_BF16>(base, at, x);
+    if (FMT <= FKV_PAGES_BF16) {
+        constexpr int DT = FMT == FKV_PAGES_F16 ? FKV_F16 : FKV_BF16;
+        unpack8<DT>(load8<DT, false>(base + 2 * at, Place8{0, 4}), x);
     } else if (FMT == FKV_PAGES_FP8 || !VALUE) {
         const uint32_t byte = (VALUE ? (const uint8_t*)pg.v_scale : pg.k_exp)[row];
         decode_fp8(*(const uint2*)(base + at), exp_byte(byte), x);
@@ -325,27 +415,36 @@ struct ReadArgs {
     TableView table;
     const int32_t* lens;
     char *k, *v;
-    uint32_t n_rows, S;
+    uint32_t n_units, S;
 };
 
-// Rows (b, h, s): neighbouring rows of a wave are neighbouring tokens of a
-// page and of the result.
+// 16 tokens of a head, which one page holds, on each wave: N rows of K and of
+// V a lane, all of their loads in flight together.
 template <int D, int FMT, int DT>
 __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs a) {
-    constexpr int LPR = D / 8;
-    const uint32_t r = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-    if (r >= a.n_rows) return;
-    const uint32_t bh = r / a.S, s = r - bh * a.S, b = bh / a.pg.H, h = bh - b * a.pg.H;
-    const int lr = threadIdx.x % LPR;
-    float k[8] = {}, v[8] = {};
-    const int64_t row = (int32_t)s < a.lens[b] ? page_row(a.pg, a.table, b, s, h) : -1;
-    if (row >= 0) {
-        load_row<D, FMT, false>(a.pg, row, lr, k);
-        load_row<D, FMT, true>(a.pg, row, lr, v);
+    constexpr int LPR = D / 8, STEP = 64 / LPR, N = 16 / STEP;
+    const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (unit >= a.n_units) return;
+    const uint32_t chunks = (a.S + 15) / 16, bh = unit / chunks, first = 16 * (unit - bh * chunks);
+    const uint32_t b = bh / a.pg.H, h = bh - b * a.pg.H, s0 = first + lane / LPR;
+    const int lr = lane % LPR;
+    const int32_t len = a.lens[b];
+    const int64_t row0 = (int32_t)first < len ? page_row(a.pg, a.table, b, first, h) : -1;
+    float k[N][8] = {}, v[N][8] = {};
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (row0 < 0 || (int32_t)(s0 + i * STEP) >= len) break;
+        load_row<D, FMT, false>(a.pg, row0 + lane / LPR + i * STEP, lr, k[i]);
+        load_row<D, FMT, true>(a.pg, row0 + lane / LPR + i * STEP, lr, v[i]);
     }
-    const int64_t at = (int64_t)r * D + 8 * lr;
-    store8f<DT>(a.k, at, k);
-    store8f<DT>(a.v, at, v);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (s0 + i * STEP >= a.S) break;
+        const int64_t at = ((int64_t)bh * a.S + s0 + i * STEP) * D;
+        const Place8 e = {8 * lr, 8 * lr + 4};
+        store8f<DT, false, true>(a.k + at * (DT == FKV_F32 ? 4 : 2), e, k[i]);
+        store8f<DT, false, true>(a.v + at * (DT == FKV_F32 ? 4 : 2), e, v[i]);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -410,13 +509,34 @@ static PositionsView positions_view(const fkv_positions* p) {
     return PositionsView{p->data, p->stride_b, p->stride_l, p->base, p->is64, p->per_token};
 }
 
+// Rows that a lane takes one after the other: with four, the angles, the
+// position and the divisions serve four rows, whose loads are in flight
+// together; with one, few rows spread over more of the chip.
+// (98K rows, four prompts' chunks of 512 tokens: 14.8 us with four, 17 with
+// one; 3K rows, a decode step of 64 sequences, 4.0 with one.)
+constexpr int64_t kFewRows = 16384;
+
+template <int D, int DT, int FMT>
+static void launch_write_f(WriteArgs& a, int64_t tokens, hipStream_t s) {
+    const int64_t heads = a.Hq + 2 * (int64_t)a.pg.H;
+    a.n_tokens = (uint32_t)tokens;
+    auto go = [&](auto n, auto pairs) {
+        constexpr int N = decltype(n)::value;
+        a.n_units = (uint32_t)(cdiv(tokens, 64 / (D / 8)) * (cdiv(a.Hq, N) + 2 * cdiv(a.pg.H, N)));
+        paged_write_kernel<D, DT, FMT, N, decltype(pairs)::value><<<(uint32_t)cdiv(a.n_units, 4), 256, 0, s>>>(a);
+    };
+    if (tokens * heads <= kFewRows) go(std::integral_constant<int, 1>{}, std::true_type{});
+    else if (a.rope.rot && !a.rope.interleaved) go(std::integral_constant<int, 4>{}, std::true_type{});
+    else go(std::integral_constant<int, 4>{}, std::false_type{});
+}
+
 template <int D, int DT>
-static void launch_write(const WriteArgs& a, int format, uint32_t blocks, hipStream_t s) {
+static void launch_write(WriteArgs& a, int format, int64_t tokens, hipStream_t s) {
     switch (format) {
-        case FKV_PAGES_F16: paged_write_kernel<D, DT, FKV_PAGES_F16><<<blocks, 256, 0, s>>>(a); break;
-        case FKV_PAGES_BF16: paged_write_kernel<D, DT, FKV_PAGES_BF16><<<blocks, 256, 0, s>>>(a); break;
-        case FKV_PAGES_FP8: paged_write_kernel<D, DT, FKV_PAGES_FP8><<<blocks, 256, 0, s>>>(a); break;
-        default: paged_write_kernel<D, DT, FKV_PAGES_FP8_INT4><<<blocks, 256, 0, s>>>(a); break;
+        case FKV_PAGES_F16: launch_write_f<D, DT, FKV_PAGES_F16>(a, tokens, s); break;
+        case FKV_PAGES_BF16: launch_write_f<D, DT, FKV_PAGES_BF16>(a, tokens, s); break;
+        case FKV_PAGES_FP8: launch_write_f<D, DT, FKV_PAGES_FP8>(a, tokens, s); break;
+        default: launch_write_f<D, DT, FKV_PAGES_FP8_INT4>(a, tokens, s); break;
     }
 }
 
@@ -449,17 +569,24 @@ int fkv_rope_apply(const fkv_rope* rope, const fkv_rows* x, const fkv_rows* out,
     if (n >= 2147483648.0) return set_error(std::string(w) + ": more than 2^31 rows");
     if (int e = check_rows(w, x)) return e;
     if (int e = check_rows(w, out)) return e;
-    const uint32_t rows = (uint32_t)((int64_t)B * H * L), lanes = D / 8, rpw = 64 / lanes;
-    const uint32_t blocks = (uint32_t)cdiv(rows, 4 * (int64_t)rpw);
+    const uint32_t lanes = D / 8, rpw = 64 / lanes;
     const RopeView rv{rope->table, rope->n_positions, rope->rot_dim, rope->interleaved};
     const PositionsView pv = positions_view(positions);
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == FKV_F16)
-        rope_kernel<FKV_F16><<<blocks, 256, 0, s>>>(rows_view(x), rows_view(out), rv, pv, rows, H, L, lanes, rpw);
-    else if (dtype == FKV_BF16)
-        rope_kernel<FKV_BF16><<<blocks, 256, 0, s>>>(rows_view(x), rows_view(out), rv, pv, rows, H, L, lanes, rpw);
-    else
-        rope_kernel<FKV_F32><<<blocks, 256, 0, s>>>(rows_view(x), rows_view(out), rv, pv, rows, H, L, lanes, rpw);
+    auto go = [&](auto dt, auto n, auto pairs) {
+        constexpr int DT = decltype(dt)::value, N = decltype(n)::value;
+        const uint32_t units = (uint32_t)((int64_t)B * L * cdiv(H, N * (int64_t)rpw));
+        rope_kernel<DT, N, decltype(pairs)::value><<<(uint32_t)cdiv(units, 4), 256, 0, s>>>(
+            rows_view(x), rows_view(out), rv, pv, units, H, L, lanes, rpw);
+    };
+    auto by_rows = [&](auto dt) {
+        if ((int64_t)B * H * L <= kFewRows) go(dt, std::integral_constant<int, 1>{}, std::true_type{});
+        else if (!rope->interleaved) go(dt, std::integral_constant<int, 4>{}, std::true_type{});
+        else go(dt, std::integral_constant<int, 4>{}, std::false_type{});
+    };
+    if (dtype == FKV_F16) by_rows(std::integral_constant<int, FKV_F16>{});
+    else if (dtype == FKV_BF16) by_rows(std::integral_constant<int, FKV_BF16>{});
+    else by_rows(std::integral_constant<int, FKV_F32>{});
     return check_hip(hipGetLastError(), w);
 }
 
@@ -498,20 +625,18 @@ int fkv_paged_write(const fkv_pages* pages, const fkv_rows* k, const fkv_rows* v
     a.start = positions_view(start);
     a.rope = rope ? RopeView{rope->table, rope->n_positions, rope->rot_dim, rope->interleaved} : RopeView{};
     a.n_new = n_new;
-    a.n_rows = (uint32_t)((int64_t)B * L * heads);
-    a.B = B;
     a.L = L;
     a.Hq = q ? Hq : 0;
-    const uint32_t blocks = (uint32_t)cdiv(a.n_rows, 256 / (pages->D / 8));
+    const int64_t tokens = (int64_t)B * L;
     hipStream_t s = (hipStream_t)stream;
     if (pages->D == 64) {
-        if (dtype == FKV_F16) launch_write<64, FKV_F16>(a, pages->format, blocks, s);
-        else if (dtype == FKV_BF16) launch_write<64, FKV_BF16>(a, pages->format, blocks, s);
-        else launch_write<64, FKV_F32>(a, pages->format, blocks, s);
+        if (dtype == FKV_F16) launch_write<64, FKV_F16>(a, pages->format, tokens, s);
+        else if (dtype == FKV_BF16) launch_write<64, FKV_BF16>(a, pages->format, tokens, s);
+        else launch_write<64, FKV_F32>(a, pages->format, tokens, s);
     } else {
-        if (dtype == FKV_F16) launch_write<128, FKV_F16>(a, pages->format, blocks, s);
-        else if (dtype == FKV_BF16) launch_write<128, FKV_BF16>(a, pages->format, blocks, s);
-        else launch_write<128, FKV_F32>(a, pages->format, blocks, s);
+        if (dtype == FKV_F16) launch_write<128, FKV_F16>(a, pages->format, tokens, s);
+        else if (dtype == FKV_BF16) launch_write<128, FKV_BF16>(a, pages->format, tokens, s);
+        else launch_write<128, FKV_F32>(a, pages->format, tokens, s);
     }
     return check_hip(hipGetLastError(), w);
 }
@@ -535,9 +660,9 @@ int fkv_paged_read(const fkv_pages* pages, const int32_t* table, int32_t n_table
     a.lens = lens;
     a.k = (char*)out_k;
     a.v = (char*)out_v;
-    a.n_rows = (uint32_t)((int64_t)B * S * pages->H);
+    a.n_units = (uint32_t)(B * pages->H * cdiv(S, 16));
     a.S = S;
-    const uint32_t blocks = (uint32_t)cdiv(a.n_rows, 256 / (pages->D / 8));
+    const uint32_t blocks = (uint32_t)cdiv(a.n_units, 4);
     hipStream_t s = (hipStream_t)stream;
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
