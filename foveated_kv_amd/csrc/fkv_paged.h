@@ -52,7 +52,8 @@ __device__ inline int64_t position_of(const PositionsView& p, int64_t b, int64_t
 // outside the table or a page id outside the pool names no row.
 __device__ inline int64_t page_row(const PageView& pg, const TableView& t, int64_t b, int64_t pos, int32_t h) {
     if (pos < 0 || pos >= (int64_t)t.n * pg.page_size) return -1;
-    const int32_t i = (int32_t)(pos / pg.page_size), off = (int32_t)(pos - (int64_t)i * pg.page_size);
+    const int32_t i = (int32_t)(pos >> (31 - __builtin_clz((unsigned)pg.page_size)));  // (a power of two)
+    const int32_t off = (int32_t)pos & (pg.page_size - 1);
     const int32_t id = t.ids[b * t.stride + i];
     if ((uint32_t)id >= (uint32_t)pg.n_pages) return -1;
     return ((int64_t)id * pg.H + h) * pg.page_size + off;

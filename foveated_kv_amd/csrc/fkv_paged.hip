@@ -3,6 +3,10 @@
 // elements a lane, a row of D elements on D / 8 neighbouring lanes, so the
 // row's reductions (largest magnitude, minimum and maximum) are DPP steps
 // within 8 or 16 lanes.
+// (Contraction would also merge the rounding of a 64-bit sum to fp32 with the
+// one to 16 bits behind it; results are rounded to fp32 first, whatever
+// follows.)
+#pragma clang fp contract(off)
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -128,30 +132,23 @@ __device__ inline Angles angles_of(const RopeView& r, int64_t pos, int lane_in_r
     return a;
 }
 
-// a b - c d.  EXACT: the products of two fp32 numbers are exact in 64 bits, so
-// the only roundings are the sum's there and its own to fp32, and what a
-// quantised key is decided from does not depend on the order of evaluation.
-// Else in fp32, with the rounding error of c d taken back out (Kahan's
-// difference of products, within 1.5 units of the last place also where the
-// two cancel), for results that are rounded to 16 bits: in 64 bits those took
-// 127 us for a 16K prompt's 32 + 8 heads, where this takes XXX.
-template <bool EXACT>
+// a b - c d.  The products of two fp32 numbers are exact in 64 bits, so the only
+// roundings are the sum's there and its own to fp32, and what a quantised key
+// is decided from does not depend on the order of evaluation.  (In fp32 the
+// 16K prompt's 32 + 8 heads took 65.3 us, so 66.0: memory is the bound.)
 __device__ inline float cross(float a, float b, float c, float d) {
-    if (EXACT) return (float)fma((double)a, (double)b, -((double)c * (double)d));
-    const float cd = c * d;
-    return fmaf(a, b, -cd) - fmaf(c, d, -cd);
+    return (float)fma((double)a, (double)b, -((double)c * (double)d));
 }
 
 // `inter`: the lane's elements are (a, b) pairs in turn, else four a, four b.
-template <bool EXACT>
 __device__ inline void rotate8(float (&x)[8], const RopeView& r, const Angles& t, int lane_in_row, bool inter) {
     if (8 * lane_in_row >= r.rot) return;
     float y[8];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const float a = inter ? x[2 * j] : x[j], b = inter ? x[2 * j + 1] : x[4 + j];
-        y[2 * j] = cross<EXACT>(a, t.c[j], b, t.s[j]);
-        y[2 * j + 1] = cross<EXACT>(b, t.c[j], a, -t.s[j]);
+        y[2 * j] = cross(a, t.c[j], b, t.s[j]);
+        y[2 * j + 1] = cross(b, t.c[j], a, -t.s[j]);
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) x[j] = inter ? y[j] : y[2 * (j & 3) + (j >> 2)];
@@ -185,7 +182,7 @@ __global__ void __launch_bounds__(256) rope_kernel(RowsView x, RowsView out, Rop
     for (int i = 0; i < N; i++) {
         float v[8];
         unpack8<DT>(raw[i], v);
-        rotate8<DT == FKV_F32>(v, rope, t, lr, N > 1 ? !PAIRS : rope.interleaved);
+        rotate8(v, rope, t, lr, N > 1 ? !PAIRS : rope.interleaved);
         if (h0 + i * step < H) store8f<DT, PAIRS, (N > 1)>(dst + (h0 + i * step) * out.sh * ES, at, v);
     }
 }
@@ -326,7 +323,6 @@ enum { kQueries, kKeys, kValues };
 template <int D, int DT, int FMT, int N, bool PAIRS, int KIND>
 __device__ inline void write_heads(const WriteArgs& a, uint32_t h0, uint32_t b, uint32_t l, int lr) {
     constexpr int ES = DT == FKV_F32 ? 4 : 2;
-    constexpr bool kExact = DT == FKV_F32 || (KIND == kKeys && FMT >= FKV_PAGES_FP8);
     const RowsView& in = KIND == kQueries ? a.q : KIND == kKeys ? a.k : a.v;
     const uint32_t heads = KIND == kQueries ? a.Hq : a.pg.H;
     const bool inter = N > 1 ? !PAIRS : a.rope.interleaved;
@@ -349,7 +345,7 @@ __device__ inline void write_heads(const WriteArgs& a, uint32_t h0, uint32_t b, 
         if (h0 + i >= heads) return;
         float x[8];
         unpack8<DT>(raw[i], x);
-        if (KIND != kValues) rotate8<kExact>(x, a.rope, t, lr, inter);
+        if (KIND != kValues) rotate8(x, a.rope, t, lr, inter);
         if (KIND == kQueries)
             store8f<DT, PAIRS, (N > 1)>(a.q_out.data + ((int64_t)b * a.q_out.sb + (h0 + i) * a.q_out.sh + (int64_t)l * a.q_out.sl) * ES,
                                         at, x);

@@ -281,27 +281,27 @@ __device__ inline void accumulate(const Step<D, FMT>& st, const float (&s)[8], S
             w[j] *= st.sz[j >> 2][(j & 3) >> 1][2 * (j & 1)];
         }
     }
-    // fp16 rows: weights to fp16 (11 bits, as the rows; 2^-12 of a weight at
-    // most).  Elsewhere: bf16 weights, which have the range that the rows'
-    // scales need but 8 bits, so each is taken as the sum of two (16 bits).
+    // Each weight as the sum of two 16-bit numbers, in the values' type (22 bits)
+    // or, for quantised rows, in bf16 (16 bits), which has the range that rows'
+    // scales need: the result is then as near to 64 bits as its own rounding
+    // allows, where one fp16 weight was 20 % further off, and the second product
+    // costs nothing beside the rows' loads.
+    constexpr bool kHalf = FMT == FKV_PAGES_F16;
     u4 hi, lo;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const float x = w[2 * j], y = w[2 * j + 1];
-        if (FMT == FKV_PAGES_F16) {
+        if (kHalf) {
             hi[j] = (uint32_t)f2h(x) | ((uint32_t)f2h(y) << 16);
+            lo[j] = (uint32_t)f2h(x - h2f((uint16_t)hi[j])) | ((uint32_t)f2h(y - h2f((uint16_t)(hi[j] >> 16))) << 16);
         } else {
             hi[j] = bf16_pair(x, y);
             lo[j] = bf16_pair(x - __uint_as_float(hi[j] << 16), y - __uint_as_float(hi[j] & 0xFFFF0000u));
         }
     }
     auto add = [&](int d, u4 v) {
-        if (FMT == FKV_PAGES_F16) {
-            u.acc[d] = mfma<false>(v, hi, u.acc[d]);
-        } else {
-            u.acc[d] = mfma<true>(v, hi, u.acc[d]);
-            u.acc[d] = mfma<true>(v, lo, u.acc[d]);
-        }
+        u.acc[d] = mfma<!kHalf>(v, hi, u.acc[d]);
+        u.acc[d] = mfma<!kHalf>(v, lo, u.acc[d]);
     };
     if (FMT <= FKV_PAGES_BF16) {
 #pragma unroll

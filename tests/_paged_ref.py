@@ -130,14 +130,14 @@ def attend(q, values, table, lens, page, n_pages, scale):
     return out, lse, spread, ds
 
 
-def attend_bound(out, spread, ds, lens, dtype, fmt):
+def attend_bound(out, spread, ds, lens, dtype):
     """What the kernel's result may be off by: its own rounding; each weight's
     relative error, from its score (exp magnifies it by 1 + ds; twice, once in
-    the sum), from exp2 (2^-22) and from its rounding (fp16 2^-11; two bf16
-    2^-16); the value of an INT4 row in fp32 (scale times code plus minimum,
+    the sum), from exp2 (2^-22) and from its rounding (as a sum of two bf16
+    numbers 2^-16, of two fp16 ones less); the value of an INT4 row in fp32 (scale times code plus minimum,
     folded into the weights: as a weight's error); fp32 sums over n tokens in
     pieces of 32 and then waves and workgroups (n / 32 + 64 roundings)."""
-    w = 2.0 ** -11 if fmt == "fp16" else 2.0 ** -16
+    w = 2.0 ** -16
     n = max(int(max(lens)), 1)
     rel = 2 * ds[..., None] * 1.01 + w + 2.0 ** -21 + (n / 32 + 64) * 2.0 ** -24
     return UNIT[dtype] * np.abs(out) + TINY[dtype] + rel * spread

@@ -292,7 +292,7 @@ def _check_attend(layer, q, table, lens, scale=None, **kw):
     add = kw.get("lens_add", 0)
     want, wlse, spread, ds = ref.attend(ref.f64(q)[:, :, 0], ref.page_values(layer), table.numpy(),
                                         [n + add for n in lens], layer.page_size, layer.n_pages, s)
-    tol = ref.attend_bound(want, spread, ds, [n + add for n in lens], q.dtype, layer.fmt)
+    tol = ref.attend_bound(want, spread, ds, [n + add for n in lens], q.dtype)
     err = np.abs(ref.f64(out)[:, :, 0] - want)
     assert (err <= tol).all(), f"error {np.nanmax(err / tol)} of the bound, NaN {np.isnan(err).sum()}"
     g = ref.f64(lse)

@@ -80,7 +80,7 @@ def test_cache_run(fkv, fmt, dtype):
                 layer = cache.layers[i]
                 want, _, spread, ds = ref.attend(ref.f64(qr)[:, :, 0], ref.page_values(layer),
                                                  cache.pages.table[seqs].cpu().numpy(), n, page, 24, D ** -0.5)
-                tol = ref.attend_bound(want, spread, ds, n, dtype, fmt)
+                tol = ref.attend_bound(want, spread, ds, n, dtype)
                 assert (np.abs(ref.f64(out)[:, :, 0] - want) <= tol).all()
 
     step([40, 1, 17])
