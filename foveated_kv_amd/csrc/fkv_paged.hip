@@ -512,27 +512,36 @@ static PositionsView positions_view(const fkv_positions* p) {
 // one; 3K rows, a decode step of 64 sequences, 4.0 with one.)
 constexpr int64_t kFewRows = 16384;
 
+// A grid has fewer than 2^32 threads: waves, four to a workgroup, that a launch
+// may have.
+constexpr int64_t kMaxUnits = 4 * ((int64_t{1} << 24) - 1);
+
+static int too_many(const char* who) { return set_error(std::string(who) + ": too many rows for one call"); }
+
 template <int D, int DT, int FMT>
-static void launch_write_f(WriteArgs& a, int64_t tokens, hipStream_t s) {
+static int launch_write_f(WriteArgs& a, int64_t tokens, hipStream_t s) {
     const int64_t heads = a.Hq + 2 * (int64_t)a.pg.H;
     a.n_tokens = (uint32_t)tokens;
     auto go = [&](auto n, auto pairs) {
         constexpr int N = decltype(n)::value;
-        a.n_units = (uint32_t)(cdiv(tokens, 64 / (D / 8)) * (cdiv(a.Hq, N) + 2 * cdiv(a.pg.H, N)));
+        const int64_t units = cdiv(tokens, 64 / (D / 8)) * (cdiv(a.Hq, N) + 2 * cdiv(a.pg.H, N));
+        if (units > kMaxUnits) return too_many("fkv_paged_write");
+        a.n_units = (uint32_t)units;
         paged_write_kernel<D, DT, FMT, N, decltype(pairs)::value><<<(uint32_t)cdiv(a.n_units, 4), 256, 0, s>>>(a);
+        return check_hip(hipGetLastError(), "fkv_paged_write");
     };
-    if (tokens * heads <= kFewRows) go(std::integral_constant<int, 1>{}, std::true_type{});
-    else if (a.rope.rot && !a.rope.interleaved) go(std::integral_constant<int, 4>{}, std::true_type{});
-    else go(std::integral_constant<int, 4>{}, std::false_type{});
+    if (tokens * heads <= kFewRows) return go(std::integral_constant<int, 1>{}, std::true_type{});
+    if (a.rope.rot && !a.rope.interleaved) return go(std::integral_constant<int, 4>{}, std::true_type{});
+    return go(std::integral_constant<int, 4>{}, std::false_type{});
 }
 
 template <int D, int DT>
-static void launch_write(WriteArgs& a, int format, int64_t tokens, hipStream_t s) {
+static int launch_write(WriteArgs& a, int format, int64_t tokens, hipStream_t s) {
     switch (format) {
-        case FKV_PAGES_F16: launch_write_f<D, DT, FKV_PAGES_F16>(a, tokens, s); break;
-        case FKV_PAGES_BF16: launch_write_f<D, DT, FKV_PAGES_BF16>(a, tokens, s); break;
-        case FKV_PAGES_FP8: launch_write_f<D, DT, FKV_PAGES_FP8>(a, tokens, s); break;
-        default: launch_write_f<D, DT, FKV_PAGES_FP8_INT4>(a, tokens, s); break;
+        case FKV_PAGES_F16: return launch_write_f<D, DT, FKV_PAGES_F16>(a, tokens, s);
+        case FKV_PAGES_BF16: return launch_write_f<D, DT, FKV_PAGES_BF16>(a, tokens, s);
+        case FKV_PAGES_FP8: return launch_write_f<D, DT, FKV_PAGES_FP8>(a, tokens, s);
+        default: return launch_write_f<D, DT, FKV_PAGES_FP8_INT4>(a, tokens, s);
     }
 }
 
@@ -571,19 +580,20 @@ int fkv_rope_apply(const fkv_rope* rope, const fkv_rows* x, const fkv_rows* out,
     hipStream_t s = (hipStream_t)stream;
     auto go = [&](auto dt, auto n, auto pairs) {
         constexpr int DT = decltype(dt)::value, N = decltype(n)::value;
-        const uint32_t units = (uint32_t)((int64_t)B * L * cdiv(H, N * (int64_t)rpw));
+        const int64_t units = (int64_t)B * L * cdiv(H, N * (int64_t)rpw);
+        if (units > kMaxUnits) return too_many(w);
         rope_kernel<DT, N, decltype(pairs)::value><<<(uint32_t)cdiv(units, 4), 256, 0, s>>>(
-            rows_view(x), rows_view(out), rv, pv, units, H, L, lanes, rpw);
+            rows_view(x), rows_view(out), rv, pv, (uint32_t)units, H, L, lanes, rpw);
+        return check_hip(hipGetLastError(), w);
     };
     auto by_rows = [&](auto dt) {
-        if ((int64_t)B * H * L <= kFewRows) go(dt, std::integral_constant<int, 1>{}, std::true_type{});
-        else if (!rope->interleaved) go(dt, std::integral_constant<int, 4>{}, std::true_type{});
-        else go(dt, std::integral_constant<int, 4>{}, std::false_type{});
+        if ((int64_t)B * H * L <= kFewRows) return go(dt, std::integral_constant<int, 1>{}, std::true_type{});
+        if (!rope->interleaved) return go(dt, std::integral_constant<int, 4>{}, std::true_type{});
+        return go(dt, std::integral_constant<int, 4>{}, std::false_type{});
     };
-    if (dtype == FKV_F16) by_rows(std::integral_constant<int, FKV_F16>{});
-    else if (dtype == FKV_BF16) by_rows(std::integral_constant<int, FKV_BF16>{});
-    else by_rows(std::integral_constant<int, FKV_F32>{});
-    return check_hip(hipGetLastError(), w);
+    if (dtype == FKV_F16) return by_rows(std::integral_constant<int, FKV_F16>{});
+    if (dtype == FKV_BF16) return by_rows(std::integral_constant<int, FKV_BF16>{});
+    return by_rows(std::integral_constant<int, FKV_F32>{});
 }
 
 int fkv_paged_write(const fkv_pages* pages, const fkv_rows* k, const fkv_rows* v, int32_t dtype, int32_t B,
@@ -626,15 +636,13 @@ int fkv_paged_write(const fkv_pages* pages, const fkv_rows* k, const fkv_rows* v
     const int64_t tokens = (int64_t)B * L;
     hipStream_t s = (hipStream_t)stream;
     if (pages->D == 64) {
-        if (dtype == FKV_F16) launch_write<64, FKV_F16>(a, pages->format, tokens, s);
-        else if (dtype == FKV_BF16) launch_write<64, FKV_BF16>(a, pages->format, tokens, s);
-        else launch_write<64, FKV_F32>(a, pages->format, tokens, s);
-    } else {
-        if (dtype == FKV_F16) launch_write<128, FKV_F16>(a, pages->format, tokens, s);
-        else if (dtype == FKV_BF16) launch_write<128, FKV_BF16>(a, pages->format, tokens, s);
-        else launch_write<128, FKV_F32>(a, pages->format, tokens, s);
+        if (dtype == FKV_F16) return launch_write<64, FKV_F16>(a, pages->format, tokens, s);
+        if (dtype == FKV_BF16) return launch_write<64, FKV_BF16>(a, pages->format, tokens, s);
+        return launch_write<64, FKV_F32>(a, pages->format, tokens, s);
     }
-    return check_hip(hipGetLastError(), w);
+    if (dtype == FKV_F16) return launch_write<128, FKV_F16>(a, pages->format, tokens, s);
+    if (dtype == FKV_BF16) return launch_write<128, FKV_BF16>(a, pages->format, tokens, s);
+    return launch_write<128, FKV_F32>(a, pages->format, tokens, s);
 }
 
 int fkv_paged_read(const fkv_pages* pages, const int32_t* table, int32_t n_table, int64_t table_stride,
@@ -656,7 +664,9 @@ int fkv_paged_read(const fkv_pages* pages, const int32_t* table, int32_t n_table
     a.lens = lens;
     a.k = (char*)out_k;
     a.v = (char*)out_v;
-    a.n_units = (uint32_t)(B * pages->H * cdiv(S, 16));
+    const int64_t units = (int64_t)B * pages->H * cdiv(S, 16);
+    if (units > kMaxUnits) return too_many(w);
+    a.n_units = (uint32_t)units;
     a.S = S;
     const uint32_t blocks = (uint32_t)cdiv(a.n_units, 4);
     hipStream_t s = (hipStream_t)stream;

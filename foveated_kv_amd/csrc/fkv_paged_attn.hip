@@ -45,7 +45,7 @@ typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxSeqs = 4096;
-constexpr float kNegBig = -1e30f;  // running maximum before the first token
+constexpr float kNegBig = -3.402823466e38f;  // running maximum before the first token: no score lies below it
 // The running maximum follows a new one only when that exceeds it by more
 // than 2^8: weights then reach 2^8 at most, which fp32 sums and 16-bit
 // weights hold alike, and most steps need no rescaling and no reduction
@@ -599,7 +599,9 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(AttnArgs a) {
             if (work) {
                 if (++hrow == rows_per_seq) {
                     hrow = 0;
-                    do len = length_of(a, ++b); while (len == 0);  // (units are left, so a sequence follows)
+                    // (units are left, so a sequence with tokens follows)
+                    do len = ++b < a.B ? length_of(a, b) : 1; while (len == 0);
+                    if (b >= a.B) break;  // (lens changed under the call)
                     nt = tiles_of<NW>(len);
                     ids = a.table.ids + b * a.table.stride;
                 }
@@ -801,7 +803,7 @@ int fkv_paged_attn(const fkv_pages* pages, const fkv_rows* query, int32_t q_dtyp
     const char* w = "fkv_paged_attn";
     if (int e = check_attn(w, pages, Hq, B, max_len)) return e;
     if (int e = check_table(w, table, n_table, table_stride, B)) return e;
-    if ((int64_t)n_table * pages->page_size > 0x7FFFFFFF) return set_error(std::string(w) + ": more than 2^31 tokens a sequence");
+    if ((int64_t)n_table * pages->page_size > 0x7FFFFFFF - 4096) return set_error(std::string(w) + ": more than 2^31 tokens a sequence");
     if (q_dtype != FKV_F16 && q_dtype != FKV_BF16) return set_error(std::string(w) + ": queries must be fp16 or bf16");
     if (pages->format <= FKV_PAGES_BF16 && (q_dtype == FKV_BF16) != (pages->format == FKV_PAGES_BF16))
         return set_error(std::string(w) + ": queries must have the 16-bit pages' type");
@@ -811,6 +813,7 @@ int fkv_paged_attn(const fkv_pages* pages, const fkv_rows* query, int32_t q_dtyp
     if (((uintptr_t)query->data | (uintptr_t)out | (uintptr_t)workspace) & 15 || (query->stride_b | query->stride_h) & 7)
         return set_error(std::string(w) + ": query, out and workspace must be 16-byte aligned, query strides multiples of 8");
     const AttnPlan p = plan_of(pages, Hq, B, max_len);
+    if (p.rows >= 1 << 24) return set_error(std::string(w) + ": more than 2^24 rows of heads");
     if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
         return set_error(std::string(w) + ": workspace of " + std::to_string(p.bytes) + " bytes needed");
     if (p.rows * (cdiv((int64_t)n_table * pages->page_size, 32 * kAttnWaves) + 1) > 0x7FFFFFFF)

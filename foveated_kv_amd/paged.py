@@ -53,22 +53,20 @@ def _no_grad(name, t):
                            "(call it under torch.no_grad())")
 
 
-class _Device:
-    """The GPU's current stream, with that GPU current inside (entering costs
-    nothing where it is already)."""
+_raw_stream, _current_gpu = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
-    def __init__(self, index):
-        self.index, self.guard = index, None
 
-    def __enter__(self):
-        if torch.cuda.current_device() != self.index:
-            self.guard = torch.cuda.device(self.index)
-            self.guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(index, what, *args):
+    """The entry point ``what`` on GPU ``index``'s current stream, that GPU
+    being current (switched to only where it is not)."""
+    fn = getattr(_lib.load(), what)
+    if _current_gpu() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, what)
 
 
 def _rows(t, shape):
@@ -90,10 +88,12 @@ def _positions(p, B, L, index, per_token_allowed=True):
     each sequence; (B, L) or (1, L): every token's."""
     if not torch.is_tensor(p):
         return _lib.PositionsC(None, 0, 0, int(p), 0, 0)
-    if p.dtype != torch.int32 and p.dtype != torch.int64:
-        raise TypeError(f"positions must be int32 or int64, got {p.dtype}")
+    dtype = p.dtype
+    is64 = dtype == torch.int64
+    if not is64 and dtype != torch.int32:
+        raise TypeError(f"positions must be int32 or int64, got {dtype}")
     _on(index, "positions", p)
-    shape, at, is64 = tuple(p.shape), p.data_ptr(), p.dtype == torch.int64
+    shape, at = p.shape, p.data_ptr()
     if shape == (B,):
         return _lib.PositionsC(at, p.stride(0), 0, 0, is64, 0)
     if shape == () or shape == (1,):
@@ -101,12 +101,12 @@ def _positions(p, B, L, index, per_token_allowed=True):
     if per_token_allowed and shape in ((B, L), (1, L)):
         return _lib.PositionsC(at, p.stride(0) if shape[0] > 1 else 0, p.stride(1), 0, is64, 1)
     raise ValueError(f"positions must be one number, one per sequence ({B},)"
-                     f"{f' or one per token {(B, L)}' if per_token_allowed else ''}, got {shape}")
+                     f"{f' or one per token {(B, L)}' if per_token_allowed else ''}, got {tuple(shape)}")
 
 
 def _lens(name, t, B, index):
     _on(index, name, t)
-    if t.dtype != torch.int32 or tuple(t.shape) != (B,):
+    if t.dtype != torch.int32 or t.shape != (B,):
         raise TypeError(f"{name} must be an int32 tensor of shape ({B},)")
     return t if B <= 1 or t.stride(0) == 1 else t.contiguous()
 
@@ -236,11 +236,9 @@ class Rope:
         pos = _positions(positions, B, L, index)
         src, held = _rows(x, shape)
         dst, result = _rows(out, shape)
-        lib = _lib.load()
-        with _Device(index) as stream:
-            check(lib.fkv_rope_apply(self._c, src, dst, code, B, H, L, D, pos, stream), "fkv_rope_apply")
-            if result is not out:
-                out.copy_(result)
+        _call(index, "fkv_rope_apply", self._c, src, dst, code, B, H, L, D, pos)
+        if result is not out:
+            out.copy_(result)
         return out
 
 
@@ -390,12 +388,10 @@ class PagedLayer:
             ro, result = _rows(q_out, qs)
         elif q_out is not None:
             raise ValueError("q_out without q")
-        lib = _lib.load()
-        with _Device(index) as stream:
-            check(lib.fkv_paged_write(self._c, rk, rv, code, B, L, table.data_ptr(), P, stride, pos, ptr(n_new),
-                                      rope_c, rq, ro, Hq, stream), "fkv_paged_write")
-            if result is not q_out:
-                q_out.copy_(result)
+        _call(index, "fkv_paged_write", self._c, rk, rv, code, B, L, table.data_ptr(), P, stride, pos,
+              None if n_new is None else n_new.data_ptr(), rope_c, rq, ro, Hq)
+        if result is not q_out:
+            q_out.copy_(result)
         return q_out
 
     def read(self, table, lens, max_len=None, dtype=None):
@@ -406,16 +402,14 @@ class PagedLayer:
         table, B, P, stride = self._table(table)
         lens = _lens("lens", lens, B, self._index)
         S = P * self.page_size if max_len is None else int(max_len)
-        if S < 0:
-            raise ValueError("max_len must not be negative")
+        if not 0 <= S < 2 ** 31:
+            raise ValueError(f"max_len must be in [0, 2^31), got {S}")
         dtype = _NEW.get(self.fmt, torch.float16) if dtype is None else dtype
         code = dtype_code(dtype)
         k = torch.empty((B, self.n_kv_heads, S, self.head_dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        lib = _lib.load()
-        with _Device(self._index) as stream:
-            check(lib.fkv_paged_read(self._c, table.data_ptr(), P, stride, lens.data_ptr(), B, S, k.data_ptr(),
-                                     v.data_ptr(), code, stream), "fkv_paged_read")
+        _call(self._index, "fkv_paged_read", self._c, table.data_ptr(), P, stride, lens.data_ptr(), B, S, k.data_ptr(),
+              v.data_ptr(), code)
         return k, v
 
     def attend(self, query, table, lens, max_len=None, lens_add=0, scale=None, out=None, return_lse=False):
@@ -443,24 +437,24 @@ class PagedLayer:
         most = P * self.page_size
         if max_len is not None and max_len < most:
             most = int(max_len)
+        if not -2 ** 31 <= lens_add < 2 ** 31:
+            raise ValueError(f"lens_add must fit 32 bits, got {lens_add}")
         rows, held = _rows(query, shape)
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=self.device)
+            out = torch.empty_like(query, memory_format=torch.contiguous_format)
         else:
             _on(index, "out", out)
             _no_grad("out", out)
             if tuple(out.shape) != shape or out.dtype != dtype or not out.is_contiguous() or out.data_ptr() % 16:
                 raise ValueError(f"out must be a contiguous, 16-byte aligned {shape} {dtype} tensor")
         lse = torch.empty((B, Hq), dtype=torch.float32, device=self.device) if return_lse else None
-        lib = _lib.load()
-        n = lib.fkv_paged_attn_workspace(self._c, Hq, B, most)
+        n = _lib.load().fkv_paged_attn_workspace(self._c, Hq, B, most)
         if n < 0:
             check(n, "fkv_paged_attn_workspace")
-        with _Device(index) as stream:
-            ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
-            check(lib.fkv_paged_attn(self._c, rows, dtype_code(dtype), Hq, B, table.data_ptr(), P, stride,
-                                     lens.data_ptr(), lens_add, most, D ** -0.5 if scale is None else scale,
-                                     out.data_ptr(), ptr(lse), ptr(ws), n, stream), "fkv_paged_attn")
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        _call(index, "fkv_paged_attn", self._c, rows, dtype_code(dtype), Hq, B, table.data_ptr(), P, stride,
+              lens.data_ptr(), lens_add, most, D ** -0.5 if scale is None else scale, out.data_ptr(), ptr(lse), ptr(ws),
+              n)
         return (out, lse) if return_lse else out
 
 

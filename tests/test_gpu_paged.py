@@ -377,6 +377,31 @@ def test_attend_nan_of_one_sequence_stays_there(paged):
     assert not bool(torch.isnan(layer.attend(q, table.cuda(), lens)).any())
 
 
+def test_attend_scores_at_the_edge_of_fp32(paged):
+    """Scores near -3e38 and far apart: a softmax like any other (a maximum
+    that starts above them would leave no weight)."""
+    H, D, page = 1, 64, 16
+    layer = paged.PagedLayer(40, H, D, page, "bf16")
+    layer.k.fill_(0.0)
+    layer.k[..., 0] = -1.0e18
+    layer.k[1, 0, 3, 0] = -0.5e18
+    layer.v.copy_(_randn(65, 40, H, page, D))
+    table = torch.arange(40, dtype=torch.int32).view(1, 40)
+    q = torch.zeros(1, 2, 1, D, dtype=torch.bfloat16, device="cuda")
+    q[0, :, 0, 0] = 1.0e18
+    for n in (10, 640):  # whole, split
+        lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+        out, lse = layer.attend(q, table.cuda(), lens, scale=128.0, return_lse=True)
+        v = layer.v.float().cpu().transpose(1, 2).reshape(-1, D)[:n]
+        want = v.double().mean(0) if n < 20 else layer.v[1, 0, 3].double().cpu()
+        err = (out[0, :, 0].double().cpu() - want).abs()
+        # equal weights or a single one: exact but for fp32 sums and the result's rounding
+        assert bool((err <= 2.0 ** -8 * want.abs() + 2.0 ** -20 * v.abs().max()).all())
+        # -128 * 1e18 * 1e18 (the bf16 numbers) or half of it
+        s = 128.0 * float(q[0, 0, 0, 0]) * float(layer.k[0, 0, 0, 0] if n < 20 else layer.k[1, 0, 3, 0])
+        assert bool(((lse.cpu().double() - s).abs() <= 2.0 ** -20 * abs(s)).all())
+
+
 def test_attend_many_sequences(paged):
     """More sequences than a workgroup has threads, most of them empty."""
     B, page, H, D = 700, 16, 2, 64

@@ -178,8 +178,8 @@ R = ctypes.byref
     ("rot_dim", {"rope": {"rot_dim": 80}}), ("rot_dim", {"rope": {"rot_dim": 0}}), ("table", {"rope": {"table": None}}),
     ("no positions", {"rope": {"n_positions": 0}}), ("NULL positions", {"pos": None}),
     ("misaligned", {"pos": {"data": 0x1002}}), ("misaligned", {"pos": {"data": 0x1004, "is64": 1}}),
-    ("2^31", {"B": 65536, "L": 65536}), ("NULL rows", {"x": None}), ("NULL rows", {"out": {"data": None}}),
-    ("aligned", {"x": {"data": 0x1008}}), ("multiples", {"out": {"stride_l": 60}})])
+    ("2^31", {"B": 65536, "L": 65536}), ("too many", {"H": 1, "L": 1 << 27}), ("NULL rows", {"x": None}),
+    ("NULL rows", {"out": {"data": None}}), ("aligned", {"x": {"data": 0x1008}}), ("multiples", {"out": {"stride_l": 60}})])
 def test_rope_apply_refusals(c, word, kw):
     a = dict(rope={}, x={}, out={}, pos={}, dtype=0, B=1, H=2, L=3, D=64, **{})
     a.update(kw)
@@ -214,7 +214,7 @@ def test_page_refusals(c, word, kw):
     ("one position", {"pos": {"per_token": 1}}), ("together", {"q": {}}), ("together", {"q_out": {}}),
     ("query head", {"q": {}, "q_out": {}, "Hq": 0}), ("rot_dim", {"rope": {"rot_dim": 72}}), ("NULL rows", {"k": None}),
     ("aligned", {"v": {"data": 0x1001}}), ("multiples", {"k": {"stride_h": 63}}), ("2^31", {"B": 40000, "L": 40000}),
-    ("aligned", {"q": {"data": 0x1008}, "q_out": {}, "Hq": 2})])
+    ("too many", {"B": 1 << 14, "L": 18000}), ("aligned", {"q": {"data": 0x1008}, "q_out": {}, "Hq": 2})])
 def test_write_refusals(c, word, kw):
     a = dict(k={}, v={}, q=None, q_out=None, pos={}, rope=None, dtype=0, B=1, L=1, table=c.at, n_table=1, stride=1, Hq=0)
     a.update(kw)
@@ -227,7 +227,8 @@ def test_write_refusals(c, word, kw):
 
 @pytest.mark.parametrize("word,kw", [
     ("dtype", {"dtype": -1}), ("negative", {"S": -1}), ("table shape", {"stride": 0, "B": 2}), ("NULL table", {"table": None}),
-    ("lens", {"lens": None}), ("aligned", {"k": None}), ("aligned", {"v": 0x1008}), ("2^31", {"S": 2 ** 31 - 1})])
+    ("lens", {"lens": None}), ("aligned", {"k": None}), ("aligned", {"v": 0x1008}), ("2^31", {"S": 2 ** 31 - 1}),
+    ("too many", {"B": 300_000_000, "stride": 1, "S": 2})])
 def test_read_refusals(c, word, kw):
     a = dict(table=c.at, n_table=1, stride=1, lens=c.at, B=1, S=1, k=c.at, v=c.at, dtype=0)
     a.update(kw)
@@ -238,7 +239,8 @@ def test_read_refusals(c, word, kw):
 
 @pytest.mark.parametrize("word,kw", [
     ("sequences", {"B": 4097}), ("sequences", {"B": -1}), ("multiple", {"Hq": 3}), ("multiple", {"Hq": 0}),
-    ("max_len", {"max_len": -1}), ("table shape", {"n_table": -1}), ("2^31 tokens", {"n_table": 2 ** 27}),
+    ("max_len", {"max_len": -1}), ("table shape", {"n_table": -1}), ("2^31 tokens", {"n_table": 2 ** 27}), ("2^24 rows", {"B": 4096, "Hq": 2 ** 18, "max_len": 100}),
+    ("2^31 tiles", {"B": 4096, "Hq": 2 ** 14, "n_table": 2 ** 20, "max_len": 100}),
     ("fp16 or bf16", {"q_dtype": 2}), ("16-bit pages' type", {"format": 0, "q_dtype": 1}),
     ("16-bit pages' type", {"format": 1, "q_dtype": 0}), ("finite", {"scale": math.nan}), ("finite", {"scale": math.inf}),
     ("NULL", {"q": None}), ("NULL", {"out": None}), ("NULL", {"lens": None}), ("aligned", {"q": {"data": 0x1008}}),
