@@ -96,7 +96,8 @@ class RopeC(ctypes.Structure):
 
 
 # name -> (restype, argtypes); every symbol include/fkv.h declares
-_PAGES, _ROWS, _POS, _ROPE = (ctypes.POINTER(t) for t in (PagesC, RowsC, PositionsC, RopeC))
+# (structs of the paged entry points: a byref, or the packed bytes of one)
+_PAGES = _ROWS = _POS = _ROPE = P
 SIGNATURES = {
     "fkv_is_available": (ctypes.c_int, []),
     "fkv_last_error": (ctypes.c_char_p, []),

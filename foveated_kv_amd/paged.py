@@ -22,7 +22,9 @@ any.  A page, once written by one stream and read by another, is ordered by
 the caller, as any tensor is.
 """
 
+import ctypes
 import math
+import struct
 
 import torch
 
@@ -32,6 +34,10 @@ from .ext import _require_device
 
 FORMATS = {"fp16": 0, "bf16": 1, "fp8": 2, "fp8_int4": 3}
 _NEW = {"fp16": torch.float16, "bf16": torch.bfloat16}
+# fkv_rows and fkv_positions (include/fkv.h) as bytes: half the time of a
+# ctypes.Structure, of which a write call needs five
+_pack_rows = struct.Struct("Pqqq").pack
+_pack_positions = struct.Struct("Pqqqii").pack
 
 
 # ---------------------------------------------------------------------------
@@ -39,15 +45,12 @@ _NEW = {"fp16": torch.float16, "bf16": torch.bfloat16}
 # ---------------------------------------------------------------------------
 
 def _on(index, name, t):
-    """Refuses what is not a tensor on GPU ``index``."""
-    if not torch.is_tensor(t):
+    """Refuses what is not a tensor on GPU ``index``, or wants a gradient."""
+    if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.get_device() != index:
         _require_device(t)
         raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
-
-
-def _no_grad(name, t):
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires grad: this package is for inference and records nothing for autograd "
                            "(call it under torch.no_grad())")
@@ -80,14 +83,14 @@ def _rows(t, shape):
         if sd != 1 or at & 15 or (sb | sh | sl) & 7:
             t = t.clone(memory_format=torch.contiguous_format)
             at, (sb, sh, sl, _) = t.data_ptr(), t.stride()
-    return _lib.RowsC(at, sb, sh, sl), t
+    return _pack_rows(at, sb, sh, sl), t
 
 
 def _positions(p, B, L, index, per_token_allowed=True):
     """int | one-element tensor | (B,) tensor: the first token's position of
     each sequence; (B, L) or (1, L): every token's."""
-    if not torch.is_tensor(p):
-        return _lib.PositionsC(None, 0, 0, int(p), 0, 0)
+    if not isinstance(p, torch.Tensor):
+        return _pack_positions(0, 0, 0, int(p), 0, 0)
     dtype = p.dtype
     is64 = dtype == torch.int64
     if not is64 and dtype != torch.int32:
@@ -95,11 +98,11 @@ def _positions(p, B, L, index, per_token_allowed=True):
     _on(index, "positions", p)
     shape, at = p.shape, p.data_ptr()
     if shape == (B,):
-        return _lib.PositionsC(at, p.stride(0), 0, 0, is64, 0)
+        return _pack_positions(at, p.stride(0), 0, 0, is64, 0)
     if shape == () or shape == (1,):
-        return _lib.PositionsC(at, 0, 0, 0, is64, 0)
+        return _pack_positions(at, 0, 0, 0, is64, 0)
     if per_token_allowed and shape in ((B, L), (1, L)):
-        return _lib.PositionsC(at, p.stride(0) if shape[0] > 1 else 0, p.stride(1), 0, is64, 1)
+        return _pack_positions(at, p.stride(0) if shape[0] > 1 else 0, p.stride(1), 0, is64, 1)
     raise ValueError(f"positions must be one number, one per sequence ({B},)"
                      f"{f' or one per token {(B, L)}' if per_token_allowed else ''}, got {tuple(shape)}")
 
@@ -207,7 +210,9 @@ class Rope:
             a = torch.arange(p, min(p + 65536, self.max_positions), dtype=torch.float64, device=device)[:, None] * inv
             self.table[p:p + 65536, 0] = a.cos() * factor
             self.table[p:p + 65536, 1] = a.sin() * factor
-        self._c = _lib.RopeC(self.table.data_ptr(), self.max_positions, self.rot_dim, int(self.interleaved))
+        self._c = ctypes.byref(_lib.RopeC(self.table.data_ptr(), self.max_positions, self.rot_dim,
+                                          int(self.interleaved)))
+        self._index = self.table.get_device()
 
     def __call__(self, x, positions=0, out=None):
         """x (B, H, L, head_dim) fp16 / bf16 / fp32, any strides -> the rotated
@@ -216,21 +221,19 @@ class Rope:
         position), a (B,) tensor (each sequence's first token's) or (B, L) /
         (1, L) (every token's); int32 or int64 tensors on the device, read
         there, so a captured call follows them."""
-        index = self.table.get_device()
+        index = self._index
         if index < 0:
             _require_device(self.table)
         _on(index, "x", x)
-        shape = tuple(x.shape)
+        shape, dtype = x.shape, x.dtype
         if len(shape) != 4 or shape[3] != self.head_dim:
-            raise ValueError(f"x must be (B, H, L, {self.head_dim}), got {shape}")
-        _no_grad("x", x)
-        code = dtype_code(x.dtype)
+            raise ValueError(f"x must be (B, H, L, {self.head_dim}), got {tuple(shape)}")
+        code = dtype_code(dtype)
         if out is None:
             out = torch.empty_like(x)
         else:
             _on(index, "out", out)
-            _no_grad("out", out)
-            if tuple(out.shape) != shape or out.dtype != x.dtype:
+            if out.shape != shape or out.dtype != dtype:
                 raise ValueError("out must have x's shape and dtype")
         B, H, L, D = shape
         pos = _positions(positions, B, L, index)
@@ -311,7 +314,8 @@ class PagedLayer:
         self.fmt, self.k, self.v, self.k_exp, self.v_scale = fmt, k, v, k_exp, v_scale
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, H, page, D
         self.device, self._index = k.device, k.get_device()
-        self._c = _lib.PagesC(k.data_ptr(), v.data_ptr(), ptr(k_exp), ptr(v_scale), n, page, H, D, FORMATS[fmt])
+        self._c = ctypes.byref(_lib.PagesC(k.data_ptr(), v.data_ptr(), ptr(k_exp), ptr(v_scale), n, page, H, D,
+                                           FORMATS[fmt]))
         check(min(int(_lib.load().fkv_paged_attn_workspace(self._c, H, 1, 0)), 0), "PagedLayer")
 
     def _table(self, table, B=None):
@@ -345,18 +349,17 @@ class PagedLayer:
         its queries come back as ``q_out`` held them (zero in a new tensor).
         Positions outside the table are not stored either.  No two tokens of
         a call may name the same slot."""
-        index, shape = self._index, tuple(k.shape)
+        index = self._index
         _on(index, "k", k)
         _on(index, "v", v)
-        if len(shape) != 4 or shape[1] != self.n_kv_heads or shape[3] != self.head_dim or tuple(v.shape) != shape or \
-                v.dtype != k.dtype:
+        shape, dtype = k.shape, k.dtype
+        if len(shape) != 4 or shape[1] != self.n_kv_heads or shape[3] != self.head_dim or v.shape != shape or \
+                v.dtype != dtype:
             raise ValueError(f"k and v must be (B, {self.n_kv_heads}, L, {self.head_dim}) of one dtype, got "
-                             f"{shape} {k.dtype} / {tuple(v.shape)} {v.dtype}")
+                             f"{tuple(shape)} {dtype} / {tuple(v.shape)} {v.dtype}")
         B, H, L, D = shape
-        code = dtype_code(k.dtype)
+        code = dtype_code(dtype)
         table, _, P, stride = self._table(table, B)
-        _no_grad("k", k)
-        _no_grad("v", v)
         rope_c = None
         if rope is not None:
             if rope.head_dim != D:
@@ -372,16 +375,14 @@ class PagedLayer:
         Hq = 0
         if q is not None:
             _on(index, "q", q)
-            _no_grad("q", q)
-            qs = tuple(q.shape)
-            if len(qs) != 4 or (qs[0], qs[2], qs[3]) != (B, L, D) or q.dtype != k.dtype:
-                raise ValueError(f"q must be ({B}, Hq, {L}, {D}) {k.dtype}, got {qs} {q.dtype}")
+            qs = q.shape
+            if len(qs) != 4 or qs[0] != B or qs[2] != L or qs[3] != D or q.dtype != dtype:
+                raise ValueError(f"q must be ({B}, Hq, {L}, {D}) {dtype}, got {tuple(qs)} {q.dtype}")
             if q_out is None:
                 q_out = torch.empty_like(q) if n_new is None else torch.zeros_like(q)
             else:
                 _on(index, "q_out", q_out)
-                _no_grad("q_out", q_out)
-                if tuple(q_out.shape) != qs or q_out.dtype != q.dtype:
+                if q_out.shape != qs or q_out.dtype != dtype:
                     raise ValueError("q_out must have q's shape and dtype")
             Hq = qs[1]
             rq, q_held = _rows(q, qs)
@@ -423,14 +424,14 @@ class PagedLayer:
         ``max_len`` is an upper bound of the lengths if the host knows one
         (default: the table's width); it decides how the work is split, not
         what is attended to.  ``scale`` defaults to D^-1/2."""
-        index, D, shape, dtype = self._index, self.head_dim, tuple(query.shape), query.dtype
+        index, D = self._index, self.head_dim
         _on(index, "query", query)
+        shape, dtype = query.shape, query.dtype
         if len(shape) != 4 or shape[2] != 1 or shape[3] != D or shape[1] % self.n_kv_heads or shape[1] == 0:
-            raise ValueError(f"query must be (B, a multiple of {self.n_kv_heads}, 1, {D}), got {shape}")
+            raise ValueError(f"query must be (B, a multiple of {self.n_kv_heads}, 1, {D}), got {tuple(shape)}")
         if dtype not in (torch.float16, torch.bfloat16) or dtype != _NEW.get(self.fmt, dtype):
             raise TypeError(f"{self.fmt} pages take {'fp16 or bf16' if self.fmt not in _NEW else self.fmt} queries, "
                             f"got {dtype}")
-        _no_grad("query", query)
         B, Hq = shape[:2]
         table, _, P, stride = self._table(table, B)
         lens = _lens("lens", lens, B, index)
@@ -444,17 +445,16 @@ class PagedLayer:
             out = torch.empty_like(query, memory_format=torch.contiguous_format)
         else:
             _on(index, "out", out)
-            _no_grad("out", out)
-            if tuple(out.shape) != shape or out.dtype != dtype or not out.is_contiguous() or out.data_ptr() % 16:
-                raise ValueError(f"out must be a contiguous, 16-byte aligned {shape} {dtype} tensor")
+            if out.shape != shape or out.dtype != dtype or not out.is_contiguous() or out.data_ptr() % 16:
+                raise ValueError(f"out must be a contiguous, 16-byte aligned {tuple(shape)} {dtype} tensor")
         lse = torch.empty((B, Hq), dtype=torch.float32, device=self.device) if return_lse else None
         n = _lib.load().fkv_paged_attn_workspace(self._c, Hq, B, most)
         if n < 0:
             check(n, "fkv_paged_attn_workspace")
         ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
         _call(index, "fkv_paged_attn", self._c, rows, dtype_code(dtype), Hq, B, table.data_ptr(), P, stride,
-              lens.data_ptr(), lens_add, most, D ** -0.5 if scale is None else scale, out.data_ptr(), ptr(lse), ptr(ws),
-              n)
+              lens.data_ptr(), lens_add, most, D ** -0.5 if scale is None else scale, out.data_ptr(), ptr(lse),
+              None if ws is None else ws.data_ptr(), n)
         return (out, lse) if return_lse else out
 
 
