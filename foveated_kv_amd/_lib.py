@@ -163,6 +163,7 @@ SIGNATURES = {
     "fkv_promoter_get_stats": (ctypes.c_int, [P, P]),
     "fkv_promoter_near_valid": (ctypes.c_int, [P, I32, P, I32]),
     "fkv_promoter_destroy": (None, [P]),
+    "fkv_rope_table": (ctypes.c_int, [P, I32, ctypes.c_double, I32, P, P]),
     "fkv_rope_apply": (ctypes.c_int, [_ROPE, _ROWS, _ROWS, I32, I32, I32, I32, I32, _POS, P]),
     "fkv_paged_write": (ctypes.c_int, [_PAGES, _ROWS, _ROWS, I32, I32, I32, P, I32, I64, _POS, P, _ROPE, _ROWS,
                                        _ROWS, I32, P]),

@@ -154,6 +154,23 @@ __device__ inline void rotate8(float (&x)[8], const RopeView& r, const Angles& t
     for (int j = 0; j < 8; j++) x[j] = inter ? y[j] : y[2 * (j & 3) + (j >> 2)];
 }
 
+// The table: one angle a thread.  Frequencies come with the launch, so that
+// there is no copy to wait for.
+struct Frequencies {
+    double f[256];
+};
+__global__ void __launch_bounds__(256) rope_table_kernel(Frequencies freq, uint32_t pairs, double factor, int64_t n,
+                                                         float* table) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t pos = i / pairs;
+        const uint32_t pair = (uint32_t)(i - pos * pairs);
+        double s, c;
+        sincos((double)pos * freq.f[pair], &s, &c);
+        table[pos * 2 * pairs + pair] = (float)(c * factor);
+        table[(pos * 2 + 1) * pairs + pair] = (float)(s * factor);
+    }
+}
+
 // One row of D elements on D / 8 lanes of one wave (each lane writes the
 // elements that it read: out may be x), the wave's rows and then N times as
 // many being consecutive heads of one token, which share the lane's angles.
@@ -559,6 +576,21 @@ static void launch_read(const ReadArgs& a, int dtype, uint32_t blocks, hipStream
 using namespace fkv;
 
 extern "C" {
+
+int fkv_rope_table(const double* frequencies, int32_t rot_dim, double factor, int32_t n_positions, float* table,
+                   void* stream) {
+    const std::string w = "fkv_rope_table";
+    if (!frequencies || !table || misaligned(table)) return set_error(w + ": NULL argument or misaligned table");
+    if (rot_dim < 16 || rot_dim > 512 || rot_dim % 16)
+        return set_error(w + ": rot_dim must be a multiple of 16 from 16 to 512, got " + std::to_string(rot_dim));
+    if (n_positions < 1) return set_error(w + ": the rotary table has no positions");
+    Frequencies f = {};
+    for (int i = 0; i < rot_dim / 2; i++) f.f[i] = frequencies[i];
+    const int64_t n = (int64_t)n_positions * (rot_dim / 2);
+    rope_table_kernel<<<(uint32_t)std::min<int64_t>(cdiv(n, 256), 65536), 256, 0, (hipStream_t)stream>>>(
+        f, rot_dim / 2, factor, n, table);
+    return check_hip(hipGetLastError(), w.c_str());
+}
 
 int fkv_rope_apply(const fkv_rope* rope, const fkv_rows* x, const fkv_rows* out, int32_t dtype, int32_t B,
                    int32_t H, int32_t L, int32_t D, const fkv_positions* positions, void* stream) {

@@ -204,12 +204,13 @@ class Rope:
         self.base, self.scaling, self.max_positions = float(base), scaling, int(max_positions)
         inv, factor = _frequencies(self.rot_dim, self.base, scaling)
         device = _index_of(device)
-        inv = inv.to(device)
         self.table = torch.empty((self.max_positions, 2, self.rot_dim // 2), dtype=torch.float32, device=device)
-        for p in range(0, self.max_positions, 65536):  # (64-bit angles of 64K positions at a time)
-            a = torch.arange(p, min(p + 65536, self.max_positions), dtype=torch.float64, device=device)[:, None] * inv
-            self.table[p:p + 65536, 0] = a.cos() * factor
-            self.table[p:p + 65536, 1] = a.sin() * factor
+        if device.type == "cuda":
+            _call(device.index, "fkv_rope_table", inv.data_ptr(), self.rot_dim, factor, self.max_positions,
+                  self.table.data_ptr())
+        else:  # (to look at: calls take tables on a GPU)
+            a = torch.arange(self.max_positions, dtype=torch.float64)[:, None] * inv
+            self.table[:, 0], self.table[:, 1] = a.cos() * factor, a.sin() * factor
         self._c = ctypes.byref(_lib.RopeC(self.table.data_ptr(), self.max_positions, self.rot_dim,
                                           int(self.interleaved)))
         self._index = self.table.get_device()

@@ -629,6 +629,13 @@ typedef struct fkv_rope {
     int32_t n_positions, rot_dim, interleaved;
 } fkv_rope;
 
+/* Fills such a table: angle p * frequencies[i] in 64 bits for position p and
+ * pair i < rot_dim / 2 (at most 256 pairs), cos and sin times factor rounded
+ * once to fp32.  frequencies is host memory, read during the call.
+ * Asynchronous, capturable. */
+int fkv_rope_table(const double* frequencies, int32_t rot_dim, double factor, int32_t n_positions, float* table,
+                   void* stream);
+
 /* out = rotated x, rows (B, H, L) of D elements (D a multiple of 8, at most
  * 1024) of dtype; out may be x.  Asynchronous, capturable. */
 int fkv_rope_apply(const fkv_rope* rope, const fkv_rows* x, const fkv_rows* out, int32_t dtype, int32_t B,

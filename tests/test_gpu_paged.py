@@ -95,6 +95,20 @@ def test_rotary(paged, dtype, D, rot, interleaved):
     _bits_equal(rope(x, 9, out=o), a, "unaligned result")
 
 
+@pytest.mark.parametrize("D,rot,scaling", [(128, 128, None), (64, 16, {"kind": "linear", "factor": 3.0}),
+                                           (512, 512, {"kind": "yarn", "factor": 16.0, "original_positions": 4096})])
+def test_rotary_table(paged, D, rot, scaling):
+    """The device's table against the host's, far positions among it."""
+    n = 70001
+    rope = paged.Rope(D, rot_dim=rot, scaling=scaling, max_positions=n)
+    inv, factor = paged._frequencies(rot, 10000.0, scaling)
+    a = np.arange(n, dtype=np.float64)[:, None] * inv.numpy()
+    t = ref.f64(rope.table)
+    for got, want in ((t[:, 0], np.cos(a) * factor), (t[:, 1], np.sin(a) * factor)):
+        # one rounding to fp32, and a sine of 64 bits
+        assert (np.abs(got - want) <= 2.0 ** -24 * np.abs(want) * 1.001 + 2.0 ** -50).all()
+
+
 def test_rotary_outside_the_table_and_empty(paged):
     rope = paged.Rope(64, rot_dim=32, max_positions=10)
     x = _randn(2, 1, 2, 4, 64).half().cuda()

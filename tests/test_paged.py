@@ -190,6 +190,13 @@ def test_rope_apply_refusals(c, word, kw):
     _refused(rc, c.lib, word)
 
 
+@pytest.mark.parametrize("word,kw", [("NULL", {"f": None}), ("NULL", {"table": None}), ("misaligned", {"table": 0x1004}),
+                                     ("rot_dim", {"rot": 24}), ("rot_dim", {"rot": 528}), ("no positions", {"n": 0})])
+def test_rope_table_refusals(c, word, kw):
+    a = {"f": c.at, "rot": 32, "n": 4, "table": c.at, **kw}
+    _refused(c.lib.fkv_rope_table(a["f"], a["rot"], 1.0, a["n"], a["table"], None), c.lib, word)
+
+
 BAD_PAGES = [("head dim", {"D": 96}), ("format", {"format": 4}), ("format", {"format": -1}), ("power of two", {"page_size": 8}),
              ("power of two", {"page_size": 48}), ("power of two", {"page_size": 2048}), ("count", {"n_pages": 0}),
              ("count", {"H": 0}), ("count", {"H": 1025}), ("NULL", {"k": None}), ("NULL", {"v": None}),
