@@ -449,7 +449,10 @@ def generate_paged(model, tokenizer, prompts, cache, max_tokens: int = 100, temp
                         out[b].append(t)
                 if all(done):
                     break
-                cache.extend(1, batch)
+                # (a finished sequence takes no more pages where the batch need not
+                # keep one length)
+                more = [0 if d else 1 for d in done] if cache.rope is not None and any(done) else 1
+                cache.extend(more, batch)
                 logits = model(tok.reshape(B, 1), cache=wrappers)[:, -1, :]
                 steps += 1
             torch.cuda.synchronize(dev)

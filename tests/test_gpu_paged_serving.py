@@ -173,6 +173,27 @@ def test_generate_paged_rotated_by_the_cache(fkv, fmt, monkeypatch):
     generate.uninstall_paged_attention()
 
 
+def test_generate_paged_stops_at_eos(fkv, monkeypatch):
+    """A sequence that ends stops growing while the others go on; the last one
+    to end ends the run."""
+    from foveated_kv_amd import generate
+
+    model, tok = _model(fkv), _tiny_lm.ByteTokenizer()
+    want = [_standard(model, tok.encode(p), 14) for p in PROMPTS]
+    monkeypatch.setattr(_tiny_lm, "_rope", lambda x, offset, base=10000.0: x)
+    tok.eos_token_id = want[1][4]
+    cut = [w[:w.index(tok.eos_token_id)] if tok.eos_token_id in w else w for w in want]
+    n = [len(tok.encode(p)) for p in PROMPTS]
+    cache = fkv.PagedKVCache(2, 2, 64, n_pages=40, max_seqs=4, max_tokens=256, page_size=16,
+                             rope=fkv.Rope(64, max_positions=512))
+    texts, stats = generate.generate_paged(model, tok, PROMPTS, cache, max_tokens=14)
+    assert texts == [tok.decode(c) for c in cut] and len(cut[1]) <= 4
+    assert stats["stored_tokens"] == [a + len(c) for a, c in zip(n, cut)]
+    texts, stats = generate.generate_paged(model, tok, PROMPTS[1], cache, max_tokens=14)
+    assert texts == tok.decode(cut[1]) and stats["model_calls"] == len(cut[1])
+    assert cache.pages.free_pages == 40
+
+
 def test_chunked_prefill_through_the_wrappers(fkv, monkeypatch):
     """A prompt fed in two chunks: the second one's queries attend to what
     the pages hold.  fp32 model, fp16 pages: logits as with whole prefill, up
