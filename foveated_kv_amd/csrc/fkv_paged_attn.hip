@@ -62,7 +62,7 @@ struct AttnArgs {
     float* lse;
     float* records;   // workspace: per workgroup two records
     int4* joins;      // workspace: per row (first workgroup, count, first slot, 0); count 0: nothing to join
-    int32_t lens_add, B, Hq, G, HT, GT;  // HT head tiles of GT heads per KV head
+    int32_t lens_add, B, Hq, G, HT, GT;  // HT passes of GT heads per KV head
     float scale;      // scale * log2(e)
 };
 
@@ -197,37 +197,42 @@ struct Sums {
     float m, l, z;   // maximum of the head, the lane's part of the sum and of INT4's minima
 };
 
-// One step: 32 tokens.  The values' registers are read after the scores, so
-// the caller may have their loads in flight until then.
-template <int D, int FMT, bool BF>
-__device__ inline void scores(const Step<D, FMT>& st, const u4 (&q)[D / 32], const Place& p, float scale, int g,
-                              float (&s)[8]) {
+// Scores of a step's 32 tokens, T tiles of 16 heads.
+template <int D, int FMT, bool BF, int T>
+__device__ inline void scores(const Step<D, FMT>& st, const u4 (&q)[T][D / 32], const Place& p, float scale, int g,
+                              float (&s)[T][8]) {
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-        f4 r = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (FMT <= FKV_PAGES_BF16) {
+        f4 r[T];
 #pragma unroll
-            for (int i = 0; i < D / 32; i++) r = mfma<BF>(st.k[t][i % Step<D, FMT>::KL], q[i], r);
-        } else {
+        for (int n = 0; n < T; n++) r[n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < D / 32; i++) {
+        for (int i = 0; i < D / 32; i++) {
+            u4 k;
+            if (FMT <= FKV_PAGES_BF16) {
+                k = st.k[t][i % Step<D, FMT>::KL];
+            } else {
                 const u4 w = st.k[t][(i / 2) % Step<D, FMT>::KL];
                 const uint32_t w0 = i & 1 ? w.z : w.x, w1 = i & 1 ? w.w : w.y;
-                const u4 k = {cvt_fp8<BF>(w0, false), cvt_fp8<BF>(w0, true), cvt_fp8<BF>(w1, false), cvt_fp8<BF>(w1, true)};
-                r = mfma<BF>(k, q[i], r);
+                k = u4{cvt_fp8<BF>(w0, false), cvt_fp8<BF>(w0, true), cvt_fp8<BF>(w1, false), cvt_fp8<BF>(w1, true)};
             }
+#pragma unroll
+            for (int n = 0; n < T; n++) r[n] = mfma<BF>(k, q[n][i], r[n]);
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float x = r[i] * scale;
-            if (FMT >= FKV_PAGES_FP8) x *= exp_byte((st.kx[t] >> (8 * i)) & 0xFF);
-            s[4 * t + i] = x;
+            float f = scale;
+            if (FMT >= FKV_PAGES_FP8) f = exp_byte((st.kx[t] >> (8 * i)) & 0xFF);
+#pragma unroll
+            for (int n = 0; n < T; n++) s[n][4 * t + i] = (FMT >= FKV_PAGES_FP8 ? r[n][i] * scale : r[n][i]) * f;
         }
     }
     if (p.n[0] < 16 || p.n[1] < 16) {  // (the same in all lanes)
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            if (4 * g + (j & 3) >= p.n[j >> 2]) s[j] = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < T; n++)
+                if (4 * g + (j & 3) >= p.n[j >> 2]) s[n][j] = -INFINITY;
     }
 }
 
@@ -249,10 +254,13 @@ __device__ inline void mask_values(Step<D, FMT>& st, const Place& p, int g) {
     }
 }
 
-// Running maximum, weights, and O^T += V^T P^T.
-template <int D, int FMT, bool BF>
-__device__ inline void accumulate(const Step<D, FMT>& st, const float (&s)[8], Sums<D>& u) {
-    constexpr int DT = D / 16, VW = Step<D, FMT>::VB < 4 ? 1 : Step<D, FMT>::VB / 4;
+// A tile's running maximum and the step's weights, each as the sum of two
+// 16-bit numbers, in the values' type (22 bits) or, for quantised rows, in bf16
+// (16 bits), which has the range that rows' scales need: the result is then as
+// near to 64 bits as its own rounding allows, where one fp16 weight was 20 %
+// further off, and the second product costs nothing beside the rows' loads.
+template <int D, int FMT>
+__device__ inline void weigh(const Step<D, FMT>& st, const float (&s)[8], Sums<D>& u, u4& hi, u4& lo) {
     float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
     if (__any(top > u.m + kSlack)) {
         top = fmaxf(top, wave_xor(top, 16));
@@ -262,7 +270,7 @@ __device__ inline void accumulate(const Step<D, FMT>& st, const float (&s)[8], S
         u.l *= f;
         u.z *= f;
 #pragma unroll
-        for (int d = 0; d < DT; d++) u.acc[d] *= f;
+        for (int d = 0; d < D / 16; d++) u.acc[d] *= f;
     }
     float w[8];
 #pragma unroll
@@ -281,17 +289,10 @@ __device__ inline void accumulate(const Step<D, FMT>& st, const float (&s)[8], S
             w[j] *= st.sz[j >> 2][(j & 3) >> 1][2 * (j & 1)];
         }
     }
-    // Each weight as the sum of two 16-bit numbers, in the values' type (22 bits)
-    // or, for quantised rows, in bf16 (16 bits), which has the range that rows'
-    // scales need: the result is then as near to 64 bits as its own rounding
-    // allows, where one fp16 weight was 20 % further off, and the second product
-    // costs nothing beside the rows' loads.
-    constexpr bool kHalf = FMT == FKV_PAGES_F16;
-    u4 hi, lo;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const float x = w[2 * j], y = w[2 * j + 1];
-        if (kHalf) {
+        if (FMT == FKV_PAGES_F16) {
             hi[j] = (uint32_t)f2h(x) | ((uint32_t)f2h(y) << 16);
             lo[j] = (uint32_t)f2h(x - h2f((uint16_t)hi[j])) | ((uint32_t)f2h(y - h2f((uint16_t)(hi[j] >> 16))) << 16);
         } else {
@@ -299,9 +300,22 @@ __device__ inline void accumulate(const Step<D, FMT>& st, const float (&s)[8], S
             lo[j] = bf16_pair(x - __uint_as_float(hi[j] << 16), y - __uint_as_float(hi[j] & 0xFFFF0000u));
         }
     }
+}
+
+// Weights, and O^T += V^T P^T.
+template <int D, int FMT, int T>
+__device__ inline void accumulate(const Step<D, FMT>& st, const float (&s)[T][8], Sums<D> (&u)[T]) {
+    constexpr int DT = D / 16, VW = Step<D, FMT>::VB < 4 ? 1 : Step<D, FMT>::VB / 4;
+    constexpr bool kBF = FMT != FKV_PAGES_F16;
+    u4 hi[T], lo[T];
+#pragma unroll
+    for (int n = 0; n < T; n++) weigh<D, FMT>(st, s[n], u[n], hi[n], lo[n]);
     auto add = [&](int d, u4 v) {
-        u.acc[d] = mfma<!kHalf>(v, hi, u.acc[d]);
-        u.acc[d] = mfma<!kHalf>(v, lo, u.acc[d]);
+#pragma unroll
+        for (int n = 0; n < T; n++) {
+            u[n].acc[d] = mfma<kBF>(v, hi[n], u[n].acc[d]);
+            u[n].acc[d] = mfma<kBF>(v, lo[n], u[n].acc[d]);
+        }
     };
     if (FMT <= FKV_PAGES_BF16) {
 #pragma unroll
@@ -350,10 +364,11 @@ struct RowLds {
     float stat[NW][16][3];
 };
 
-// Joins the waves' sums in the LDS and writes the row's result (whole) or its
-// record.  Every wave of the workgroup calls it.
+// Joins the waves' sums of one tile of heads in the LDS and writes the row's
+// result (whole) or its record.  Every wave of the workgroup calls it.
 template <int D, int FMT, bool BF, int NW>
-__device__ inline void finish_row(const AttnArgs& a, Sums<D>& u, RowLds<D, NW>& lds, int b, int hrow, float* record) {
+__device__ inline void finish_row(const AttnArgs& a, Sums<D>& u, RowLds<D, NW>& lds, int b, int hrow, int tile,
+                                  float* record) {
     constexpr int DT = D / 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
     u.l += wave_xor(u.l, 16);
@@ -372,9 +387,9 @@ __device__ inline void finish_row(const AttnArgs& a, Sums<D>& u, RowLds<D, NW>& 
             *(f4*)&lds.num[wave][c][DT * (4 * g + i) + d] = f4{u.acc[d][i], u.acc[d + 1][i], u.acc[d + 2][i], u.acc[d + 3][i]};
     __syncthreads();
     // 16 threads a head, D / 16 dims a thread
-    const int head = threadIdx.x >> 4, r = threadIdx.x & 15, d0 = r * DT;
+    const int head = threadIdx.x >> 4, of_row = 16 * tile + head, r = threadIdx.x & 15, d0 = r * DT;
     const int h = hrow / a.HT, g0 = (hrow - h * a.HT) * a.GT;
-    if (head < a.GT && g0 + head < a.G) {
+    if (head < 16 && of_row < a.GT && g0 + of_row < a.G) {
         float m = kNegBig, l = 0.0f, z = 0.0f, y[DT] = {}, x[DT];
 #pragma unroll
         for (int w = 0; w < NW; w++) m = fmaxf(m, lds.stat[w][head][0]);
@@ -398,12 +413,12 @@ __device__ inline void finish_row(const AttnArgs& a, Sums<D>& u, RowLds<D, NW>& 
             x[i] = FMT == FKV_PAGES_FP8_INT4 ? fmaf(y[from], 512.0f, z) : y[from];
         }
         if (record) {
-            float* out = record + head * (D + 4);
+            float* out = record + of_row * (D + 4);
 #pragma unroll
             for (int i = 0; i < DT; i += 4) *(f4*)(out + d0 + i) = f4{x[i], x[i + 1], x[i + 2], x[i + 3]};
             if (r == 0) *(float2*)(out + D) = make_float2(m, l);
         } else {
-            const int64_t at = (int64_t)b * a.Hq + h * a.G + g0 + head;
+            const int64_t at = (int64_t)b * a.Hq + h * a.G + g0 + of_row;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             uint32_t o[DT / 2];
 #pragma unroll
@@ -496,7 +511,7 @@ __device__ inline Run run_of(const AttnArgs& a, uint32_t rows_per_seq) {
 
 // NW waves of 32 tokens a step.  SPLIT: runs of tiles dealt to the grid's
 // workgroups, see the file's head; else one workgroup per row.
-template <int D, int FMT, bool BF, int NW, bool SPLIT>
+template <int D, int FMT, bool BF, int NW, bool SPLIT, int T>
 __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(AttnArgs a) {
     constexpr int kStep = 32 * NW;
     __shared__ RowLds<D, NW> lds;
@@ -539,21 +554,26 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(AttnArgs a) {
     }
 
     while (work) {
-        u4 q[D / 32];
-        {
-            const bool real = c < a.GT && g0 + c < a.G;
-            const char* row = a.q + 2 * (b * a.q_sb + (int64_t)(h * a.G + g0 + (real ? c : 0)) * a.q_sh);
+        u4 q[T][D / 32];
+#pragma unroll
+        for (int n = 0; n < T; n++) {
+            const int of_row = 16 * n + c;
+            const bool real = of_row < a.GT && g0 + of_row < a.G;
+            const char* row = a.q + 2 * (b * a.q_sb + (int64_t)(h * a.G + g0 + (real ? of_row : 0)) * a.q_sh);
 #pragma unroll
             for (int i = 0; i < D / 32; i++) {
                 const int d = FMT <= FKV_PAGES_BF16 ? 32 * i + 8 * g : 64 * (i / 2) + 16 * g + 8 * (i & 1);
                 const u4 x = *(const u4*)(row + 2 * d), none = {0, 0, 0, 0};
-                q[i] = real ? x : none;
+                q[n][i] = real ? x : none;
             }
         }
-        Sums<D> u;
-        u.m = kNegBig, u.l = 0.0f, u.z = 0.0f;
+        Sums<D> u[T];
 #pragma unroll
-        for (int d = 0; d < D / 16; d++) u.acc[d] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int n = 0; n < T; n++) {
+            u[n].m = kNegBig, u[n].l = 0.0f, u[n].z = 0.0f;
+#pragma unroll
+            for (int d = 0; d < D / 16; d++) u[n].acc[d] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
 
         // One step; with `more`, the next one's ids first, its keys into the
         // same registers once these are used, its values once these are: 8 KB
@@ -566,14 +586,14 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(AttnArgs a) {
             tok += kStep;
             const int2 id = more ? ids_of(ids, sh, tok, len) : make_int2(0, 0);
             const Place p = place;
-            float s[8];
-            scores<D, FMT, BF>(st, q, p, a.scale, g, s);
+            float s[T][8];
+            scores<D, FMT, BF, T>(st, q, p, a.scale, g, s);
             if (more) {
                 place = place_of(a, id, sh, tok, len, h);
                 load_keys(st, a, place, g, c);
             }
             if (p.n[0] < 16 || p.n[1] < 16) mask_values(st, p, g);
-            accumulate<D, FMT, BF>(st, s, u);
+            accumulate<D, FMT, T>(st, s, u);
             if (more) load_values(st, a, place, g, c);
         };
         for (int t = t0; t < t1 - 1; t++) step(true);
@@ -614,7 +634,8 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(AttnArgs a) {
                 load_values(st, a, place, g, c);
             }
         }
-        finish_row<D, FMT, BF, NW>(a, u, lds, done_b, done_row, record);
+#pragma unroll
+        for (int n = 0; n < T; n++) finish_row<D, FMT, BF, NW>(a, u[n], lds, done_b, done_row, n, record);
         if (!SPLIT) return;
     }
 
@@ -721,7 +742,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, int n_rows)
 // ---------------------------------------------------------------------------
 
 struct AttnPlan {
-    int G, HT, GT, blocks;
+    int G, tiles, HT, GT, blocks;
     bool split;
     int64_t rows, records_at, bytes;
 };
@@ -743,10 +764,17 @@ constexpr int64_t kWholeRows = 512;
 static AttnPlan plan_of(const fkv_pages* p, int32_t Hq, int32_t B, int64_t max_len) {
     AttnPlan r;
     r.G = Hq / p->H;
-    r.HT = (r.G + 15) / 16;
+    r.split = max_len > kWholeRows;
+    // Groups of more than 16 heads: two tiles of heads a pass over the rows.  32
+    // heads on each of 2 KV heads, 16K tokens of 16 sequences, D = 128: 56 us and
+    // 88 with one (fp16), 37 and 50 (fp8).  Not for rows that are not split, whose
+    // time is a workgroup's (64 heads, 400 tokens of 32 sequences 10.2 us, 9.2 with
+    // one), nor for quantised rows of 64 dims, whose second pass costs what the
+    // second tile does (71 heads, 8K tokens of 8 sequences 15.8, 14.9 with one).
+    r.tiles = r.G > 16 && r.split && (p->D == 128 || p->format <= FKV_PAGES_BF16) ? 2 : 1;
+    r.HT = (r.G + 16 * r.tiles - 1) / (16 * r.tiles);
     r.GT = (r.G + r.HT - 1) / r.HT;
     r.rows = (int64_t)B * p->H * r.HT;
-    r.split = max_len > kWholeRows;
     const int64_t tiles = r.rows * std::max<int64_t>(1, cdiv(max_len, 32 * kAttnWaves));
     r.blocks = (int)(r.split ? std::min<int64_t>(tiles, kAttnGroups) : r.rows);
     r.records_at = round_up(16 * r.rows, 256);
@@ -765,11 +793,15 @@ static int check_attn(const char* who, const fkv_pages* p, int32_t Hq, int32_t B
 
 template <int D, int FMT, bool BF>
 static void launch_attn(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+    constexpr int threads = 64 * kAttnWaves;
     if (!p.split) {
-        paged_attn_kernel<D, FMT, BF, kAttnWaves, false><<<p.blocks, 64 * kAttnWaves, 0, s>>>(a);
+        paged_attn_kernel<D, FMT, BF, kAttnWaves, false, 1><<<p.blocks, threads, 0, s>>>(a);
         return;
     }
-    paged_attn_kernel<D, FMT, BF, kAttnWaves, true><<<p.blocks, 64 * kAttnWaves, 0, s>>>(a);
+    if constexpr (D == 128 || FMT <= FKV_PAGES_BF16) {
+        if (p.tiles == 2) paged_attn_kernel<D, FMT, BF, kAttnWaves, true, 2><<<p.blocks, threads, 0, s>>>(a);
+    }
+    if (p.tiles == 1) paged_attn_kernel<D, FMT, BF, kAttnWaves, true, 1><<<p.blocks, threads, 0, s>>>(a);
     const int rows = (int)std::min<int64_t>(p.rows, 1024);
     if (p.rows * p.GT <= 1024) paged_join_kernel<D, BF, 1><<<dim3(rows, p.GT), 256, 0, s>>>(a, (int)p.rows);
     else paged_join_kernel<D, BF, 4><<<dim3(rows, (p.GT + 3) / 4), 256, 0, s>>>(a, (int)p.rows);

@@ -78,9 +78,15 @@ def int4_encode(rows):
 
 
 def page_values(layer):
-    """Every row of a layer's pages (n_pages,H,page,D) in float64."""
+    """Every row of a layer's pages (n_pages,H,page,D) in float64: keys,
+    values, and what a value's error in attention is relative to, its
+    magnitude.  For INT4 that is |scale * code| + |min|: the kernel sums
+    w scale code and w min apart, the first with weights w scale rounded to 16
+    bits, so its error is 2^-16 of sum w |scale code|, and more than that of
+    sum w |v| where scale * code and min cancel."""
     if layer.k_exp is None:
-        return f64(layer.k), f64(layer.v)
+        v = f64(layer.v)
+        return f64(layer.k), v, np.abs(v)
 
     def scale(t):
         b = t.cpu().numpy().astype(np.int64)
@@ -88,11 +94,12 @@ def page_values(layer):
 
     k = e4m3_value(layer.k.cpu().numpy()) * scale(layer.k_exp)
     if layer.fmt == "fp8":
-        return k, e4m3_value(layer.v.cpu().numpy()) * scale(layer.v_scale)
+        v = e4m3_value(layer.v.cpu().numpy()) * scale(layer.v_scale)
+        return k, v, np.abs(v)
     c = layer.v.cpu().numpy()
     c = np.stack([c & 15, c >> 4], -1).reshape(*c.shape[:-1], -1).astype(np.float64)
     sz = f64(layer.v_scale)
-    return k, c * sz[..., :1] + sz[..., 1:]
+    return k, c * sz[..., :1] + sz[..., 1:], np.abs(c * sz[..., :1]) + np.abs(sz[..., 1:])
 
 
 def sequence(values, table, b, n, page, n_pages):
@@ -103,7 +110,7 @@ def sequence(values, table, b, n, page, n_pages):
 
 
 def attend(q, values, table, lens, page, n_pages, scale):
-    """-> out, lse and the error scale sum_t w_t |v_t| with the largest error of
+    """-> out, lse and the error scale sum_t w_t |v_t| (see page_values) with the largest error of
     a score, both per head (see bound)."""
     B, Hq, D = q.shape
     H = values[0].shape[1]
@@ -112,8 +119,8 @@ def attend(q, values, table, lens, page, n_pages, scale):
     spread, ds = np.zeros((B, Hq, D)), np.zeros((B, Hq))
     for b in range(B):
         n = int(min(max(lens[b], 0), table.shape[1] * page))
-        (k, v), ok = sequence(values, table, b, n, page, n_pages)
-        k, v = k[:, ok], v[:, ok]
+        (k, v, mag), ok = sequence(values, table, b, n, page, n_pages)
+        k, v, mag = k[:, ok], v[:, ok], mag[:, ok]
         if k.shape[1] == 0:
             continue
         for h in range(Hq):
@@ -123,7 +130,7 @@ def attend(q, values, table, lens, page, n_pages, scale):
             lse[b, h] = m + math.log(w.sum())
             w /= w.sum()
             out[b, h] = w @ v[h // G]
-            spread[b, h] = w @ np.abs(v[h // G])
+            spread[b, h] = w @ mag[h // G]
             # fp32 accumulation of D exact products, and the scale's and
             # log2 e's rounding
             ds[b, h] = (D + 4) * 2.0 ** -24 * (np.abs(k[h // G]) @ np.abs(q[b, h]) * abs(scale)).max()

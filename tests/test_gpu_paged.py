@@ -360,6 +360,22 @@ def test_attend_split(paged, fmt, lens):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,H,G", [(128, 1, 32), (128, 2, 17), (64, 1, 71)])
+def test_attend_wide_groups(paged, fmt, D, H, G):
+    """More than 16 heads on a KV head, over split rows: two tiles of heads a
+    pass, the last one partly filled."""
+    _flush("wide", fmt, D, H, G)
+    lens, page = [700, 1, 0, 3001], 64
+    counts = [-(-n // page) for n in lens]
+    layer = _filled(paged, fmt, sum(counts) + 1, H, D, page, 35)
+    table = _table(36, sum(counts) + 1, counts)
+    _spoil(layer, table, lens)
+    q = _randn(37, 4, H * G, 1, D).to(DTYPES.get(fmt, torch.float16)).cuda()
+    out = _check_attend(layer, q, table, lens)
+    assert bool((out[2] == 0).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_attend_pages_outside_the_pool_and_long_lens(paged, fmt):
     page, H, G, D = 16, 2, 3, 64
     layer = _filled(paged, fmt, 30, H, D, page, 40)
