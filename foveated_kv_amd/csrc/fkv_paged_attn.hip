@@ -605,9 +605,12 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(AttnArgs a) {
         float* record = nullptr;
         if (SPLIT) {
             const int slot = at > run.begin ? 1 : 0;
-            if (t0 == 0 && tid == 0)
+            if (t0 == 0 && tid == 0) {
+                // (no further than the records go, whatever was done to lens meanwhile)
+                const uint32_t last = min(owner_of(run.deal, at - u0 + kRowCost + nt - 1), gridDim.x - 1);
                 a.joins[(int64_t)b * rows_per_seq + hrow] =
-                    make_int4(blockIdx.x, whole ? 0 : (int)(owner_of(run.deal, at - u0 + kRowCost + nt - 1) - blockIdx.x + 1), slot, 0);
+                    make_int4(blockIdx.x, whole ? 0 : (int)(last - blockIdx.x + 1), slot, 0);
+            }
             if (!whole) record = a.records + ((int64_t)blockIdx.x * 2 + slot) * a.GT * (D + 4);
         }
         const int done_b = b, done_row = hrow;

@@ -331,12 +331,13 @@ class PagedCacheWrapper:
     ``update_and_fetch`` with several tokens (prefill) stores them and hands
     back every key (rotated, where the cache rotates) and value for the
     original attention; with one token it leaves the write to the attention
-    call that follows, which rotates the query in the same launch."""
+    call that follows, which rotates the query in the same launch and attends
+    to every stored token (``attn_mask`` is not looked at)."""
 
     def __init__(self, cache, layer_idx, seqs=None):
         self.cache, self.layer_idx, self.seqs = cache, layer_idx, cache.pages._range(seqs)
         self.rope = cache.rope
-        self._new = None
+        self._new, self._n_new = None, 0
 
     @property
     def offset(self):
@@ -350,7 +351,8 @@ class PagedCacheWrapper:
         if _paged_state["original"] is None:
             raise RuntimeError("paged attention is not installed")
         _paged_state["pending"] = self
-        if keys.shape[2] == 1:
+        self._n_new = keys.shape[2]
+        if self._n_new == 1:
             self._new = keys, values
             return keys, values
         self.cache.write(self.layer_idx, keys, values, seqs=self.seqs)
@@ -370,8 +372,11 @@ class PagedCacheWrapper:
 
 def _paged_interceptor(query, key, value, attn_mask=None, dropout_p=0.0, is_causal=False, scale=None, **kwargs):
     w, _paged_state["pending"] = _paged_state["pending"], None
-    if w is not None and query.dim() == 4:
-        if query.shape[2] == 1:
+    if w is not None:
+        if query.dim() != 4 or query.shape[2] != w._n_new:
+            raise RuntimeError(f"update_and_fetch took {w._n_new} tokens, the attention call has queries "
+                               f"{tuple(query.shape)}")
+        if w._n_new == 1:
             return w._answer(query, scale)
         if w.rope is not None:
             query = w.rope(query, w.offset)

@@ -86,6 +86,15 @@ def _rows(t, shape):
     return _pack_rows(at, sb, sh, sl), t
 
 
+def _result(index, name, t, shape, dtype):
+    """Refuses a result tensor that does not fit, or whose rows share memory."""
+    _on(index, name, t)
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{name} must have shape {tuple(shape)} and dtype {dtype}, got {tuple(t.shape)} {t.dtype}")
+    if 0 in t.stride() and any(s == 0 and n > 1 for s, n in zip(t.stride(), shape)):
+        raise ValueError(f"{name} is an expanded tensor: its rows share memory")
+
+
 def _positions(p, B, L, index, per_token_allowed=True):
     """int | one-element tensor | (B,) tensor: the first token's position of
     each sequence; (B, L) or (1, L): every token's."""
@@ -233,9 +242,7 @@ class Rope:
         if out is None:
             out = torch.empty_like(x)
         else:
-            _on(index, "out", out)
-            if out.shape != shape or out.dtype != dtype:
-                raise ValueError("out must have x's shape and dtype")
+            _result(index, "out", out, shape, dtype)
         B, H, L, D = shape
         pos = _positions(positions, B, L, index)
         src, held = _rows(x, shape)
@@ -382,9 +389,7 @@ class PagedLayer:
             if q_out is None:
                 q_out = torch.empty_like(q) if n_new is None else torch.zeros_like(q)
             else:
-                _on(index, "q_out", q_out)
-                if q_out.shape != qs or q_out.dtype != dtype:
-                    raise ValueError("q_out must have q's shape and dtype")
+                _result(index, "q_out", q_out, qs, dtype)
             Hq = qs[1]
             rq, q_held = _rows(q, qs)
             ro, result = _rows(q_out, qs)
@@ -514,10 +519,16 @@ class PageTable:
             raise ValueError(f"seqs must be a slice of neighbouring sequences, got {seqs}")
         return slice(first, stop)
 
+    def _not_captured(self):
+        if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("pages are handed out on the host: extend, reserve and free outside of a capture, or "
+                               "capture the layer's calls with lengths of your own")
+
     def reserve(self, tokens, seqs=None):
         """Gives each sequence the pages for ``tokens`` tokens (a number, or one
         per sequence) in all; those it holds stay.  Raises MemoryError, and
         changes nothing, where the pool or a sequence's row is too small."""
+        self._not_captured()
         sl = self._range(seqs)
         each = range(sl.start, sl.stop)
         want = [int(tokens)] * len(each) if isinstance(tokens, int) else [int(t) for t in tokens]
@@ -543,9 +554,7 @@ class PageTable:
     def extend(self, n=1, seqs=None):
         """``n`` more tokens (a number, or one per sequence): reserves their
         pages and advances start, new and lens."""
-        if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("pages are handed out on the host: extend before the capture, or capture the layer's "
-                               "calls with lengths of your own")
+        self._not_captured()
         sl = self._range(seqs)
         count = sl.stop - sl.start
         each = [int(n)] * count if isinstance(n, int) else [int(t) for t in n]
@@ -565,6 +574,7 @@ class PageTable:
         """Sequence ``seq`` is over: its pages go back to the pool."""
         if not 0 <= seq < self.max_seqs:
             raise ValueError(f"no sequence {seq}")
+        self._not_captured()
         self._free.extend(reversed(self._pages[seq]))
         self._pages[seq] = []
         self._lens[seq] = self._new[seq] = 0

@@ -636,8 +636,8 @@ typedef struct fkv_rope {
 int fkv_rope_table(const double* frequencies, int32_t rot_dim, double factor, int32_t n_positions, float* table,
                    void* stream);
 
-/* out = rotated x, rows (B, H, L) of D elements (D a multiple of 8, at most
- * 1024) of dtype; out may be x.  Asynchronous, capturable. */
+/* out = rotated x, rows (B, H, L) of D elements (D a multiple of 8 from
+ * 16 to 512) of dtype; out may be x.  Asynchronous, capturable. */
 int fkv_rope_apply(const fkv_rope* rope, const fkv_rows* x, const fkv_rows* out, int32_t dtype, int32_t B,
                    int32_t H, int32_t L, int32_t D, const fkv_positions* positions, void* stream);
 

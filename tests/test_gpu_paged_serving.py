@@ -326,3 +326,41 @@ def _lib_error():
     from foveated_kv_amd import _lib
 
     return _lib.FkvLibraryError
+
+
+def test_pages_are_not_handed_out_in_a_capture(fkv):
+    t = fkv.PageTable(4, 16, 2, 32)
+    t.extend(3)
+    x = torch.ones(4, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        graph.capture_begin()
+        try:
+            x.add_(1)
+            for call in (lambda: t.extend(1), lambda: t.reserve(20), lambda: t.free(0)):
+                with pytest.raises(RuntimeError, match="outside of a capture"):
+                    call()
+        finally:
+            graph.capture_end()
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(3):
+        graph.replay()
+    assert x.tolist() == [4.0] * 4
+    assert t.lengths() == [3, 3] and t.free_pages == 2 and t.lens.tolist() == [3, 3]
+    assert [t.table[b, 0].item() for b in range(2)] == [t.pages(b)[0] for b in range(2)]
+
+
+def test_expanded_results_are_refused(fkv):
+    from foveated_kv_amd import paged
+
+    layer = paged.PagedLayer(4, 2, 64, 16, "fp16")
+    rope = paged.Rope(64, max_positions=8)
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    kv = torch.ones(1, 1, 3, 64, dtype=torch.float16, device="cuda").expand(-1, 2, -1, -1)
+    for call in (lambda: rope(kv, 1, out=kv), lambda: layer.write(kv, kv, table, 0, q=kv, q_out=kv)):
+        with pytest.raises(ValueError, match="share memory"):
+            call()
+    assert bool((layer.k == 0).all()) and bool((kv == 1).all())
+    assert torch.equal(rope(kv, 1), rope(kv.contiguous(), 1))

@@ -302,3 +302,48 @@ def test_reference_codecs():
     back = c * s[:, None].astype(np.float64) + z[:, None]
     # half a step, and the scale's rounding 15 times over
     assert (np.abs(back - rows) <= s[:, None] * (0.5 + 15 * 2.0 ** -24) * 1.0000001).all()
+
+
+# ---------------------------------------------------------------------------
+# results and model calls
+# ---------------------------------------------------------------------------
+
+def test_results_whose_rows_share_memory_are_refused():
+    x = torch.zeros(2, 3, 5, 64)
+    shape, dtype = x.shape, x.dtype
+    paged._result(-1, "out", x, shape, dtype)
+    paged._result(-1, "out", torch.zeros(2, 5, 3, 64).transpose(1, 2), shape, dtype)
+    one = torch.zeros(1, 3, 5, 64)
+    # (one sequence: its stride says nothing)
+    paged._result(-1, "out", one.as_strided(one.shape, (0, 320, 64, 1)), one.shape, dtype)
+    for bad in (x[:1].expand(2, -1, -1, -1), x[:, :1].expand(-1, 3, -1, -1), x[..., :1].expand(-1, -1, -1, 64), x[:1],
+                x.half()):
+        with pytest.raises(ValueError):
+            paged._result(-1, "out", bad, shape, dtype)
+
+
+def test_attention_call_must_have_the_written_tokens():
+    from foveated_kv_amd import generate
+
+    class Cache:
+        rope, layers, pages = None, [None], PageTable(4, 16, 2, 32, device="cpu")
+        written = 0
+
+        def write(self, *args, **kw):
+            Cache.written += 1
+
+    cache = Cache()
+    kv, original = torch.zeros(2, 1, 5, 64), torch.nn.functional.scaled_dot_product_attention
+    w, = generate.install_paged_attention(cache)
+    try:
+        for keys, queries in ((kv[:, :, :1], kv), (kv, kv[:, :, :1]), (kv, kv[:, :, :4]), (kv[:, :, :1], kv[0])):
+            w.update_and_fetch(keys, keys)
+            with pytest.raises(RuntimeError, match="update_and_fetch took"):
+                torch.nn.functional.scaled_dot_product_attention(queries, keys, keys)
+        assert Cache.written == 2
+        k, v = w.update_and_fetch(kv, kv)
+        torch.nn.functional.scaled_dot_product_attention(kv, k, v)
+        torch.nn.functional.scaled_dot_product_attention(kv[0], kv[0], kv[0])  # (another attention than the cache's)
+    finally:
+        generate.uninstall_paged_attention()
+    assert torch.nn.functional.scaled_dot_product_attention is original
