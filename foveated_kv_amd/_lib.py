@@ -180,7 +180,7 @@ STATS_FIELDS = ("spikes_detected", "spikes_queued", "spikes_deduplicated", "spik
 class PromoterStatsC(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint64) for n in STATS_FIELDS]
 
-_lib = None
+_lib = _calls = None
 _load_error = None
 
 
@@ -206,6 +206,23 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def calls():
+    """The compiled calls of the paged cache (csrc/fkv_calls.cpp), bound to
+    the loaded library."""
+    global _calls
+    if _calls is None:
+        lib = load()
+        try:
+            from . import _fkv_calls
+        except ImportError as e:
+            raise FkvLibraryError(f"cannot load {_HERE}/_fkv_calls.so: {e}; run `make -C foveated_kv_amd/csrc` "
+                                  "or __graft_entry__.build()") from e
+        _fkv_calls.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
+            "fkv_rope_apply", "fkv_paged_write", "fkv_paged_read", "fkv_paged_attn_workspace", "fkv_paged_attn")))
+        _calls = _fkv_calls
+    return _calls
 
 
 def check(rc, what=""):

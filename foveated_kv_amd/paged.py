@@ -34,8 +34,11 @@ from .ext import _require_device
 
 FORMATS = {"fp16": 0, "bf16": 1, "fp8": 2, "fp8_int4": 3}
 _NEW = {"fp16": torch.float16, "bf16": torch.bfloat16}
-# fkv_rows and fkv_positions (include/fkv.h) as bytes: half the time of a
-# ctypes.Structure, of which a write call needs five
+# A plain call goes through the compiled module of csrc/fkv_calls.cpp, which
+# does what stands here behind it; NotImplemented: it has done nothing, and the
+# call is checked, and its arguments copied where they must be, here.
+#
+# fkv_rows and fkv_positions (include/fkv.h) as bytes
 _pack_rows = struct.Struct("Pqqq").pack
 _pack_positions = struct.Struct("Pqqqii").pack
 
@@ -220,9 +223,9 @@ class Rope:
         else:  # (to look at: calls take tables on a GPU)
             a = torch.arange(self.max_positions, dtype=torch.float64)[:, None] * inv
             self.table[:, 0], self.table[:, 1] = a.cos() * factor, a.sin() * factor
-        self._c = ctypes.byref(_lib.RopeC(self.table.data_ptr(), self.max_positions, self.rot_dim,
-                                          int(self.interleaved)))
-        self._index = self.table.get_device()
+        c = _lib.RopeC(self.table.data_ptr(), self.max_positions, self.rot_dim, int(self.interleaved))
+        self._c, self._index = ctypes.byref(c), self.table.get_device()
+        self._key = ctypes.addressof(c), self._index, self.head_dim
 
     def __call__(self, x, positions=0, out=None):
         """x (B, H, L, head_dim) fp16 / bf16 / fp32, any strides -> the rotated
@@ -231,6 +234,9 @@ class Rope:
         position), a (B,) tensor (each sequence's first token's) or (B, L) /
         (1, L) (every token's); int32 or int64 tensors on the device, read
         there, so a captured call follows them."""
+        done = _lib.calls().rope(self._key, x, positions, out)
+        if done is not NotImplemented:
+            return done
         index = self._index
         if index < 0:
             _require_device(self.table)
@@ -322,8 +328,8 @@ class PagedLayer:
         self.fmt, self.k, self.v, self.k_exp, self.v_scale = fmt, k, v, k_exp, v_scale
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, H, page, D
         self.device, self._index = k.device, k.get_device()
-        self._c = ctypes.byref(_lib.PagesC(k.data_ptr(), v.data_ptr(), ptr(k_exp), ptr(v_scale), n, page, H, D,
-                                           FORMATS[fmt]))
+        c = _lib.PagesC(k.data_ptr(), v.data_ptr(), ptr(k_exp), ptr(v_scale), n, page, H, D, FORMATS[fmt])
+        self._c, self._key = ctypes.byref(c), (ctypes.addressof(c), self._index)
         check(min(int(_lib.load().fkv_paged_attn_workspace(self._c, H, 1, 0)), 0), "PagedLayer")
 
     def _table(self, table, B=None):
@@ -357,6 +363,9 @@ class PagedLayer:
         its queries come back as ``q_out`` held them (zero in a new tensor).
         Positions outside the table are not stored either.  No two tokens of
         a call may name the same slot."""
+        done = _lib.calls().write(self._key, k, v, table, start, n_new, q, None if rope is None else rope._key, q_out)
+        if done is not NotImplemented:
+            return done
         index = self._index
         _on(index, "k", k)
         _on(index, "v", v)
@@ -406,6 +415,9 @@ class PagedLayer:
         ``dtype`` (default: the pages' own, fp16 for quantised ones); rows
         past lens[b] ((B,) int32 on the device) are zero.  ``max_len``
         defaults to the table's width in tokens."""
+        done = _lib.calls().read(self._key, table, lens, max_len, dtype)
+        if done is not NotImplemented:
+            return done
         table, B, P, stride = self._table(table)
         lens = _lens("lens", lens, B, self._index)
         S = P * self.page_size if max_len is None else int(max_len)
@@ -430,6 +442,9 @@ class PagedLayer:
         ``max_len`` is an upper bound of the lengths if the host knows one
         (default: the table's width); it decides how the work is split, not
         what is attended to.  ``scale`` defaults to D^-1/2."""
+        done = _lib.calls().attend(self._key, query, table, lens, max_len, lens_add, scale, out, return_lse)
+        if done is not NotImplemented:
+            return done
         index, D = self._index, self.head_dim
         _on(index, "query", query)
         shape, dtype = query.shape, query.dtype

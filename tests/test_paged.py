@@ -347,3 +347,27 @@ def test_attention_call_must_have_the_written_tokens():
     finally:
         generate.uninstall_paged_attention()
     assert torch.nn.functional.scaled_dot_product_attention is original
+
+
+def test_compiled_calls_leave_what_is_not_plain():
+    calls, x = _lib.calls(), torch.zeros(2, 3, 5, 64)
+    rope = Rope(64, max_positions=8, device="cpu")
+    i = torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: calls.rope(rope._key, x, 0, None), lambda: calls.rope(rope._key, None, "0", 3), lambda: calls.rope(),
+                 lambda: calls.rope(None, x, 0, None), lambda: calls.rope((1, 2), x, 2 ** 70, None),
+                 lambda: calls.write((0, 0), x, x, i[None], 0, None, None, None, None), lambda: calls.write((0, 0)),
+                 lambda: calls.read((0, 0), i[None], i, None, None), lambda: calls.read("pages", 1, 2, 3, 4),
+                 lambda: calls.attend((0, 0), x, i[None], i, None, 0, None, None, False), lambda: calls.attend(*[x] * 9)):
+        assert call() is NotImplemented
+
+
+def test_compiled_calls_that_are_missing_raise(monkeypatch):
+    import sys
+
+    import foveated_kv_amd
+
+    monkeypatch.setattr(_lib, "_calls", None)
+    monkeypatch.setitem(sys.modules, "foveated_kv_amd._fkv_calls", None)
+    monkeypatch.delattr(foveated_kv_amd, "_fkv_calls", raising=False)
+    with pytest.raises(_lib.FkvLibraryError, match="make -C"):
+        _lib.calls()
