@@ -141,11 +141,19 @@ __device__ inline Place place_of(const AttnArgs& a, int2 ids, int sh, int32_t to
 }
 
 // 16, 8, 4 or 2 bytes at a uniform base plus a lane's offset.  The cache is
-// read once, so its lines are not kept.
-template <typename T>
+// read once, so its lines are not kept.  But a key row of 128 bytes takes two
+// loads, each of half its line, as the lines of scales do: beside 64-byte rows
+// of values, KEEP for both is worth more than it displaces (INT4, D = 128, 4096
+// tokens of 64 sequences 75 us and 83.5 without, one sequence of 64K tokens 28.1
+// and 30.1; E4M3 values 89 and 90.5, but one sequence of 4096 tokens 10.0 and
+// 9.7; D = 64 or 16 bits no gain, or a loss of up to 5 %).
+template <typename T, bool KEEP = false>
 __device__ inline T load_at(const char* base, uint32_t off) {
+    if (KEEP) return *(const T*)(base + off);
     return __builtin_nontemporal_load((const T*)(base + off));
 }
+template <int D, int FMT>
+constexpr bool kKeep = FMT == FKV_PAGES_FP8_INT4 && D == 128;
 
 template <int D, int FMT>
 __device__ inline void load_keys(Step<D, FMT>& st, const AttnArgs& a, const Place& p, int g, int c) {
@@ -155,8 +163,8 @@ __device__ inline void load_keys(Step<D, FMT>& st, const AttnArgs& a, const Plac
     for (int t = 0; t < 2; t++) {
         const char* base = a.pg.k + p.row[t] * RB;
 #pragma unroll
-        for (int i = 0; i < Step<D, FMT>::KL; i++) st.k[t][i] = load_at<u4>(base, off + 64 * i);
-        if (FMT >= FKV_PAGES_FP8) st.kx[t] = load_at<uint32_t>((const char*)a.pg.k_exp + p.row[t], 4 * g);
+        for (int i = 0; i < Step<D, FMT>::KL; i++) st.k[t][i] = load_at<u4, kKeep<D, FMT>>(base, off + 64 * i);
+        if (FMT >= FKV_PAGES_FP8) st.kx[t] = load_at<uint32_t, kKeep<D, FMT>>((const char*)a.pg.k_exp + p.row[t], 4 * g);
     }
 }
 
@@ -184,8 +192,8 @@ __device__ inline void load_values(Step<D, FMT>& st, const AttnArgs& a, const Pl
         }
         if (FMT == FKV_PAGES_FP8) st.vx[t] = load_at<uint32_t>(a.pg.v_scale + p.row[t], 4 * g);
         if (FMT == FKV_PAGES_FP8_INT4) {
-            st.sz[t][0] = load_at<f4>(a.pg.v_scale + 8 * p.row[t], 32 * g);
-            st.sz[t][1] = load_at<f4>(a.pg.v_scale + 8 * p.row[t], 32 * g + 16);
+            st.sz[t][0] = load_at<f4, kKeep<D, FMT>>(a.pg.v_scale + 8 * p.row[t], 32 * g);
+            st.sz[t][1] = load_at<f4, kKeep<D, FMT>>(a.pg.v_scale + 8 * p.row[t], 32 * g + 16);
         }
     }
 }
