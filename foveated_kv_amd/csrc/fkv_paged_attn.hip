@@ -16,7 +16,9 @@
 // same), so the weights never cross lanes.  V^T's operand is made in
 // registers: a lane loads 16 (8, 4) bytes of D / 16 neighbouring dims of its
 // eight tokens -- 16 lanes a row, coalesced -- and pairs tokens by byte
-// permutes.  The LDS holds nothing but the waves' results at a row's end.
+// permutes.  Keys of 128 bytes a row and more go through the LDS, into which
+// they are loaded whole lines at a time; the rest of it holds the waves' results
+// at a row's end.
 //
 // Work: every (sequence, KV head) row is cut into tiles of 128 tokens (32 per
 // wave), and all tiles (with a unit per row for its beginning and end) are
@@ -26,9 +28,10 @@
 // sum, numerators) per workgroup, joined by a second kernel in a fixed order.
 //
 // Measured (kernel alone; 6.3 TB/s is what a streaming read reaches here):
-// 16K tokens of 8 sequences, 8 KV heads, bf16, 537 MB: 81.4 us, 6.6 TB/s;
-// 64K tokens, fp8 / INT4, 105 MB: 23.7 us, of which about 7 are the chain
-// lengths -> page ids -> first rows, and the rows' ends; the join 4 us.
+// 16K tokens of 8 sequences, 8 KV heads, bf16, 537 MB: 81 us, 6.6 TB/s; 64K
+// tokens, fp8 / INT4, 105 MB: 21 us, of which about 5 are the chain lengths ->
+// page ids -> first rows, and the rows' ends; the join 4 to 5 us.  Times below
+// are of both, over layers of 1.5 GB in turn, so that no cache holds one.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -101,10 +104,12 @@ __device__ inline uint32_t bf16_pair(float a, float b) {
 // Registers of one step: 32 tokens of a wave, as they were loaded.
 template <int D, int FMT>
 struct Step {
-    static constexpr int KL = FMT <= FKV_PAGES_BF16 ? D / 32 : D / 64;  // 16-byte key loads per 16-token tile
+    static constexpr int RB = FMT <= FKV_PAGES_BF16 ? 2 * D : D;  // bytes of a key row
+    static constexpr int KL = RB / 64;                            // 16-byte key loads per 16-token tile
+    static constexpr bool LDS = RB >= 128;                        // keys go to the wave's part of the LDS
     // value bytes of a lane per token: D / 16 dims
     static constexpr int VB = FMT <= FKV_PAGES_BF16 ? D / 8 : FMT == FKV_PAGES_FP8 ? D / 16 : D / 32;
-    u4 k[2][KL];
+    u4 k[2][LDS ? 1 : KL];
     uint32_t v[8][VB < 4 ? 1 : VB / 4];
     uint32_t kx[2], vx[2];  // exponent bytes of the lane's four tokens per tile
     f4 sz[2][2];            // INT4: (scale, min) of the lane's four tokens
@@ -141,30 +146,60 @@ __device__ inline Place place_of(const AttnArgs& a, int2 ids, int sh, int32_t to
 }
 
 // 16, 8, 4 or 2 bytes at a uniform base plus a lane's offset.  The cache is
-// read once, so its lines are not kept.  But a key row of 128 bytes takes two
-// loads, each of half its line, as the lines of scales do: beside 64-byte rows
-// of values, KEEP for both is worth more than it displaces (INT4, D = 128, 4096
-// tokens of 64 sequences 75 us and 83.5 without, one sequence of 64K tokens 28.1
-// and 30.1; E4M3 values 89 and 90.5, but one sequence of 4096 tokens 10.0 and
-// 9.7; D = 64 or 16 bits no gain, or a loss of up to 5 %).
-template <typename T, bool KEEP = false>
+// read once, so its lines are not kept.
+template <typename T>
 __device__ inline T load_at(const char* base, uint32_t off) {
-    if (KEEP) return *(const T*)(base + off);
     return __builtin_nontemporal_load((const T*)(base + off));
 }
-template <int D, int FMT>
-constexpr bool kKeep = FMT == FKV_PAGES_FP8_INT4 && D == 128;
+
+// Keys: the matrix instruction wants 16 bytes of each of 16 rows from 16
+// neighbouring lanes, which a load into registers fetches as 64 lookups of 16
+// bytes, and a row of 128 bytes or more line by line twice and more (INT4, D =
+// 128: 2.0 requests to the L2 for a line, and loads that keep lines only moved
+// others out).  A load into the LDS takes whole rows by neighbouring lanes, and
+// leaves 16 to 64 registers free: 4096 tokens of 64 sequences 83.5 -> 71.7 us
+// (INT4), 90.6 -> 88.4 (fp8), 168 -> 167 (bf16); 11003 tokens of 3 sequences,
+// 4 KV heads, 15.1 -> 14.1, 15.1 -> 14.2 and 20.6 -> 19.0.  Rows of 64 bytes
+// (E4M3, D = 64), 16 of which are neighbours anyway, keep to registers: 50.0 and
+// 50.9 through the LDS (INT4), 50.6 and 50.4 (fp8).
+
+// Where 16-byte chunk `chunk` of row `row` of a tile lies in the LDS: eight
+// neighbouring lanes' reads of one chunk of eight rows fall on all banks.
+template <int RB>
+__device__ inline uint32_t key_at(int row, int chunk) { return row * RB + 16 * (chunk ^ (row & 7)); }
+
+// 16 bytes a lane from a uniform base (of `size` bytes) plus a lane's and a
+// uniform offset into 1024 bytes of LDS, streamed past the caches (2: nt).  (A
+// buffer load: beside global loads into the LDS the compiler waits for all loads
+// wherever it waits for one.)
+__device__ inline void load_to_lds(char* lds, const char* base, int size, uint32_t off, int uniform_off) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, size, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, off, uniform_off, 0, 2);
+}
 
 template <int D, int FMT>
-__device__ inline void load_keys(Step<D, FMT>& st, const AttnArgs& a, const Place& p, int g, int c) {
-    constexpr int RB = FMT <= FKV_PAGES_BF16 ? 2 * D : D;  // bytes of a key row
-    const uint32_t off = c * RB + 16 * g;
+__device__ inline void load_keys(Step<D, FMT>& st, const AttnArgs& a, const Place& p, int g, int c, char* keys) {
+    constexpr int RB = Step<D, FMT>::RB, KL = Step<D, FMT>::KL;
+    if (FMT >= FKV_PAGES_FP8) {
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-        const char* base = a.pg.k + p.row[t] * RB;
+        for (int t = 0; t < 2; t++) st.kx[t] = load_at<uint32_t>((const char*)a.pg.k_exp + p.row[t], 4 * g);
+    }
+    if constexpr (Step<D, FMT>::LDS) {
+        constexpr int CHUNKS = RB / 16, ROWS = 64 / CHUNKS;  // of a row, and rows of a load
+        const int lane = 16 * g + c, row = lane / CHUNKS, chunk = lane % CHUNKS;
+        asm volatile("" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < Step<D, FMT>::KL; i++) st.k[t][i] = load_at<u4, kKeep<D, FMT>>(base, off + 64 * i);
-        if (FMT >= FKV_PAGES_FP8) st.kx[t] = load_at<uint32_t, kKeep<D, FMT>>((const char*)a.pg.k_exp + p.row[t], 4 * g);
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int i = 0; i < KL; i++)
+                load_to_lds(keys + 16 * RB * t + 1024 * i, a.pg.k + p.row[t] * RB, 16 * RB,
+                            key_at<RB>(row + ROWS * i % 8, chunk) - ROWS * i % 8 * RB, 1024 * i);
+        asm volatile("" ::: "memory");  // (the values' loads, which read_keys() counts, come behind these)
+    } else {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int i = 0; i < KL; i++) st.k[t][i] = load_at<u4>(a.pg.k + p.row[t] * RB, c * RB + 16 * g + 64 * i);
     }
 }
 
@@ -192,9 +227,46 @@ __device__ inline void load_values(Step<D, FMT>& st, const AttnArgs& a, const Pl
         }
         if (FMT == FKV_PAGES_FP8) st.vx[t] = load_at<uint32_t>(a.pg.v_scale + p.row[t], 4 * g);
         if (FMT == FKV_PAGES_FP8_INT4) {
-            st.sz[t][0] = load_at<f4, kKeep<D, FMT>>(a.pg.v_scale + 8 * p.row[t], 32 * g);
-            st.sz[t][1] = load_at<f4, kKeep<D, FMT>>(a.pg.v_scale + 8 * p.row[t], 32 * g + 16);
+            st.sz[t][0] = load_at<f4>(a.pg.v_scale + 8 * p.row[t], 32 * g);
+            st.sz[t][1] = load_at<f4>(a.pg.v_scale + 8 * p.row[t], 32 * g + 16);
         }
+    }
+}
+
+// The step's keys out of the LDS, once they are there.  Loads end in the order of
+// their issue, so all but load_values()'s, which come next and are counted here,
+// must be done; what else was issued since only makes the wait longer.
+template <int D, int FMT>
+__device__ inline void read_keys(const char* keys, u4 (&k)[2][Step<D, FMT>::KL], int g, int c) {
+    constexpr int RB = Step<D, FMT>::RB;
+    constexpr int kBehind = 2 * (4 + (FMT == FKV_PAGES_FP8 ? 1 : FMT == FKV_PAGES_FP8_INT4 ? 2 : 0));
+    const uint32_t base = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)keys;
+    const uint32_t a0 = base + key_at<RB>(c, g), a1 = base + key_at<RB>(c, g + 4);
+    if constexpr (RB == 128) {
+        asm volatile("s_waitcnt vmcnt(%6)\n\t"
+                     "ds_read_b128 %0, %4\n\t"
+                     "ds_read_b128 %1, %5\n\t"
+                     "ds_read_b128 %2, %4 offset:2048\n\t"
+                     "ds_read_b128 %3, %5 offset:2048\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[1][0]), "=&v"(k[1][1])
+                     : "v"(a0), "v"(a1), "n"(kBehind)
+                     : "memory");
+    } else {
+        asm volatile("s_waitcnt vmcnt(%10)\n\t"
+                     "ds_read_b128 %0, %8\n\t"
+                     "ds_read_b128 %1, %9\n\t"
+                     "ds_read_b128 %2, %8 offset:128\n\t"
+                     "ds_read_b128 %3, %9 offset:128\n\t"
+                     "ds_read_b128 %4, %8 offset:4096\n\t"
+                     "ds_read_b128 %5, %9 offset:4096\n\t"
+                     "ds_read_b128 %6, %8 offset:4224\n\t"
+                     "ds_read_b128 %7, %9 offset:4224\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[0][2]), "=&v"(k[0][3]), "=&v"(k[1][0]), "=&v"(k[1][1]),
+                       "=&v"(k[1][2]), "=&v"(k[1][3])
+                     : "v"(a0), "v"(a1), "n"(kBehind)
+                     : "memory");
     }
 }
 
@@ -207,8 +279,8 @@ struct Sums {
 
 // Scores of a step's 32 tokens, T tiles of 16 heads.
 template <int D, int FMT, bool BF, int T>
-__device__ inline void scores(const Step<D, FMT>& st, const u4 (&q)[T][D / 32], const Place& p, float scale, int g,
-                              float (&s)[T][8]) {
+__device__ inline void scores(const Step<D, FMT>& st, const u4 (&keys)[2][Step<D, FMT>::KL],
+                              const u4 (&q)[T][D / 32], const Place& p, float scale, int g, float (&s)[T][8]) {
 #pragma unroll
     for (int t = 0; t < 2; t++) {
         f4 r[T];
@@ -218,9 +290,9 @@ __device__ inline void scores(const Step<D, FMT>& st, const u4 (&q)[T][D / 32], 
         for (int i = 0; i < D / 32; i++) {
             u4 k;
             if (FMT <= FKV_PAGES_BF16) {
-                k = st.k[t][i % Step<D, FMT>::KL];
+                k = keys[t][i % Step<D, FMT>::KL];
             } else {
-                const u4 w = st.k[t][(i / 2) % Step<D, FMT>::KL];
+                const u4 w = keys[t][i / 2 % Step<D, FMT>::KL];
                 const uint32_t w0 = i & 1 ? w.z : w.x, w1 = i & 1 ? w.w : w.y;
                 k = u4{cvt_fp8<BF>(w0, false), cvt_fp8<BF>(w0, true), cvt_fp8<BF>(w1, false), cvt_fp8<BF>(w1, true)};
             }
@@ -523,8 +595,10 @@ template <int D, int FMT, bool BF, int NW, bool SPLIT, int T>
 __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(AttnArgs a) {
     constexpr int kStep = 32 * NW;
     __shared__ RowLds<D, NW> lds;
+    __shared__ __attribute__((aligned(16))) char key_lds[NW][Step<D, FMT>::LDS ? 32 * Step<D, FMT>::RB : 16];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    char* keys = key_lds[wave];
     const int rows_per_seq = a.pg.H * a.HT;
     const int sh = 31 - __builtin_clz((unsigned)a.pg.page_size);
 
@@ -557,7 +631,7 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(AttnArgs a) {
     // (one workgroup per row: the first ids are loaded beside the length)
     Place place = place_of(a, ids_of(ids, sh, tok, SPLIT ? len : a.table.n << sh), sh, tok, len, h);
     if (work) {
-        load_keys(st, a, place, g, c);
+        load_keys(st, a, place, g, c, keys);
         load_values(st, a, place, g, c);
     }
 
@@ -584,21 +658,28 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(AttnArgs a) {
         }
 
         // One step; with `more`, the next one's ids first, its keys into the
-        // same registers once these are used, its values once these are: 8 KB
-        // to 16 KB of a wave in flight at D = 128 in 16 bits.  (The last step
+        // same place once these are used, its values once these are: 8 KB to 16
+        // KB of a wave in flight at D = 128 in 16 bits.  (The last step
         // stands apart: loads under a condition inside the loop made every wait
         // in it one for all loads, 16K tokens of 8 sequences 83.5 us, not 81.9.
         // A second set of registers, loaded a step further ahead, gained 2 %
         // there and lost 7 to 20 % with quantised rows.)
         auto step = [&](bool more) {
+            u4 k[2][Step<D, FMT>::KL];
+            if constexpr (Step<D, FMT>::LDS) {
+                read_keys<D, FMT>(keys, k, g, c);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2 * Step<D, FMT>::KL; i++) k[i & 1][i / 2] = st.k[i & 1][i / 2];
+            }
             tok += kStep;
             const int2 id = more ? ids_of(ids, sh, tok, len) : make_int2(0, 0);
             const Place p = place;
             float s[T][8];
-            scores<D, FMT, BF, T>(st, q, p, a.scale, g, s);
+            scores<D, FMT, BF, T>(st, k, q, p, a.scale, g, s);
             if (more) {
                 place = place_of(a, id, sh, tok, len, h);
-                load_keys(st, a, place, g, c);
+                load_keys(st, a, place, g, c, keys);
             }
             if (p.n[0] < 16 || p.n[1] < 16) mask_values(st, p, g);
             accumulate<D, FMT, T>(st, s, u);
@@ -641,7 +722,7 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(AttnArgs a) {
                 h = hrow / a.HT, g0 = (hrow - h * a.HT) * a.GT;
                 tok = 32 * wave;
                 place = place_of(a, ids_of(ids, sh, tok, len), sh, tok, len, h);
-                load_keys(st, a, place, g, c);
+                load_keys(st, a, place, g, c, keys);
                 load_values(st, a, place, g, c);
             }
         }
