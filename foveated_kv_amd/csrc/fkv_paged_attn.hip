@@ -661,8 +661,9 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(AttnArgs a) {
         // same place once these are used, its values once these are: 8 KB to 16
         // KB of a wave in flight at D = 128 in 16 bits.  (The last step
         // stands apart: loads under a condition inside the loop made every wait
-        // in it one for all loads, 16K tokens of 8 sequences 83.5 us, not 81.9.
-        // A second set of registers, loaded a step further ahead, gained 2 %
+        // in it one for all loads, and read_keys() counts on those of the step.
+        // Keys in registers then, 16K tokens of 8 sequences took 83.5 us, not 81.9,
+        // and a second set of registers, loaded a step further ahead, gained 2 %
         // there and lost 7 to 20 % with quantised rows.)
         auto step = [&](bool more) {
             u4 k[2][Step<D, FMT>::KL];
@@ -843,24 +844,34 @@ struct AttnPlan {
 // 3 sequences 21 us, not 19; one row of 512 tokens 7.8 us, not 7.3: a row's
 // time is what one CU can load.)
 constexpr int kAttnWaves = 4;
-// Two workgroups per CU, each with its part of all rows.  (Three: 16K tokens of
-// 8 sequences 83.6 us, not 81.4; four: 88.)
+// Two workgroups per CU, each with its part of all rows.  (Three: 4096 tokens of
+// 64 sequences 173.8 us, not 167.6 (bf16), 75.8 and 71.8 (INT4); 11003 tokens of
+// 3 sequences 23.3 and 18.9.)
 constexpr int kAttnGroups = 512;
 // Rows up to this long are not split: one launch, no records.  512 tokens of
-// one sequence's 8 KV heads 7.4 us and split 7.7 (bf16, D = 128), 5.1 and 6.9
-// (fp16, D = 64), 64 sequences 21 and 26; 1024 tokens of one sequence 11.7 us
-// and split 7.7.
+// one sequence's 8 KV heads 5.7 us and split 8.0 (bf16, D = 128), 4.9 and 7.4
+// (fp16, D = 64), of 64 sequences 19.8 and 22.1; 1024 tokens of one sequence 11.7
+// us and split 9.3.
 constexpr int64_t kWholeRows = 512;
+// Twice as long with as many rows as this, which then keep enough of the chip
+// busy: 1024 tokens of 16 sequences 15.6 us and split 19.0 (bf16), 12.8 and 13.8
+// (fp8), of 24 sequences with 5 KV heads 15.7 and 18.2, lengths at random up to
+// 1024 13.7 and 14.0; where one sequence has 1024 and the others 128, 12.6 and
+// 11.4.  8 sequences: 13.9 and 13.5.  (2048 tokens of 32 sequences 43.1 and 48.8,
+// but with one that is longer than the others 22.5 and 15.7.)
+constexpr int64_t kManyRows = 96;
 
 // Workgroups and workspace of a call (a function of sizes alone).
 static AttnPlan plan_of(const fkv_pages* p, int32_t Hq, int32_t B, int64_t max_len) {
     AttnPlan r;
     r.G = Hq / p->H;
-    r.split = max_len > kWholeRows;
+    const int64_t rows16 = (int64_t)B * p->H * ((r.G + 15) / 16);
+    r.split = max_len > (rows16 >= kManyRows ? 2 * kWholeRows : kWholeRows);
     // Groups of more than 16 heads: two tiles of heads a pass over the rows.  32
-    // heads on each of 2 KV heads, 16K tokens of 16 sequences, D = 128: 56 us and
-    // 88 with one (fp16), 37 and 50 (fp8).  Not for rows that are not split, whose
-    // time is a workgroup's (64 heads, 400 tokens of 32 sequences 10.2 us, 9.2 with
+    // heads on each of 2 KV heads, 16K tokens of 16 sequences, D = 128: 53 us and
+    // 81 with one (fp16), 36.5 and 43.5 (fp8), 35.3 and 39.3 (INT4; 17 heads, 2000
+    // tokens, 4 KV heads 18.3 and 17.0).  Not for rows that are not split, whose
+    // time is a workgroup's (64 heads, 400 tokens of 32 sequences 9.9 us, 7.7 with
     // one), nor for quantised rows of 64 dims, whose second pass costs what the
     // second tile does (71 heads, 8K tokens of 8 sequences 15.8, 14.9 with one).
     r.tiles = r.G > 16 && r.split && (p->D == 128 || p->format <= FKV_PAGES_BF16) ? 2 : 1;

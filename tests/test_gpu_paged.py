@@ -360,6 +360,25 @@ def test_attend_split(paged, fmt, lens):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,H,G,B", [(128, 2, 4, 50), (64, 3, 5, 40), (64, 1, 40, 40)])
+def test_attend_many_rows(paged, fmt, D, H, G, B):
+    """Many rows of up to 1024 tokens, a workgroup each, and the same rows split
+    (by a larger max_len), and longer ones than max_len says."""
+    _flush("many rows", fmt, D, H, G, B)
+    page, n = 64, [0, 1, 513, 1024, 130, 1023, 640, 900]
+    lens = [n[b % len(n)] for b in range(B)]
+    lens[3] = 1500
+    counts = [-(-x // page) for x in lens]
+    layer = _filled(paged, fmt, sum(counts) + 1, H, D, page, 38)
+    table = _table(39, sum(counts) + 1, counts)
+    _spoil(layer, table, lens)
+    q = _randn(40, B, H * G, 1, D).to(DTYPES.get(fmt, torch.bfloat16)).cuda()
+    for max_len in (1024, 513, 1500):
+        out = _check_attend(layer, q, table, lens, max_len=max_len)
+        assert bool((out[0] == 0).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("D,H,G", [(128, 1, 32), (128, 2, 17), (64, 1, 71)])
 def test_attend_wide_groups(paged, fmt, D, H, G):
     """More than 16 heads on a KV head, over split rows: two tiles of heads a
