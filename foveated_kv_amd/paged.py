@@ -539,6 +539,10 @@ class PageTable:
             raise RuntimeError("pages are handed out on the host: extend, reserve and free outside of a capture, or "
                                "capture the layer's calls with lengths of your own")
 
+    def _view(self, t, sl):
+        # (a slice of a tensor takes longer than a decode step's kernel launch)
+        return t if sl.stop - sl.start == self.max_seqs else t[sl]
+
     def reserve(self, tokens, seqs=None):
         """Gives each sequence the pages for ``tokens`` tokens (a number, or one
         per sequence) in all; those it holds stay.  Raises MemoryError, and
@@ -578,11 +582,12 @@ class PageTable:
         if each and min(each) < 0:
             raise ValueError("sequences do not shrink (free them)")
         self.reserve([a + t for a, t in zip(self._lens[sl], each)], seqs=sl)
-        self.start[sl].copy_(self.lens[sl])
+        start, new, lens = (self._view(t, sl) for t in (self.start, self.new, self.lens))
+        start.copy_(lens)
         if self._new[sl] != each:
-            self.new[sl].copy_(torch.tensor(each, dtype=torch.int32))
+            new.copy_(torch.tensor(each, dtype=torch.int32))
             self._new[sl] = each
-        self.lens[sl].add_(self.new[sl])
+        lens.add_(new)
         self._lens[sl] = [a + t for a, t in zip(self._lens[sl], each)]
 
     def free(self, seq):
@@ -629,7 +634,7 @@ class PagedKVCache:
 
     def _batch(self, seqs):
         sl = self.pages._range(seqs)
-        return sl, self.pages.table[sl]
+        return sl, self.pages._view(self.pages.table, sl)
 
     def write(self, layer, k, v, q=None, seqs=None, q_out=None):
         """The new tokens of the last ``extend`` of the same sequences; see
@@ -638,20 +643,20 @@ class PagedKVCache:
         new = self.pages._new[sl]
         if new and max(new) != k.shape[2]:
             raise ValueError(f"k holds {k.shape[2]} tokens, the last extend made room for {max(new)}")
-        n_new = None if len(set(new)) <= 1 else self.pages.new[sl]
-        return self.layers[layer].write(k, v, table, self.pages.start[sl], n_new=n_new, q=q, rope=self.rope,
+        n_new = None if len(set(new)) <= 1 else self.pages._view(self.pages.new, sl)
+        return self.layers[layer].write(k, v, table, self.pages._view(self.pages.start, sl), n_new=n_new, q=q, rope=self.rope,
                                         q_out=q_out)
 
     def attend(self, layer, query, seqs=None, scale=None, out=None):
         sl, table = self._batch(seqs)
-        return self.layers[layer].attend(query, table, self.pages.lens[sl], max(self.pages._lens[sl], default=0),
+        return self.layers[layer].attend(query, table, self.pages._view(self.pages.lens, sl), max(self.pages._lens[sl], default=0),
                                          scale=scale, out=out)
 
     def read(self, layer, seqs=None, dtype=None):
         """K, V (B, H, longest length, D); rows past a sequence's length are
         zero."""
         sl, table = self._batch(seqs)
-        return self.layers[layer].read(table, self.pages.lens[sl], max(self.pages._lens[sl], default=0), dtype)
+        return self.layers[layer].read(table, self.pages._view(self.pages.lens, sl), max(self.pages._lens[sl], default=0), dtype)
 
     def to_foveated(self, cfg=None, seqs=None, importance=None):
         """A ``FoveatedKVCache`` of the sequences' contexts, compressed into
