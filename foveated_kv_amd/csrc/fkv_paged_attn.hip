@@ -334,13 +334,18 @@ __device__ inline void mask_values(Step<D, FMT>& st, const Place& p, int g) {
     }
 }
 
-// A tile's running maximum and the step's weights, each as the sum of two
-// 16-bit numbers, in the values' type (22 bits) or, for quantised rows, in bf16
-// (16 bits), which has the range that rows' scales need: the result is then as
-// near to 64 bits as its own rounding allows, where one fp16 weight was 20 %
-// further off, and the second product costs nothing beside the rows' loads.
+// Numbers of 16 bits that a weight is the sum of.  bf16: three, which hold all
+// of its 24 bits (each the upper half of what is left, so there is no rounding)
+// and have the range that rows' scales need.  (Two, rounded, hold 16 bits; the
+// third product costs 0 to 2 %: 64 sequences of 4096 tokens 167.1 us with either
+// (bf16, D = 128), 88.5 and 88.6 (fp8), 71.8 and 72.3 (INT4), 50.2 and 51.4 (INT4,
+// D = 64).)  fp16: two, 22 bits.
+template <int FMT>
+constexpr int kParts = FMT == FKV_PAGES_F16 ? 2 : 3;
+
+// A tile's running maximum and the step's weights.
 template <int D, int FMT>
-__device__ inline void weigh(const Step<D, FMT>& st, const float (&s)[8], Sums<D>& u, u4& hi, u4& lo) {
+__device__ inline void weigh(const Step<D, FMT>& st, const float (&s)[8], Sums<D>& u, u4 (&part)[kParts<FMT>]) {
     float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
     if (__any(top > u.m + kSlack)) {
         top = fmaxf(top, wave_xor(top, 16));
@@ -371,13 +376,19 @@ __device__ inline void weigh(const Step<D, FMT>& st, const float (&s)[8], Sums<D
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const float x = w[2 * j], y = w[2 * j + 1];
-        if (FMT == FKV_PAGES_F16) {
-            hi[j] = (uint32_t)f2h(x) | ((uint32_t)f2h(y) << 16);
-            lo[j] = (uint32_t)f2h(x - h2f((uint16_t)hi[j])) | ((uint32_t)f2h(y - h2f((uint16_t)(hi[j] >> 16))) << 16);
+        float x = w[2 * j], y = w[2 * j + 1];
+        if constexpr (FMT == FKV_PAGES_F16) {
+            const uint32_t hi = (uint32_t)f2h(x) | ((uint32_t)f2h(y) << 16);
+            part[0][j] = hi;
+            part[1][j] = (uint32_t)f2h(x - h2f((uint16_t)hi)) | ((uint32_t)f2h(y - h2f((uint16_t)(hi >> 16))) << 16);
         } else {
-            hi[j] = bf16_pair(x, y);
-            lo[j] = bf16_pair(x - __uint_as_float(hi[j] << 16), y - __uint_as_float(hi[j] & 0xFFFF0000u));
+#pragma unroll
+            for (int i = 0; i < kParts<FMT>; i++) {
+                const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+                part[i][j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+                x -= __uint_as_float(a & 0xFFFF0000u);
+                y -= __uint_as_float(b & 0xFFFF0000u);
+            }
         }
     }
 }
@@ -387,15 +398,14 @@ template <int D, int FMT, int T>
 __device__ inline void accumulate(const Step<D, FMT>& st, const float (&s)[T][8], Sums<D> (&u)[T]) {
     constexpr int DT = D / 16, VW = Step<D, FMT>::VB < 4 ? 1 : Step<D, FMT>::VB / 4;
     constexpr bool kBF = FMT != FKV_PAGES_F16;
-    u4 hi[T], lo[T];
+    u4 part[T][kParts<FMT>];
 #pragma unroll
-    for (int n = 0; n < T; n++) weigh<D, FMT>(st, s[n], u[n], hi[n], lo[n]);
+    for (int n = 0; n < T; n++) weigh<D, FMT>(st, s[n], u[n], part[n]);
     auto add = [&](int d, u4 v) {
 #pragma unroll
-        for (int n = 0; n < T; n++) {
-            u[n].acc[d] = mfma<kBF>(v, hi[n], u[n].acc[d]);
-            u[n].acc[d] = mfma<kBF>(v, lo[n], u[n].acc[d]);
-        }
+        for (int n = 0; n < T; n++)
+#pragma unroll
+            for (int i = 0; i < kParts<FMT>; i++) u[n].acc[d] = mfma<kBF>(v, part[n][i], u[n].acc[d]);
     };
     if (FMT <= FKV_PAGES_BF16) {
 #pragma unroll
