@@ -54,6 +54,11 @@ constexpr float kNegBig = -3.402823466e38f;  // running maximum before the first
 // weights hold alike, and most steps need no rescaling and no reduction
 // across lanes.
 constexpr float kSlack = 8.0f;
+// What the running maximum of fp16 pages stays below the scores': their largest
+// weight is 2^7 to 2^15, so that small ones are as far as may be from the end of
+// fp16's range.
+template <int FMT>
+constexpr float kBias = FMT == FKV_PAGES_F16 ? 7.0f : 0.0f;
 
 struct AttnArgs {
     PageView pg;
@@ -334,23 +339,44 @@ __device__ inline void mask_values(Step<D, FMT>& st, const Place& p, int g) {
     }
 }
 
-// Numbers of 16 bits that a weight is the sum of.  bf16: three, which hold all
-// of its 24 bits (each the upper half of what is left, so there is no rounding)
-// and have the range that rows' scales need.  (Two, rounded, hold 16 bits; the
-// third product costs 0 to 2 %: 64 sequences of 4096 tokens 167.1 us with either
-// (bf16, D = 128), 88.5 and 88.6 (fp8), 71.8 and 72.3 (INT4), 50.2 and 51.4 (INT4,
-// D = 64).)  fp16: two, 22 bits.
-template <int FMT>
-constexpr int kParts = FMT == FKV_PAGES_F16 ? 2 : 3;
+// A weight enters as three 16-bit numbers, for which there are matrix
+// instructions.
+// bf16: their sum is the weight, all 24 bits of it, each being the upper half of
+// what is left; they have the range that rows' scales need.  (Two, rounded, hold
+// 16 bits; the third product costs 0 to 2 %: 64 sequences of 4096 tokens 167.1 us
+// with either (bf16, D = 128), 88.5 and 88.6 (fp8), 71.8 and 72.3 (INT4), 50.2 and
+// 51.4 (INT4, D = 64).)
+// fp16, the type of the values that it is for: the weight cut off to fp16, and
+// 2^10 times what that leaves, twice.  Large weights have 24 bits and small ones
+// steps of 2^-44, which is 2^-51 of the row's largest; fp16 alone ends at 2^-24,
+// and a token 14 to 24 nats above the others, with a value of zero, left 10 to
+// no bits of theirs.  (Beside two parts of one scale: 64 sequences of 4096 tokens
+// 167.0 us and 167.8, 11003 tokens of 3 19.0 and 19.6, 512 of one 7.6 and 8.0;
+// D = 64 85.8, 86.2; 13.2, 13.5; 5.7, 5.9.  Values taken apart into bf16, for which
+// weights are as above, cost 1 % and, 512 tokens of one sequence, 2.1 to 2.7 us.)
+constexpr int kParts = 3;
+constexpr float kUp = 1024.0f;
+__device__ inline uint32_t take_bf16(float& x, float& y) {
+    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+    x -= __uint_as_float(a & 0xFFFF0000u);
+    y -= __uint_as_float(b & 0xFFFF0000u);
+    return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+__device__ inline uint32_t take_fp16(float& x, float& y) {
+    const fkv_h2 h = __builtin_bit_cast(fkv_h2, __builtin_amdgcn_cvt_pkrtz(x, y));
+    x = fmaf(-kUp, (float)h.x, kUp * x);
+    y = fmaf(-kUp, (float)h.y, kUp * y);
+    return as_u32(h);
+}
 
 // A tile's running maximum and the step's weights.
 template <int D, int FMT>
-__device__ inline void weigh(const Step<D, FMT>& st, const float (&s)[8], Sums<D>& u, u4 (&part)[kParts<FMT>]) {
+__device__ inline void weigh(const Step<D, FMT>& st, const float (&s)[8], Sums<D>& u, u4 (&part)[kParts]) {
     float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-    if (__any(top > u.m + kSlack)) {
+    if (__any(top > u.m + (kSlack + kBias<FMT>))) {
         top = fmaxf(top, wave_xor(top, 16));
         top = fmaxf(top, wave_xor(top, 32));
-        const float m = fmaxf(u.m, top), f = __builtin_amdgcn_exp2f(u.m - m);
+        const float m = fmaxf(u.m, top - kBias<FMT>), f = __builtin_amdgcn_exp2f(u.m - m);
         u.m = m;
         u.l *= f;
         u.z *= f;
@@ -376,20 +402,9 @@ __device__ inline void weigh(const Step<D, FMT>& st, const float (&s)[8], Sums<D
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        float x = w[2 * j], y = w[2 * j + 1];
-        if constexpr (FMT == FKV_PAGES_F16) {
-            const uint32_t hi = (uint32_t)f2h(x) | ((uint32_t)f2h(y) << 16);
-            part[0][j] = hi;
-            part[1][j] = (uint32_t)f2h(x - h2f((uint16_t)hi)) | ((uint32_t)f2h(y - h2f((uint16_t)(hi >> 16))) << 16);
-        } else {
 #pragma unroll
-            for (int i = 0; i < kParts<FMT>; i++) {
-                const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
-                part[i][j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-                x -= __uint_as_float(a & 0xFFFF0000u);
-                y -= __uint_as_float(b & 0xFFFF0000u);
-            }
-        }
+        for (int i = 0; i < kParts; i++)
+            part[i][j] = FMT == FKV_PAGES_F16 ? take_fp16(w[2 * j], w[2 * j + 1]) : take_bf16(w[2 * j], w[2 * j + 1]);
     }
 }
 
@@ -398,14 +413,24 @@ template <int D, int FMT, int T>
 __device__ inline void accumulate(const Step<D, FMT>& st, const float (&s)[T][8], Sums<D> (&u)[T]) {
     constexpr int DT = D / 16, VW = Step<D, FMT>::VB < 4 ? 1 : Step<D, FMT>::VB / 4;
     constexpr bool kBF = FMT != FKV_PAGES_F16;
-    u4 part[T][kParts<FMT>];
+    u4 part[T][kParts];
 #pragma unroll
     for (int n = 0; n < T; n++) weigh<D, FMT>(st, s[n], u[n], part[n]);
     auto add = [&](int d, u4 v) {
 #pragma unroll
-        for (int n = 0; n < T; n++)
+        for (int n = 0; n < T; n++) {
+            f4& acc = u[n].acc[d];
+            if (kBF) {
 #pragma unroll
-            for (int i = 0; i < kParts<FMT>; i++) u[n].acc[d] = mfma<kBF>(v, part[n][i], u[n].acc[d]);
+                for (int i = 0; i < kParts; i++) acc = mfma<kBF>(v, part[n][i], acc);
+            } else {
+                f4 low = mfma<kBF>(v, part[n][2], f4{0.0f, 0.0f, 0.0f, 0.0f});
+                low = mfma<kBF>(v, part[n][1], low * (1.0f / kUp));
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[i] = fmaf(low[i], 1.0f / kUp, acc[i]);
+                acc = mfma<kBF>(v, part[n][0], acc);
+            }
+        }
     };
     if (FMT <= FKV_PAGES_BF16) {
 #pragma unroll

@@ -1,8 +1,6 @@
 """How exactly the paged attention weighs values: results that are small
 beside their terms show what a weight was rounded to."""
 
-import math
-
 import numpy as np
 import pytest
 import torch
@@ -42,8 +40,8 @@ def _cancelling(fmt, w):
     return np.stack(out, -1)
 
 
-@pytest.mark.parametrize("fmt,qd", [("bf16", "bf16"), ("fp8", "bf16"), ("fp8", "fp16"), ("fp8_int4", "bf16"),
-                                    ("fp8_int4", "fp16")])
+@pytest.mark.parametrize("fmt,qd", [("fp16", "fp16"), ("bf16", "bf16"), ("fp8", "bf16"), ("fp8", "fp16"),
+                                    ("fp8_int4", "bf16"), ("fp8_int4", "fp16")])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("G,split", [(3, False), (3, True), (20, True)])
 def test_weights_are_held_in_32_bits(paged, fmt, qd, D, G, split):
@@ -79,3 +77,36 @@ def test_weights_are_held_in_32_bits(paged, fmt, qd, D, G, split):
     tol = (ref.UNIT[q.dtype] + 2.0 ** -20) * np.abs(want) + ref.TINY[q.dtype] + rel * spread
     err = np.abs(ref.f64(got)[:, :, 0] - want)
     assert (err <= tol).all(), f"error {(err / tol).max()} of the bound"
+
+
+@pytest.mark.parametrize("fmt,qd", [("fp16", "fp16"), ("bf16", "bf16"), ("fp8", "fp16"), ("fp8_int4", "bf16")])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,G", [(40, 4), (512, 4), (1500, 4), (1500, 20)])
+def test_a_token_above_the_others_whose_value_is_zero(paged, fmt, qd, D, n, G):
+    """A sink: it has nearly all of the weight and adds nothing, so that the
+    result is the others', whose weights are e^-10 and less of its own."""
+    above = [10.0, 14.0, 16.0, 18.0, 20.0, 24.0]  # nats, of each sequence's first token
+    B, H, page = len(above), 2, 16
+    P = -(-n // page)
+    g = torch.Generator().manual_seed(n + D + G)
+    k, v = torch.randn(B, H, n, D, generator=g), torch.randn(B, H, n, D, generator=g) * 2.0 ** 12
+    q = torch.randn(B, H * G, 1, D, generator=g)
+    k[..., 0] = 0.0
+    q[..., 0] = 4.0
+    k[:, :, 0] = 0.0
+    k[:, :, 0, 0] = torch.tensor(above)[:, None] * D ** 0.5 / 4.0
+    v[:, :, 0] = 0.0
+    layer = paged.PagedLayer(B * P, H, D, page, fmt)
+    table = torch.arange(B * P, dtype=torch.int32).view(B, P)
+    layer.write(k.cuda(), v.cuda(), table.cuda(), 0)
+    q = q.to(DTYPES[qd])
+    got, lse = layer.attend(q.cuda(), table.cuda(), torch.full((B,), n, dtype=torch.int32, device="cuda"),
+                            return_lse=True)
+    want, wlse, spread, ds = ref.attend(ref.f64(q)[:, :, 0], ref.page_values(layer), table.numpy(), [n] * B, page,
+                                        B * P, D ** -0.5)
+    tol = ref.attend_bound(want, spread, ds, [n] * B, q.dtype)
+    err = np.abs(ref.f64(got)[:, :, 0] - want)
+    # (24 nats leave results that end in the result type's smallest numbers)
+    assert np.abs(want[:3]).max(-1).min() > 1e3 * ref.TINY[q.dtype], "too small to see"
+    assert (err <= tol).all(), f"error {(err / tol).max()} of the bound"
+    assert (np.abs(ref.f64(lse) - wlse) <= 2 * ds + 2.0 ** -20 + 2.0 ** -22 * np.abs(wlse)).all()
