@@ -220,7 +220,7 @@ def calls():
             raise FkvLibraryError(f"cannot load {_HERE}/_fkv_calls.so: {e}; run `make -C foveated_kv_amd/csrc` "
                                   "or __graft_entry__.build()") from e
         _fkv_calls.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
-            "fkv_rope_apply", "fkv_paged_write", "fkv_paged_read", "fkv_paged_attn_workspace", "fkv_paged_attn")))
+            "fkv_rope_apply", "fkv_paged_write", "fkv_paged_read", "fkv_paged_attn_workspace", "fkv_paged_attn")), check)
         _calls = _fkv_calls
     return _calls
 

@@ -9,8 +9,11 @@
 //
 // Each function returns NotImplemented for whatever is not plain -- a wrong
 // argument, a tensor to be copied first, one of another GPU than the current
-// one, an error -- and has done nothing then: paged.py goes on with its own
-// checks, which raise or handle it.  So there is one place that words errors.
+// one -- and has done nothing then: paged.py goes on with its own checks, which
+// raise or handle it.  So there is one place that words refusals.  An entry
+// point that failed otherwise than by refusing its arguments may have started
+// work, which must not be done twice (rows rotated in place): that is raised
+// here, by _lib.py's check().
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -35,9 +38,15 @@ struct {
     decltype(&fkv_paged_attn_workspace) workspace;
     decltype(&fkv_paged_attn) attn;
 } lib;
+PyObject* check = nullptr;  // _lib.check(code, name), which raises
 
 // What a call meets that paged.py has to look at.
 struct NotPlain {};
+// An entry point's error that is not a refusal.
+struct Failed {
+    int code;
+    const char* name;
+};
 void need(bool ok) {
     if (!ok) throw NotPlain{};
 }
@@ -134,19 +143,29 @@ void* stream_of(int64_t index) {
     return (void*)c10::hip::getCurrentHIPStream((c10::DeviceIndex)index).stream();
 }
 
-// Runs f, which returns a new reference.
+// Runs f(begun), which checks a call's arguments, launches it and returns a new
+// reference.
 template <typename F>
 PyObject* plain(Py_ssize_t n, Py_ssize_t wanted, F f) {
+    bool begun = false;
     try {
-        if (n == wanted) return f();
-    } catch (...) {  // (paged.py meets the same, and words it)
-        PyErr_Clear();
+        if (n == wanted) return f(begun);
+    } catch (const Failed& e) {
+        PyObject* none = PyObject_CallFunction(check, "is", e.code, e.name);
+        Py_XDECREF(none);
+        return nullptr;
+    } catch (...) {
+        if (begun) {  // (no memory for the result's Python object)
+            if (!PyErr_Occurred()) PyErr_NoMemory();
+            return nullptr;
+        }
+        PyErr_Clear();  // (paged.py meets the same, and words it)
     }
     Py_RETURN_NOTIMPLEMENTED;
 }
 
 template <typename F>
-void launch(F f) {
+void launch(bool& begun, const char* name, F f) {
     struct Released {  // (other threads run while a full queue makes the launch wait)
         PyThreadState* state = PyEval_SaveThread();
         ~Released() { PyEval_RestoreThread(state); }
@@ -156,7 +175,9 @@ void launch(F f) {
         Released gil;
         rc = f();
     }
-    need(rc == FKV_OK);
+    need(rc != FKV_EINVAL);  // (arguments are refused before anything is done)
+    begun = true;
+    if (rc != FKV_OK) throw Failed{rc, name};
 }
 
 // A rotary table's (fkv_rope's address, GPU, head dim).
@@ -183,7 +204,7 @@ struct PagesKey {
 
 // rope(key, x, positions, out)
 PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return plain(n, 4, [&] {
+    return plain(n, 4, [&](bool& begun) {
         const RopeKey key(a[0]);
         void* stream = stream_of(key.index);
         const at::Tensor& x = tensor(a[1], key.index);
@@ -194,14 +215,16 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const fkv_rows src = rows(x);
         at::Tensor out = result(a[3], key.index, x, false);
         const fkv_rows dst = rows(out);
-        launch([&] { return lib.rope(key.rope, &src, &dst, dt, B, H, L, (int32_t)key.D, &pos, stream); });
+        launch(begun, "fkv_rope_apply", [&] {
+            return lib.rope(key.rope, &src, &dst, dt, B, H, L, (int32_t)key.D, &pos, stream);
+        });
         return THPVariable_Wrap(std::move(out));
     });
 }
 
 // write(key, k, v, table, start, n_new, q, rope's key, q_out)
 PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return plain(n, 9, [&]() -> PyObject* {
+    return plain(n, 9, [&](bool& begun) -> PyObject* {
         const PagesKey key(a[0]);
         const fkv_pages* pg = key.pages;
         void* stream = stream_of(key.index);
@@ -235,7 +258,7 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
         } else {
             need(a[8] == Py_None);
         }
-        launch([&] {
+        launch(begun, "fkv_paged_write", [&] {
             return lib.write(pg, &rk, &rv, dt, B, L, t.ids, t.n, t.stride, &start, n_new, rope, queries ? &rq : nullptr,
                              queries ? &ro : nullptr, Hq, stream);
         });
@@ -246,7 +269,7 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // read(key, table, lens, max_len, dtype)
 PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return plain(n, 5, [&] {
+    return plain(n, 5, [&](bool& begun) {
         const PagesKey key(a[0]);
         const fkv_pages* pg = key.pages;
         void* stream = stream_of(key.index);
@@ -262,7 +285,7 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int32_t dt = dtype_code(dtype);
         const auto options = THPVariable_Unpack(a[1]).options().dtype(dtype);
         at::Tensor k = at::empty({t.B, pg->H, S, pg->D}, options), v = at::empty({t.B, pg->H, S, pg->D}, options);
-        launch([&] {
+        launch(begun, "fkv_paged_read", [&] {
             return lib.read(pg, t.ids, t.n, t.stride, lens, t.B, S, k.data_ptr(), v.data_ptr(), dt, stream);
         });
         return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(k)), THPVariable_Wrap(std::move(v)));
@@ -271,7 +294,7 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // attend(key, query, table, lens, max_len, lens_add, scale, out, return_lse)
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return plain(n, 9, [&] {
+    return plain(n, 9, [&](bool& begun) {
         const PagesKey key(a[0]);
         const fkv_pages* pg = key.pages;
         void* stream = stream_of(key.index);
@@ -303,7 +326,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int64_t bytes = lib.workspace(pg, Hq, B, most);
         need(bytes >= 0);
         if (bytes) work = at::empty({bytes}, q.options().dtype(at::kByte));
-        launch([&] {
+        launch(begun, "fkv_paged_attn", [&] {
             return lib.attn(pg, &rq, dt, Hq, B, t.ids, t.n, t.stride, lens, lens_add, most, (float)scale, out.data_ptr(),
                             want_lse && lse.numel() ? (float*)lse.data_ptr() : nullptr, bytes ? work.data_ptr() : nullptr,
                             bytes, stream);
@@ -314,17 +337,20 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // bind(addresses of fkv_rope_apply, fkv_paged_write, fkv_paged_read,
-// fkv_paged_attn_workspace, fkv_paged_attn)
+// fkv_paged_attn_workspace, fkv_paged_attn; _lib.check)
 PyObject* bind(PyObject*, PyObject* args) {
     unsigned long long p[5];
-    if (!PyArg_ParseTuple(args, "KKKKK", p, p + 1, p + 2, p + 3, p + 4)) return nullptr;
+    PyObject* raise;
+    if (!PyArg_ParseTuple(args, "KKKKKO", p, p + 1, p + 2, p + 3, p + 4, &raise)) return nullptr;
+    Py_INCREF(raise);
+    Py_XSETREF(check, raise);
     lib = {(decltype(lib.rope))p[0], (decltype(lib.write))p[1], (decltype(lib.read))p[2],
            (decltype(lib.workspace))p[3], (decltype(lib.attn))p[4]};
     Py_RETURN_NONE;
 }
 
 PyMethodDef methods[] = {
-    {"bind", bind, METH_VARARGS, "addresses of libfkv's entry points"},
+    {"bind", bind, METH_VARARGS, "addresses of libfkv's entry points, _lib.check"},
     {"rope", (PyCFunction)(void (*)())rope, METH_FASTCALL, "Rope.__call__"},
     {"write", (PyCFunction)(void (*)())write, METH_FASTCALL, "PagedLayer.write"},
     {"read", (PyCFunction)(void (*)())read, METH_FASTCALL, "PagedLayer.read"},

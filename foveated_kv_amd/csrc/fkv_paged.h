@@ -62,6 +62,22 @@ __device__ inline int64_t page_row(const PageView& pg, const TableView& t, int64
 // 2^e of an exponent byte (e + 127).
 __device__ inline float exp_byte(uint32_t byte) { return __uint_as_float(byte << 23); }
 
+// Starts a kernel -> FKV_OK, or this launch's own error with nothing started.
+// (hipGetLastError() after a launch also reports, and clears, what an earlier
+// call of the program's left behind: a failure although the kernel runs.)
+template <typename T>
+struct AsDeclared {
+    using type = T;
+};
+template <typename... P>
+int start_kernel(const char* who, void (*kernel)(P...), dim3 grid, uint32_t threads, hipStream_t s,
+                 typename AsDeclared<P>::type... args) {
+    void* p[] = {&args...};
+    const hipError_t e = hipLaunchKernel((const void*)kernel, grid, dim3(threads), p, 0, s);
+    if (e != hipSuccess) (void)hipGetLastError();  // (reported here, not by the next one to ask)
+    return check_hip(e, who);
+}
+
 int check_pages(const char* who, const fkv_pages* p);
 int check_table(const char* who, const int32_t* table, int32_t n_table, int64_t stride, int32_t B);
 PageView page_view(const fkv_pages* p);

@@ -544,8 +544,8 @@ static int launch_write_f(WriteArgs& a, int64_t tokens, hipStream_t s) {
         const int64_t units = cdiv(tokens, 64 / (D / 8)) * (cdiv(a.Hq, N) + 2 * cdiv(a.pg.H, N));
         if (units > kMaxUnits) return too_many("fkv_paged_write");
         a.n_units = (uint32_t)units;
-        paged_write_kernel<D, DT, FMT, N, decltype(pairs)::value><<<(uint32_t)cdiv(a.n_units, 4), 256, 0, s>>>(a);
-        return check_hip(hipGetLastError(), "fkv_paged_write");
+        return start_kernel("fkv_paged_write", paged_write_kernel<D, DT, FMT, N, decltype(pairs)::value>,
+                            (uint32_t)cdiv(a.n_units, 4), 256, s, a);
     };
     if (tokens * heads <= kFewRows) return go(std::integral_constant<int, 1>{}, std::true_type{});
     if (a.rope.rot && !a.rope.interleaved) return go(std::integral_constant<int, 4>{}, std::true_type{});
@@ -563,11 +563,12 @@ static int launch_write(WriteArgs& a, int format, int64_t tokens, hipStream_t s)
 }
 
 template <int D, int FMT>
-static void launch_read(const ReadArgs& a, int dtype, uint32_t blocks, hipStream_t s) {
+static int launch_read(const ReadArgs& a, int dtype, uint32_t blocks, hipStream_t s) {
+    const char* w = "fkv_paged_read";
     switch (dtype) {
-        case FKV_F16: paged_read_kernel<D, FMT, FKV_F16><<<blocks, 256, 0, s>>>(a); break;
-        case FKV_BF16: paged_read_kernel<D, FMT, FKV_BF16><<<blocks, 256, 0, s>>>(a); break;
-        default: paged_read_kernel<D, FMT, FKV_F32><<<blocks, 256, 0, s>>>(a); break;
+        case FKV_F16: return start_kernel(w, paged_read_kernel<D, FMT, FKV_F16>, blocks, 256, s, a);
+        case FKV_BF16: return start_kernel(w, paged_read_kernel<D, FMT, FKV_BF16>, blocks, 256, s, a);
+        default: return start_kernel(w, paged_read_kernel<D, FMT, FKV_F32>, blocks, 256, s, a);
     }
 }
 
@@ -587,9 +588,8 @@ int fkv_rope_table(const double* frequencies, int32_t rot_dim, double factor, in
     Frequencies f = {};
     for (int i = 0; i < rot_dim / 2; i++) f.f[i] = frequencies[i];
     const int64_t n = (int64_t)n_positions * (rot_dim / 2);
-    rope_table_kernel<<<(uint32_t)std::min<int64_t>(cdiv(n, 256), 65536), 256, 0, (hipStream_t)stream>>>(
-        f, rot_dim / 2, factor, n, table);
-    return check_hip(hipGetLastError(), w.c_str());
+    return start_kernel(w.c_str(), rope_table_kernel, (uint32_t)std::min<int64_t>(cdiv(n, 256), 65536), 256,
+                        (hipStream_t)stream, f, rot_dim / 2, factor, n, table);
 }
 
 int fkv_rope_apply(const fkv_rope* rope, const fkv_rows* x, const fkv_rows* out, int32_t dtype, int32_t B,
@@ -614,9 +614,8 @@ int fkv_rope_apply(const fkv_rope* rope, const fkv_rows* x, const fkv_rows* out,
         constexpr int DT = decltype(dt)::value, N = decltype(n)::value;
         const int64_t units = (int64_t)B * L * cdiv(H, N * (int64_t)rpw);
         if (units > kMaxUnits) return too_many(w);
-        rope_kernel<DT, N, decltype(pairs)::value><<<(uint32_t)cdiv(units, 4), 256, 0, s>>>(
-            rows_view(x), rows_view(out), rv, pv, (uint32_t)units, H, L, lanes, rpw);
-        return check_hip(hipGetLastError(), w);
+        return start_kernel(w, rope_kernel<DT, N, decltype(pairs)::value>, (uint32_t)cdiv(units, 4), 256, s, rows_view(x),
+                            rows_view(out), rv, pv, (uint32_t)units, H, L, lanes, rpw);
     };
     auto by_rows = [&](auto dt) {
         if ((int64_t)B * H * L <= kFewRows) return go(dt, std::integral_constant<int, 1>{}, std::true_type{});
@@ -705,15 +704,14 @@ int fkv_paged_read(const fkv_pages* pages, const int32_t* table, int32_t n_table
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
         switch (pages->format) {
-            case FKV_PAGES_F16: launch_read<D, FKV_PAGES_F16>(a, out_dtype, blocks, s); break;
-            case FKV_PAGES_BF16: launch_read<D, FKV_PAGES_BF16>(a, out_dtype, blocks, s); break;
-            case FKV_PAGES_FP8: launch_read<D, FKV_PAGES_FP8>(a, out_dtype, blocks, s); break;
-            default: launch_read<D, FKV_PAGES_FP8_INT4>(a, out_dtype, blocks, s); break;
+            case FKV_PAGES_F16: return launch_read<D, FKV_PAGES_F16>(a, out_dtype, blocks, s);
+            case FKV_PAGES_BF16: return launch_read<D, FKV_PAGES_BF16>(a, out_dtype, blocks, s);
+            case FKV_PAGES_FP8: return launch_read<D, FKV_PAGES_FP8>(a, out_dtype, blocks, s);
+            default: return launch_read<D, FKV_PAGES_FP8_INT4>(a, out_dtype, blocks, s);
         }
     };
-    if (pages->D == 64) go(std::integral_constant<int, 64>{});
-    else go(std::integral_constant<int, 128>{});
-    return check_hip(hipGetLastError(), w);
+    if (pages->D == 64) return go(std::integral_constant<int, 64>{});
+    return go(std::integral_constant<int, 128>{});
 }
 
 }  // extern "C"

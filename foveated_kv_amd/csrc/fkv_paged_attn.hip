@@ -930,29 +930,30 @@ static int check_attn(const char* who, const fkv_pages* p, int32_t Hq, int32_t B
 }
 
 template <int D, int FMT, bool BF>
-static void launch_attn(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+static int launch_attn(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+    const char* w = "fkv_paged_attn";
     constexpr int threads = 64 * kAttnWaves;
-    if (!p.split) {
-        paged_attn_kernel<D, FMT, BF, kAttnWaves, false, 1><<<p.blocks, threads, 0, s>>>(a);
-        return;
-    }
+    if (!p.split)
+        return start_kernel(w, paged_attn_kernel<D, FMT, BF, kAttnWaves, false, 1>, p.blocks, threads, s, a);
+    auto kernel = paged_attn_kernel<D, FMT, BF, kAttnWaves, true, 1>;
     if constexpr (D == 128 || FMT <= FKV_PAGES_BF16) {
-        if (p.tiles == 2) paged_attn_kernel<D, FMT, BF, kAttnWaves, true, 2><<<p.blocks, threads, 0, s>>>(a);
+        if (p.tiles == 2) kernel = paged_attn_kernel<D, FMT, BF, kAttnWaves, true, 2>;
     }
-    if (p.tiles == 1) paged_attn_kernel<D, FMT, BF, kAttnWaves, true, 1><<<p.blocks, threads, 0, s>>>(a);
+    if (int e = start_kernel(w, kernel, p.blocks, threads, s, a)) return e;
     const int rows = (int)std::min<int64_t>(p.rows, 1024);
-    if (p.rows * p.GT <= 1024) paged_join_kernel<D, BF, 1><<<dim3(rows, p.GT), 256, 0, s>>>(a, (int)p.rows);
-    else paged_join_kernel<D, BF, 4><<<dim3(rows, (p.GT + 3) / 4), 256, 0, s>>>(a, (int)p.rows);
+    if (p.rows * p.GT <= 1024)
+        return start_kernel(w, paged_join_kernel<D, BF, 1>, dim3(rows, p.GT), 256, s, a, (int)p.rows);
+    return start_kernel(w, paged_join_kernel<D, BF, 4>, dim3(rows, (p.GT + 3) / 4), 256, s, a, (int)p.rows);
 }
 
 template <int D>
-static void launch_attn_d(const AttnArgs& a, const AttnPlan& p, int format, bool bf, hipStream_t s) {
-    if (format == FKV_PAGES_F16) launch_attn<D, FKV_PAGES_F16, false>(a, p, s);
-    else if (format == FKV_PAGES_BF16) launch_attn<D, FKV_PAGES_BF16, true>(a, p, s);
-    else if (format == FKV_PAGES_FP8 && bf) launch_attn<D, FKV_PAGES_FP8, true>(a, p, s);
-    else if (format == FKV_PAGES_FP8) launch_attn<D, FKV_PAGES_FP8, false>(a, p, s);
-    else if (bf) launch_attn<D, FKV_PAGES_FP8_INT4, true>(a, p, s);
-    else launch_attn<D, FKV_PAGES_FP8_INT4, false>(a, p, s);
+static int launch_attn_d(const AttnArgs& a, const AttnPlan& p, int format, bool bf, hipStream_t s) {
+    if (format == FKV_PAGES_F16) return launch_attn<D, FKV_PAGES_F16, false>(a, p, s);
+    if (format == FKV_PAGES_BF16) return launch_attn<D, FKV_PAGES_BF16, true>(a, p, s);
+    if (format == FKV_PAGES_FP8 && bf) return launch_attn<D, FKV_PAGES_FP8, true>(a, p, s);
+    if (format == FKV_PAGES_FP8) return launch_attn<D, FKV_PAGES_FP8, false>(a, p, s);
+    if (bf) return launch_attn<D, FKV_PAGES_FP8_INT4, true>(a, p, s);
+    return launch_attn<D, FKV_PAGES_FP8_INT4, false>(a, p, s);
 }
 
 }  // namespace fkv
@@ -1007,9 +1008,8 @@ int fkv_paged_attn(const fkv_pages* pages, const fkv_rows* query, int32_t q_dtyp
     a.GT = p.GT;
     a.scale = scale * 1.4426950408889634f;
     const bool bf = q_dtype == FKV_BF16;
-    if (pages->D == 64) launch_attn_d<64>(a, p, pages->format, bf, (hipStream_t)stream);
-    else launch_attn_d<128>(a, p, pages->format, bf, (hipStream_t)stream);
-    return check_hip(hipGetLastError(), w);
+    if (pages->D == 64) return launch_attn_d<64>(a, p, pages->format, bf, (hipStream_t)stream);
+    return launch_attn_d<128>(a, p, pages->format, bf, (hipStream_t)stream);
 }
 
 }  // extern "C"
