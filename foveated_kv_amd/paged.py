@@ -140,7 +140,7 @@ def _index_of(device):
 def _frequencies(rot_dim, base, scaling):
     """Angle per position of each pair in 64 bits, and the factor that cos and
     sin carry."""
-    i = torch.arange(rot_dim // 2, dtype=torch.float64)
+    i = torch.arange(rot_dim // 2, dtype=torch.float64, device="cpu")  # (whose numbers the library reads on the host)
     inv = base ** (-2.0 * i / rot_dim)
     if scaling is None:
         return inv, 1.0
@@ -221,7 +221,7 @@ class Rope:
             _call(device.index, "fkv_rope_table", inv.data_ptr(), self.rot_dim, factor, self.max_positions,
                   self.table.data_ptr())
         else:  # (to look at: calls take tables on a GPU)
-            a = torch.arange(self.max_positions, dtype=torch.float64)[:, None] * inv
+            a = torch.arange(self.max_positions, dtype=torch.float64, device="cpu")[:, None] * inv
             self.table[:, 0], self.table[:, 1] = a.cos() * factor, a.sin() * factor
         c = _lib.RopeC(self.table.data_ptr(), self.max_positions, self.rot_dim, int(self.interleaved))
         self._c, self._index = ctypes.byref(c), self.table.get_device()
