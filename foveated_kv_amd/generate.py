@@ -330,9 +330,11 @@ class PagedCacheWrapper:
 
     ``update_and_fetch`` with several tokens (prefill) stores them and hands
     back every key (rotated, where the cache rotates) and value for the
-    original attention; with one token it leaves the write to the attention
-    call that follows, which rotates the query in the same launch and attends
-    to every stored token (``attn_mask`` is not looked at)."""
+    original attention, whose mask is the model's: query l of sequence b stands
+    at position start(b) + l of the rows handed back, of which those past the
+    sequence's tokens are zeros or padding.  With one token it leaves the write
+    to the attention call that follows, which rotates the query in the same
+    launch and attends to every stored token (``attn_mask`` is not looked at)."""
 
     def __init__(self, cache, layer_idx, seqs=None):
         self.cache, self.layer_idx, self.seqs = cache, layer_idx, cache.pages._range(seqs)
@@ -350,15 +352,17 @@ class PagedCacheWrapper:
                                "F.scaled_dot_product_attention after each update_and_fetch")
         if _paged_state["original"] is None:
             raise RuntimeError("paged attention is not installed")
-        _paged_state["pending"] = self
-        self._n_new = keys.shape[2]
-        if self._n_new == 1:
-            self._new = keys, values
-            return keys, values
-        self.cache.write(self.layer_idx, keys, values, seqs=self.seqs)
-        if self.offset == 0:
-            return (keys if self.rope is None else self.rope(keys, 0)), values
-        return self.cache.read(self.layer_idx, self.seqs, keys.dtype)
+        fetched, n = (keys, values), keys.shape[2]
+        if n == 1:
+            self._new = fetched
+        else:
+            self.cache.write(self.layer_idx, keys, values, seqs=self.seqs)
+            if any(self.cache.pages.starts(self.seqs)):
+                fetched = self.cache.read(self.layer_idx, self.seqs, keys.dtype)
+            elif self.rope is not None:
+                fetched = self.rope(keys, 0), values
+        self._n_new, _paged_state["pending"] = n, self
+        return fetched
 
     def _answer(self, query, scale):
         keys, values = self._new

@@ -34,3 +34,47 @@ def test_a_cuda_default_device(paged):
     with torch.device("cuda"):
         got = run()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_chunk_for_sequences_of_different_lengths(paged):
+    """A follow-up of five tokens for a sequence of 20 and a new one: what the
+    model gets back is what each sequence gets alone."""
+    from foveated_kv_amd import generate
+
+    H, D, first, more = 2, 64, [20, 0], 5
+    rope = paged.Rope(D, max_positions=64)
+    g = torch.Generator().manual_seed(3)
+    k, v, q = (torch.randn(2, h, 25, D, generator=g).half().cuda() for h in (H, H, 2 * H))
+    seen = []
+
+    def attention(query, key, value, **kw):
+        seen.append((query, key, value))
+        return query
+
+    def run(seqs):
+        """The chunk of these sequences, each behind its own beginning."""
+        cache = paged.PagedKVCache(1, H, D, n_pages=8, max_seqs=len(seqs), max_tokens=64, page_size=16, rope=rope)
+        for i, b in enumerate(seqs):
+            if first[b]:
+                cache.extend(first[b], slice(i, i + 1))
+                cache.write(0, k[b:b + 1, :, :first[b]], v[b:b + 1, :, :first[b]], seqs=slice(i, i + 1))
+        part = [torch.cat([t[b:b + 1, :, first[b]:first[b] + more] for b in seqs]) for t in (k, v, q)]
+        w, = generate.install_paged_attention(cache)
+        generate._paged_state["original"], original = attention, generate._paged_state["original"]
+        try:
+            cache.extend(more)
+            kk, vv = w.update_and_fetch(*part[:2])
+            torch.nn.functional.scaled_dot_product_attention(part[2], kk, vv)
+        finally:
+            generate._paged_state["original"] = original
+            generate.uninstall_paged_attention()
+        return seen.pop()
+
+    both = run([0, 1])
+    assert both[1].shape == (2, H, 25, D)
+    for b in (0, 1):
+        n = first[b] + more
+        alone = run([b])
+        assert torch.equal(both[0][b], alone[0][0])
+        for t, a in zip(both[1:], alone[1:]):
+            assert torch.equal(t[b, :, :n], a[0]) and not bool(t[b, :, n:].any())
