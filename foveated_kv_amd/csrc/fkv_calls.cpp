@@ -321,6 +321,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
             out = result(a[7], key.index, q, false);
             need(out.is_contiguous() && !((uintptr_t)out.data_ptr() & 15));
         }
+        need(PyBool_Check(a[8]));
         const bool want_lse = a[8] == Py_True;
         if (want_lse) lse = at::empty({B, Hq}, q.options().dtype(at::kFloat));
         const int64_t bytes = lib.workspace(pg, Hq, B, most);

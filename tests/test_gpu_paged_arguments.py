@@ -1,5 +1,6 @@
 """What the paged cache's calls take and refuse beside plain arguments (GPU)."""
 
+import numpy as np
 import pytest
 import torch
 
@@ -78,3 +79,14 @@ def test_a_chunk_for_sequences_of_different_lengths(paged):
         assert torch.equal(both[0][b], alone[0][0])
         for t, a in zip(both[1:], alone[1:]):
             assert torch.equal(t[b, :, :n], a[0]) and not bool(t[b, :, n:].any())
+
+
+@pytest.mark.parametrize("yes,no", [(True, False), (1, 0), (np.True_, np.False_), ("yes", None)])
+def test_return_lse_by_its_truth(paged, yes, no):
+    layer = paged.PagedLayer(2, 1, 64, 16, "fp16")
+    table = torch.arange(2, dtype=torch.int32, device="cuda").view(2, 1)
+    lens = torch.full((2,), 9, dtype=torch.int32, device="cuda")
+    q = torch.ones(2, 4, 1, 64, dtype=torch.float16, device="cuda")
+    out, lse = layer.attend(q, table, lens, return_lse=yes)
+    assert out.shape == q.shape and lse.shape == (2, 4)
+    assert torch.equal(layer.attend(q, table, lens, return_lse=no), out)
