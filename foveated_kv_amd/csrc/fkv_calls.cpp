@@ -64,11 +64,12 @@ int32_t int32_of(int64_t v) {
     return (int32_t)v;
 }
 
-// A tensor proper on GPU `index` that wants no gradient.
+// A tensor proper on GPU `index` that wants no gradient and has no tangent.
 const at::Tensor& tensor(PyObject* o, int64_t index) {
     need(THPVariable_CheckExact(o));
     const at::Tensor& t = THPVariable_Unpack(o);
-    need(t.is_cuda() && t.layout() == at::kStrided && t.get_device() == index && !t.requires_grad());
+    need(t.is_cuda() && t.layout() == at::kStrided && t.get_device() == index && !t.requires_grad() &&
+         !t._fw_grad(0).defined());
     return t;
 }
 

@@ -27,6 +27,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, dtype_code, ptr
@@ -48,7 +49,8 @@ _pack_positions = struct.Struct("Pqqqii").pack
 # ---------------------------------------------------------------------------
 
 def _on(index, name, t):
-    """Refuses what is not a tensor on GPU ``index``, or wants a gradient."""
+    """Refuses what is not a tensor on GPU ``index``, wants a gradient or
+    carries a forward-mode tangent."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.get_device() != index:
@@ -57,6 +59,8 @@ def _on(index, name, t):
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires grad: this package is for inference and records nothing for autograd "
                            "(call it under torch.no_grad())")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{name} has a forward-mode tangent: this package is for inference and would drop it")
 
 
 _raw_stream, _current_gpu = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice

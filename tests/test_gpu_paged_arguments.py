@@ -90,3 +90,20 @@ def test_return_lse_by_its_truth(paged, yes, no):
     out, lse = layer.attend(q, table, lens, return_lse=yes)
     assert out.shape == q.shape and lse.shape == (2, 4)
     assert torch.equal(layer.attend(q, table, lens, return_lse=no), out)
+
+
+def test_a_forward_tangent_is_refused(paged):
+    from torch.autograd import forward_ad
+
+    rope, layer = paged.Rope(64, max_positions=8), paged.PagedLayer(1, 1, 64, 16, "fp16")
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    lens = torch.ones(1, dtype=torch.int32, device="cuda")
+    x = torch.ones(1, 1, 1, 64, dtype=torch.float16, device="cuda")
+    with forward_ad.dual_level(), torch.no_grad():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: rope(d), lambda: rope(x, out=d), lambda: layer.write(d, x, table, 0),
+                     lambda: layer.write(x, x, table, 0, q=d), lambda: layer.attend(d, table, lens)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+        assert torch.equal(rope(x, 0), x)
+    assert bool((layer.k == 0).all())

@@ -68,3 +68,13 @@ def test_a_failed_update_leaves_nothing_pending():
         torch.nn.functional.scaled_dot_product_attention(kv[:, :, :2], kv, kv)  # (another attention)
     finally:
         generate.uninstall_paged_attention()
+
+
+def test_a_forward_tangent_is_refused():
+    from torch.autograd import forward_ad
+
+    x = torch.zeros(1, 2, 3, 64)
+    with forward_ad.dual_level():
+        paged._on(-1, "x", x)
+        with pytest.raises(RuntimeError, match="tangent"):
+            paged._on(-1, "x", forward_ad.make_dual(x, torch.ones_like(x)))
