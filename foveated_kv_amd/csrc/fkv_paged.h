@@ -78,6 +78,18 @@ int start_kernel(const char* who, void (*kernel)(P...), dim3 grid, uint32_t thre
     return check_hip(e, who);
 }
 
+// Rows of a call: (B, H, L) of D elements of es bytes.
+struct RowsShape {
+    int64_t B, H, L, D, es;
+};
+// Refuses a result whose rows share memory with one another, or with rows that
+// the call reads elsewhere.  Rows that are the very ones read (the same address
+// and strides) may be written, each by the lanes that read it.  (k and the like:
+// NULL for none, `in_place` whether those may be the result's own.)
+int check_result_rows(const char* who, const char* name, const fkv_rows* out, const RowsShape& shape);
+int check_apart(const char* who, const char* what, const fkv_rows* out, const RowsShape& out_shape, const fkv_rows* in,
+                const RowsShape& in_shape, bool in_place);
+
 int check_pages(const char* who, const fkv_pages* p);
 int check_table(const char* who, const int32_t* table, int32_t n_table, int64_t stride, int32_t B);
 PageView page_view(const fkv_pages* p);

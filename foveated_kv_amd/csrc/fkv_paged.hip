@@ -9,6 +9,7 @@
 #pragma clang fp contract(off)
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -499,6 +500,97 @@ static int check_rows(const std::string& w, const fkv_rows* r) {
     return FKV_OK;
 }
 
+// One dimension of the difference of two rows' addresses: k * stride for a k of
+// [lo, hi].
+struct Steps {
+    int64_t stride, lo, hi;
+};
+
+// Whether numbers k of the steps [i, n) bring `from` (elements) within D of 0;
+// with `moved` false, numbers that are not all 0.  `left` bounds the search, and
+// the answer is yes where it ends: strides are nested in any layout of a tensor,
+// which leaves two or three k of each dimension to look at.
+static bool can_meet(const Steps* st, int n, int i, int64_t from, int64_t D, bool moved, int& left) {
+    if (i == n) return moved && from < D && -from < D;
+    if (--left <= 0) return true;
+    int64_t reach = D - 1;
+    for (int j = i + 1; j < n; j++) reach += st[j].stride * std::max(-st[j].lo, st[j].hi);
+    const Steps s = st[i];
+    // |from + k stride| <= reach
+    const int64_t lo = std::max(s.lo, -((from + reach) / s.stride)), hi = std::min(s.hi, (reach - from) / s.stride);
+    for (int64_t k = lo; k <= hi; k++)
+        if (can_meet(st, n, i + 1, from + k * s.stride, D, moved || k != 0, left)) return true;
+    return false;
+}
+
+static bool can_meet(Steps* st, int n, int64_t from, int64_t D, bool moved) {
+    int m = 0;
+    for (int i = 0; i < n; i++) {
+        Steps s = st[i];
+        if (s.stride < 0) s = Steps{-s.stride, -s.hi, -s.lo};
+        if (s.lo == 0 && s.hi == 0) continue;
+        if (s.stride == 0) {
+            moved = true;
+            continue;
+        }
+        st[m++] = s;
+    }
+    std::sort(st, st + m, [](const Steps& a, const Steps& b) { return a.stride > b.stride; });
+    int left = 4096;
+    return can_meet(st, m, 0, from, D, moved, left);
+}
+
+// Whether strides are nested: each passes all that the smaller ones cover, as in
+// any slice of a tensor.  (Found without a division, which each call would notice.)
+static bool nested(const fkv_rows* r, const RowsShape& s) {
+    int64_t stride[3] = {r->stride_b, r->stride_h, r->stride_l}, n[3] = {s.B, s.H, s.L};
+    auto order = [&](int i, int j) {
+        if (stride[i] < stride[j]) std::swap(stride[i], stride[j]), std::swap(n[i], n[j]);
+    };
+    order(0, 1), order(1, 2), order(0, 1);
+    int64_t covered = s.D;
+    for (int d = 2; d >= 0; d--) {
+        if (n[d] > 1 && stride[d] < covered) return false;
+        covered += n[d] > 1 ? (n[d] - 1) * stride[d] : 0;
+    }
+    return true;
+}
+
+int check_result_rows(const char* who, const char* name, const fkv_rows* out, const RowsShape& s) {
+    if (nested(out, s)) return FKV_OK;
+    Steps st[3] = {{out->stride_b, 1 - s.B, s.B - 1}, {out->stride_h, 1 - s.H, s.H - 1}, {out->stride_l, 1 - s.L, s.L - 1}};
+    if (!can_meet(st, 3, 0, s.D, false)) return FKV_OK;
+    return set_error(std::string(who) + ": rows of " + name + " share memory");
+}
+
+int check_apart(const char* who, const char* what, const fkv_rows* out, const RowsShape& o, const fkv_rows* in,
+                const RowsShape& r, bool in_place) {
+    const int64_t so[3] = {out->stride_b, out->stride_h, out->stride_l}, no[3] = {o.B, o.H, o.L},
+                  si[3] = {in->stride_b, in->stride_h, in->stride_l}, ni[3] = {r.B, r.H, r.L};
+    int64_t lo = 0, hi = 0, first = 0, last = 0;  // elements that each covers, from its address on
+    bool same = in_place && out->data == in->data;
+    for (int d = 0; d < 3; d++) {
+        (so[d] < 0 ? lo : hi) += (no[d] - 1) * so[d];
+        (si[d] < 0 ? first : last) += (ni[d] - 1) * si[d];
+        same = same && no[d] == ni[d] && (no[d] == 1 || so[d] == si[d]);
+    }
+    const int64_t bytes = (const char*)out->data - (const char*)in->data;
+    if (same || bytes + (hi + o.D) * o.es <= first * o.es || (last + r.D) * o.es <= bytes + lo * o.es) return FKV_OK;
+    const int64_t from = bytes / o.es;
+    Steps st[6];
+    int n = 0;
+    for (int d = 0; d < 3; d++) {
+        if (so[d] == si[d]) {
+            st[n++] = Steps{so[d], 1 - ni[d], no[d] - 1};
+        } else {
+            st[n++] = Steps{so[d], 0, no[d] - 1};
+            st[n++] = Steps{si[d], 1 - ni[d], 0};
+        }
+    }
+    if (!can_meet(st, n, from, o.D, true)) return FKV_OK;
+    return set_error(std::string(who) + ": " + what + " share memory");
+}
+
 static RowsView rows_view(const fkv_rows* r) {
     return RowsView{(char*)r->data, r->stride_b, r->stride_h, r->stride_l};
 }
@@ -606,6 +698,9 @@ int fkv_rope_apply(const fkv_rope* rope, const fkv_rows* x, const fkv_rows* out,
     if (n >= 2147483648.0) return set_error(std::string(w) + ": more than 2^31 rows");
     if (int e = check_rows(w, x)) return e;
     if (int e = check_rows(w, out)) return e;
+    const RowsShape shape{B, H, L, D, dtype == FKV_F32 ? 4 : 2};
+    if (int e = check_result_rows(w, "out", out, shape)) return e;
+    if (int e = check_apart(w, "out, which is not x, and x", out, shape, x, shape, true)) return e;
     const uint32_t lanes = D / 8, rpw = 64 / lanes;
     const RopeView rv{rope->table, rope->n_positions, rope->rot_dim, rope->interleaved};
     const PositionsView pv = positions_view(positions);
@@ -651,6 +746,11 @@ int fkv_paged_write(const fkv_pages* pages, const fkv_rows* k, const fkv_rows* v
     if (q) {
         if (int e = check_rows(w, q)) return e;
         if (int e = check_rows(w, q_out)) return e;
+        const RowsShape sq{B, Hq, L, pages->D, dtype == FKV_F32 ? 4 : 2}, sk{B, pages->H, L, pages->D, sq.es};
+        if (int e = check_result_rows(w, "q_out", q_out, sq)) return e;
+        if (int e = check_apart(w, "q_out, which is not q, and q", q_out, sq, q, sq, true)) return e;
+        if (int e = check_apart(w, "q_out and k", q_out, sq, k, sk, false)) return e;
+        if (int e = check_apart(w, "q_out and v", q_out, sq, v, sk, false)) return e;
     }
     WriteArgs a;
     a.pg = page_view(pages);

@@ -989,6 +989,9 @@ int fkv_paged_attn(const fkv_pages* pages, const fkv_rows* query, int32_t q_dtyp
         return set_error(std::string(w) + ": workspace of " + std::to_string(p.bytes) + " bytes needed");
     if (p.rows * (cdiv((int64_t)n_table * pages->page_size, 32 * kAttnWaves) + 1) > 0x7FFFFFFF)
         return set_error(std::string(w) + ": the tables hold more than 2^31 tiles of 128 tokens over all heads");
+    const RowsShape heads{B, Hq, 1, pages->D, 2};
+    const fkv_rows result{out, (int64_t)Hq * pages->D, pages->D, 0};
+    if (int e = check_apart(w, "out, which is not the query, and the query", &result, heads, query, heads, true)) return e;
     AttnArgs a;
     a.pg = page_view(pages);
     a.table = TableView{table, table_stride, n_table};

@@ -233,7 +233,8 @@ class Rope:
 
     def __call__(self, x, positions=0, out=None):
         """x (B, H, L, head_dim) fp16 / bf16 / fp32, any strides -> the rotated
-        rows, in ``out`` (may be x itself; else a new tensor like x).
+        rows, in ``out`` (may be x itself, and shares no memory with it
+        otherwise; default a new tensor like x).
         ``positions``: a number or one-element tensor (the first token's
         position), a (B,) tensor (each sequence's first token's) or (B, L) /
         (1, L) (every token's); int32 or int64 tensors on the device, read
@@ -359,8 +360,8 @@ class PagedLayer:
         sequence (``start``: a number, a one-element tensor or (B,), int32 or
         int64 on the device).  Keys, and the queries q (B, Hq, L, D) of the
         same dtype where given, are rotated by ``rope`` first; returns the
-        rotated queries (``q_out``, which may be q, else a new tensor), or
-        None without q.
+        rotated queries (``q_out``, which may be q, and shares no memory with
+        q, k or v otherwise; default a new tensor), or None without q.
 
         ``n_new`` (B,) int32 on the device: only the first n_new[b] tokens of
         sequence b are real; the rest of a padded batch is not stored, and
@@ -443,7 +444,8 @@ class PagedLayer:
         fp32 of each head's sum of exponentials (by which several such results
         are joined).  A sequence without tokens gives zeros and -inf.
 
-        ``max_len`` is an upper bound of the lengths if the host knows one
+        ``out`` may be the query where that is contiguous.  ``max_len`` is an
+        upper bound of the lengths if the host knows one
         (default: the table's width); it decides how the work is split, not
         what is attended to.  ``scale`` defaults to D^-1/2."""
         done = _lib.calls().attend(self._key, query, table, lens, max_len, lens_add, scale, out, return_lse)

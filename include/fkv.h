@@ -637,7 +637,9 @@ int fkv_rope_table(const double* frequencies, int32_t rot_dim, double factor, in
                    void* stream);
 
 /* out = rotated x, rows (B, H, L) of D elements (D a multiple of 8 from
- * 16 to 512) of dtype; out may be x.  Asynchronous, capturable. */
+ * 16 to 512) of dtype; out may be x (the same address and strides), and else
+ * shares no memory with it, nor its rows with one another.  Asynchronous,
+ * capturable. */
 int fkv_rope_apply(const fkv_rope* rope, const fkv_rows* x, const fkv_rows* out, int32_t dtype, int32_t B,
                    int32_t H, int32_t L, int32_t D, const fkv_positions* positions, void* stream);
 
@@ -648,9 +650,9 @@ int fkv_rope_apply(const fkv_rope* rope, const fkv_rows* x, const fkv_rows* out,
  * n_new (B) int32 in device memory, or NULL: the tokens l < n_new[b] alone.
  * A token whose position lies outside the table, or whose page id lies
  * outside the pool, is not stored.  q, q_out (both or neither; rows (B, Hq, L)
- * of the same dtype, q_out may be q): queries rotated by the same
- * positions, or copied without rope; those past n_new are not written.  Two
- * tokens of one call must not name the same row.  Asynchronous, capturable. */
+ * of the same dtype, q_out may be q, and else shares no memory with q, k or
+ * v): queries rotated by the same positions, or copied without rope; those past
+ * n_new are not written.  Two tokens of one call must not name the same row.  Asynchronous, capturable. */
 int fkv_paged_write(const fkv_pages* pages, const fkv_rows* k, const fkv_rows* v, int32_t dtype, int32_t B,
                     int32_t L, const int32_t* table, int32_t n_table, int64_t table_stride,
                     const fkv_positions* start, const int32_t* n_new, const fkv_rope* rope, const fkv_rows* q,
@@ -667,7 +669,8 @@ int fkv_paged_read(const fkv_pages* pages, const int32_t* table, int32_t n_table
 /* Attention of one new token per sequence over its first lens[b] + lens_add
  * cached tokens (clamped to [0, n_table * page_size]): query rows (B, Hq) of
  * q_dtype (fp16 or bf16, the pages' own for the 16-bit formats; stride_l is
- * not read), out (B, Hq, D) contiguous of the same type, lse (B, Hq) fp32 or
+ * not read), out (B, Hq, D) contiguous of the same type (it may be the query,
+ * if that is contiguous, and else shares no memory with it), lse (B, Hq) fp32 or
  * NULL: the natural logarithm of each head's sum of exp(scale * score).  Query
  * heads [h * Hq/H, (h + 1) * Hq/H) attend to KV head h.  No tokens: out 0,
  * lse -inf.  Tokens of a page id outside the pool take no part.  max_len: an

@@ -107,3 +107,96 @@ def test_a_forward_tangent_is_refused(paged):
                 call()
         assert torch.equal(rope(x, 0), x)
     assert bool((layer.k == 0).all())
+
+
+def _elements(t):
+    """Storage offsets of a view's elements."""
+    at = torch.zeros((), dtype=torch.int64) + t.storage_offset()
+    for n, s in zip(t.shape, t.stride()):
+        at = at[..., None] + torch.arange(n) * s
+    return at.flatten()
+
+
+def test_rows_that_share_memory(paged):
+    """Random views of one buffer, read and written: refused where some element
+    is in two rows (found here by listing them) unless the views are the same,
+    and right where not."""
+    import random
+
+    from foveated_kv_amd import _lib
+
+    D, rng, counts = 16, random.Random(11), {"same": 0, "apart": 0, "meet": 0}
+    rope = paged.Rope(D, max_positions=64)
+    table = rope.table.cpu().double()
+    buf = torch.zeros(4096, dtype=torch.float32, device="cuda")
+
+    def view(shape):
+        kind = rng.choice(["nested", "nested", "any"])
+        if kind == "any":
+            strides = [8 * rng.randint(0, 20) for _ in shape]
+        else:
+            strides, order, s = [0] * 3, rng.sample(range(3), 3), D + 8 * rng.choice([0, 0, 1, 4])
+            for d in order:
+                strides[d] = s
+                s = s * shape[d] + 8 * rng.choice([0, 0, 2])
+        at = 8 * rng.randint(0, 60)
+        if at + sum((n - 1) * s for n, s in zip(shape, strides)) + D > buf.numel():
+            return view(shape)
+        return torch.as_strided(buf, (*shape, D), (*strides, 1), at)
+
+    for _ in range(400):
+        shape = [rng.randint(1, 4) for _ in range(3)]
+        x = view(shape)
+        out = x if rng.random() < 0.2 else torch.as_strided(buf, x.shape, x.stride(), 8 * rng.randint(0, 60)) \
+            if rng.random() < 0.5 and _elements(x).max() + 480 < buf.numel() else view(shape)
+        ex, eo = _elements(x), _elements(out)
+        inside = len(set(eo.tolist())) < len(eo)
+        same = out.data_ptr() == x.data_ptr() and all(n == 1 or s == t for n, s, t in zip(shape, out.stride(), x.stride()))
+        meet = inside or (not same and bool(torch.isin(eo, ex).any()))
+        counts["meet" if meet else "same" if same else "apart"] += 1
+        buf.copy_(torch.arange(4096))
+        before = x.cpu().double()
+        if meet:
+            with pytest.raises((ValueError, _lib.FkvLibraryError), match="share memory"):
+                rope(x, 3, out=out)
+            assert torch.equal(buf, torch.arange(4096, device="cuda", dtype=torch.float32))
+            continue
+        rope(x, 3, out=out)
+        c, s = (t[3:3 + shape[2]] for t in (table[:, 0], table[:, 1]))
+        a, b = before[..., :D // 2], before[..., D // 2:]
+        want = torch.cat([a * c - b * s, b * c + a * s], -1)
+        # (one rounding to fp32 of a 64-bit sum of numbers up to 4096)
+        assert bool(((out.cpu().double() - want).abs() <= 2.0 ** -24 * want.abs() + 2.0 ** -38).all())
+    assert min(counts.values()) >= 40, counts
+
+
+def test_heads_of_one_projection_in_place(paged):
+    """q, k and v as one projection leaves them, interleaved in one buffer:
+    nothing is shared, and q is rotated where it lies."""
+    B, L, Hq, H, D = 2, 7, 4, 2, 64
+    g = torch.Generator().manual_seed(1)
+    for layout in ("blhd", "bhld"):
+        x = torch.randn(B, L, Hq + 2 * H, D, generator=g).half().cuda()
+        if layout == "bhld":
+            x = x.transpose(1, 2).contiguous().transpose(1, 2)
+        q, k, v = (t.transpose(1, 2) for t in x.split([Hq, H, H], 2))
+        rope, want = paged.Rope(D, max_positions=32), x.clone()
+        layers = [paged.PagedLayer(B, H, D, 16, "fp16") for _ in range(2)]
+        table = torch.arange(B, dtype=torch.int32, device="cuda").view(B, 1)
+        qr = layers[0].write(k.clone(), v.clone(), table, 3, q=q.clone(), rope=rope)
+        assert layers[1].write(k, v, table, 3, q=q, q_out=q, rope=rope) is q
+        assert torch.equal(q, qr) and torch.equal(x[:, :, Hq:], want[:, :, Hq:])
+        assert torch.equal(layers[0].k, layers[1].k) and torch.equal(layers[0].v, layers[1].v)
+
+
+def test_attention_in_the_place_of_its_query(paged):
+    layer = paged.PagedLayer(80, 2, 64, 16, "bf16")
+    g = torch.Generator().manual_seed(2)
+    layer.k.copy_(torch.randn(layer.k.shape, generator=g))
+    layer.v.copy_(torch.randn(layer.v.shape, generator=g))
+    q = torch.randn(2, 80, 1, 64, generator=g).bfloat16().cuda()
+    table = torch.arange(80, dtype=torch.int32, device="cuda").view(2, 40)
+    for n in (0, 100, 640):  # none, whole, split with two tiles of heads
+        lens = torch.tensor([n, n // 2], dtype=torch.int32, device="cuda")
+        want, x = layer.attend(q, table, lens), q.clone()
+        assert torch.equal(layer.attend(x, table, lens, out=x), want) and torch.equal(x, want)

@@ -1,9 +1,11 @@
 """What the paged cache's calls take and refuse beside plain arguments (CPU)."""
 
+import ctypes
+
 import pytest
 import torch
 
-from foveated_kv_amd import Rope, paged
+from foveated_kv_amd import Rope, _lib, paged
 from test_paged import SCALINGS
 
 
@@ -78,3 +80,45 @@ def test_a_forward_tangent_is_refused():
         paged._on(-1, "x", x)
         with pytest.raises(RuntimeError, match="tangent"):
             paged._on(-1, "x", forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+# ---------------------------------------------------------------------------
+# rows that share memory (entry points refuse them before any launch)
+# ---------------------------------------------------------------------------
+
+def _entry(name, *args):
+    lib = _lib.load()
+    rc = getattr(lib, name)(*args)
+    assert rc == _lib.FKV_EINVAL, rc
+    return lib.fkv_last_error().decode()
+
+
+def _rows(at, sb, sh, sl):
+    return ctypes.byref(_lib.RowsC(at, sb, sh, sl))
+
+
+def test_results_that_share_memory_are_refused():
+    """B, H, L, D = 2, 3, 4, 64 of fp16; addresses and strides in one buffer
+    that is never touched."""
+    at = 1 << 20
+    rope = ctypes.byref(_lib.RopeC(at, 4, 64, 0))
+    pos = ctypes.byref(_lib.PositionsC(None))
+    x = (at, 768, 256, 64)
+    for out, word in [((at, 768, 256, 0), "rows of out"), ((at, 768, 256, 56), "rows of out"), ((at, 512, 256, 64), "rows of out"),
+                      ((at, 256, 256, 64), "rows of out"), ((at, 768, 256, -32), "rows of out"),
+                      ((at + 128, *x[1:]), "out, which is not x"), ((at + 16, *x[1:]), "out, which is not x"),
+                      ((at - 2 * 704, *x[1:]), "out, which is not x"), ((at, 768, 64, 192), "out, which is not x"),
+                      ((at + 2 * 1472, 64, 128, 512), "out, which is not x"), ((at + 384, 768, 256, -64), "out, which is not x")]:
+        msg = _entry("fkv_rope_apply", rope, _rows(*x), _rows(*out), 0, 2, 3, 4, 64, pos, None)
+        assert word in msg and "share memory" in msg, (out, msg)
+    pages = ctypes.byref(_lib.PagesC(at, at, None, None, 2, 16, 3, 64, 0))
+    far = (at + (1 << 18), 768, 256, 64)
+    for q, q_out, k, v, word in [(x, (at + 128, *x[1:]), far, far, "q_out, which is not q"), (x, x, x, far, "q_out and k"),
+                                 (x, x, far, x, "q_out and v"), (far, x, (at + 2 * 768, *x[1:]), far, "q_out and k"),
+                                 (far, (at, 768, 256, 32), far, far, "rows of q_out")]:
+        msg = _entry("fkv_paged_write", pages, _rows(*k), _rows(*v), 0, 2, 4, at, 1, 1, pos, None, None, _rows(*q),
+                     _rows(*q_out), 3, None)
+        assert word in msg and "share memory" in msg, (word, msg)
+    for q, out in [((at, 192, 64, 0), at + 128), ((at, 384, 128, 0), at), ((at, 192, 64, 0), at - 2 * 320)]:
+        msg = _entry("fkv_paged_attn", pages, _rows(*q), 0, 3, 2, at, 1, 1, at, 0, 16, 1.0, out, None, None, 0, None)
+        assert "out, which is not the query" in msg
