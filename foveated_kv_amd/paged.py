@@ -137,6 +137,16 @@ def _index_of(device):
     return device
 
 
+class _Fixed:
+    """An object whose attributes say what its calls, which know addresses
+    and sizes, work on: another value would change nothing there."""
+
+    def __setattr__(self, name, value):
+        if "_key" in self.__dict__ and name in self.__dict__:
+            raise AttributeError(f"{name} cannot be set: a {type(self).__name__} is made for what it holds (make another one)")
+        super().__setattr__(name, value)
+
+
 # ---------------------------------------------------------------------------
 # rotary positions
 # ---------------------------------------------------------------------------
@@ -183,7 +193,7 @@ def _frequencies(rot_dim, base, scaling):
     raise ValueError(f"unknown scaling kind {kind!r} (linear, ntk, yarn, bands)")
 
 
-class Rope:
+class Rope(_Fixed):
     """Rotary positions.  Pair i of a row at position p turns by the angle
     p * f_i, f_i = base^(-2 i / rot_dim) in 64 bits, the pairs being elements
     (i, i + rot_dim / 2), or (2 i, 2 i + 1) with ``interleaved``, of the row's
@@ -268,7 +278,7 @@ class Rope:
 # one layer
 # ---------------------------------------------------------------------------
 
-class PagedLayer:
+class PagedLayer(_Fixed):
     """One layer's pages: ``n_pages`` pages of ``page_size`` tokens (a power
     of two from 16 to 1024) for ``n_kv_heads`` heads of 64 or 128 dims.
 
@@ -334,8 +344,9 @@ class PagedLayer:
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, H, page, D
         self.device, self._index = k.device, k.get_device()
         c = _lib.PagesC(k.data_ptr(), v.data_ptr(), ptr(k_exp), ptr(v_scale), n, page, H, D, FORMATS[fmt])
-        self._c, self._key = ctypes.byref(c), (ctypes.addressof(c), self._index)
+        self._c = ctypes.byref(c)
         check(min(int(_lib.load().fkv_paged_attn_workspace(self._c, H, 1, 0)), 0), "PagedLayer")
+        self._key = ctypes.addressof(c), self._index
 
     def _table(self, table, B=None):
         """-> table, its rows, pages per sequence and row stride."""

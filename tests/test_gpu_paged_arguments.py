@@ -200,3 +200,18 @@ def test_attention_in_the_place_of_its_query(paged):
         lens = torch.tensor([n, n // 2], dtype=torch.int32, device="cuda")
         want, x = layer.attend(q, table, lens), q.clone()
         assert torch.equal(layer.attend(x, table, lens, out=x), want) and torch.equal(x, want)
+
+
+def test_what_a_layer_holds_is_fixed(paged):
+    import copy
+
+    layer = paged.PagedLayer(2, 1, 64, 16, "fp8")
+    for name in ("k", "v", "k_exp", "v_scale", "page_size", "fmt"):
+        with pytest.raises(AttributeError, match=f"{name} cannot be set"):
+            setattr(layer, name, getattr(layer, name))
+    with pytest.raises(TypeError):
+        copy.deepcopy(layer)
+    other = paged.PagedLayer.wrap("fp8", layer.k.clone(), layer.v.clone(), layer.k_exp.clone(), layer.v_scale.clone())
+    x = torch.ones(1, 1, 1, 64, dtype=torch.float16, device="cuda")
+    other.write(x, x, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), 0)
+    assert bool(other.k.any()) and not bool(layer.k.any())

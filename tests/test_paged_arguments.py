@@ -122,3 +122,24 @@ def test_results_that_share_memory_are_refused():
     for q, out in [((at, 192, 64, 0), at + 128), ((at, 384, 128, 0), at), ((at, 192, 64, 0), at - 2 * 320)]:
         msg = _entry("fkv_paged_attn", pages, _rows(*q), 0, 3, 2, at, 1, 1, at, 0, 16, 1.0, out, None, None, 0, None)
         assert "out, which is not the query" in msg
+
+
+# ---------------------------------------------------------------------------
+# objects
+# ---------------------------------------------------------------------------
+
+def test_what_a_rope_is_made_for_is_fixed():
+    """Its calls know the table's address: another table, or another way to
+    pair, would have been ignored."""
+    import copy
+
+    rope = Rope(64, max_positions=8, device="cpu")
+    for name, value in (("table", rope.table * 0), ("interleaved", True), ("rot_dim", 32), ("head_dim", 128)):
+        with pytest.raises(AttributeError, match=f"{name} cannot be set"):
+            setattr(rope, name, value)
+        with pytest.raises(AttributeError):
+            setattr(copy.copy(rope), name, value)
+    with pytest.raises(TypeError):  # (a copy of the table at another address)
+        copy.deepcopy(rope)
+    assert not rope.interleaved and rope.table.any()
+    rope.note = "mine"  # (a program's own)
