@@ -24,6 +24,7 @@ the caller, as any tensor is.
 
 import ctypes
 import math
+import operator
 import struct
 
 import torch
@@ -551,6 +552,16 @@ class PageTable:
             raise ValueError(f"seqs must be a slice of neighbouring sequences, got {seqs}")
         return slice(first, stop)
 
+    @staticmethod
+    def _each(n, count):
+        """A number for all of them, or one for each."""
+        if hasattr(n, "__index__") and not getattr(n, "ndim", 0):
+            return [operator.index(n)] * count
+        each = [int(t) for t in n]
+        if len(each) != count:
+            raise ValueError(f"{len(each)} numbers of tokens for {count} sequences")
+        return each
+
     def _not_captured(self):
         if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("pages are handed out on the host: extend, reserve and free outside of a capture, or "
@@ -567,9 +578,7 @@ class PageTable:
         self._not_captured()
         sl = self._range(seqs)
         each = range(sl.start, sl.stop)
-        want = [int(tokens)] * len(each) if isinstance(tokens, int) else [int(t) for t in tokens]
-        if len(want) != len(each):
-            raise ValueError(f"{len(want)} lengths for {len(each)} sequences")
+        want = self._each(tokens, len(each))
         if want and max(want) > self.max_tokens:
             raise MemoryError(f"a sequence of {max(want)} tokens: the table holds {self.max_tokens}")
         more = [max(0, -(-t // self.page_size) - len(self._pages[b])) for b, t in zip(each, want)]
@@ -592,10 +601,7 @@ class PageTable:
         pages and advances start, new and lens."""
         self._not_captured()
         sl = self._range(seqs)
-        count = sl.stop - sl.start
-        each = [int(n)] * count if isinstance(n, int) else [int(t) for t in n]
-        if len(each) != count:
-            raise ValueError(f"{len(each)} numbers of tokens for {count} sequences")
+        each = self._each(n, sl.stop - sl.start)
         if each and min(each) < 0:
             raise ValueError("sequences do not shrink (free them)")
         self.reserve([a + t for a, t in zip(self._lens[sl], each)], seqs=sl)

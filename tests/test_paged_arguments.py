@@ -143,3 +143,23 @@ def test_what_a_rope_is_made_for_is_fixed():
         copy.deepcopy(rope)
     assert not rope.interleaved and rope.table.any()
     rope.note = "mine"  # (a program's own)
+
+
+def test_numbers_of_tokens():
+    """Anything that is an integer, or a sequence of them."""
+    import numpy as np
+
+    t = paged.PageTable(16, 16, 2, 100, device="cpu")
+    for n, lens in ((np.int64(3), [3, 3]), (torch.tensor(2), [5, 5]), (np.array([1, 0]), [6, 5]), (torch.tensor([0, 4]), [6, 9]),
+                    ((1, np.int32(1)), [7, 10]), (True, [8, 11])):
+        t.extend(n)
+        assert t.lengths() == lens and t.lens.tolist() == lens
+    t.reserve(np.int32(40))
+    assert [len(t.pages(b)) for b in (0, 1)] == [3, 3]
+    for bad in (1.5, None, torch.tensor(0.5)):
+        with pytest.raises(TypeError):
+            t.extend(bad)
+    for bad in ([1, 1, 1], torch.tensor([1])):
+        with pytest.raises(ValueError, match="for 2 sequences"):
+            t.extend(bad)
+    assert t.lengths() == [8, 11]
