@@ -110,3 +110,29 @@ def test_a_token_above_the_others_whose_value_is_zero(paged, fmt, qd, D, n, G):
     assert np.abs(want[:3]).max(-1).min() > 1e3 * ref.TINY[q.dtype], "too small to see"
     assert (err <= tol).all(), f"error {(err / tol).max()} of the bound"
     assert (np.abs(ref.f64(lse) - wlse) <= 2 * ds + 2.0 ** -20 + 2.0 ** -22 * np.abs(wlse)).all()
+
+
+@pytest.mark.parametrize("fmt", ["fp16", "bf16"])
+@pytest.mark.parametrize("scores", [2.0 ** 27 + 2.0 ** 14, 2.0 ** 26 + 2.0 ** 14, 2.0 ** 24 + 2.0 ** 14])
+def test_scores_whose_steps_are_as_large_as_the_slack(paged, fmt, scores):
+    """Scores (in powers of two) with a step of 16 or 8 beside a running
+    maximum that lets them pass it by 15: the later token, 16 above the earlier
+    one, has a weight of 2^16 of it, and the result is its value but for that."""
+    D, page, n = 64, 16, 256
+    half = scores - 2.0 ** 14
+    layer = paged.PagedLayer(n // page, 1, D, page, fmt)
+    k, v = torch.zeros(1, 1, n, D), torch.zeros(1, 1, n, D)
+    k[..., 0], k[..., 1] = half / 2.0 ** 13, 2.0 ** 7
+    k[:, :, 1:] *= -1.0  # (far below: no weight)
+    k[:, :, 128] = k[:, :, 0]
+    k[:, :, 128, 2] = 4.0
+    v[:, :, 0], v[:, :, 128] = 3.0, 5.0
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda").view(1, -1)
+    layer.write(k.cuda(), v.cuda(), table, 0)
+    q = torch.zeros(1, 2, 1, D, dtype=DTYPES[fmt])
+    q[..., 0], q[..., 1], q[..., 2] = 2.0 ** 13, 2.0 ** 7, 4.0
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    # (the scale times log2 e is 1 or next to it: scores off by 2^-23 of themselves, 16 at most)
+    for wide in (table, torch.nn.functional.pad(table, (0, 64), value=-1)):  # (a table of 1280 tokens is split)
+        out = layer.attend(q.cuda(), wide, lens, scale=float(np.log(2.0)))
+        assert bool(((out.float() - 5.0).abs() <= 5.0 * ref.UNIT[q.dtype] + 2.0 * 2.0 ** -15).all()), out.unique()
