@@ -3,9 +3,9 @@
 // as they are, check them, allocate results and call libfkv's entry points.
 //
 // A decode step's kernels take 4 to 5 us and their launch 3, which the checks in
-// Python more than doubled.  Per call, a step of 64 sequences with 32 query and
-// 8 KV heads: rotation 7.6 us from Python, 4.9 so; write 10.0 and 5.0; attention
-// over 512 tokens 8.9 and 5.1.
+// Python more than doubled.  Host time of a call, a step of 64 sequences with 32
+// query and 8 KV heads: rotation 8.1 us from Python, 4.6 so; write 10.9 and 5.1;
+// attention over 512 tokens of one 9.5 and 4.6.
 //
 // Each function returns NotImplemented for whatever is not plain -- a wrong
 // argument, a tensor to be copied first, one of another GPU than the current

@@ -6,8 +6,9 @@
 // in one pass over the rows with the running maximum m and sum l of the
 // softmax (in powers of two: exp(s) = 2^(s log2 e)).
 //
-// Bound: the cache's bytes.  Each row is read once for up to 16 query heads;
-// the products run on the matrix cores, whose 16 columns are those heads:
+// Bound: the cache's bytes.  Each row is read once for up to 16 query heads, or
+// 32 of a long row (plan_of); the products run on the matrix cores, whose 16
+// columns are heads:
 //   S^T (16 tokens x 16 heads) = K (16 x 32 dims) Q^T,  v_mfma_f32_16x16x32
 //   O^T (16 dims x 16 heads)  += V^T (16 x 32 tokens) P^T
 // A lane of S^T holds four tokens of one head, which is where P^T's operand
@@ -27,11 +28,13 @@
 // cache.  A row that ends up in several workgroups leaves one record (maximum,
 // sum, numerators) per workgroup, joined by a second kernel in a fixed order.
 //
-// Measured (kernel alone; 6.3 TB/s is what a streaming read reaches here):
-// 16K tokens of 8 sequences, 8 KV heads, bf16, 537 MB: 81 us, 6.6 TB/s; 64K
-// tokens, fp8 / INT4, 105 MB: 21 us, of which about 5 are the chain lengths ->
-// page ids -> first rows, and the rows' ends; the join 4 to 5 us.  Times below
-// are of both, over layers of 1.5 GB in turn, so that no cache holds one.
+// Measured: 4096 tokens of 64 sequences, 8 KV heads, bf16, 1.07 GB, 167 us with
+// the join, 6.4 TB/s, over layers of 1.5 GB in turn, so that no cache holds one,
+// as all times below; 16K tokens of 8 sequences, 537 MB, 88.  With three sets of
+// 537 MB in turn, of which the last-level cache keeps a part, the kernel alone
+// takes 81 us (6.6 TB/s).  64K tokens, fp8 / INT4, 105 MB: 21 us alone, of which
+// about 5 are the chain lengths -> page ids -> first rows, and the rows' ends; the
+// join 4 to 5 us.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -884,9 +887,9 @@ constexpr int kAttnWaves = 4;
 // 3 sequences 23.3 and 18.9.)
 constexpr int kAttnGroups = 512;
 // Rows up to this long are not split: one launch, no records.  512 tokens of
-// one sequence's 8 KV heads 5.7 us and split 8.0 (bf16, D = 128), 4.9 and 7.4
-// (fp16, D = 64), of 64 sequences 19.8 and 22.1; 1024 tokens of one sequence 11.7
-// us and split 9.3.
+// one sequence's 8 KV heads 7.6 us and split 9.1 (bf16, D = 128), 8.0 and 9.6
+// (fp16), 6.0 and 8.0 (fp16, 2 heads of 64 dims), of 64 sequences 22.2 and 22.0;
+// 1024 tokens of one sequence 11.7 us and split 9.3.
 constexpr int64_t kWholeRows = 512;
 // Twice as long with as many rows as this, which then keep enough of the chip
 // busy: 1024 tokens of 16 sequences 15.6 us and split 19.0 (bf16), 12.8 and 13.8

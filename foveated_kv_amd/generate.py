@@ -415,7 +415,8 @@ def generate_paged(model, tokenizer, prompts, cache, max_tokens: int = 100, temp
     """Prefill ``prompts`` (a list, or one string) into sequences 0, 1, ... of
     the ``PagedKVCache`` ``cache``, which must be free, and decode them
     together for up to ``max_tokens`` tokens each -> (texts, stats); one text
-    for one string.  The sequences are freed at the end.
+    for one string.  The sequences are freed at the end; the cache needs room
+    for ``max_tokens`` tokens beside each prompt (MemoryError where it has not).
 
     Where ``cache.rope`` is set the model must leave the rotation to the
     cache, and prompts may have different lengths.  Without it the model

@@ -454,7 +454,8 @@ class PagedLayer(_Fixed):
         lens[b] + lens_add tokens of its pages -> out (B, Hq, 1, D) of the
         query's type, and with ``return_lse`` the natural logarithm (B, Hq)
         fp32 of each head's sum of exponentials (by which several such results
-        are joined).  A sequence without tokens gives zeros and -inf.
+        are joined).  A sequence without tokens gives zeros and -inf; one that
+        has an infinite value among its tokens NaN or infinity in that dim.
 
         ``out`` may be the query where that is contiguous.  ``max_len`` is an
         upper bound of the lengths if the host knows one
