@@ -62,13 +62,13 @@ __device__ inline int64_t page_row(const PageView& pg, const TableView& t, int64
 // 2^e of an exponent byte (e + 127).
 __device__ inline float exp_byte(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// Starts a kernel -> FKV_OK, or this launch's own error with nothing started.
-// (hipGetLastError() after a launch also reports, and clears, what an earlier
-// call of the program's left behind: a failure although the kernel runs.)
 template <typename T>
 struct AsDeclared {
     using type = T;
 };
+// Starts a kernel -> FKV_OK, or this launch's own error with nothing started.
+// (hipGetLastError() after a launch also reports, and clears, what an earlier
+// call of the program's left behind: a failure although the kernel runs.)
 template <typename... P>
 int start_kernel(const char* who, void (*kernel)(P...), dim3 grid, uint32_t threads, hipStream_t s,
                  typename AsDeclared<P>::type... args) {
@@ -83,9 +83,8 @@ struct RowsShape {
     int64_t B, H, L, D, es;
 };
 // Refuses a result whose rows share memory with one another, or with rows that
-// the call reads elsewhere.  Rows that are the very ones read (the same address
-// and strides) may be written, each by the lanes that read it.  (k and the like:
-// NULL for none, `in_place` whether those may be the result's own.)
+// the call reads elsewhere.  `in_place`: rows that are the very ones read (the
+// same address and strides) may be written, each by the lanes that read it.
 int check_result_rows(const char* who, const char* name, const fkv_rows* out, const RowsShape& shape);
 int check_apart(const char* who, const char* what, const fkv_rows* out, const RowsShape& out_shape, const fkv_rows* in,
                 const RowsShape& in_shape, bool in_place);

@@ -650,7 +650,15 @@ class PagedKVCache:
 
     def extend(self, n=1, seqs=None):
         """As ``PageTable.extend``; with one number per sequence, a write's
-        batch is padded to the largest of them."""
+        batch is padded to the largest of them.  Raises ValueError, and changes
+        nothing, where a token would stand past the rotary table, whose keys
+        would be NaN."""
+        if self.rope is not None:
+            sl = self.pages._range(seqs)
+            n = self.pages._each(n, sl.stop - sl.start)
+            most = max((a + t for a, t in zip(self.pages._lens[sl], n) if t > 0), default=0)
+            if most > self.rope.max_positions:
+                raise ValueError(f"a sequence of {most} tokens: the rotary table holds {self.rope.max_positions} positions")
         self.pages.extend(n, seqs)
 
     def free(self, seq):

@@ -163,3 +163,23 @@ def test_numbers_of_tokens():
         with pytest.raises(ValueError, match="for 2 sequences"):
             t.extend(bad)
     assert t.lengths() == [8, 11]
+
+
+def test_a_cache_does_not_grow_past_its_rotary_table():
+    """Keys there would be NaN, and with them all that the sequence attends
+    to."""
+    cache = paged.PagedKVCache.__new__(paged.PagedKVCache)
+    cache.pages = paged.PageTable(8, 16, 2, 64, device="cpu")
+    cache.rope = Rope(64, max_positions=20, device="cpu")
+    cache.extend([20, 3])
+    for n, seqs in ((1, None), ([1, 0], None), ([0, 18], None), (1, slice(0, 1))):
+        with pytest.raises(ValueError, match="20 positions"):
+            cache.extend(n, seqs)
+        assert cache.pages.lengths() == [20, 3] and cache.pages.starts() == [0, 0]
+    cache.extend([0, 17])
+    cache.extend(0)
+    assert cache.pages.lengths() == [20, 20]
+    cache.rope = None
+    cache.extend(1)
+    with pytest.raises(MemoryError):
+        cache.extend(44)
