@@ -3,7 +3,7 @@ alike, drafted tokens and long contexts.
 
 Kinds of call:
 
-  rows    ``PagedLayer.attend`` of several new tokens a sequence, each over
+  rows    ``PagedLayer.attend_tokens`` of several new tokens a sequence, each over
           the tokens up to itself: drafted tokens to be verified, a prompt's
           chunk.
   shared  the same where all sequences begin with the same pages
@@ -402,7 +402,7 @@ def run(state):
                                              return_pages=True))
     if not own:
         return _plain_rows(case, x)
-    return x["layer"].attend(x["q"], x["table"], x["lens"], x["max_len"], n_new=x["n_new"], shared=case["shared"])
+    return x["layer"].attend_tokens(x["q"], x["table"], x["lens"], x["max_len"], n_new=x["n_new"], shared=case["shared"])
 
 
 # ---------------------------------------------------------------------------
