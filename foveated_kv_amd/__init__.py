@@ -19,6 +19,7 @@ from .tier_cache import (
     standard_attention,
     standard_attention_mlx,
 )
+from .drafts import verify_drafts
 from .ext import is_available
 from .paged import PagedKVCache, PagedLayer, PageTable, Rope
 
@@ -36,4 +37,5 @@ __all__ = [
     "PagedLayer",
     "PageTable",
     "Rope",
+    "verify_drafts",
 ]

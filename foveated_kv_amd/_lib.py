@@ -171,6 +171,15 @@ SIGNATURES = {
     "fkv_paged_attn_workspace": (I64, [_PAGES, I32, I32, I64]),
     "fkv_paged_attn": (ctypes.c_int, [_PAGES, _ROWS, I32, I32, I32, P, I32, I64, P, I32, I64, F32, P, P, P, I64,
                                       P]),
+    "fkv_paged_attn_rows_workspace": (I64, [_PAGES, I32, I32, I32, I64, I64]),
+    "fkv_paged_attn_rows": (ctypes.c_int, [_PAGES, _ROWS, I32, I32, I32, I32, P, I32, I64, P, I32, P, I64, I64, F32,
+                                           _ROWS, P, P, I64, P]),
+    "fkv_paged_bounds": (ctypes.c_int, [_PAGES, P, I32, I32, P, I32, I64, _POS, P, P]),
+    "fkv_paged_attn_sparse_workspace": (I64, [_PAGES, I32, I32, I32, I32, I64]),
+    "fkv_paged_attn_sparse": (ctypes.c_int, [_PAGES, P, _ROWS, I32, I32, I32, P, I32, I64, P, I32, I64, I32, F32, P, P,
+                                             P, P, I64, P]),
+    "fkv_verify_drafts_workspace": (I64, [I32, I32, I32]),
+    "fkv_verify_drafts": (ctypes.c_int, [_ROWS, _ROWS, I32, I32, I32, I32, P, I32, P, P, P, P, P, I64, P]),
 }
 
 STATS_FIELDS = ("spikes_detected", "spikes_queued", "spikes_deduplicated", "spikes_cooled_down",

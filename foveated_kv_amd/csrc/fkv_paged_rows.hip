@@ -1,0 +1,765 @@
+// Attention of several new tokens per sequence over a paged KV cache, and of
+// sequences whose first pages are the same.
+//
+// A row is one query head at one new token.  Row (b, l, g) of KV head h attends
+// to the first lim = len_b - n_b + l + 1 tokens of its sequence (n_b new ones, of
+// which it is the l-th), as the one-token kernel does:
+//   s_t = scale * q . k_t,   out = sum_t exp(s_t) v_t / sum_t exp(s_t).
+// Tokens below `shared` lie in the same pages for all sequences: the rows of all
+// of them attend to these together, so that they are read once per 256 rows, and
+// each sequence's rows to its own tokens.  Every part leaves a record (maximum,
+// sum, numerators) per row, which a second kernel joins in a fixed order; a call
+// that is not split writes its results at once.
+//
+// Matrix products, 32 rows a wave, 32 tokens a step:
+//   S^T (32 tokens x 32 rows) = K (32 x 16 dims) Q^T,   v_mfma_f32_32x32x16
+//   O^T (32 dims x 32 rows)  += V^T (32 x 16 tokens) P^T
+// A lane of S^T holds 16 tokens of one row, the lane 32 further the other 16; in
+// groups of 8 they are P^T's operand as they stand, since the order of the 16
+// tokens within a product is free as long as V^T's is the same: tokens 4 h + i
+// and 8 + 4 h + i of lanes' half h.  V^T comes out of the LDS by transposing
+// reads, which hand a lane four tokens of one dim.
+//
+// A workgroup has eight waves and takes 128 tokens a tile, which its threads
+// decode to 16 bits once into the LDS, the next tile's loads being in flight
+// meanwhile.  WR waves stand for 32 rows each and WT = min(4, 8 / WR) for parts
+// of the tile's tokens: few rows (drafted tokens) are bound by the cache's bytes
+// and take one wave each for their rows, many (a prompt's chunk, a shared
+// beginning) by the products.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "fkv_paged.h"
+
+namespace fkv {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+constexpr int kRowsMaxSeqs = 4096;
+constexpr int kTileTokens = 128;
+constexpr int kRowWaves = 8;
+constexpr float kLowest = -3.402823466e38f;  // running maximum before the first token: no score lies below it
+// As in the one-token kernel: the running maximum follows a score that exceeds
+// it by more than 2^8, and stays 2^7 below the scores of fp16 pages, whose
+// weights (2^15 at most) so keep away from the end of fp16's range.
+constexpr float kRowSlack = 8.0f;
+template <int FMT>
+constexpr float kRowBias = FMT == FKV_PAGES_F16 ? 7.0f : 0.0f;
+
+// How one kind of part (the shared tokens, the sequences' own) is cut up.
+struct RowParts {
+    int32_t wr;      // waves of 32 rows per workgroup: 1, 2, 4 or 8
+    int32_t tiles;   // workgroups of 32 * wr rows (per sequence, for the own tokens)
+    int32_t splits;  // parts of the tokens
+    int32_t chunk;   // tokens of a part; the last one of the own tokens takes what is left
+};
+
+struct RowsArgs {
+    PageView pg;
+    TableView table;
+    RowsView q, out;
+    const int32_t* lens;
+    const int32_t* n_new;
+    float* lse;
+    float* records;  // workspace: per row and part D numerators, maximum, sum
+    RowParts common, own;
+    int32_t lens_add, B, Hq, G, L, shared;
+    float scale;  // scale * log2(e)
+};
+
+typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
+__device__ inline int32_t scalar_load(const int32_t* p, int64_t i) { return ((scalar_ints)(uintptr_t)p)[i]; }
+
+// How many tokens row (b, l) attends to; -1 for a padded token's.
+__device__ inline int32_t limit_of(const RowsArgs& a, int b, int l) {
+    const int64_t cap = (int64_t)a.table.n * a.pg.page_size;  // (below 2^31)
+    int64_t len = (int64_t)a.lens[b] + a.lens_add;
+    len = len < 0 ? 0 : len > cap ? cap : len;
+    int32_t n = a.L;
+    if (a.n_new) n = min(max(a.n_new[b], 0), a.L);
+    const int64_t lim = len - n + l + 1;
+    return l >= n ? -1 : lim < 0 ? 0 : (int32_t)lim;
+}
+
+template <bool BF>
+__device__ inline f16v mfma32(u4 x, u4 y, f16v c) {
+    if (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), c, 0, 0, 0);
+}
+
+// Two E4M3 codes (the chosen half of w) times a power of two, exact.
+template <bool BF, bool HI>
+__device__ inline uint32_t cvt_codes(uint32_t w, float scale) {
+    if (BF) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
+}
+__device__ inline uint32_t round_pair_bf16(float a, float b) {
+    const b2 v = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+// A tile's tokens as a thread loads them: 16 (INT4 of 64 dims: 8) bytes of a row
+// at a time, neighbouring threads a row.
+template <int D, int FMT>
+struct Rows {
+    static constexpr bool k16 = FMT <= FKV_PAGES_BF16;
+    static constexpr int KB = k16 ? 2 * D : D;                                 // bytes of a key row
+    static constexpr int VB = k16 ? 2 * D : FMT == FKV_PAGES_FP8 ? D : D / 2;  // and of a value row
+    static constexpr int KT = KB / 16, VT = VB == 32 ? 4 : VB / 16;            // threads a row
+    static constexpr int KP = KT / 4, VP = VT / 4;                             // passes of 512 threads over 128 rows
+    u4 k[KP], v[VP];
+    uint32_t vx[VP];    // E4M3 values: the rows' exponent bytes
+    uint32_t kx;        // of token threadIdx.x: the key's exponent byte,
+    float2 sz;          // INT4 values: scale and minimum
+};
+
+template <int D>
+struct RowsLds {
+    static constexpr int kRow = 2 * D;                 // bytes of a row in 16 bits
+    static constexpr int kTileBytes = kTileTokens * kRow;
+    static constexpr int kNumerators = kRowWaves * 32 * (D + 4) * 4;
+    static constexpr int kBytes = 4 * kTileBytes > kNumerators ? 4 * kTileBytes : kNumerators;
+};
+
+// Where 16-byte chunk `chunk` of row `row` lies in a tile of keys (eight
+// neighbouring lanes read one chunk of eight rows: all banks) and of values (a
+// transposing read takes 64 bytes of each of four rows).
+template <int D>
+__device__ inline uint32_t key_place(uint32_t row, uint32_t chunk) { return row * 2 * D + 16 * (chunk ^ (row & 7)); }
+template <int D>
+__device__ inline uint32_t value_turn(uint32_t row) { return D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
+template <int D>
+__device__ inline uint32_t value_place(uint32_t row, uint32_t chunk) {
+    return row * 2 * D + 16 * (chunk ^ value_turn<D>(row));
+}
+
+// Are any of two packed 16-bit numbers infinite or NaN?
+template <bool BF>
+__device__ inline bool any_not_finite(uint32_t w) {
+    const uint32_t e = BF ? 0x7F80u : 0x7C00u;
+    return (w & e) == e || ((w >> 16) & e) == e;
+}
+template <bool BF>
+__device__ inline uint32_t finite_or_zero(uint32_t w) {
+    const uint32_t e = BF ? 0x7F80u : 0x7C00u;
+    return ((w & e) == e ? 0 : w & 0xFFFFu) | (((w >> 16) & e) == e ? 0 : w & 0xFFFF0000u);
+}
+
+template <int D, int FMT, bool BF>
+__global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs a) {
+    using R = Rows<D, FMT>;
+    constexpr bool kVB = FMT != FKV_PAGES_F16;  // values and weights are bf16 numbers
+    constexpr int DT = D / 32;
+    __shared__ __attribute__((aligned(16))) char tiles[RowsLds<D>::kBytes];
+    __shared__ __attribute__((aligned(16))) float key_factor[2][kTileTokens], value_scale[2][kTileTokens],
+        value_min[2][kTileTokens];
+    __shared__ float stat[kRowWaves][32][3];
+    __shared__ int32_t least[kRowWaves], most[kRowWaves], run_tokens[2][8], odd_tile[2];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int sh = 31 - __builtin_clz((unsigned)a.pg.page_size);
+
+    // the part: shared tokens (seq < 0) or sequence seq's own
+    const int h = blockIdx.x % a.pg.H;
+    int rest = blockIdx.x / a.pg.H, seq = -1, tile, split;
+    RowParts p = a.common;
+    if (rest < a.common.tiles * a.common.splits) {
+        tile = rest / a.common.splits, split = rest - tile * a.common.splits;
+    } else {
+        rest -= a.common.tiles * a.common.splits;
+        p = a.own;
+        // (the last rows attend to the most tokens: they come first)
+        const int per_tile = a.own.splits * a.B, t = rest / per_tile;
+        tile = a.own.tiles - 1 - t;
+        rest -= t * per_tile;
+        seq = rest / a.own.splits, split = rest - seq * a.own.splits;
+    }
+    const int rows = seq < 0 ? a.B * a.L * a.G : a.L * a.G;
+    const int wr = p.wr, wt = min(4, kRowWaves / wr), rg = wave & (wr - 1), tg = wave / wr;
+    const int row0 = tile * 32 * wr;
+    // row r of the part -> (b, l, query head); -1: none
+    auto place = [&](int r, int& b, int& l, int& hq) {
+        const int token = r / a.G;
+        b = seq < 0 ? token / a.L : seq;
+        l = seq < 0 ? token - b * a.L : token;
+        hq = h * a.G + r - token * a.G;
+        return r < rows ? limit_of(a, b, l) : -1;
+    };
+    int b, l, hq;
+    const int row = row0 + 32 * rg + c;
+    int32_t lim = place(row, b, l, hq);
+    const bool real = lim >= 0;
+    if (seq < 0) lim = min(lim, a.shared);
+
+    const int32_t begin = (seq < 0 ? 0 : a.shared) + split * p.chunk;
+    int32_t wave_most = lim, wave_least = real ? lim : 0x7FFFFFFF;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        wave_most = max(wave_most, wave_xor(wave_most, o));
+        wave_least = min(wave_least, wave_xor(wave_least, o));
+    }
+    wave_most = __builtin_amdgcn_readfirstlane(wave_most);
+    wave_least = __builtin_amdgcn_readfirstlane(wave_least);
+    if (lane == 0) least[wave] = wave_least, most[wave] = wave_most;
+    if (tid < 2) odd_tile[tid] = -1;
+    __syncthreads();
+    int32_t end = most[0], all_least = least[0];
+#pragma unroll
+    for (int w = 1; w < kRowWaves; w++) end = max(end, most[w]), all_least = min(all_least, least[w]);
+    end = __builtin_amdgcn_readfirstlane(end);
+    all_least = __builtin_amdgcn_readfirstlane(all_least);
+    if (seq < 0 || split + 1 < p.splits) end = min(end, begin + p.chunk);
+    const int nt = end > begin ? (end - begin + kTileTokens - 1) / kTileTokens : 0;
+    const int parts = a.common.splits + a.own.splits;
+    if (nt == 0 && parts > 1) return;
+
+    u4 q[D / 16];
+    {
+        const char* at = a.q.data + 2 * (b * a.q.sb + hq * a.q.sh + l * a.q.sl);
+        const u4 none = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) q[i] = real ? *(const u4*)(at + 32 * i + 16 * hf) : none;
+    }
+
+    const int32_t* ids = a.table.ids + (seq < 0 ? 0 : seq) * a.table.stride;
+    R st;
+    // page of run `run` (16 tokens) of the tile at tok -> first row of its tokens, how many there are
+    auto run_of = [&](int32_t tok, int run, int& n) {
+        const int32_t at = tok + 16 * run;
+        n = min(max(end - at, 0), 16);
+        int32_t id = n > 0 ? scalar_load(ids, at >> sh) : 0;
+        if ((uint32_t)id >= (uint32_t)a.pg.n_pages) id = 0, n = 0;
+        return (((int64_t)id * a.pg.H + h) << sh) + (n > 0 ? at & (a.pg.page_size - 1) : 0);
+    };
+    // A tile's loads.  A wave's rows of one pass lie in one run.
+    auto load = [&](int32_t tok) {
+        constexpr u4 none = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < R::KP; i++) {
+            constexpr int per = 512 / R::KT;  // rows a pass
+            int n;
+            const int64_t first = run_of(tok, (per * i + (64 / R::KT) * wave) / 16, n);
+            const int r = (tid / R::KT) & 15;
+            const u4 x = *(const u4*)(a.pg.k + first * R::KB + (uint32_t)(r * R::KB + 16 * (tid % R::KT)));
+            st.k[i] = r < n ? x : none;
+        }
+#pragma unroll
+        for (int i = 0; i < R::VP; i++) {
+            constexpr int per = 512 / R::VT;
+            int n;
+            const int64_t first = run_of(tok, (per * i + (64 / R::VT) * wave) / 16, n);
+            const int r = (tid / R::VT) & 15;
+            const char* at = a.pg.v + first * R::VB;
+            if (R::VB == 32) {
+                const u2 x = *(const u2*)(at + (uint32_t)(r * R::VB + 8 * (tid % R::VT)));
+                st.v[i] = u4{r < n ? x.x : 0, r < n ? x.y : 0, 0, 0};
+            } else {
+                const u4 x = *(const u4*)(at + (uint32_t)(r * R::VB + 16 * (tid % R::VT)));
+                st.v[i] = r < n ? x : none;
+            }
+            if (FMT == FKV_PAGES_FP8) st.vx[i] = r < n ? ((const uint8_t*)a.pg.v_scale)[first + r] : 0;
+        }
+        if (FMT >= FKV_PAGES_FP8 && wave < 2) {
+            // (token tid of the tile: runs 4 wave to 4 wave + 3, 16 lanes each)
+            int64_t at = 0;
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                int m;
+                const int64_t first = run_of(tok, 4 * wave + i, m);
+                if (lane >> 4 == i) at = first, n = m;
+            }
+            const bool in = (lane & 15) < n;
+            st.kx = in ? a.pg.k_exp[at + (lane & 15)] : 0;
+            if (FMT == FKV_PAGES_FP8_INT4) {
+                const float2 x = ((const float2*)a.pg.v_scale)[at + (in ? lane & 15 : 0)];
+                st.sz = in ? x : make_float2(0.0f, 0.0f);
+            }
+        }
+    };
+    // ... and into the LDS, in 16 bits.
+    auto store = [&](int32_t tok, int t, int buf) {
+        char* keys = tiles + buf * 2 * RowsLds<D>::kTileBytes;
+        char* values = keys + RowsLds<D>::kTileBytes;
+        const bool look = tok + kTileTokens > all_least;  // (tokens that not all rows attend to)
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < R::KP; i++) {
+            const int r = (512 / R::KT) * i + tid / R::KT, ch = tid % R::KT;
+            const u4 x = st.k[i];
+            if (R::k16) {
+                *(u4*)(keys + key_place<D>(r, ch)) = x;
+            } else {
+                *(u4*)(keys + key_place<D>(r, 2 * ch)) = u4{cvt_codes<BF, false>(x.x, 1.0f), cvt_codes<BF, true>(x.x, 1.0f),
+                                                            cvt_codes<BF, false>(x.y, 1.0f), cvt_codes<BF, true>(x.y, 1.0f)};
+                *(u4*)(keys + key_place<D>(r, 2 * ch + 1)) =
+                    u4{cvt_codes<BF, false>(x.z, 1.0f), cvt_codes<BF, true>(x.z, 1.0f), cvt_codes<BF, false>(x.w, 1.0f),
+                       cvt_codes<BF, true>(x.w, 1.0f)};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < R::VP; i++) {
+            const int r = (512 / R::VT) * i + tid / R::VT, ch = tid % R::VT;
+            const u4 x = st.v[i];
+            if (R::k16) {
+                *(u4*)(values + value_place<D>(r, ch)) = x;
+                if (look)
+                    odd = odd || any_not_finite<kVB>(x.x) || any_not_finite<kVB>(x.y) || any_not_finite<kVB>(x.z) ||
+                          any_not_finite<kVB>(x.w);
+            } else if (FMT == FKV_PAGES_FP8) {
+                // (times the row's power of two, which bf16 numbers carry exactly; byte 0 stands for a factor of 0)
+                const float e = exp_byte(st.vx[i]);
+                const bool none = st.vx[i] == 0;
+                uint32_t y[8];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    y[2 * j] = none ? 0 : cvt_codes<true, false>(x[j], e);
+                    y[2 * j + 1] = none ? 0 : cvt_codes<true, true>(x[j], e);
+                }
+                *(u4*)(values + value_place<D>(r, 2 * ch)) = u4{y[0], y[1], y[2], y[3]};
+                *(u4*)(values + value_place<D>(r, 2 * ch + 1)) = u4{y[4], y[5], y[6], y[7]};
+                if (look) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) odd = odd || any_not_finite<true>(y[j]);
+                }
+            } else {
+                // codes 0 to 15 are the E4M3 numbers code * 2^-9
+                constexpr int NW = R::VB == 32 ? 2 : 4;  // dwords of eight codes: a chunk each
+#pragma unroll
+                for (int j = 0; j < NW; j++) {
+                    const uint32_t even = x[j] & 0x0F0F0F0Fu, other = (x[j] >> 4) & 0x0F0F0F0Fu;
+                    const uint32_t lo = __builtin_amdgcn_perm(other, even, 0x05010400u);
+                    const uint32_t hi = __builtin_amdgcn_perm(other, even, 0x07030602u);
+                    *(u4*)(values + value_place<D>(r, NW * ch + j)) =
+                        u4{cvt_codes<true, false>(lo, 512.0f), cvt_codes<true, true>(lo, 512.0f),
+                           cvt_codes<true, false>(hi, 512.0f), cvt_codes<true, true>(hi, 512.0f)};
+                }
+            }
+        }
+        if (FMT >= FKV_PAGES_FP8 && wave < 2) {
+            key_factor[buf][tid] = exp_byte(st.kx);
+            if (FMT == FKV_PAGES_FP8_INT4) value_scale[buf][tid] = st.sz.x, value_min[buf][tid] = st.sz.y;
+        }
+        if (lane == 0) {
+            int n;
+            (void)run_of(tok, wave, n);
+            run_tokens[buf][wave] = n;
+        }
+        if (odd) odd_tile[buf] = t;
+    };
+
+    f16v acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
+    float m = kLowest, sum = 0.0f, z = 0.0f;
+
+    // V^T's operand: this lane's row and bytes of a transposing read
+    const uint32_t tr_row = 4 * hf + ((lane & 15) >> 2), tr_byte = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    auto step = [&](int32_t tok, int t, int buf, int sub) {
+        const char* keys = tiles + buf * 2 * RowsLds<D>::kTileBytes;
+        const char* values = keys + RowsLds<D>::kTileBytes;
+        f16v s;
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++)
+            s = mfma32<BF>(*(const u4*)(keys + key_place<D>(32 * sub + c, 2 * i + hf)), q[i], s);
+        // this lane's tokens: 8 (i / 4) + 4 hf + i % 4
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            f4 f = {1.0f, 1.0f, 1.0f, 1.0f};
+            if (FMT >= FKV_PAGES_FP8) f = *(const f4*)&key_factor[buf][32 * sub + 8 * j + 4 * hf];
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[4 * j + i] = FMT >= FKV_PAGES_FP8 ? s[4 * j + i] * a.scale * f[i] : s[4 * j + i] * a.scale;
+        }
+        const int n0 = __builtin_amdgcn_readfirstlane(run_tokens[buf][2 * sub]);
+        const int n1 = __builtin_amdgcn_readfirstlane(run_tokens[buf][2 * sub + 1]);
+        const bool part = tok + 32 > wave_least;
+        const bool masked = part || n0 < 16 || n1 < 16;
+        if (masked) {
+            const int left = lim - tok;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int at = 8 * (i >> 2) + 4 * hf + (i & 3);
+                if (at >= left || (at & 15) >= (i < 8 ? n0 : n1)) s[i] = -INFINITY;
+            }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+        if (__any(top > m + (kRowSlack + kRowBias<FMT>))) {
+            top = fmaxf(top, wave_xor(top, 32));
+            const float up = fmaxf(m, top - kRowBias<FMT>), f = __builtin_amdgcn_exp2f(m - up);
+            m = up;
+            sum *= f;
+            z *= f;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[d][i] *= f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            s[i] = __builtin_amdgcn_exp2f(s[i] - m);
+            sum += s[i];
+        }
+        if (FMT == FKV_PAGES_FP8_INT4) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const f4 scale = *(const f4*)&value_scale[buf][32 * sub + 8 * j + 4 * hf];
+                const f4 low = *(const f4*)&value_min[buf][32 * sub + 8 * j + 4 * hf];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    // (a token that takes no part may have any scale, NaN among them)
+                    const bool in = !masked || 8 * j + 4 * hf + i < lim - tok;
+                    z = in ? fmaf(s[4 * j + i], low[i], z) : z;
+                    s[4 * j + i] = in ? s[4 * j + i] * scale[i] : 0.0f;
+                }
+            }
+        }
+        // Weights as two 16-bit numbers, the first cut off and the second what
+        // that leaves, rounded: 16 bits (bf16) or 22 (fp16, down to steps of
+        // 2^-24, 2^-39 of the row's largest weight).
+        u4 part_of[2][2];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            float x = s[2 * j], y = s[2 * j + 1];
+            uint32_t first;
+            if (kVB) {
+                first = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+                x -= __uint_as_float(first << 16);
+                y -= __uint_as_float(first & 0xFFFF0000u);
+            } else {
+                const fkv_h2 w = __builtin_bit_cast(fkv_h2, __builtin_amdgcn_cvt_pkrtz(x, y));
+                first = as_u32(w);
+                x -= (float)w.x;
+                y -= (float)w.y;
+            }
+            part_of[0][j >> 2][j & 3] = first;
+            part_of[1][j >> 2][j & 3] = kVB ? round_pair_bf16(x, y) : (uint32_t)f2h(x) | ((uint32_t)f2h(y) << 16);
+        }
+        const bool odd = part && FMT != FKV_PAGES_FP8_INT4 && __builtin_amdgcn_readfirstlane(odd_tile[buf]) == t;
+        auto products = [&](bool clean) {
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    u4 v;
+#pragma unroll
+                    for (int jj = 0; jj < 2; jj++) {
+                        const uint32_t r = 32 * sub + 16 * g + 8 * jj + tr_row;
+                        const char* at = values + value_place<D>(r, 4 * d + (tr_byte >> 4)) + (tr_byte & 15);
+                        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)at);
+                        const u2 w = __builtin_bit_cast(u2, x);
+                        v[2 * jj] = clean ? finite_or_zero<kVB>(w.x) : w.x;
+                        v[2 * jj + 1] = clean ? finite_or_zero<kVB>(w.y) : w.y;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; i++) acc[d] = mfma32<kVB>(v, part_of[i][g], acc[d]);
+                }
+        };
+        if (!odd) {
+            products(false);
+        } else {
+            // Infinite or NaN values among tokens that not all rows attend to: a
+            // weight of 0 would carry them into every row, so the products are
+            // made without them, and they join the rows that attend to them.
+            products(true);
+            for (int r = 0; r < 32; r++) {
+                const bool in = r < lim - tok && (r & 15) < (r < 16 ? n0 : n1);
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int dim = 32 * d + 8 * j + 4 * hf;
+                        const u2 w = *(const u2*)(values + value_place<D>(32 * sub + r, dim >> 3) + 2 * (dim & 7));
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t x = (w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu;
+                            if (in && any_not_finite<kVB>(x)) acc[d][4 * j + i] += kVB ? bf2f(x) : h2f(x);
+                        }
+                    }
+            }
+        }
+    };
+
+    if (nt > 0) load(begin);
+    for (int t = 0; t < nt; t++) {
+        const int32_t tok = begin + t * kTileTokens;
+        const int buf = t & 1;
+        store(tok, t, buf);
+        if (t + 1 < nt) load(tok + kTileTokens);
+        __syncthreads();
+        if (tg < wt)
+            for (int sub = tg; sub < 4; sub += wt)
+                if (tok + 32 * sub < wave_most) step(tok + 32 * sub, t, buf, sub);
+    }
+
+    // The waves' sums meet in the LDS: 16 threads a row, D / 16 dims a thread.
+    sum += wave_xor(sum, 32);
+    z += wave_xor(z, 32);
+    __syncthreads();
+    float* num = (float*)tiles;
+    if (tg < wt) {
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                *(f4*)(num + (wave * 32 + c) * (D + 4) + 32 * d + 8 * j + 4 * hf) =
+                    f4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
+        if (hf == 0) stat[wave][c][0] = m, stat[wave][c][1] = sum, stat[wave][c][2] = z;
+    }
+    __syncthreads();
+    constexpr int N = D / 16;
+    for (int i = 0; i < wr; i++) {
+        const int rr = tid >> 4, d0 = (tid & 15) * N;
+        int b, l, hq;
+        const int32_t lim = place(row0 + 32 * i + rr, b, l, hq);
+        const int64_t at = ((int64_t)b * a.Hq + hq) * a.L + l;
+        if (lim < 0) {
+            if (parts == 1 && a.lse && (tid & 15) == 0 && row0 + 32 * i + rr < rows) a.lse[at] = -INFINITY;
+            continue;
+        }
+        float top = kLowest, all = 0.0f, low = 0.0f, x[N] = {};
+        for (int w = 0; w < wt; w++) top = fmaxf(top, stat[w * wr + i][rr][0]);
+        for (int w = 0; w < wt; w++) {
+            const float* s = stat[w * wr + i][rr];
+            const float f = __builtin_amdgcn_exp2f(s[0] - top);
+            all = fmaf(f, s[1], all);
+            low = fmaf(f, s[2], low);
+            const float* n = num + ((w * wr + i) * 32 + rr) * (D + 4) + d0;
+#pragma unroll
+            for (int j = 0; j < N; j++) x[j] = fmaf(f, n[j], x[j]);
+        }
+        if (FMT == FKV_PAGES_FP8_INT4) {
+#pragma unroll
+            for (int j = 0; j < N; j++) x[j] += low;
+        }
+        if (parts > 1) {
+            float* out = a.records + (at * parts + (seq < 0 ? split : a.common.splits + split)) * (D + 4);
+#pragma unroll
+            for (int j = 0; j < N; j += 4) *(f4*)(out + d0 + j) = f4{x[j], x[j + 1], x[j + 2], x[j + 3]};
+            if ((tid & 15) == 0) *(float2*)(out + D) = make_float2(top, all);
+        } else {
+            const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+            uint32_t o[N / 2];
+#pragma unroll
+            for (int j = 0; j < N / 2; j++) {
+                const float u = x[2 * j] * inv, v = x[2 * j + 1] * inv;
+                o[j] = BF ? round_pair_bf16(u, v) : (uint32_t)f2h(u) | ((uint32_t)f2h(v) << 16);
+            }
+            char* dst = a.out.data + 2 * (b * a.out.sb + hq * a.out.sh + l * a.out.sl + d0);
+            if (N == 8) *(uint4*)dst = make_uint4(o[0], o[1], o[2 % (N / 2)], o[3 % (N / 2)]);
+            else *(uint2*)dst = make_uint2(o[0], o[1]);
+            if (a.lse && (tid & 15) == 0) a.lse[at] = (top + __builtin_amdgcn_logf(all)) * 0.69314718055994531f;
+        }
+    }
+}
+
+// The records of a row, in order: a wave a row.
+template <int D, bool BF>
+__global__ void __launch_bounds__(256) paged_rows_join_kernel(RowsArgs a, int64_t n_rows) {
+    constexpr int N = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (at >= n_rows) return;
+    const int64_t bh = at / a.L;
+    const int l = (int)(at - bh * a.L), b = (int)(bh / a.Hq), hq = (int)(bh - (int64_t)b * a.Hq);
+    const int32_t lim = limit_of(a, b, l);
+    if (lim < 0) {
+        if (a.lse && lane == 0) a.lse[at] = -INFINITY;
+        return;
+    }
+    const int parts = a.common.splits + a.own.splits;
+    // (parts whose tokens begin below the row's end have a record)
+    const int n_common = a.common.splits ? min(a.common.splits, (min(lim, a.shared) + a.common.chunk - 1) / a.common.chunk) : 0;
+    const int n_own = lim > a.shared ? min(a.own.splits, (lim - a.shared + a.own.chunk - 1) / a.own.chunk) : 0;
+    const int n = n_common + n_own;
+    const float* rec = a.records + at * parts * (D + 4);
+    float m = kLowest, sum = 0.0f, x[N] = {};
+    constexpr int U = 8;  // records a step, their loads in flight together
+    for (int i = 0; i < n; i += U) {
+        float2 st[U];
+        float v[U][N];
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            const int r = min(i + k, n - 1);
+            const float* p = rec + (r < n_common ? r : a.common.splits + r - n_common) * (D + 4);
+            st[k] = *(const float2*)(p + D);
+#pragma unroll
+            for (int j = 0; j < N; j++) v[k][j] = p[64 * j + lane];
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < U; k++) top = fmaxf(top, st[k].x);
+        const float f = __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        sum *= f;
+#pragma unroll
+        for (int j = 0; j < N; j++) x[j] *= f;
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            if (i + k < n) {
+                const float w = __builtin_amdgcn_exp2f(st[k].x - m);
+                sum = fmaf(w, st[k].y, sum);
+#pragma unroll
+                for (int j = 0; j < N; j++) x[j] = fmaf(w, v[k][j], x[j]);
+            }
+        }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint16_t* out = (uint16_t*)a.out.data + b * a.out.sb + hq * a.out.sh + l * a.out.sl;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const float y = x[j] * inv;
+        out[64 * j + lane] = BF ? __builtin_bit_cast(uint16_t, (__bf16)y) : f2h(y);
+    }
+    if (a.lse && lane == 0) a.lse[at] = (m + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+}
+
+// ---------------------------------------------------------------------------
+// launch
+// ---------------------------------------------------------------------------
+
+struct RowsPlan {
+    RowParts common, own;
+    int64_t blocks, bytes;
+};
+
+static int waves_for(int64_t rows) { return rows > 128 ? 8 : rows > 64 ? 4 : rows > 32 ? 2 : 1; }
+
+// Workgroups and workspace of a call (a function of sizes alone).
+static RowsPlan plan_rows(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, int64_t shared, int64_t max_len) {
+    RowsPlan r;
+    const int64_t G = Hq / p->H, own_rows = L * G, all_rows = B * own_rows;
+    const int64_t own_tokens = std::max<int64_t>(1, max_len - shared);
+    r.own.wr = waves_for(own_rows);
+    r.own.tiles = (int32_t)cdiv(own_rows, 32 * r.own.wr);
+    r.common.wr = waves_for(all_rows);
+    r.common.tiles = shared ? (int32_t)cdiv(all_rows, 32 * r.common.wr) : 0;
+    // tiles of 128 tokens in all, dealt to 512 workgroups of two tiles at least
+    const int64_t tiles = p->H * (r.common.tiles * cdiv(shared, kTileTokens) + B * r.own.tiles * cdiv(own_tokens, kTileTokens));
+    const int64_t per = std::max<int64_t>(2, cdiv(tiles, 512));
+    auto cut = [&](RowParts& part, int64_t tokens, int64_t groups) {
+        // (workgroups enough without parts: none)
+        const int64_t n = groups >= 256 ? 1 : cdiv(cdiv(tokens, kTileTokens), per);
+        part.chunk = (int32_t)(cdiv(cdiv(tokens, kTileTokens), std::max<int64_t>(n, 1)) * kTileTokens);
+        part.splits = (int32_t)cdiv(tokens, part.chunk);
+    };
+    r.common.chunk = kTileTokens;
+    r.common.splits = 0;
+    if (shared) cut(r.common, shared, p->H * r.common.tiles);
+    cut(r.own, own_tokens, p->H * B * r.own.tiles);
+    r.blocks = p->H * ((int64_t)r.common.tiles * r.common.splits + (int64_t)B * r.own.tiles * r.own.splits);
+    const int64_t parts = r.common.splits + r.own.splits;
+    r.bytes = parts > 1 ? (int64_t)B * Hq * L * parts * (p->D + 4) * 4 : 0;
+    return r;
+}
+
+static int check_rows(const char* who, const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, int64_t shared, int64_t max_len) {
+    const std::string w = who;
+    if (int e = check_pages(who, p)) return e;
+    if (B < 0 || B > kRowsMaxSeqs) return set_error(w + ": at most " + std::to_string(kRowsMaxSeqs) + " sequences");
+    if (Hq < 1 || Hq % p->H) return set_error(w + ": query heads must be a multiple of the KV heads");
+    if (L < 0 || (int64_t)B * L * Hq >= 1 << 28) return set_error(w + ": at most 2^28 rows of queries");
+    if (max_len < 0) return set_error(w + ": negative max_len");
+    if (shared < 0 || shared % p->page_size || shared > 0x7FFFFFFF - 4096)
+        return set_error(w + ": shared tokens must fill whole pages");
+    return FKV_OK;
+}
+
+template <int D, int FMT, bool BF>
+static int launch_rows(const RowsArgs& a, const RowsPlan& p, hipStream_t s) {
+    const char* w = "fkv_paged_attn_rows";
+    if (int e = start_kernel(w, paged_rows_kernel<D, FMT, BF>, (uint32_t)p.blocks, 64 * kRowWaves, s, a)) return e;
+    if (p.bytes == 0) return FKV_OK;
+    const int64_t rows = (int64_t)a.B * a.Hq * a.L;
+    return start_kernel(w, paged_rows_join_kernel<D, BF>, (uint32_t)cdiv(rows, 4), 256, s, a, rows);
+}
+
+template <int D>
+static int launch_rows_d(const RowsArgs& a, const RowsPlan& p, int format, bool bf, hipStream_t s) {
+    if (format == FKV_PAGES_F16) return launch_rows<D, FKV_PAGES_F16, false>(a, p, s);
+    if (format == FKV_PAGES_BF16) return launch_rows<D, FKV_PAGES_BF16, true>(a, p, s);
+    if (format == FKV_PAGES_FP8 && bf) return launch_rows<D, FKV_PAGES_FP8, true>(a, p, s);
+    if (format == FKV_PAGES_FP8) return launch_rows<D, FKV_PAGES_FP8, false>(a, p, s);
+    if (bf) return launch_rows<D, FKV_PAGES_FP8_INT4, true>(a, p, s);
+    return launch_rows<D, FKV_PAGES_FP8_INT4, false>(a, p, s);
+}
+
+}  // namespace fkv
+
+using namespace fkv;
+
+extern "C" {
+
+int64_t fkv_paged_attn_rows_workspace(const fkv_pages* pages, int32_t Hq, int32_t B, int32_t L, int64_t shared,
+                                      int64_t max_len) {
+    if (int e = check_rows("fkv_paged_attn_rows_workspace", pages, Hq, B, L, shared, max_len)) return e;
+    return plan_rows(pages, Hq, B, L, shared, max_len).bytes;
+}
+
+int fkv_paged_attn_rows(const fkv_pages* pages, const fkv_rows* query, int32_t q_dtype, int32_t Hq, int32_t B, int32_t L,
+                        const int32_t* table, int32_t n_table, int64_t table_stride, const int32_t* lens,
+                        int32_t lens_add, const int32_t* n_new, int64_t shared, int64_t max_len, float scale,
+                        const fkv_rows* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* w = "fkv_paged_attn_rows";
+    if (int e = check_rows(w, pages, Hq, B, L, shared, max_len)) return e;
+    if (int e = check_table(w, table, n_table, table_stride, B)) return e;
+    const int64_t cap = (int64_t)n_table * pages->page_size;
+    if (cap > 0x7FFFFFFF - 4096) return set_error(std::string(w) + ": more than 2^31 tokens a sequence");
+    if (shared > cap) return set_error(std::string(w) + ": more shared tokens than the table holds");
+    if (q_dtype != FKV_F16 && q_dtype != FKV_BF16) return set_error(std::string(w) + ": queries must be fp16 or bf16");
+    if (pages->format <= FKV_PAGES_BF16 && (q_dtype == FKV_BF16) != (pages->format == FKV_PAGES_BF16))
+        return set_error(std::string(w) + ": queries must have the 16-bit pages' type");
+    if (!std::isfinite(scale)) return set_error(std::string(w) + ": scale must be finite");
+    if (B == 0 || L == 0) return FKV_OK;
+    if (!query || !query->data || !out || !out->data || !lens) return set_error(std::string(w) + ": NULL argument");
+    for (const fkv_rows* r : {query, out})
+        if ((uintptr_t)r->data & 15 || (r->stride_b | r->stride_h | r->stride_l) & 7)
+            return set_error(std::string(w) + ": query and out must be 16-byte aligned, their strides multiples of 8");
+    if ((uintptr_t)workspace & 15) return set_error(std::string(w) + ": workspace must be 16-byte aligned");
+    const RowsPlan p = plan_rows(pages, Hq, B, L, shared, max_len);
+    if (p.blocks > 0x7FFFFFFF / 512) return set_error(std::string(w) + ": more than 2^22 workgroups of rows");
+    if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
+        return set_error(std::string(w) + ": workspace of " + std::to_string(p.bytes) + " bytes needed");
+    const RowsShape shape{B, Hq, L, pages->D, 2};
+    if (int e = check_result_rows(w, "out", out, shape)) return e;
+    // (a workgroup reads its rows' queries before it writes their results)
+    if (int e = check_apart(w, "out, which is not the query, and the query", out, shape, query, shape, true)) return e;
+    RowsArgs a;
+    a.pg = page_view(pages);
+    a.table = TableView{table, table_stride, n_table};
+    a.q = RowsView{(char*)query->data, query->stride_b, query->stride_h, query->stride_l};
+    a.out = RowsView{(char*)out->data, out->stride_b, out->stride_h, out->stride_l};
+    a.lens = lens;
+    a.n_new = n_new;
+    a.lse = lse;
+    a.records = (float*)workspace;
+    a.common = p.common;
+    a.own = p.own;
+    a.lens_add = lens_add;
+    a.B = B;
+    a.Hq = Hq;
+    a.G = Hq / pages->H;
+    a.L = L;
+    a.shared = (int32_t)shared;
+    a.scale = scale * 1.4426950408889634f;
+    const bool bf = q_dtype == FKV_BF16;
+    if (pages->D == 64) return launch_rows_d<64>(a, p, pages->format, bf, (hipStream_t)stream);
+    return launch_rows_d<128>(a, p, pages->format, bf, (hipStream_t)stream);
+}
+
+}  // extern "C"

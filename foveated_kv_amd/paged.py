@@ -6,9 +6,13 @@ attended to in place.
   Rope            rotary positions: half or interleaved pairs, part of the
                   head, scaled for long contexts
   PagedLayer      one layer's pages: write (rotate, encode, store), read
-                  (decode, gather) and attend (one new token a sequence)
+                  (decode, gather), attend (one new token a sequence),
+                  attend_tokens (several; a beginning that all sequences share
+                  is read once) and attend_sparse (over a few pages of a long
+                  context)
   PagedKVCache    layers that share one page table and one set of lengths,
-                  pages handed out as sequences grow
+                  pages handed out as sequences grow and held in common where
+                  they begin alike
 
 The reference has no such cache: it keeps a prompt's K and V whole until
 they are compressed into tiers.  ``PagedKVCache.to_foveated`` does the latter
@@ -295,9 +299,14 @@ class PagedLayer(_Fixed):
     [i * page_size, (i + 1) * page_size) at (b, i).  A page id outside
     [0, n_pages) holds no tokens: nothing is stored there, it reads as zeros
     and takes no part in attention.  Entries past a sequence's last page are
-    not read."""
+    not read.
 
-    def __init__(self, n_pages, n_kv_heads, head_dim, page_size=64, fmt="fp16", device="cuda"):
+    With ``bounds`` the layer keeps, per page, KV head and dim, the least and
+    the largest key (bounds (n_pages, H, 2, D) bf16), by which
+    ``attend_sparse`` chooses pages; ``write`` then ends its sequences: tokens
+    behind the last one written count as not there."""
+
+    def __init__(self, n_pages, n_kv_heads, head_dim, page_size=64, fmt="fp16", device="cuda", bounds=False):
         if fmt not in FORMATS:
             raise ValueError(f"fmt must be one of {sorted(FORMATS)}, got {fmt!r}")
         shape = (int(n_pages), int(n_kv_heads), int(page_size))
@@ -313,19 +322,21 @@ class PagedLayer(_Fixed):
             k_exp = torch.full(shape, 127, dtype=torch.uint8, **new)
             v_scale = torch.full(shape, 127, dtype=torch.uint8, **new) if fmt == "fp8" else \
                 torch.zeros((*shape, 2), dtype=torch.float32, **new)
-        self._take(fmt, k, v, k_exp, v_scale)
+        b = torch.zeros((*shape[:2], 2, D), dtype=torch.bfloat16, **new) if bounds else None
+        self._take(fmt, k, v, k_exp, v_scale, b)
 
     @classmethod
-    def wrap(cls, fmt, k, v, k_exp=None, v_scale=None):
-        """A layer over existing page tensors (kept, not copied)."""
+    def wrap(cls, fmt, k, v, k_exp=None, v_scale=None, bounds=None):
+        """A layer over existing page tensors (kept, not copied).  ``bounds``
+        must be those of the keys that are there (see ``bound``)."""
         self = cls.__new__(cls)
-        self._take(fmt, k, v, k_exp, v_scale)
+        self._take(fmt, k, v, k_exp, v_scale, bounds)
         return self
 
-    def _take(self, fmt, k, v, k_exp, v_scale):
+    def _take(self, fmt, k, v, k_exp, v_scale, bounds):
         if fmt not in FORMATS:
             raise ValueError(f"fmt must be one of {sorted(FORMATS)}, got {fmt!r}")
-        _require_device(k, v, k_exp, v_scale)
+        _require_device(k, v, k_exp, v_scale, bounds)
         if k.dim() != 4:
             raise ValueError(f"k must be (n_pages, H, page_size, D), got {tuple(k.shape)}")
         n, H, page, D = k.shape
@@ -337,11 +348,13 @@ class PagedLayer(_Fixed):
                 (v_scale, (n, H, page, 2), torch.float32)
         elif k_exp is not None or v_scale is not None:
             raise ValueError(f"{fmt} pages have no scales")
+        if bounds is not None:
+            want["bounds"] = (bounds, (n, H, 2, D), torch.bfloat16)
         for name, (t, shape, dtype) in want.items():
             if t is None or tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous {shape} {dtype} tensor")
             _on(k.get_device(), name, t)
-        self.fmt, self.k, self.v, self.k_exp, self.v_scale = fmt, k, v, k_exp, v_scale
+        self.fmt, self.k, self.v, self.k_exp, self.v_scale, self.bounds = fmt, k, v, k_exp, v_scale, bounds
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, H, page, D
         self.device, self._index = k.device, k.get_device()
         c = _lib.PagesC(k.data_ptr(), v.data_ptr(), ptr(k_exp), ptr(v_scale), n, page, H, D, FORMATS[fmt])
@@ -364,7 +377,8 @@ class PagedLayer(_Fixed):
         return table, rows, P, stride if rows > 1 else P
 
     def memory_bytes(self):
-        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_exp, self.v_scale) if t is not None)
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_exp, self.v_scale, self.bounds)
+                   if t is not None)
 
     def write(self, k, v, table, start, n_new=None, q=None, rope=None, q_out=None):
         """Stores L new tokens of B sequences: k, v (B, H, L, D) fp16 / bf16 /
@@ -381,8 +395,13 @@ class PagedLayer(_Fixed):
         Positions outside the table are not stored either.  No two tokens of
         a call may name the same slot."""
         done = _lib.calls().write(self._key, k, v, table, start, n_new, q, None if rope is None else rope._key, q_out)
-        if done is not NotImplemented:
-            return done
+        if done is NotImplemented:
+            done = self._write(k, v, table, start, n_new, q, rope, q_out)
+        if self.bounds is not None:
+            self.bound(table, start, k.shape[2], n_new)
+        return done
+
+    def _write(self, k, v, table, start, n_new, q, rope, q_out):
         index = self._index
         _on(index, "k", k)
         _on(index, "v", v)
@@ -427,6 +446,24 @@ class PagedLayer(_Fixed):
             q_out.copy_(result)
         return q_out
 
+    def bound(self, table, start, n, n_new=None):
+        """The bounds of the pages that hold tokens start(b) to start(b) + n - 1
+        of each sequence (``start`` and ``n_new`` as for ``write``), from their
+        keys: what ``write`` does by itself, and what a layer over pages that
+        were filled otherwise needs once."""
+        if self.bounds is None:
+            raise ValueError("the layer keeps no bounds (PagedLayer(bounds=True), or wrap(bounds=...))")
+        index = self._index
+        table, B, P, stride = self._table(table)
+        n = int(n)
+        if not 0 <= n < 2 ** 31:
+            raise ValueError(f"n must be in [0, 2^31), got {n}")
+        pos = _positions(start, B, n, index, per_token_allowed=False)
+        if n_new is not None:
+            n_new = _lens("n_new", n_new, B, index)
+        _call(index, "fkv_paged_bounds", self._c, self.bounds.data_ptr(), B, n, table.data_ptr(), P, stride, pos,
+              None if n_new is None else n_new.data_ptr())
+
     def read(self, table, lens, max_len=None, dtype=None):
         """K and V (B, H, max_len, D) of B sequences out of their pages, in
         ``dtype`` (default: the pages' own, fp16 for quantised ones); rows
@@ -465,21 +502,8 @@ class PagedLayer(_Fixed):
         if done is not NotImplemented:
             return done
         index, D = self._index, self.head_dim
-        _on(index, "query", query)
-        shape, dtype = query.shape, query.dtype
-        if len(shape) != 4 or shape[2] != 1 or shape[3] != D or shape[1] % self.n_kv_heads or shape[1] == 0:
-            raise ValueError(f"query must be (B, a multiple of {self.n_kv_heads}, 1, {D}), got {tuple(shape)}")
-        if dtype not in (torch.float16, torch.bfloat16) or dtype != _NEW.get(self.fmt, dtype):
-            raise TypeError(f"{self.fmt} pages take {'fp16 or bf16' if self.fmt not in _NEW else self.fmt} queries, "
-                            f"got {dtype}")
+        shape, dtype, table, P, stride, lens, most = self._attention(query, table, lens, max_len, lens_add, True)
         B, Hq = shape[:2]
-        table, _, P, stride = self._table(table, B)
-        lens = _lens("lens", lens, B, index)
-        most = P * self.page_size
-        if max_len is not None and max_len < most:
-            most = int(max_len)
-        if not -2 ** 31 <= lens_add < 2 ** 31:
-            raise ValueError(f"lens_add must fit 32 bits, got {lens_add}")
         rows, held = _rows(query, shape)
         if out is None:
             out = torch.empty_like(query, memory_format=torch.contiguous_format)
@@ -496,6 +520,108 @@ class PagedLayer(_Fixed):
               lens.data_ptr(), lens_add, most, D ** -0.5 if scale is None else scale, out.data_ptr(), ptr(lse),
               None if ws is None else ws.data_ptr(), n)
         return (out, lse) if return_lse else out
+
+    def _attention(self, query, table, lens, max_len, lens_add, one):
+        """An attention call's arguments -> the query's shape and type, the table
+        with its width and stride, the lengths, their upper bound."""
+        index, D = self._index, self.head_dim
+        _on(index, "query", query)
+        shape, dtype = query.shape, query.dtype
+        if len(shape) != 4 or (one and shape[2] != 1) or shape[3] != D or shape[1] % self.n_kv_heads or shape[1] == 0:
+            raise ValueError(f"query must be (B, a multiple of {self.n_kv_heads}, {1 if one else 'L'}, {D}), "
+                             f"got {tuple(shape)}")
+        if dtype not in (torch.float16, torch.bfloat16) or dtype != _NEW.get(self.fmt, dtype):
+            raise TypeError(f"{self.fmt} pages take {'fp16 or bf16' if self.fmt not in _NEW else self.fmt} queries, "
+                            f"got {dtype}")
+        table, _, P, stride = self._table(table, shape[0])
+        lens = _lens("lens", lens, shape[0], index)
+        most = P * self.page_size
+        if max_len is not None and max_len < most:
+            most = int(max_len)
+        if not -2 ** 31 <= lens_add < 2 ** 31:
+            raise ValueError(f"lens_add must fit 32 bits, got {lens_add}")
+        return shape, dtype, table, P, stride, lens, most
+
+    def attend_tokens(self, query, table, lens, max_len=None, lens_add=0, scale=None, out=None, return_lse=False,
+                      n_new=None, shared=0):
+        """``attend`` of the newest L tokens of each sequence (drafted tokens, a
+        prompt's chunk), query (B, Hq, L, D): query l sees the tokens up to
+        itself, all of the first lens[b] + lens_add but the last L - 1 - l.
+        -> out (B, Hq, L, D), and with ``return_lse`` (B, Hq, L) fp32.
+
+        ``n_new`` (B,) int32 on the device: only the first n_new[b] queries of
+        sequence b are real, and its tokens end with theirs; the rest of a padded
+        batch comes back as ``out`` held it (zero in a new tensor), -inf in lse.
+
+        ``shared`` tokens at the beginning (whole pages) lie in the pages of the
+        table's first row for all sequences: they are read from that row alone,
+        once for all.
+
+        ``out`` may have any strides, and be the query."""
+        index = self._index
+        shape, dtype, table, P, stride, lens, most = self._attention(query, table, lens, max_len, lens_add, False)
+        B, Hq, L, D = shape
+        shared = operator.index(shared)
+        if not 0 <= shared <= P * self.page_size or shared % self.page_size:
+            raise ValueError(f"shared must be whole pages of {self.page_size} tokens within the table's "
+                             f"{P * self.page_size}, got {shared}")
+        if n_new is not None:
+            n_new = _lens("n_new", n_new, B, index)
+        if out is None:
+            out = torch.empty_like(query) if n_new is None else torch.zeros_like(query)
+        else:
+            _result(index, "out", out, shape, dtype)
+        rows, held = _rows(query, shape)
+        dst, result = _rows(out, shape)
+        lse = torch.empty((B, Hq, L), dtype=torch.float32, device=self.device) if return_lse else None
+        n = _lib.load().fkv_paged_attn_rows_workspace(self._c, Hq, B, L, shared, most)
+        if n < 0:
+            check(n, "fkv_paged_attn_rows_workspace")
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        _call(index, "fkv_paged_attn_rows", self._c, rows, dtype_code(dtype), Hq, B, L, table.data_ptr(), P, stride,
+              lens.data_ptr(), lens_add, None if n_new is None else n_new.data_ptr(), shared, most,
+              D ** -0.5 if scale is None else scale, dst, ptr(lse), None if ws is None else ws.data_ptr(), n)
+        if result is not out:
+            out.copy_(result)
+        return (out, lse) if return_lse else out
+
+    def attend_sparse(self, query, table, lens, n_select, max_len=None, lens_add=0, scale=None, out=None,
+                      return_lse=False, return_pages=False):
+        """``attend`` of one new token per sequence over ``n_select`` pages of it
+        for each KV head: its newest page, and those whose bounds (the layer's
+        ``bounds``) promise the largest scores with any of the head's queries; all
+        pages of a sequence that has no more.  ``return_pages``: also which,
+        (B, H, n_select) int32, ascending, as entries of the sequence's table row,
+        then -1.  ``scale`` must not be negative."""
+        if self.bounds is None:
+            raise ValueError("the layer keeps no bounds (PagedLayer(bounds=True), or wrap(bounds=...))")
+        index = self._index
+        shape, dtype, table, P, stride, lens, most = self._attention(query, table, lens, max_len, lens_add, True)
+        B, Hq, _, D = shape
+        n_select = operator.index(n_select)
+        if n_select < 1:
+            raise ValueError(f"n_select must be positive, got {n_select}")
+        n_select = min(n_select, 2 ** 31 - 1)
+        if B > 1 and query.stride(0) != Hq * query.stride(1):
+            query = query.contiguous()
+        rows, held = _rows(query, shape)
+        if out is None:
+            out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        else:
+            _on(index, "out", out)
+            if out.shape != shape or out.dtype != dtype or not out.is_contiguous() or out.data_ptr() % 16:
+                raise ValueError(f"out must be a contiguous, 16-byte aligned {tuple(shape)} {dtype} tensor")
+        lse = torch.empty((B, Hq), dtype=torch.float32, device=self.device) if return_lse else None
+        pages = torch.empty((B, self.n_kv_heads, n_select), dtype=torch.int32, device=self.device) if return_pages else None
+        n = _lib.load().fkv_paged_attn_sparse_workspace(self._c, Hq, B, P, n_select, most)
+        if n < 0:
+            check(n, "fkv_paged_attn_sparse_workspace")
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+        _call(index, "fkv_paged_attn_sparse", self._c, self.bounds.data_ptr(), rows, dtype_code(dtype), Hq, B,
+              table.data_ptr(), P, stride, lens.data_ptr(), lens_add, most, n_select, D ** -0.5 if scale is None else scale,
+              out.data_ptr(), ptr(lse), ptr(pages), ptr(ws), n)
+        done = (out,) + ((lse,) if return_lse else ()) + ((pages,) if return_pages else ())
+        return done if len(done) > 1 else out
 
 
 # ---------------------------------------------------------------------------

@@ -685,6 +685,74 @@ int fkv_paged_attn(const fkv_pages* pages, const fkv_rows* query, int32_t q_dtyp
                    int32_t lens_add, int64_t max_len, float scale, void* out, float* lse, void* workspace,
                    int64_t workspace_bytes, void* stream);
 
+/* Attention of L new tokens per sequence, of which n_new[b] (int32 in device
+ * memory, NULL: L) are real: query rows (B, Hq, L) of q_dtype, query l of
+ * sequence b over the first len_b - n_new[b] + l + 1 tokens, len_b = lens[b] +
+ * lens_add clamped to [0, n_table * page_size], out rows of the same type (they
+ * may be the query's, and else share no memory with them or one another), lse
+ * (B, Hq, L) fp32 or NULL.  A query without tokens gives 0 and -inf; a padded
+ * one is not written, its lse -inf.  The first `shared` tokens (whole pages, at
+ * most the table's; 0: none) lie in the pages of the table's first row for every
+ * sequence, and are read there alone, for as many of them as a sequence has.
+ * Tokens that a query does not attend to take no part in it, whatever they are.
+ * Types, max_len and workspace as for fkv_paged_attn.  Asynchronous,
+ * capturable. */
+int64_t fkv_paged_attn_rows_workspace(const fkv_pages* pages, int32_t Hq, int32_t B, int32_t L, int64_t shared,
+                                      int64_t max_len);
+int fkv_paged_attn_rows(const fkv_pages* pages, const fkv_rows* query, int32_t q_dtype, int32_t Hq, int32_t B,
+                        int32_t L, const int32_t* table, int32_t n_table, int64_t table_stride,
+                        const int32_t* lens, int32_t lens_add, const int32_t* n_new, int64_t shared,
+                        int64_t max_len, float scale, const fkv_rows* out, float* lse, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
+/* Bounds of the pages' keys: bounds (n_pages, H, 2, D) bf16, 16-byte aligned,
+ * the least and the largest element per dim of each page's keys as they are
+ * stored, rounded downwards and upwards (a NaN counts as none).  Computed anew for
+ * the pages that hold tokens start(b) to start(b) + min(n_new[b], L) - 1 of B
+ * sequences, from each one's first token to the last new one: tokens behind that
+ * count as not there.  Pages outside the table or the pool are left out.
+ * Asynchronous, capturable. */
+int fkv_paged_bounds(const fkv_pages* pages, void* bounds, int32_t B, int32_t L, const int32_t* table,
+                     int32_t n_table, int64_t table_stride, const fkv_positions* start, const int32_t* n_new,
+                     void* stream);
+
+/* Attention of one new token per sequence over n_select pages of its cache for
+ * each KV head: the newest one and those whose bounds promise the largest scores,
+ * max over the KV head's queries of sum_d max(q_d least_d, q_d largest_d), computed
+ * in 64 bits (equal ones: the lower page; a bound that is not finite: first; a
+ * page id outside the pool: last); all pages where there are no more.  selected (B,
+ * H, n_select) int32 or NULL: the pages, ascending, as entries of the sequence's
+ * table row, then -1.  scale must not be negative; the query's rows of neighbouring
+ * sequences follow one another (stride_b = Hq * stride_h).  Otherwise as
+ * fkv_paged_attn, over the selected pages' tokens.  At most 4096 sequences times
+ * KV heads. */
+int64_t fkv_paged_attn_sparse_workspace(const fkv_pages* pages, int32_t Hq, int32_t B, int32_t n_table,
+                                        int32_t n_select, int64_t max_len);
+int fkv_paged_attn_sparse(const fkv_pages* pages, const void* bounds, const fkv_rows* query, int32_t q_dtype,
+                          int32_t Hq, int32_t B, const int32_t* table, int32_t n_table, int64_t table_stride,
+                          const int32_t* lens, int32_t lens_add, int64_t max_len, int32_t n_select, float scale,
+                          void* out, float* lse, int32_t* selected, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+
+/* Verification of n_draft[b] (int32 in device memory, clamped to [0, K]; NULL:
+ * K <= 63) drafted tokens of B sequences.  target rows (b, i), i <= K: the
+ * target's probabilities after i drafted tokens, V numbers of dtype at data +
+ * b * stride_b + i * stride_l (stride_h is not read; any alignment); draft rows
+ * (b, i), i < K: those that token i was drawn from (NULL: all on that token);
+ * tokens (B, K) int32, or int64 with tokens64; uniforms (B, K + 1) fp32 in [0, 1).
+ * Token i stands while uniforms[b][i] * draft(token) < target(token), a token
+ * outside the vocabulary never; accepted (B) int32 counts them up to the first
+ * that does not.  The next token is the first at which the running sum of the
+ * weights exceeds uniforms[b][K] times their sum: max(target - draft, 0) where a
+ * token was refused (the target's own where that leaves nothing), the target's
+ * where all stand; -1 where the sum is not a positive number.  out_tokens (B, K + 1)
+ * of the tokens' type: the accepted ones, the next one, then -1.  Products and
+ * sums are in 64 bits.  Asynchronous, capturable. */
+int64_t fkv_verify_drafts_workspace(int32_t B, int32_t K, int32_t V);
+int fkv_verify_drafts(const fkv_rows* target, const fkv_rows* draft, int32_t dtype, int32_t B, int32_t K, int32_t V,
+                      const void* tokens, int32_t tokens64, const float* uniforms, const int32_t* n_draft,
+                      void* out_tokens, int32_t* accepted, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Benchmark utility with no counterpart in the reference: streams `bytes`
  * (a multiple of 16) from device buffer `buf` with 16-byte lane loads,
  * `unroll` (1, 2, 4, 8) loads in flight per lane, optionally non-temporal,
