@@ -44,7 +44,9 @@ computed as ``offset + arange(L)``).
 Extension: ``generate_paged`` serves a batch of prompts from a
 ``PagedKVCache`` (paged.py): each prompt is prefilled into its own pages, then
 all sequences decode together, every layer's one-token call being answered by
-the cache's paged attention (``install_paged_attention``).
+the cache's paged attention (``install_paged_attention``).  Prompts that begin
+alike can hold that beginning in common, and a smaller model can draft tokens
+that the model then verifies several at a time.
 """
 
 import shutil
@@ -57,6 +59,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
+from .drafts import verify_drafts
 from .promotion import PromotionPipeline
 from .tier_cache import MLXFoveatedKVCache, MLXTierConfig
 
@@ -334,11 +337,13 @@ class PagedCacheWrapper:
     at position start(b) + l of the rows handed back, of which those past the
     sequence's tokens are zeros or padding.  With one token it leaves the write
     to the attention call that follows, which rotates the query in the same
-    launch and attends to every stored token (``attn_mask`` is not looked at)."""
+    launch and attends to every stored token (``attn_mask`` is not looked at);
+    with ``in_place`` so it does with several, each of which sees the tokens up to
+    itself."""
 
-    def __init__(self, cache, layer_idx, seqs=None):
+    def __init__(self, cache, layer_idx, seqs=None, in_place=False):
         self.cache, self.layer_idx, self.seqs = cache, layer_idx, cache.pages._range(seqs)
-        self.rope = cache.rope
+        self.rope, self.in_place = cache.rope, in_place
         self._new, self._n_new = None, 0
 
     @property
@@ -353,7 +358,7 @@ class PagedCacheWrapper:
         if _paged_state["original"] is None:
             raise RuntimeError("paged attention is not installed")
         fetched, n = (keys, values), keys.shape[2]
-        if n == 1:
+        if n == 1 or self.in_place:
             self._new = fetched
         else:
             self.cache.write(self.layer_idx, keys, values, seqs=self.seqs)
@@ -371,7 +376,8 @@ class PagedCacheWrapper:
         layer = self.cache.layers[self.layer_idx]
         want = {"fp16": torch.float16, "bf16": torch.bfloat16}.get(
             layer.fmt, query.dtype if query.dtype != torch.float32 else torch.float16)
-        return self.cache.attend(self.layer_idx, q.to(want), seqs=self.seqs, scale=scale).to(query.dtype)
+        attend = self.cache.attend if self._n_new == 1 else self.cache.attend_tokens
+        return attend(self.layer_idx, q.to(want), seqs=self.seqs, scale=scale).to(query.dtype)
 
 
 def _paged_interceptor(query, key, value, attn_mask=None, dropout_p=0.0, is_causal=False, scale=None, **kwargs):
@@ -380,7 +386,7 @@ def _paged_interceptor(query, key, value, attn_mask=None, dropout_p=0.0, is_caus
         if query.dim() != 4 or query.shape[2] != w._n_new:
             raise RuntimeError(f"update_and_fetch took {w._n_new} tokens, the attention call has queries "
                                f"{tuple(query.shape)}")
-        if w._n_new == 1:
+        if w._n_new == 1 or w.in_place:
             return w._answer(query, scale)
         if w.rope is not None:
             query = w.rope(query, w.offset)
@@ -400,9 +406,9 @@ def install_paged_attention(cache, seqs=None) -> list:
     return paged_wrappers(cache, seqs)
 
 
-def paged_wrappers(cache, seqs=None) -> list:
+def paged_wrappers(cache, seqs=None, in_place=False) -> list:
     """One ``PagedCacheWrapper`` per layer for the sequences ``seqs``."""
-    return [PagedCacheWrapper(cache, i, seqs) for i in range(len(cache.layers))]
+    return [PagedCacheWrapper(cache, i, seqs, in_place) for i in range(len(cache.layers))]
 
 
 def uninstall_paged_attention() -> None:
@@ -411,7 +417,106 @@ def uninstall_paged_attention() -> None:
         _paged_state["original"] = _paged_state["pending"] = None
 
 
-def generate_paged(model, tokenizer, prompts, cache, max_tokens: int = 100, temp: float = 0.0):
+def _common_tokens(ids, page_size):
+    """Tokens that all prompts begin with, in whole pages, leaving each prompt one
+    more at least."""
+    n = 0
+    for column in zip(*ids):
+        if len(set(column)) > 1:
+            break
+        n += 1
+    return min(n, min(len(i) for i in ids) - 1) // page_size * page_size
+
+
+def _prefill_paged(model, cache, ids, shared, device):
+    """Every prompt into its own sequence, the first ``shared`` tokens held in
+    common -> the logits of each one's last token."""
+    logits = []
+    for b, tok in enumerate(ids):
+        at = slice(b, b + 1)
+        held = shared if b else 0
+        if held:
+            cache.share(0, held, at)
+        cache.extend(len(tok) - held, at)
+        x = torch.tensor([tok[held:]], dtype=torch.long, device=device)
+        logits.append(model(x, cache=paged_wrappers(cache, at, in_place=held > 0))[:, -1, :])
+    return torch.cat(logits)
+
+
+def _probabilities(logits, temp):
+    """What tokens are drawn from: softmax(logits / temp), or all of it on the
+    largest."""
+    if temp == 0:
+        return torch.zeros_like(logits, dtype=torch.float32).scatter_(-1, logits.argmax(-1, keepdim=True), 1.0)
+    return torch.softmax(logits.float() / temp, dim=-1)
+
+
+class _Drafter:
+    """Tokens drafted by a smaller model with a ``PagedKVCache`` of its own, which
+    holds the same tokens of the same sequences as the target's."""
+
+    def __init__(self, model, cache, n):
+        self.model, self.cache, self.n = model, cache, n
+
+    def draft(self, tok, counts, temp):
+        """counts[b] tokens after tok (B,) for each sequence (-1: a finished one)
+        -> tokens (B, most), and the probabilities that they were drawn from
+        (None where none were).  Stores tok and every drafted token."""
+        B, most = len(counts), max(counts)
+        wrappers = paged_wrappers(self.cache, slice(0, B))
+        tokens, probs = [], []
+        for i in range(most + 1):
+            self.cache.extend([int(i <= n) for n in counts], slice(0, B))
+            logits = self.model(tok.reshape(B, 1), cache=wrappers)[:, -1, :]
+            if i < most:
+                tok = _next_token(logits, temp)
+                tokens.append(tok)
+                probs.append(_probabilities(logits, temp) if temp else None)
+        if not tokens:
+            return torch.zeros((B, 0), dtype=torch.long, device=tok.device), None
+        return torch.stack(tokens, 1), torch.stack(probs, 1) if temp else None
+
+
+def _decode_drafted(model, cache, drafter, tok, out, done, max_tokens, temp, eos):
+    """Rounds of drafting and verifying: each appends to every sequence the
+    drafted tokens that stand and the one that follows them.  -> (model calls,
+    drafted tokens, accepted tokens)"""
+    B = len(out)
+    batch, wrappers = slice(0, B), paged_wrappers(cache, slice(0, B), in_place=True)
+    calls = drafted = stood = 0
+    done[:] = [d or len(o) >= max_tokens for d, o in zip(done, out)]
+    while not all(done):
+        # (a sequence near its end drafts no more than it may still take)
+        counts = [-1 if d else min(drafter.n, max_tokens - len(o)) for d, o in zip(done, out)]
+        tokens, probs = drafter.draft(tok, counts, temp)
+        cache.extend([n + 1 for n in counts], batch)
+        logits = model(torch.cat([tok.reshape(B, 1), tokens], 1), cache=wrappers)
+        calls += 1
+        K = tokens.shape[1]
+        uniforms = torch.rand((B, K + 1), device=tok.device) if temp else torch.full((B, K + 1), 0.5, device=tok.device)
+        n_draft = torch.tensor([max(n, 0) for n in counts], dtype=torch.int32, device=tok.device)
+        taken, accepted = verify_drafts(_probabilities(logits, temp), probs, tokens, uniforms, n_draft=n_draft)
+        tok = taken.gather(1, accepted.long()[:, None]).clamp_min(0)[:, 0]
+        back = []
+        for b, (row, a, n) in enumerate(zip(taken.tolist(), accepted.tolist(), counts)):
+            back.append(n - a if n > 0 else 0)
+            if done[b]:
+                continue
+            drafted, stood = drafted + n, stood + a
+            if row[a] < 0:
+                raise RuntimeError(f"the model's logits for sequence {b} are not numbers that tokens can be drawn by")
+            for t in row[:a + 1]:
+                done[b] = done[b] or t == eos or len(out[b]) == max_tokens
+                if not done[b]:
+                    out[b].append(t)
+            done[b] = done[b] or len(out[b]) == max_tokens
+        cache.rollback(back, batch)
+        drafter.cache.rollback(back, batch)
+    return calls, drafted, stood
+
+
+def generate_paged(model, tokenizer, prompts, cache, max_tokens: int = 100, temp: float = 0.0, share_prefix=False,
+                   draft_model=None, draft_cache=None, n_draft: int = 4):
     """Prefill ``prompts`` (a list, or one string) into sequences 0, 1, ... of
     the ``PagedKVCache`` ``cache``, which must be free, and decode them
     together for up to ``max_tokens`` tokens each -> (texts, stats); one text
@@ -421,31 +526,48 @@ def generate_paged(model, tokenizer, prompts, cache, max_tokens: int = 100, temp
     Where ``cache.rope`` is set the model must leave the rotation to the
     cache, and prompts may have different lengths.  Without it the model
     rotates by ``cache.offset``, a number for the whole batch: prompts then
-    need one length."""
+    need one length.
+
+    ``share_prefix``: the whole pages that all prompts begin with alike are
+    prefilled once, held in common, and attended to once for all sequences.
+
+    ``draft_model`` with ``draft_cache``, a ``PagedKVCache`` of its own with the
+    same room: it drafts ``n_draft`` tokens a round, which the model verifies in
+    one call (``verify_drafts``).  Tokens are distributed as the model's own, and
+    with temp=0 they are its largest.  Both caches must rotate."""
     one = isinstance(prompts, str)
     dev = _model_device(model)
     ids = [tokenizer.encode(p) for p in ([prompts] if one else prompts)]
     B = len(ids)
     if B == 0 or min(len(i) for i in ids) == 0:
         raise ValueError("generate_paged needs prompts of at least one token")
-    if B > cache.pages.max_seqs or any(cache.pages.lengths(slice(0, B))):
-        raise ValueError(f"sequences 0 to {B - 1} of the cache must be there and free")
     if cache.rope is None and len({len(i) for i in ids}) > 1:
         raise ValueError("prompts of different lengths need a cache that rotates (PagedKVCache(rope=...))")
+    drafter = None
+    if draft_model is not None or draft_cache is not None:
+        if draft_model is None or draft_cache is None:
+            raise ValueError("drafting needs draft_model and draft_cache")
+        if cache.rope is None or draft_cache.rope is None or draft_cache is cache:
+            raise ValueError("drafting needs two caches that rotate (PagedKVCache(rope=...))")
+        if not 1 <= n_draft <= 63:
+            raise ValueError(f"n_draft must be from 1 to 63, got {n_draft}")
+        drafter = _Drafter(draft_model, draft_cache, n_draft)
+    caches = [cache] + ([draft_cache] if drafter else [])
+    if any(B > c.pages.max_seqs or any(c.pages.lengths(slice(0, B))) for c in caches):
+        raise ValueError(f"sequences 0 to {B - 1} of the cache must be there and free")
     batch = slice(0, B)
     eos = getattr(tokenizer, "eos_token_id", None)
     out = [[] for _ in range(B)]
     done = [False] * B
+    shared = [_common_tokens(ids, c.pages.page_size) if share_prefix and B > 1 else 0 for c in caches]
+    drafted = stood = 0
     install_paged_attention(cache)
     try:
         with torch.no_grad():
             t0 = time.perf_counter()
-            logits = []
-            for b, tok in enumerate(ids):
-                cache.extend(len(tok), slice(b, b + 1))
-                x = torch.tensor([tok], dtype=torch.long, device=dev)
-                logits.append(model(x, cache=paged_wrappers(cache, slice(b, b + 1)))[:, -1, :])
-            logits = torch.cat(logits)
+            logits = _prefill_paged(model, cache, ids, shared[0], dev)
+            if drafter:
+                _prefill_paged(draft_model, draft_cache, ids, shared[1], dev)
             torch.cuda.synchronize(dev)
             t_prefill = time.perf_counter() - t0
             t0 = time.perf_counter()
@@ -459,6 +581,9 @@ def generate_paged(model, tokenizer, prompts, cache, max_tokens: int = 100, temp
                         out[b].append(t)
                 if all(done):
                     break
+                if drafter:
+                    steps, drafted, stood = _decode_drafted(model, cache, drafter, tok, out, done, max_tokens, temp, eos)
+                    break
                 # (a finished sequence takes no more pages where the batch need not
                 # keep one length)
                 more = [0 if d else 1 for d in done] if cache.rope is not None and any(done) else 1
@@ -470,13 +595,18 @@ def generate_paged(model, tokenizer, prompts, cache, max_tokens: int = 100, temp
     finally:
         uninstall_paged_attention()
         stored = cache.pages.lengths(batch)
-        for b in range(B):
-            cache.free(b)
+        for c in caches:
+            for b in range(B):
+                c.free(b)
     texts = [tokenizer.decode(o) for o in out]
     n = sum(len(o) for o in out)
     stats = {"prompt_tokens": [len(i) for i in ids], "generated_tokens": [len(o) for o in out],
              "stored_tokens": stored, "model_calls": steps, "prefill_time_s": t_prefill, "decode_time_s": t_decode,
              "tokens_per_second": n / max(t_decode, 1e-6), "cache_mb": cache.memory_bytes() / 2 ** 20}
+    if share_prefix:
+        stats["shared_tokens"] = shared[0]
+    if drafter:
+        stats["drafted_tokens"], stats["accepted_tokens"] = drafted, stood
     return (texts[0] if one else texts), stats
 
 

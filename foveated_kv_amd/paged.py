@@ -636,7 +636,11 @@ class PageTable:
     nothing is held, ``lens``, ``start`` and ``new`` (max_seqs,) int32: the
     tokens of each sequence now, before its last ``extend``, and their
     difference.  The host keeps its own copy and hands out pages; device
-    updates are work on the current stream."""
+    updates are work on the current stream.
+
+    Sequences may hold their first pages in common (``share``): a page goes back
+    to the pool when the last of them is freed.  The last tokens of a sequence
+    can be taken back (``rollback``), as those of refused drafts."""
 
     def __init__(self, n_pages, page_size, max_seqs, max_tokens, device="cuda"):
         n_pages, page_size, max_seqs, max_tokens = (int(x) for x in (n_pages, page_size, max_seqs, max_tokens))
@@ -652,6 +656,8 @@ class PageTable:
         self._pages = [[] for _ in range(max_seqs)]
         self._lens = [0] * max_seqs
         self._new = [0] * max_seqs
+        self._holders = [0] * n_pages  # sequences that hold each page
+        self._common = {}  # (first, stop) -> pages that those sequences begin with in common
 
     @property
     def free_pages(self):
@@ -718,6 +724,7 @@ class PageTable:
                 cols.append(len(self._pages[b]))
                 ids.append(self._free.pop())
                 self._pages[b].append(ids[-1])
+                self._holders[ids[-1]] = 1
         if ids:
             d = self.table.device
             self.table[torch.tensor(rows, device=d), torch.tensor(cols, device=d)] = \
@@ -730,7 +737,7 @@ class PageTable:
         sl = self._range(seqs)
         each = self._each(n, sl.stop - sl.start)
         if each and min(each) < 0:
-            raise ValueError("sequences do not shrink (free them)")
+            raise ValueError("sequences do not shrink (rollback, or free them)")
         self.reserve([a + t for a, t in zip(self._lens[sl], each)], seqs=sl)
         start, new, lens = (self._view(t, sl) for t in (self.start, self.new, self.lens))
         start.copy_(lens)
@@ -740,13 +747,84 @@ class PageTable:
         lens.add_(new)
         self._lens[sl] = [a + t for a, t in zip(self._lens[sl], each)]
 
+    def share(self, src, tokens, seqs=None):
+        """The sequences, which must be free, begin with the first ``tokens``
+        tokens of sequence ``src``: whole pages, held in common."""
+        self._not_captured()
+        sl = self._range(seqs)
+        src, tokens = operator.index(src), operator.index(tokens)
+        if not 0 <= src < self.max_seqs:
+            raise ValueError(f"no sequence {src}")
+        if tokens % self.page_size or not 0 <= tokens <= self._lens[src]:
+            raise ValueError(f"shared tokens must fill whole pages of {self.page_size} within the {self._lens[src]} of "
+                             f"sequence {src}, got {tokens}")
+        if any(self._pages[sl]):
+            raise ValueError("sequences that take a beginning from another one must be free")
+        n = tokens // self.page_size
+        pages = self._pages[src][:n]
+        if sl.stop == sl.start:
+            return
+        for b in range(sl.start, sl.stop):
+            self._pages[b] = list(pages)
+            self._lens[b], self._new[b] = tokens, 0
+        for p in pages:
+            self._holders[p] += sl.stop - sl.start
+        self.table[sl, :n] = self.table[src, :n].clone()
+        self.lens[sl].fill_(tokens)
+        self.start[sl].fill_(tokens)
+        self.new[sl].fill_(0)
+        self._common.clear()
+
+    def common_tokens(self, seqs=None):
+        """Tokens that the sequences (two or more) begin with in the same pages."""
+        sl = self._range(seqs)
+        key = sl.start, sl.stop
+        n = self._common.get(key)
+        if n is None:
+            n = 0
+            if sl.stop - sl.start > 1:
+                # (pages held by one sequence alone are the last ones)
+                for column in zip(*self._pages[sl]):
+                    if self._holders[column[0]] == 1 or len(set(column)) > 1:
+                        break
+                    n += 1
+            self._common[key] = n
+        return n * self.page_size
+
+    def rollback(self, n=1, seqs=None):
+        """Takes back each sequence's last ``n`` tokens (a number, or one per
+        sequence); its pages stay with it.  Tokens in pages that other sequences
+        hold too cannot be taken back."""
+        self._not_captured()
+        sl = self._range(seqs)
+        each = self._each(n, sl.stop - sl.start)
+        for b, t in zip(range(sl.start, sl.stop), each):
+            if not 0 <= t <= self._lens[b]:
+                raise ValueError(f"sequence {b} has {self._lens[b]} tokens, {t} cannot be taken back")
+            kept = self._lens[b] - t
+            held = -(-self._lens[b] // self.page_size)
+            if t and any(self._holders[p] > 1 for p in self._pages[b][kept // self.page_size:held]):
+                raise ValueError(f"sequence {b} shares pages of the tokens to be taken back")
+        if not any(each):
+            return
+        self._lens[sl] = [a - t for a, t in zip(self._lens[sl], each)]
+        self._new[sl] = [max(a - t, 0) for a, t in zip(self._new[sl], each)]
+        for t, kept in ((self.lens, self._lens), (self.new, self._new)):
+            self._view(t, sl).copy_(torch.tensor(kept[sl], dtype=torch.int32))
+        torch.sub(self._view(self.lens, sl), self._view(self.new, sl), out=self._view(self.start, sl))
+
     def free(self, seq):
-        """Sequence ``seq`` is over: its pages go back to the pool."""
+        """Sequence ``seq`` is over: its pages go back to the pool, but for those
+        that other sequences hold too."""
         if not 0 <= seq < self.max_seqs:
             raise ValueError(f"no sequence {seq}")
         self._not_captured()
-        self._free.extend(reversed(self._pages[seq]))
+        for p in reversed(self._pages[seq]):
+            self._holders[p] -= 1
+            if self._holders[p] == 0:
+                self._free.append(p)
         self._pages[seq] = []
+        self._common.clear()
         self._lens[seq] = self._new[seq] = 0
         self.table[seq].fill_(-1)
         for t in (self.lens, self.start, self.new):
@@ -760,17 +838,27 @@ class PagedKVCache:
         cache.extend(n)                          # n tokens more per sequence
         q = cache.write(layer, k, v, q)          # rotated, encoded, stored
         out = cache.attend(layer, q)             # one-token queries
+        out = cache.attend_tokens(layer, q)      # queries of all the new tokens
         k, v = cache.read(layer)                 # what is stored
+        cache.share(0, 512, slice(1, 8))         # free sequences begin as sequence 0
+        cache.rollback(n)                        # the last n tokens again
 
     ``seqs`` (a slice, default all sequences) picks the neighbouring
     sequences that a call's batch stands for.  With ``rope`` the cache rotates
-    what it is handed; without it keys and queries come rotated."""
+    what it is handed; without it keys and queries come rotated.  Pages that all
+    sequences of a call begin with are attended to once for all of them.  With
+    ``sparse_pages`` layers keep bounds of their pages, and ``attend`` takes that
+    many pages of each sequence (``PagedLayer.attend_sparse``)."""
 
     def __init__(self, n_layers, n_kv_heads, head_dim, n_pages, max_seqs=1, max_tokens=32768, page_size=64,
-                 fmt="fp16", rope=None, device="cuda"):
+                 fmt="fp16", rope=None, device="cuda", sparse_pages=0):
         if rope is not None and rope.head_dim != head_dim:
             raise ValueError(f"rope is for head dim {rope.head_dim}, not {head_dim}")
-        self.layers = [PagedLayer(n_pages, n_kv_heads, head_dim, page_size, fmt, device) for _ in range(n_layers)]
+        if operator.index(sparse_pages) < 0:
+            raise ValueError(f"sparse_pages must not be negative, got {sparse_pages}")
+        self.sparse_pages = operator.index(sparse_pages)
+        self.layers = [PagedLayer(n_pages, n_kv_heads, head_dim, page_size, fmt, device, bounds=self.sparse_pages > 0)
+                       for _ in range(n_layers)]
         self.pages = PageTable(n_pages, page_size, max_seqs, max_tokens, device)
         self.rope, self.fmt = rope, fmt
 
@@ -790,6 +878,14 @@ class PagedKVCache:
     def free(self, seq):
         self.pages.free(seq)
 
+    def share(self, src, tokens, seqs=None):
+        """As ``PageTable.share``: the sequences begin with ``src``'s first tokens."""
+        self.pages.share(src, tokens, seqs)
+
+    def rollback(self, n=1, seqs=None):
+        """As ``PageTable.rollback``: takes back each sequence's last tokens."""
+        self.pages.rollback(n, seqs)
+
     def _batch(self, seqs):
         sl = self.pages._range(seqs)
         return sl, self.pages._view(self.pages.table, sl)
@@ -807,8 +903,26 @@ class PagedKVCache:
 
     def attend(self, layer, query, seqs=None, scale=None, out=None):
         sl, table = self._batch(seqs)
-        return self.layers[layer].attend(query, table, self.pages._view(self.pages.lens, sl), max(self.pages._lens[sl], default=0),
-                                         scale=scale, out=out)
+        lens, most = self.pages._view(self.pages.lens, sl), max(self.pages._lens[sl], default=0)
+        if self.sparse_pages:
+            return self.layers[layer].attend_sparse(query, table, lens, self.sparse_pages, most, scale=scale, out=out)
+        shared = self.pages.common_tokens(sl)
+        if shared:
+            return self.layers[layer].attend_tokens(query, table, lens, most, scale=scale, out=out, shared=shared)
+        return self.layers[layer].attend(query, table, lens, most, scale=scale, out=out)
+
+    def attend_tokens(self, layer, query, seqs=None, scale=None, out=None):
+        """Attention of all new tokens of the last ``extend`` of the same
+        sequences, each over those up to itself; see
+        ``PagedLayer.attend_tokens``."""
+        sl, table = self._batch(seqs)
+        new = self.pages._new[sl]
+        if new and max(new) != query.shape[2]:
+            raise ValueError(f"query holds {query.shape[2]} tokens, the last extend made room for {max(new)}")
+        n_new = None if len(set(new)) <= 1 else self.pages._view(self.pages.new, sl)
+        return self.layers[layer].attend_tokens(query, table, self.pages._view(self.pages.lens, sl),
+                                                max(self.pages._lens[sl], default=0), scale=scale, out=out, n_new=n_new,
+                                                shared=self.pages.common_tokens(sl))
 
     def read(self, layer, seqs=None, dtype=None):
         """K, V (B, H, longest length, D); rows past a sequence's length are
