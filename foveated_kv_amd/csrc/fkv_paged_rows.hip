@@ -53,6 +53,10 @@ constexpr float kLowest = -3.402823466e38f;  // running maximum before the first
 // it by more than 2^8, and stays 2^7 below the scores of fp16 pages, whose
 // weights (2^15 at most) so keep away from the end of fp16's range.
 constexpr float kRowSlack = 8.0f;
+// Scores are scaled and the maximum taken off by one fma, whose product is not
+// rounded as the maximum was: a difference of 2^-4 at most up to here; beyond,
+// where it would be a power, in two steps.
+constexpr float kWide = 1048576.0f;
 template <int FMT>
 constexpr float kRowBias = FMT == FKV_PAGES_F16 ? 7.0f : 0.0f;
 
@@ -74,7 +78,8 @@ struct RowsArgs {
     float* records;  // workspace: per row and part D numerators, maximum, sum
     RowParts common, own;
     int32_t lens_add, B, Hq, G, L, shared;
-    float scale;  // scale * log2(e)
+    float scale;      // |scale| * log2(e)
+    uint32_t q_sign, q_mask;  // its sign, for two 16-bit numbers; 0 where it is 0 (and |scale| 1)
 };
 
 typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
@@ -228,7 +233,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
         const char* at = a.q.data + 2 * (b * a.q.sb + hq * a.q.sh + l * a.q.sl);
         const u4 none = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < D / 16; i++) q[i] = real ? *(const u4*)(at + 32 * i + 16 * hf) : none;
+        for (int i = 0; i < D / 16; i++) q[i] = real ? (*(const u4*)(at + 32 * i + 16 * hf) & a.q_mask) ^ a.q_sign : none;
     }
 
     const int32_t* ids = a.table.ids + (seq < 0 ? 0 : seq) * a.table.stride;
@@ -364,30 +369,41 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
     float m = kLowest, sum = 0.0f, z = 0.0f;
+    bool wide = false;  // (of any of the wave's rows)
 
-    // V^T's operand: this lane's row and bytes of a transposing read
-    const uint32_t tr_row = 4 * hf + ((lane & 15) >> 2), tr_byte = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-    auto step = [&](int32_t tok, int t, int buf, int sub) {
-        const char* keys = tiles + buf * 2 * RowsLds<D>::kTileBytes;
+    // Lane constants of the LDS reads.  Keys: 16-byte chunk 2 i + hf of token c,
+    // the chunk's upper bit a constant offset; values: of each 32 dims the rows and
+    // bytes of a transposing read (tokens 8 and 16 further lie a constant further).
+    constexpr int kKeys = 4, kRow = RowsLds<D>::kRow;
+    uint32_t key_lane[kKeys], value_lane[DT];
+    {
+        const uint32_t tr_row = 4 * hf + ((lane & 15) >> 2), tr_byte = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < kKeys; i++) key_lane[i] = key_place<D>(c, 2 * i + hf);
+#pragma unroll
+        for (int d = 0; d < DT; d++) value_lane[d] = value_place<D>(tr_row, 4 * d + (tr_byte >> 4)) + (tr_byte & 15);
+    }
+    auto step = [&](int32_t tok, int buf, int sub) {
+        const char* keys = tiles + buf * 2 * RowsLds<D>::kTileBytes + 32 * sub * kRow;
         const char* values = keys + RowsLds<D>::kTileBytes;
         f16v s;
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = 0.0f;
 #pragma unroll
         for (int i = 0; i < D / 16; i++)
-            s = mfma32<BF>(*(const u4*)(keys + key_place<D>(32 * sub + c, 2 * i + hf)), q[i], s);
+            s = mfma32<BF>(*(const u4*)(keys + key_lane[i % kKeys] + i / kKeys * 128), q[i], s);
         // this lane's tokens: 8 (i / 4) + 4 hf + i % 4
+        if (FMT >= FKV_PAGES_FP8) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            f4 f = {1.0f, 1.0f, 1.0f, 1.0f};
-            if (FMT >= FKV_PAGES_FP8) f = *(const f4*)&key_factor[buf][32 * sub + 8 * j + 4 * hf];
+            for (int j = 0; j < 4; j++) {
+                const f4 f = *(const f4*)&key_factor[buf][32 * sub + 8 * j + 4 * hf];
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[4 * j + i] = FMT >= FKV_PAGES_FP8 ? s[4 * j + i] * a.scale * f[i] : s[4 * j + i] * a.scale;
+                for (int i = 0; i < 4; i++) s[4 * j + i] *= f[i];
+            }
         }
         const int n0 = __builtin_amdgcn_readfirstlane(run_tokens[buf][2 * sub]);
         const int n1 = __builtin_amdgcn_readfirstlane(run_tokens[buf][2 * sub + 1]);
-        const bool part = tok + 32 > wave_least;
-        const bool masked = part || n0 < 16 || n1 < 16;
+        const bool masked = tok + 32 > wave_least || n0 < 16 || n1 < 16;
         if (masked) {
             const int left = lim - tok;
 #pragma unroll
@@ -396,13 +412,15 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
                 if (at >= left || (at & 15) >= (i < 8 ? n0 : n1)) s[i] = -INFINITY;
             }
         }
-        float top = s[0];
-#pragma unroll
-        for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+        // (the scale is not negative: the queries carry its sign)
+        float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        top = fmaxf(top, fmaxf(fmaxf(fmaxf(s[8], s[9]), fmaxf(s[10], s[11])), fmaxf(fmaxf(s[12], s[13]), fmaxf(s[14], s[15]))));
+        top *= a.scale;
         if (__any(top > m + (kRowSlack + kRowBias<FMT>))) {
             top = fmaxf(top, wave_xor(top, 32));
             const float up = fmaxf(m, top - kRowBias<FMT>), f = __builtin_amdgcn_exp2f(m - up);
             m = up;
+            wide = __any(fabsf(m) > kWide && m != kLowest);
             sum *= f;
             z *= f;
 #pragma unroll
@@ -410,11 +428,24 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
 #pragma unroll
                 for (int i = 0; i < 16; i++) acc[d][i] *= f;
         }
+        if (wide) {
+#pragma clang fp contract(off)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float x = s[i] * a.scale;
+                s[i] = x - m;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[i] = fmaf(s[i], a.scale, -m);
+        }
+        float part_sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            s[i] = __builtin_amdgcn_exp2f(s[i] - m);
-            sum += s[i];
+            s[i] = __builtin_amdgcn_exp2f(s[i]);
+            part_sum += s[i];
         }
+        sum += part_sum;
         if (FMT == FKV_PAGES_FP8_INT4) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -439,8 +470,8 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
             uint32_t first;
             if (kVB) {
                 first = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
-                x -= __uint_as_float(first << 16);
-                y -= __uint_as_float(first & 0xFFFF0000u);
+                x -= __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+                y -= __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
             } else {
                 const fkv_h2 w = __builtin_bit_cast(fkv_h2, __builtin_amdgcn_cvt_pkrtz(x, y));
                 first = as_u32(w);
@@ -450,49 +481,49 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
             part_of[0][j >> 2][j & 3] = first;
             part_of[1][j >> 2][j & 3] = kVB ? round_pair_bf16(x, y) : (uint32_t)f2h(x) | ((uint32_t)f2h(y) << 16);
         }
-        const bool odd = part && FMT != FKV_PAGES_FP8_INT4 && __builtin_amdgcn_readfirstlane(odd_tile[buf]) == t;
-        auto products = [&](bool clean) {
 #pragma unroll
-            for (int g = 0; g < 2; g++)
+        for (int g = 0; g < 2; g++)
 #pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    u4 v;
+            for (int d = 0; d < DT; d++) {
+                u4 v;
 #pragma unroll
-                    for (int jj = 0; jj < 2; jj++) {
-                        const uint32_t r = 32 * sub + 16 * g + 8 * jj + tr_row;
-                        const char* at = values + value_place<D>(r, 4 * d + (tr_byte >> 4)) + (tr_byte & 15);
-                        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)at);
-                        const u2 w = __builtin_bit_cast(u2, x);
-                        v[2 * jj] = clean ? finite_or_zero<kVB>(w.x) : w.x;
-                        v[2 * jj + 1] = clean ? finite_or_zero<kVB>(w.y) : w.y;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 2; i++) acc[d] = mfma32<kVB>(v, part_of[i][g], acc[d]);
+                for (int jj = 0; jj < 2; jj++) {
+                    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s4*)(values + value_lane[d] + (16 * g + 8 * jj) * kRow));
+                    const u2 w = __builtin_bit_cast(u2, x);
+                    v[2 * jj] = w.x, v[2 * jj + 1] = w.y;
                 }
-        };
-        if (!odd) {
-            products(false);
-        } else {
-            // Infinite or NaN values among tokens that not all rows attend to: a
-            // weight of 0 would carry them into every row, so the products are
-            // made without them, and they join the rows that attend to them.
-            products(true);
-            for (int r = 0; r < 32; r++) {
-                const bool in = r < lim - tok && (r & 15) < (r < 16 ? n0 : n1);
+#pragma unroll
+                for (int i = 0; i < 2; i++) acc[d] = mfma32<kVB>(v, part_of[i][g], acc[d]);
+            }
+    };
+    // Infinite or NaN values among tokens that not all rows attend to: a weight of
+    // 0 would carry them into every row.  So they join the rows that attend to them
+    // here, and the products find zeros in their place.
+    auto settle = [&](int32_t tok, int buf) {
+        char* values = tiles + (buf * 2 + 1) * RowsLds<D>::kTileBytes;
+        if (tg < wt)
+            for (int r = 0; r < kTileTokens; r++) {
+                if (((r >> 5) & (wt - 1)) != tg) continue;
+                const bool in = r < lim - tok && (r & 15) < run_tokens[buf][r >> 4];
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const int dim = 32 * d + 8 * j + 4 * hf;
-                        const u2 w = *(const u2*)(values + value_place<D>(32 * sub + r, dim >> 3) + 2 * (dim & 7));
+                        const u2 w = *(const u2*)(values + value_place<D>(r, 4 * d + j) + 8 * hf);
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const uint32_t x = (w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu;
-                            if (in && any_not_finite<kVB>(x)) acc[d][4 * j + i] += kVB ? bf2f(x) : h2f(x);
+                            acc[d][4 * j + i] += in && any_not_finite<kVB>(x) ? (kVB ? bf2f(x) : h2f(x)) : 0.0f;
                         }
                     }
             }
+        __syncthreads();
+        for (int i = tid; i < RowsLds<D>::kTileBytes / 8; i += 64 * kRowWaves) {
+            const u2 w = *(const u2*)(values + 8 * i);
+            *(u2*)(values + 8 * i) = u2{finite_or_zero<kVB>(w.x), finite_or_zero<kVB>(w.y)};
         }
+        __syncthreads();
     };
 
     if (nt > 0) load(begin);
@@ -502,9 +533,10 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
         store(tok, t, buf);
         if (t + 1 < nt) load(tok + kTileTokens);
         __syncthreads();
+        if (FMT != FKV_PAGES_FP8_INT4 && __builtin_amdgcn_readfirstlane(odd_tile[buf]) == t) settle(tok, buf);
         if (tg < wt)
             for (int sub = tg; sub < 4; sub += wt)
-                if (tok + 32 * sub < wave_most) step(tok + 32 * sub, t, buf, sub);
+                if (tok + 32 * sub < wave_most) step(tok + 32 * sub, buf, sub);
     }
 
     // The waves' sums meet in the LDS: 16 threads a row, D / 16 dims a thread.
@@ -756,7 +788,10 @@ int fkv_paged_attn_rows(const fkv_pages* pages, const fkv_rows* query, int32_t q
     a.G = Hq / pages->H;
     a.L = L;
     a.shared = (int32_t)shared;
-    a.scale = scale * 1.4426950408889634f;
+    a.scale = std::fabs(scale) * 1.4426950408889634f;
+    a.q_sign = std::signbit(scale) ? 0x80008000u : 0;
+    a.q_mask = ~0u;
+    if (a.scale < 1e-37f) a.scale = 1.0f, a.q_mask = a.q_sign = 0;  // (scores that are all 0: -inf times 0 would not be)
     const bool bf = q_dtype == FKV_BF16;
     if (pages->D == 64) return launch_rows_d<64>(a, p, pages->format, bf, (hipStream_t)stream);
     return launch_rows_d<128>(a, p, pages->format, bf, (hipStream_t)stream);
