@@ -96,6 +96,18 @@ __device__ inline int32_t limit_of(const RowsArgs& a, int b, int l) {
     return l >= n ? -1 : lim < 0 ? 0 : (int32_t)lim;
 }
 
+// 16-bit numbers that a weight enters the products as.  One, rounded, for results
+// of its own precision: 2^-8 of each weight at most for bf16 results, as their own
+// rounding is (on independent values their error grows by a fifth), 2^-11 for fp16
+// pages (down to steps of 2^-24, 2^-31 of the row's largest weight or less).  Two
+// bf16 numbers, the first cut off and the second what that leaves, 2^-15, for fp16
+// results over quantised pages, whose values' scales need bf16's range, and for INT4
+// values, whose codes and minima may cancel.  The products are what a prompt's chunk is bound by: half
+// as many again, two numbers, cost FIGURE.
+constexpr int row_parts(int fmt, bool bf) {
+    return fmt == FKV_PAGES_FP8_INT4 || (fmt == FKV_PAGES_FP8 && !bf) ? 2 : 1;
+}
+
 template <bool BF>
 __device__ inline f16v mfma32(u4 x, u4 y, f16v c) {
     if (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), c, 0, 0, 0);
@@ -124,7 +136,7 @@ struct Rows {
     static constexpr int KP = KT / 4, VP = VT / 4;                             // passes of 512 threads over 128 rows
     u4 k[KP], v[VP];
     uint32_t vx[VP];    // E4M3 values: the rows' exponent bytes
-    uint32_t kx;        // of token threadIdx.x: the key's exponent byte,
+    uint32_t kx;        // of run `wave`, token `lane`: the key's exponent byte,
     float2 sz;          // INT4 values: scale and minimum
 };
 
@@ -164,6 +176,7 @@ template <int D, int FMT, bool BF>
 __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs a) {
     using R = Rows<D, FMT>;
     constexpr bool kVB = FMT != FKV_PAGES_F16;  // values and weights are bf16 numbers
+    constexpr int kParts = row_parts(FMT, BF);
     constexpr int DT = D / 32;
     __shared__ __attribute__((aligned(16))) char tiles[RowsLds<D>::kBytes];
     __shared__ __attribute__((aligned(16))) float key_factor[2][kTileTokens], value_scale[2][kTileTokens],
@@ -238,62 +251,74 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
 
     const int32_t* ids = a.table.ids + (seq < 0 ? 0 : seq) * a.table.stride;
     R st;
-    // page of run `run` (16 tokens) of the tile at tok -> first row of its tokens, how many there are
-    auto run_of = [&](int32_t tok, int run, int& n) {
-        const int32_t at = tok + 16 * run;
-        n = min(max(end - at, 0), 16);
-        int32_t id = n > 0 ? scalar_load(ids, at >> sh) : 0;
-        if ((uint32_t)id >= (uint32_t)a.pg.n_pages) id = 0, n = 0;
-        return (((int64_t)id * a.pg.H + h) << sh) + (n > 0 ? at & (a.pg.page_size - 1) : 0);
+    // Runs of 16 tokens lie in one page.  A wave's loads are rows of KP runs of keys,
+    // VP of values (the same ones where rows have as many bytes) and, for the rows'
+    // scales, run `wave`; their pages' ids are loaded a tile ahead.
+    constexpr bool kSame = R::KT == R::VT;
+    constexpr int kIds = R::KP + (kSame ? 0 : R::VP) + 1;
+    int32_t id[kIds];
+    auto run_at = [&](int i) {
+        return i < R::KP ? (512 / R::KT * i + (64 / R::KT) * wave) / 16
+               : i < kIds - 1 ? (512 / R::VT * (i - R::KP) + (64 / R::VT) * wave) / 16 : wave;
     };
-    // A tile's loads.  A wave's rows of one pass lie in one run.
-    auto load = [&](int32_t tok) {
-        constexpr u4 none = {0, 0, 0, 0};
+    auto fetch = [&](int32_t tok) {
 #pragma unroll
-        for (int i = 0; i < R::KP; i++) {
-            constexpr int per = 512 / R::KT;  // rows a pass
-            int n;
-            const int64_t first = run_of(tok, (per * i + (64 / R::KT) * wave) / 16, n);
-            const int r = (tid / R::KT) & 15;
-            const u4 x = *(const u4*)(a.pg.k + first * R::KB + (uint32_t)(r * R::KB + 16 * (tid % R::KT)));
-            st.k[i] = r < n ? x : none;
+        for (int i = 0; i < kIds; i++) id[i] = scalar_load(ids, min(tok + 16 * run_at(i), end - 1) >> sh);
+    };
+    // -> the run's first row in the pages (any that is there, where the run has none), how many of its tokens take part
+    auto run_of = [&](int32_t tok, int i, int& n) {
+        const int32_t at = tok + 16 * run_at(i);
+        const bool in = (uint32_t)id[i] < (uint32_t)a.pg.n_pages;
+        n = in ? min(max(end - at, 0), 16) : 0;
+        return (((int64_t)(in ? id[i] : 0) * a.pg.H + h) << sh) + (at & (a.pg.page_size - 1));
+    };
+    // A tile's loads, as they are (what waits for them is store()).  `taken`: tokens
+    // of each run that take part; `whole`: all 16 of all.
+    bool whole = true;
+    int taken[kIds];
+    auto load = [&](int32_t tok) {
+        int64_t first[kIds];
+        whole = true;
+#pragma unroll
+        for (int i = 0; i < kIds; i++) {
+            first[i] = run_of(tok, i, taken[i]);
+            whole = whole && taken[i] == 16;
         }
+        if (tok + kTileTokens < end) fetch(tok + kTileTokens);
+#pragma unroll
+        for (int i = 0; i < R::KP; i++)
+            st.k[i] = *(const u4*)(a.pg.k + first[i] * R::KB + (uint32_t)(((tid / R::KT) & 15) * R::KB + 16 * (tid % R::KT)));
 #pragma unroll
         for (int i = 0; i < R::VP; i++) {
-            constexpr int per = 512 / R::VT;
-            int n;
-            const int64_t first = run_of(tok, (per * i + (64 / R::VT) * wave) / 16, n);
-            const int r = (tid / R::VT) & 15;
-            const char* at = a.pg.v + first * R::VB;
+            const int64_t row = first[kSame ? i : R::KP + i];
+            const uint32_t r = (tid / R::VT) & 15;
+            const char* at = a.pg.v + row * R::VB;
             if (R::VB == 32) {
-                const u2 x = *(const u2*)(at + (uint32_t)(r * R::VB + 8 * (tid % R::VT)));
-                st.v[i] = u4{r < n ? x.x : 0, r < n ? x.y : 0, 0, 0};
+                const u2 x = *(const u2*)(at + r * R::VB + 8 * (tid % R::VT));
+                st.v[i] = u4{x.x, x.y, 0, 0};
             } else {
-                const u4 x = *(const u4*)(at + (uint32_t)(r * R::VB + 16 * (tid % R::VT)));
-                st.v[i] = r < n ? x : none;
+                st.v[i] = *(const u4*)(at + r * R::VB + 16 * (tid % R::VT));
             }
-            if (FMT == FKV_PAGES_FP8) st.vx[i] = r < n ? ((const uint8_t*)a.pg.v_scale)[first + r] : 0;
+            if (FMT == FKV_PAGES_FP8) st.vx[i] = ((const uint8_t*)a.pg.v_scale)[row + r];
         }
-        if (FMT >= FKV_PAGES_FP8 && wave < 2) {
-            // (token tid of the tile: runs 4 wave to 4 wave + 3, 16 lanes each)
-            int64_t at = 0;
-            int n = 0;
+        if (FMT >= FKV_PAGES_FP8 && lane < 16) {
+            st.kx = a.pg.k_exp[first[kIds - 1] + lane];
+            if (FMT == FKV_PAGES_FP8_INT4) st.sz = ((const float2*)a.pg.v_scale)[first[kIds - 1] + lane];
+        }
+    };
+    // Zeros in the place of what takes no part (of a tile that is not whole).
+    auto blank = [&]() {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                int m;
-                const int64_t first = run_of(tok, 4 * wave + i, m);
-                if (lane >> 4 == i) at = first, n = m;
-            }
-            const bool in = (lane & 15) < n;
-            st.kx = in ? a.pg.k_exp[at + (lane & 15)] : 0;
-            if (FMT == FKV_PAGES_FP8_INT4) {
-                const float2 x = ((const float2*)a.pg.v_scale)[at + (in ? lane & 15 : 0)];
-                st.sz = in ? x : make_float2(0.0f, 0.0f);
-            }
-        }
+        for (int i = 0; i < R::KP; i++)
+            if ((int)((tid / R::KT) & 15) >= taken[i]) st.k[i] = u4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < R::VP; i++)
+            if ((int)((tid / R::VT) & 15) >= taken[kSame ? i : R::KP + i]) st.v[i] = u4{0, 0, 0, 0}, st.vx[i] = 0;
+        if (lane >= taken[kIds - 1]) st.kx = 0, st.sz = make_float2(0.0f, 0.0f);
     };
     // ... and into the LDS, in 16 bits.
     auto store = [&](int32_t tok, int t, int buf) {
+        if (!whole) blank();
         char* keys = tiles + buf * 2 * RowsLds<D>::kTileBytes;
         char* values = keys + RowsLds<D>::kTileBytes;
         const bool look = tok + kTileTokens > all_least;  // (tokens that not all rows attend to)
@@ -351,15 +376,12 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
                 }
             }
         }
-        if (FMT >= FKV_PAGES_FP8 && wave < 2) {
-            key_factor[buf][tid] = exp_byte(st.kx);
-            if (FMT == FKV_PAGES_FP8_INT4) value_scale[buf][tid] = st.sz.x, value_min[buf][tid] = st.sz.y;
+        if (FMT >= FKV_PAGES_FP8 && lane < 16) {
+            key_factor[buf][16 * wave + lane] = exp_byte(st.kx);
+            if (FMT == FKV_PAGES_FP8_INT4)
+                value_scale[buf][16 * wave + lane] = st.sz.x, value_min[buf][16 * wave + lane] = st.sz.y;
         }
-        if (lane == 0) {
-            int n;
-            (void)run_of(tok, wave, n);
-            run_tokens[buf][wave] = n;
-        }
+        if (lane == 0) run_tokens[buf][wave] = taken[kIds - 1];
         if (odd) odd_tile[buf] = t;
     };
 
@@ -383,39 +405,52 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
 #pragma unroll
         for (int d = 0; d < DT; d++) value_lane[d] = value_place<D>(tr_row, 4 * d + (tr_byte >> 4)) + (tr_byte & 15);
     }
-    auto step = [&](int32_t tok, int buf, int sub) {
+    // Matrix products take their pipe 32 cycles and the issue of vector
+    // instructions 9 of these, so a wave's stream is one product, then about six
+    // vector instructions, and so on: the weights of these tokens beside the next
+    // ones' scores and their own products.  (A wave by itself issues a vector
+    // instruction every 6.4 cycles, and two that each do one kind at a time mostly
+    // wait for each other.)  The fences keep the order.
+#define FENCE __builtin_amdgcn_sched_barrier(0)
+    auto key_of = [&](const char* keys, int i) { return *(const u4*)(keys + key_lane[i % kKeys] + i / kKeys * 128); };
+    // Scores (not scaled) of the tile's 32 tokens `sub`; the lane's are 8 (i / 4) + 4 hf + i % 4.
+    auto score = [&](int buf, int sub) {
         const char* keys = tiles + buf * 2 * RowsLds<D>::kTileBytes + 32 * sub * kRow;
-        const char* values = keys + RowsLds<D>::kTileBytes;
         f16v s;
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 16; i++)
-            s = mfma32<BF>(*(const u4*)(keys + key_lane[i % kKeys] + i / kKeys * 128), q[i], s);
-        // this lane's tokens: 8 (i / 4) + 4 hf + i % 4
+        for (int i = 0; i < D / 16; i++) s = mfma32<BF>(key_of(keys, i), q[i], s);
+        return s;
+    };
+    // Keys' factors, and the largest score.
+    auto factors = [&](f16v& s, int buf, int sub, int j) {
         if (FMT >= FKV_PAGES_FP8) {
+            const f4 f = *(const f4*)&key_factor[buf][32 * sub + 8 * j + 4 * hf];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const f4 f = *(const f4*)&key_factor[buf][32 * sub + 8 * j + 4 * hf];
-#pragma unroll
-                for (int i = 0; i < 4; i++) s[4 * j + i] *= f[i];
-            }
+            for (int i = 0; i < 4; i++) s[4 * j + i] *= f[i];
         }
+    };
+    auto largest = [](float x, float y) { return __builtin_elementwise_maximum(x, y); };  // (NaN where one is)
+    auto max4 = [&](const f16v& s, int j) {
+        return largest(largest(s[4 * j], s[4 * j + 1]), largest(s[4 * j + 2], s[4 * j + 3]));
+    };
+    // What takes no part, and the running maximum.
+    bool masked = false;
+    auto settle_scores = [&](f16v& s, float top, int32_t tok, int buf, int sub) {
         const int n0 = __builtin_amdgcn_readfirstlane(run_tokens[buf][2 * sub]);
         const int n1 = __builtin_amdgcn_readfirstlane(run_tokens[buf][2 * sub + 1]);
-        const bool masked = tok + 32 > wave_least || n0 < 16 || n1 < 16;
+        masked = tok + 32 > wave_least || n0 < 16 || n1 < 16;
         if (masked) {
-            const int left = lim - tok;
+            const int left = lim - tok - 4 * hf, left0 = n0 - 4 * hf, left1 = n1 - 4 * hf;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const int at = 8 * (i >> 2) + 4 * hf + (i & 3);
-                if (at >= left || (at & 15) >= (i < 8 ? n0 : n1)) s[i] = -INFINITY;
+                const int at = 8 * (i >> 2) + (i & 3);
+                if (at >= left || (at & 15) >= (i < 8 ? left0 : left1)) s[i] = -INFINITY;
             }
+            top = largest(largest(max4(s, 0), max4(s, 1)), largest(max4(s, 2), max4(s, 3)));
         }
-        // (the scale is not negative: the queries carry its sign)
-        float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-        top = fmaxf(top, fmaxf(fmaxf(fmaxf(s[8], s[9]), fmaxf(s[10], s[11])), fmaxf(fmaxf(s[12], s[13]), fmaxf(s[14], s[15]))));
-        top *= a.scale;
+        top *= a.scale;  // (not negative: the queries carry its sign)
         if (__any(top > m + (kRowSlack + kRowBias<FMT>))) {
             top = fmaxf(top, wave_xor(top, 32));
             const float up = fmaxf(m, top - kRowBias<FMT>), f = __builtin_amdgcn_exp2f(m - up);
@@ -435,67 +470,115 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
                 const float x = s[i] * a.scale;
                 s[i] = x - m;
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = fmaf(s[i], a.scale, -m);
         }
-        float part_sum = 0.0f;
+    };
+    // Weights of the scores s (whose tokens begin at tok), O^T += V^T P^T, and the
+    // scores of the tokens `next` of the tile in next_buf, whose largest is returned
+    // (of whatever lies there where these were the last ones).
+    auto step = [&](f16v& s, int32_t tok, int buf, int sub, int next_buf, int next) {
+        const char* values = tiles + (buf * 2 + 1) * RowsLds<D>::kTileBytes + 32 * sub * kRow;
+        const char* keys = tiles + next_buf * 2 * RowsLds<D>::kTileBytes + 32 * next * kRow;
+        const float by = wide ? 1.0f : a.scale, off = wide ? 0.0f : m;
+        float w[16], part_sum = 0.0f;
+        u4 part_of[2][kParts];  // [16 tokens][part]
+        f4 v_scale[2], v_low[2];
+        auto constants = [&](int g) {
+            if (FMT != FKV_PAGES_FP8_INT4) return;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            s[i] = __builtin_amdgcn_exp2f(s[i]);
-            part_sum += s[i];
-        }
-        sum += part_sum;
-        if (FMT == FKV_PAGES_FP8_INT4) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const f4 scale = *(const f4*)&value_scale[buf][32 * sub + 8 * j + 4 * hf];
-                const f4 low = *(const f4*)&value_min[buf][32 * sub + 8 * j + 4 * hf];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    // (a token that takes no part may have any scale, NaN among them)
-                    const bool in = !masked || 8 * j + 4 * hf + i < lim - tok;
-                    z = in ? fmaf(s[4 * j + i], low[i], z) : z;
-                    s[4 * j + i] = in ? s[4 * j + i] * scale[i] : 0.0f;
-                }
+            for (int j = 0; j < 2; j++) {
+                v_scale[j] = *(const f4*)&value_scale[buf][32 * sub + 16 * g + 8 * j + 4 * hf];
+                v_low[j] = *(const f4*)&value_min[buf][32 * sub + 16 * g + 8 * j + 4 * hf];
             }
-        }
-        // Weights as two 16-bit numbers, the first cut off and the second what
-        // that leaves, rounded: 16 bits (bf16) or 22 (fp16, down to steps of
-        // 2^-24, 2^-39 of the row's largest weight).
-        u4 part_of[2][2];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            float x = s[2 * j], y = s[2 * j + 1];
-            uint32_t first;
-            if (kVB) {
-                first = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+        };
+        auto weigh = [&](int i) {
+            w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], by, -off));
+            part_sum += w[i];
+            if (FMT == FKV_PAGES_FP8_INT4) {
+                // (a token that takes no part may have any scale, NaN among them)
+                const bool in = !masked || 8 * (i >> 2) + (i & 3) < lim - tok - 4 * hf;
+                z = in ? fmaf(w[i], v_low[(i >> 2) & 1][i & 3], z) : z;
+                w[i] = in ? w[i] * v_scale[(i >> 2) & 1][i & 3] : 0.0f;
+            }
+        };
+        auto halve = [&](int j) {
+            float x = w[2 * j], y = w[2 * j + 1];
+            u4* part = part_of[j >> 2];
+            if (kParts == 1) {
+                part[0][j & 3] = kVB ? round_pair_bf16(x, y) : (uint32_t)f2h(x) | ((uint32_t)f2h(y) << 16);
+            } else {
+                part[0][j & 3] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
                 x -= __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
                 y -= __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
-            } else {
-                const fkv_h2 w = __builtin_bit_cast(fkv_h2, __builtin_amdgcn_cvt_pkrtz(x, y));
-                first = as_u32(w);
-                x -= (float)w.x;
-                y -= (float)w.y;
+                part[kParts - 1][j & 3] = round_pair_bf16(x, y);
             }
-            part_of[0][j >> 2][j & 3] = first;
-            part_of[1][j >> 2][j & 3] = kVB ? round_pair_bf16(x, y) : (uint32_t)f2h(x) | ((uint32_t)f2h(y) << 16);
+        };
+        auto value_of = [&](int g, int d) {
+            u4 v;
+#pragma unroll
+            for (int jj = 0; jj < 2; jj++) {
+                const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s4*)(values + value_lane[d] + (16 * g + 8 * jj) * kRow));
+                const u2 y = __builtin_bit_cast(u2, x);
+                v[2 * jj] = y.x, v[2 * jj + 1] = y.y;
+            }
+            return v;
+        };
+        f16v after;
+        u4 v[DT];
+        constexpr int NQ = D / 16, AHEAD = 3;
+        constants(0);
+#pragma unroll
+        for (int i = 0; i < 16; i++) after[i] = 0.0f;
+        u4 k[NQ];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) k[i] = key_of(keys, i);
+        FENCE;
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            if (i + AHEAD < NQ) k[i + AHEAD] = key_of(keys, i + AHEAD);
+            else if (i + AHEAD - NQ < DT) v[i + AHEAD - NQ] = value_of(0, i + AHEAD - NQ);
+            after = mfma32<BF>(k[i], q[i], after);
+#pragma unroll
+            for (int j = 8 / NQ * i; j < 8 / NQ * (i + 1); j++) {
+                weigh(j);
+                if (j & 1) halve(j >> 1);
+            }
+            FENCE;
         }
+        constants(1);
+        // two blocks of 32 dims at a time, so that no product waits for the one before
+        float top = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < 2; g++)
+        for (int g = 0; g < 2; g++) {
 #pragma unroll
-            for (int d = 0; d < DT; d++) {
-                u4 v;
+            for (int d0 = 0; d0 < DT; d0 += 2)
 #pragma unroll
-                for (int jj = 0; jj < 2; jj++) {
-                    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s4*)(values + value_lane[d] + (16 * g + 8 * jj) * kRow));
-                    const u2 w = __builtin_bit_cast(u2, x);
-                    v[2 * jj] = w.x, v[2 * jj + 1] = w.y;
+                for (int e = 0; e < 2 * kParts; e++) {
+                    const int d = d0 + (e & 1), n = kParts * d0 + e;  // product n of kParts * DT
+                    if (e < 2 && g == 0 && d + AHEAD < DT) v[d + AHEAD] = value_of(g, d + AHEAD);
+                    acc[d] = mfma32<kVB>(v[d], part_of[g][e >> 1], acc[d]);
+                    if (e >= 2 * kParts - 2 && g == 0) v[d] = value_of(1, d);  // (its last use was the product above)
+                    if (g == 0) {
+                        constexpr int PER = 8 / (kParts * DT);
+#pragma unroll
+                        for (int j = 8 + PER * n; j < 8 + PER * (n + 1); j++) {
+                            weigh(j);
+                            if (j & 1) halve(j >> 1);
+                        }
+                    } else {
+                        constexpr int PER = kParts * DT < 4 ? 4 / (kParts * DT) : 1;
+#pragma unroll
+                        for (int j = PER * n; j < PER * (n + 1) && j < 4; j++) {
+                            factors(after, next_buf, next, j);
+                            top = largest(top, max4(after, j));
+                        }
+                    }
+                    FENCE;
                 }
-#pragma unroll
-                for (int i = 0; i < 2; i++) acc[d] = mfma32<kVB>(v, part_of[i][g], acc[d]);
-            }
+        }
+        sum += part_sum;
+        s = after;
+        return top;
     };
     // Infinite or NaN values among tokens that not all rows attend to: a weight of
     // 0 would carry them into every row.  So they join the rows that attend to them
@@ -526,17 +609,45 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
         __syncthreads();
     };
 
-    if (nt > 0) load(begin);
+    // A tile's last step takes the next tile's first scores, so this is stored
+    // before it; the other buffer is free once all waves are that far.
+    f16v s;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; i++) s[i] = 0.0f;
+    if (nt > 0) {
+        fetch(begin);
+        load(begin);
+        store(begin, 0, 0);
+        if (nt > 1) load(begin + kTileTokens);
+        __syncthreads();
+        if (tg < wt) {
+            s = score(0, tg);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                factors(s, 0, tg, j);
+                top = largest(top, max4(s, j));
+            }
+        }
+    }
     for (int t = 0; t < nt; t++) {
         const int32_t tok = begin + t * kTileTokens;
         const int buf = t & 1;
-        store(tok, t, buf);
-        if (t + 1 < nt) load(tok + kTileTokens);
-        __syncthreads();
         if (FMT != FKV_PAGES_FP8_INT4 && __builtin_amdgcn_readfirstlane(odd_tile[buf]) == t) settle(tok, buf);
-        if (tg < wt)
-            for (int sub = tg; sub < 4; sub += wt)
-                if (tok + 32 * sub < wave_most) step(tok + 32 * sub, buf, sub);
+        for (int j = wt; j <= 4; j += wt) {
+            const bool last = j == 4;
+            if (last && t + 1 < nt) {
+                __syncthreads();
+                store(tok + kTileTokens, t + 1, buf ^ 1);
+                if (t + 2 < nt) load(tok + 2 * kTileTokens);
+                __syncthreads();
+            }
+            const int sub = tg + j - wt;
+            if (tg < wt && tok + 32 * sub < wave_most) {
+                settle_scores(s, top, tok + 32 * sub, buf, sub);
+                top = step(s, tok + 32 * sub, buf, sub, last ? buf ^ 1 : buf, last ? tg : sub + wt);
+            }
+        }
     }
 
     // The waves' sums meet in the LDS: 16 threads a row, D / 16 dims a thread.

@@ -31,16 +31,18 @@ def _i32(x):
     return torch.tensor(x, dtype=torch.int32, device="cuda")
 
 
-def _bound(out, spread, ds, n, dtype, mag):
-    """What a result may be off by, as for the one-token kernel: its own
-    rounding; each weight's relative error, from its score (twice, once in the
-    sum), from exp2 (2^-22) and from being two 16-bit numbers (bf16: 8 bits cut
-    off and 8 rounded, 2^-16; fp16: less, down to steps of 2^-24 where the
-    largest weight is 2^7 or more, 2^-32 of it, times the largest value); fp32
-    sums: of 32 tokens four products of 16, each rounded twice at most, then
-    waves and workgroups."""
+def _bound(out, spread, ds, n, fmt, dtype, mag):
+    """What a result may be off by: its own rounding; each weight's relative
+    error, from its score (twice, once in the sum), from exp2 (2^-22) and from its
+    16-bit form (half a step of n bits is 2^-n): bf16 results over bf16 and E4M3 pages
+    one rounded bf16 number, 2^-8; fp16 pages one fp16 number, 2^-11, or 2^-25 where it
+    is small (the largest weight is 2^7 or more: 2^-32 of it, times the largest
+    value); otherwise two bf16 numbers, the first cut off, which leaves less than 2^-7,
+    and that rounded, 2^-15.  fp32 sums: of 32 tokens four products of 16,
+    each rounded twice at most, then waves and workgroups."""
     n = max(int(n), 1)
-    rel = 2 * ds[..., None] * 1.01 + 2.0 ** -16 + 2.0 ** -21 + (n / 4 + 64) * 2.0 ** -24
+    one = 2.0 ** -11 if fmt == "fp16" else 2.0 ** -8 if fmt in ("bf16", "fp8") and dtype == torch.bfloat16 else 2.0 ** -15
+    rel = 2 * ds[..., None] * 1.01 + one + 2.0 ** -21 + (n / 4 + 64) * 2.0 ** -24
     return ref.UNIT[dtype] * np.abs(out) + ref.TINY[dtype] + rel * spread + n * 2.0 ** -32 * mag
 
 
@@ -62,7 +64,7 @@ def _check(layer, q, table, lens, n_new=None, shared=0, scale=None, read_table=N
         limit = [max(h - n + l + 1, 0) if l < n else 0 for h, n in zip(have, new)]
         want, wlse, spread, ds = ref.attend(q64[:, :, l], values, t, limit, layer.page_size, layer.n_pages, s)
         real = np.array([l < n for n in new])
-        tol = _bound(want, spread, ds, max(limit), q.dtype, mag)
+        tol = _bound(want, spread, ds, max(limit), layer.fmt, q.dtype, mag)
         err = np.abs(got[:, :, l] - want)[real]
         assert (err <= tol[real]).all(), f"token {l}: {np.nanmax(err / tol[real])} of the bound, NaN {np.isnan(err).sum()}"
         none = np.isinf(wlse)
