@@ -101,12 +101,10 @@ __device__ inline int32_t limit_of(const RowsArgs& a, int b, int l) {
 // rounding is (on independent values their error grows by a fifth), 2^-11 for fp16
 // pages (down to steps of 2^-24, 2^-31 of the row's largest weight or less).  Two
 // bf16 numbers, the first cut off and the second what that leaves, 2^-15, for fp16
-// results over quantised pages, whose values' scales need bf16's range, and for INT4
-// values, whose codes and minima may cancel.  The products are what a prompt's chunk is bound by: half
-// as many again, two numbers, cost FIGURE.
-constexpr int row_parts(int fmt, bool bf) {
-    return fmt == FKV_PAGES_FP8_INT4 || (fmt == FKV_PAGES_FP8 && !bf) ? 2 : 1;
-}
+// results over quantised pages, whose values' scales need bf16's range.  The
+// products are what a prompt's chunk is bound by: 2K tokens after 14K take 602 us
+// with one number, 796 with two.
+constexpr int row_parts(int fmt, bool bf) { return fmt >= FKV_PAGES_FP8 && !bf ? 2 : 1; }
 
 template <bool BF>
 __device__ inline f16v mfma32(u4 x, u4 y, f16v c) {
@@ -119,6 +117,23 @@ template <bool BF, bool HI>
 __device__ inline uint32_t cvt_codes(uint32_t w, float scale) {
     if (BF) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
+}
+// 16 codes of a row with exponent byte e (0 stands for a factor of 0) as 16-bit numbers.
+template <typename B>
+__device__ inline void decode(u4 x, uint32_t e, B, uint32_t (&y)[8]) {
+    const float scale = exp_byte(e);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t w = e ? x[j] : 0;
+        y[2 * j] = cvt_codes<B::value, false>(w, scale);
+        y[2 * j + 1] = cvt_codes<B::value, true>(w, scale);
+    }
+}
+// Codes c of 0 to 15, a byte each, as the E4M3 numbers (c - 8) * 2^-9 (0 to 7 times
+// that are subnormal numbers, 8 times the first normal one).
+__device__ inline uint32_t less_eight(uint32_t c) {
+    const uint32_t x = c ^ 0x08080808u, n = x & 0x08080808u;  // n: 8 where c < 8, and x is c + 8
+    return ((x ^ ((n << 1) - (n >> 3))) + (n >> 3)) | n << 4;
 }
 __device__ inline uint32_t round_pair_bf16(float a, float b) {
     const b2 v = {(__bf16)a, (__bf16)b};
@@ -135,9 +150,9 @@ struct Rows {
     static constexpr int KT = KB / 16, VT = VB == 32 ? 4 : VB / 16;            // threads a row
     static constexpr int KP = KT / 4, VP = VT / 4;                             // passes of 512 threads over 128 rows
     u4 k[KP], v[VP];
-    uint32_t vx[VP];    // E4M3 values: the rows' exponent bytes
-    uint32_t kx;        // of run `wave`, token `lane`: the key's exponent byte,
-    float2 sz;          // INT4 values: scale and minimum
+    uint32_t kx[KP], vx[VP];  // exponent bytes of the rows (E4M3; of keys for bf16 queries)
+    uint32_t ke;              // of run `wave`, token `lane`: the key's (for fp16 queries),
+    float2 sz;                // an INT4 value's scale and minimum
 };
 
 template <int D>
@@ -177,10 +192,13 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
     using R = Rows<D, FMT>;
     constexpr bool kVB = FMT != FKV_PAGES_F16;  // values and weights are bf16 numbers
     constexpr int kParts = row_parts(FMT, BF);
+    // E4M3 keys as bf16 numbers hold their row's power of two; as fp16 numbers the
+    // scores are multiplied by it
+    constexpr bool kFactors = FMT >= FKV_PAGES_FP8 && !BF;
     constexpr int DT = D / 32;
     __shared__ __attribute__((aligned(16))) char tiles[RowsLds<D>::kBytes];
     __shared__ __attribute__((aligned(16))) float key_factor[2][kTileTokens], value_scale[2][kTileTokens],
-        value_min[2][kTileTokens];
+        value_min[2][kTileTokens];  // (the latter min + 8 scale)
     __shared__ float stat[kRowWaves][32][3];
     __shared__ int32_t least[kRowWaves], most[kRowWaves], run_tokens[2][8], odd_tile[2];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hf = lane >> 5;
@@ -286,8 +304,10 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
         }
         if (tok + kTileTokens < end) fetch(tok + kTileTokens);
 #pragma unroll
-        for (int i = 0; i < R::KP; i++)
+        for (int i = 0; i < R::KP; i++) {
             st.k[i] = *(const u4*)(a.pg.k + first[i] * R::KB + (uint32_t)(((tid / R::KT) & 15) * R::KB + 16 * (tid % R::KT)));
+            if (FMT >= FKV_PAGES_FP8 && !kFactors) st.kx[i] = (a.pg.k_exp + first[i])[(tid / R::KT) & 15];
+        }
 #pragma unroll
         for (int i = 0; i < R::VP; i++) {
             const int64_t row = first[kSame ? i : R::KP + i];
@@ -302,7 +322,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
             if (FMT == FKV_PAGES_FP8) st.vx[i] = ((const uint8_t*)a.pg.v_scale)[row + r];
         }
         if (FMT >= FKV_PAGES_FP8 && lane < 16) {
-            st.kx = a.pg.k_exp[first[kIds - 1] + lane];
+            if (kFactors) st.ke = a.pg.k_exp[first[kIds - 1] + lane];
             if (FMT == FKV_PAGES_FP8_INT4) st.sz = ((const float2*)a.pg.v_scale)[first[kIds - 1] + lane];
         }
     };
@@ -310,11 +330,11 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
     auto blank = [&]() {
 #pragma unroll
         for (int i = 0; i < R::KP; i++)
-            if ((int)((tid / R::KT) & 15) >= taken[i]) st.k[i] = u4{0, 0, 0, 0};
+            if ((int)((tid / R::KT) & 15) >= taken[i]) st.k[i] = u4{0, 0, 0, 0}, st.kx[i] = 0;
 #pragma unroll
         for (int i = 0; i < R::VP; i++)
             if ((int)((tid / R::VT) & 15) >= taken[kSame ? i : R::KP + i]) st.v[i] = u4{0, 0, 0, 0}, st.vx[i] = 0;
-        if (lane >= taken[kIds - 1]) st.kx = 0, st.sz = make_float2(0.0f, 0.0f);
+        if (lane >= taken[kIds - 1]) st.ke = 0, st.sz = make_float2(0.0f, 0.0f);
     };
     // ... and into the LDS, in 16 bits.
     auto store = [&](int32_t tok, int t, int buf) {
@@ -330,11 +350,10 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
             if (R::k16) {
                 *(u4*)(keys + key_place<D>(r, ch)) = x;
             } else {
-                *(u4*)(keys + key_place<D>(r, 2 * ch)) = u4{cvt_codes<BF, false>(x.x, 1.0f), cvt_codes<BF, true>(x.x, 1.0f),
-                                                            cvt_codes<BF, false>(x.y, 1.0f), cvt_codes<BF, true>(x.y, 1.0f)};
-                *(u4*)(keys + key_place<D>(r, 2 * ch + 1)) =
-                    u4{cvt_codes<BF, false>(x.z, 1.0f), cvt_codes<BF, true>(x.z, 1.0f), cvt_codes<BF, false>(x.w, 1.0f),
-                       cvt_codes<BF, true>(x.w, 1.0f)};
+                uint32_t y[8];
+                decode(x, kFactors ? 127 : st.kx[i], std::integral_constant<bool, BF>{}, y);
+                *(u4*)(keys + key_place<D>(r, 2 * ch)) = u4{y[0], y[1], y[2], y[3]};
+                *(u4*)(keys + key_place<D>(r, 2 * ch + 1)) = u4{y[4], y[5], y[6], y[7]};
             }
         }
 #pragma unroll
@@ -347,15 +366,8 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
                     odd = odd || any_not_finite<kVB>(x.x) || any_not_finite<kVB>(x.y) || any_not_finite<kVB>(x.z) ||
                           any_not_finite<kVB>(x.w);
             } else if (FMT == FKV_PAGES_FP8) {
-                // (times the row's power of two, which bf16 numbers carry exactly; byte 0 stands for a factor of 0)
-                const float e = exp_byte(st.vx[i]);
-                const bool none = st.vx[i] == 0;
                 uint32_t y[8];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    y[2 * j] = none ? 0 : cvt_codes<true, false>(x[j], e);
-                    y[2 * j + 1] = none ? 0 : cvt_codes<true, true>(x[j], e);
-                }
+                decode(x, st.vx[i], std::true_type{}, y);
                 *(u4*)(values + value_place<D>(r, 2 * ch)) = u4{y[0], y[1], y[2], y[3]};
                 *(u4*)(values + value_place<D>(r, 2 * ch + 1)) = u4{y[4], y[5], y[6], y[7]};
                 if (look) {
@@ -363,11 +375,12 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
                     for (int j = 0; j < 8; j++) odd = odd || any_not_finite<true>(y[j]);
                 }
             } else {
-                // codes 0 to 15 are the E4M3 numbers code * 2^-9
+                // code - 8 in place of the code and min + 8 scale in place of min: both
+                // are then of the values' size, and so is what rounding a weight costs
                 constexpr int NW = R::VB == 32 ? 2 : 4;  // dwords of eight codes: a chunk each
 #pragma unroll
                 for (int j = 0; j < NW; j++) {
-                    const uint32_t even = x[j] & 0x0F0F0F0Fu, other = (x[j] >> 4) & 0x0F0F0F0Fu;
+                    const uint32_t even = less_eight(x[j] & 0x0F0F0F0Fu), other = less_eight((x[j] >> 4) & 0x0F0F0F0Fu);
                     const uint32_t lo = __builtin_amdgcn_perm(other, even, 0x05010400u);
                     const uint32_t hi = __builtin_amdgcn_perm(other, even, 0x07030602u);
                     *(u4*)(values + value_place<D>(r, NW * ch + j)) =
@@ -377,9 +390,12 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
             }
         }
         if (FMT >= FKV_PAGES_FP8 && lane < 16) {
-            key_factor[buf][16 * wave + lane] = exp_byte(st.kx);
-            if (FMT == FKV_PAGES_FP8_INT4)
-                value_scale[buf][16 * wave + lane] = st.sz.x, value_min[buf][16 * wave + lane] = st.sz.y;
+            if (kFactors) key_factor[buf][16 * wave + lane] = exp_byte(st.ke);
+            if (FMT == FKV_PAGES_FP8_INT4) {
+                const float low = fmaf(8.0f, st.sz.x, st.sz.y);
+                value_scale[buf][16 * wave + lane] = st.sz.x, value_min[buf][16 * wave + lane] = low;
+                if (look) odd = odd || !(fabsf(low) < INFINITY);
+            }
         }
         if (lane == 0) run_tokens[buf][wave] = taken[kIds - 1];
         if (odd) odd_tile[buf] = t;
@@ -425,7 +441,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
     };
     // Keys' factors, and the largest score.
     auto factors = [&](f16v& s, int buf, int sub, int j) {
-        if (FMT >= FKV_PAGES_FP8) {
+        if (kFactors) {
             const f4 f = *(const f4*)&key_factor[buf][32 * sub + 8 * j + 4 * hf];
 #pragma unroll
             for (int i = 0; i < 4; i++) s[4 * j + i] *= f[i];
@@ -494,10 +510,8 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
             w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], by, -off));
             part_sum += w[i];
             if (FMT == FKV_PAGES_FP8_INT4) {
-                // (a token that takes no part may have any scale, NaN among them)
-                const bool in = !masked || 8 * (i >> 2) + (i & 3) < lim - tok - 4 * hf;
-                z = in ? fmaf(w[i], v_low[(i >> 2) & 1][i & 3], z) : z;
-                w[i] = in ? w[i] * v_scale[(i >> 2) & 1][i & 3] : 0.0f;
+                z = fmaf(w[i], v_low[(i >> 2) & 1][i & 3], z);
+                w[i] *= v_scale[(i >> 2) & 1][i & 3];
             }
         };
         auto halve = [&](int j) {
@@ -589,6 +603,11 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
             for (int r = 0; r < kTileTokens; r++) {
                 if (((r >> 5) & (wt - 1)) != tg) continue;
                 const bool in = r < lim - tok && (r & 15) < run_tokens[buf][r >> 4];
+                if (FMT == FKV_PAGES_FP8_INT4) {
+                    const float low = value_min[buf][r];
+                    z += in && !(fabsf(low) < INFINITY) ? low : 0.0f;
+                    continue;
+                }
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -602,9 +621,13 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
                     }
             }
         __syncthreads();
-        for (int i = tid; i < RowsLds<D>::kTileBytes / 8; i += 64 * kRowWaves) {
-            const u2 w = *(const u2*)(values + 8 * i);
-            *(u2*)(values + 8 * i) = u2{finite_or_zero<kVB>(w.x), finite_or_zero<kVB>(w.y)};
+        if (FMT == FKV_PAGES_FP8_INT4) {
+            if (tid < kTileTokens && !(fabsf(value_min[buf][tid]) < INFINITY)) value_scale[buf][tid] = value_min[buf][tid] = 0.0f;
+        } else {
+            for (int i = tid; i < RowsLds<D>::kTileBytes / 8; i += 64 * kRowWaves) {
+                const u2 w = *(const u2*)(values + 8 * i);
+                *(u2*)(values + 8 * i) = u2{finite_or_zero<kVB>(w.x), finite_or_zero<kVB>(w.y)};
+            }
         }
         __syncthreads();
     };
@@ -633,7 +656,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
     for (int t = 0; t < nt; t++) {
         const int32_t tok = begin + t * kTileTokens;
         const int buf = t & 1;
-        if (FMT != FKV_PAGES_FP8_INT4 && __builtin_amdgcn_readfirstlane(odd_tile[buf]) == t) settle(tok, buf);
+        if (__builtin_amdgcn_readfirstlane(odd_tile[buf]) == t) settle(tok, buf);
         for (int j = wt; j <= 4; j += wt) {
             const bool last = j == 4;
             if (last && t + 1 < nt) {

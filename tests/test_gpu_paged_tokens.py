@@ -34,16 +34,28 @@ def _i32(x):
 def _bound(out, spread, ds, n, fmt, dtype, mag):
     """What a result may be off by: its own rounding; each weight's relative
     error, from its score (twice, once in the sum), from exp2 (2^-22) and from its
-    16-bit form (half a step of n bits is 2^-n): bf16 results over bf16 and E4M3 pages
-    one rounded bf16 number, 2^-8; fp16 pages one fp16 number, 2^-11, or 2^-25 where it
+    16-bit form (half a step of n bits is 2^-n): bf16 results one rounded bf16
+    number, 2^-8; fp16 pages one fp16 number, 2^-11, or 2^-25 where it
     is small (the largest weight is 2^7 or more: 2^-32 of it, times the largest
     value); otherwise two bf16 numbers, the first cut off, which leaves less than 2^-7,
     and that rounded, 2^-15.  fp32 sums: of 32 tokens four products of 16,
     each rounded twice at most, then waves and workgroups."""
     n = max(int(n), 1)
-    one = 2.0 ** -11 if fmt == "fp16" else 2.0 ** -8 if fmt in ("bf16", "fp8") and dtype == torch.bfloat16 else 2.0 ** -15
+    one = 2.0 ** -11 if fmt == "fp16" else 2.0 ** -8 if fmt != "fp16" and dtype == torch.bfloat16 else 2.0 ** -15
     rel = 2 * ds[..., None] * 1.01 + one + 2.0 ** -21 + (n / 4 + 64) * 2.0 ** -24
     return ref.UNIT[dtype] * np.abs(out) + ref.TINY[dtype] + rel * spread + n * 2.0 ** -32 * mag
+
+
+def _values(layer):
+    """As ``ref.page_values``; an INT4 value is scale (code - 8) + (min + 8 scale)
+    here, and its error relative to the magnitudes of both."""
+    k, v, mag = ref.page_values(layer)
+    if layer.fmt == "fp8_int4":
+        sz = ref.f64(layer.v_scale)
+        with np.errstate(invalid="ignore"):
+            shift = sz[..., 1:] + 8 * sz[..., :1]
+            mag = np.abs(v - shift) + np.abs(shift)
+    return k, v, mag
 
 
 def _check(layer, q, table, lens, n_new=None, shared=0, scale=None, read_table=None, **kw):
@@ -55,7 +67,7 @@ def _check(layer, q, table, lens, n_new=None, shared=0, scale=None, read_table=N
     assert out.shape == q.shape and out.dtype == q.dtype and lse.shape == (B, Hq, L)
     s = D ** -0.5 if scale is None else scale
     t = (table if read_table is None else read_table).numpy()
-    values, q64 = ref.page_values(layer), ref.f64(q)
+    values, q64 = _values(layer), ref.f64(q)
     mag = max(1.0, float(np.nanmax(np.where(np.isfinite(values[1]), np.abs(values[1]), 0.0))))
     got, glse = ref.f64(out), ref.f64(lse)
     new = [L] * B if n_new is None else [min(max(n, 0), L) for n in n_new]
