@@ -46,8 +46,10 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRowsMaxSeqs = 4096;
-constexpr int kTileTokens = 128;
-constexpr int kRowWaves = 8;
+// More rows than this on a KV head: workgroups of eight waves and 128 tokens a tile
+// in place of four and 64, of which a CU has two at once.
+constexpr int64_t kFewRows = 256;
+constexpr float kBegin = 6.0f, kJoin = 4.0f;  // us, see plan_rows()
 constexpr float kLowest = -3.402823466e38f;  // running maximum before the first token: no score lies below it
 // As in the one-token kernel: the running maximum follows a score that exceeds
 // it by more than 2^8, and stays 2^7 below the scores of fp16 pages, whose
@@ -85,15 +87,14 @@ struct RowsArgs {
 typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
 __device__ inline int32_t scalar_load(const int32_t* p, int64_t i) { return ((scalar_ints)(uintptr_t)p)[i]; }
 
+__device__ inline int32_t length_of(const RowsArgs& a, int32_t len) {
+    const int64_t n = (int64_t)len + a.lens_add, cap = (int64_t)a.table.n * a.pg.page_size;  // (cap < 2^31)
+    return (int32_t)(n < 0 ? 0 : n > cap ? cap : n);
+}
 // How many tokens row (b, l) attends to; -1 for a padded token's.
 __device__ inline int32_t limit_of(const RowsArgs& a, int b, int l) {
-    const int64_t cap = (int64_t)a.table.n * a.pg.page_size;  // (below 2^31)
-    int64_t len = (int64_t)a.lens[b] + a.lens_add;
-    len = len < 0 ? 0 : len > cap ? cap : len;
-    int32_t n = a.L;
-    if (a.n_new) n = min(max(a.n_new[b], 0), a.L);
-    const int64_t lim = len - n + l + 1;
-    return l >= n ? -1 : lim < 0 ? 0 : (int32_t)lim;
+    const int32_t n = a.n_new ? min(max(a.n_new[b], 0), a.L) : a.L;
+    return l >= n ? -1 : max(length_of(a, a.lens[b]) - n + l + 1, 0);
 }
 
 // 16-bit numbers that a weight enters the products as.  One, rounded, for results
@@ -148,18 +149,18 @@ struct Rows {
     static constexpr int KB = k16 ? 2 * D : D;                                 // bytes of a key row
     static constexpr int VB = k16 ? 2 * D : FMT == FKV_PAGES_FP8 ? D : D / 2;  // and of a value row
     static constexpr int KT = KB / 16, VT = VB == 32 ? 4 : VB / 16;            // threads a row
-    static constexpr int KP = KT / 4, VP = VT / 4;                             // passes of 512 threads over 128 rows
+    static constexpr int KP = KT / 4, VP = VT / 4;                             // passes over a tile's rows
     u4 k[KP], v[VP];
     uint32_t kx[KP], vx[VP];  // exponent bytes of the rows (E4M3; of keys for bf16 queries)
     uint32_t ke;              // of run `wave`, token `lane`: the key's (for fp16 queries),
     float2 sz;                // an INT4 value's scale and minimum
 };
 
-template <int D>
+template <int D, int NW>
 struct RowsLds {
     static constexpr int kRow = 2 * D;                 // bytes of a row in 16 bits
-    static constexpr int kTileBytes = kTileTokens * kRow;
-    static constexpr int kNumerators = kRowWaves * 32 * (D + 4) * 4;
+    static constexpr int kTileBytes = 16 * NW * kRow;
+    static constexpr int kNumerators = NW * 32 * (D + 4) * 4;
     static constexpr int kBytes = 4 * kTileBytes > kNumerators ? 4 * kTileBytes : kNumerators;
 };
 
@@ -187,20 +188,21 @@ __device__ inline uint32_t finite_or_zero(uint32_t w) {
     return ((w & e) == e ? 0 : w & 0xFFFFu) | (((w >> 16) & e) == e ? 0 : w & 0xFFFF0000u);
 }
 
-template <int D, int FMT, bool BF>
-__global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs a) {
+template <int D, int FMT, bool BF, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) paged_rows_kernel(RowsArgs a) {
     using R = Rows<D, FMT>;
+    constexpr int kRowWaves = NW, kTileTokens = 16 * NW, kSubs = NW / 2, kThreads = 64 * NW;
     constexpr bool kVB = FMT != FKV_PAGES_F16;  // values and weights are bf16 numbers
     constexpr int kParts = row_parts(FMT, BF);
     // E4M3 keys as bf16 numbers hold their row's power of two; as fp16 numbers the
     // scores are multiplied by it
     constexpr bool kFactors = FMT >= FKV_PAGES_FP8 && !BF;
     constexpr int DT = D / 32;
-    __shared__ __attribute__((aligned(16))) char tiles[RowsLds<D>::kBytes];
+    __shared__ __attribute__((aligned(16))) char tiles[RowsLds<D, NW>::kBytes];
     __shared__ __attribute__((aligned(16))) float key_factor[2][kTileTokens], value_scale[2][kTileTokens],
         value_min[2][kTileTokens];  // (the latter min + 8 scale)
     __shared__ float stat[kRowWaves][32][3];
-    __shared__ int32_t least[kRowWaves], most[kRowWaves], run_tokens[2][8], odd_tile[2];
+    __shared__ int32_t least[kRowWaves], most[kRowWaves], run_tokens[2][kRowWaves], odd_tile[2];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sh = 31 - __builtin_clz((unsigned)a.pg.page_size);
@@ -221,7 +223,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
         seq = rest / a.own.splits, split = rest - seq * a.own.splits;
     }
     const int rows = seq < 0 ? a.B * a.L * a.G : a.L * a.G;
-    const int wr = p.wr, wt = min(4, kRowWaves / wr), rg = wave & (wr - 1), tg = wave / wr;
+    const int wr = p.wr, wt = min(kSubs, kRowWaves / wr), rg = wave & (wr - 1), tg = wave / wr;
     const int row0 = tile * 32 * wr;
     // row r of the part -> (b, l, query head); -1: none
     auto place = [&](int r, int& b, int& l, int& hq) {
@@ -231,33 +233,52 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
         hq = h * a.G + r - token * a.G;
         return r < rows ? limit_of(a, b, l) : -1;
     };
-    int b, l, hq;
-    const int row = row0 + 32 * rg + c;
-    int32_t lim = place(row, b, l, hq);
-    const bool real = lim >= 0;
-    if (seq < 0) lim = min(lim, a.shared);
-
     const int32_t begin = (seq < 0 ? 0 : a.shared) + split * p.chunk;
-    int32_t wave_most = lim, wave_least = real ? lim : 0x7FFFFFFF;
+    const int parts = a.common.splits + a.own.splits;
+    // The ends of rows [first, last): the most tokens that one attends to (-1: none
+    // is real) and the least that a real one does.  A sequence's own rows come by
+    // their tokens, so these are its length and their numbers; the shared tokens'
+    // rows are looked at one by one.
+    int32_t wave_most, wave_least, end, all_least;
+    int b, l, hq;
+    int32_t lim;
+    if (seq >= 0) {
+        const int32_t len = length_of(a, scalar_load(a.lens, seq));
+        const int32_t n = a.n_new ? min(max(scalar_load(a.n_new, seq), 0), a.L) : a.L;
+        auto ends = [&](int first, int last, int32_t& most, int32_t& least) {
+            last = min(last, rows);
+            const int l0 = first / a.G, l1 = min((last - 1) / a.G, n - 1);
+            most = first < last && l0 < n ? max(len - n + l1 + 1, 0) : -1;
+            least = first < last && l0 < n ? max(len - n + l0 + 1, 0) : 0x7FFFFFFF;
+        };
+        ends(row0, row0 + 32 * wr, end, all_least);
+        if (end <= begin && parts > 1) return;
+        ends(row0 + 32 * rg, row0 + 32 * rg + 32, wave_most, wave_least);
+        lim = place(row0 + 32 * rg + c, b, l, hq);
+    } else {
+        lim = min(place(row0 + 32 * rg + c, b, l, hq), a.shared);
+        wave_most = lim, wave_least = lim >= 0 ? lim : 0x7FFFFFFF;
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-        wave_most = max(wave_most, wave_xor(wave_most, o));
-        wave_least = min(wave_least, wave_xor(wave_least, o));
+        for (int o = 16; o >= 1; o >>= 1) {
+            wave_most = max(wave_most, wave_xor(wave_most, o));
+            wave_least = min(wave_least, wave_xor(wave_least, o));
+        }
+        wave_most = __builtin_amdgcn_readfirstlane(wave_most);
+        wave_least = __builtin_amdgcn_readfirstlane(wave_least);
+        if (lane == 0) least[wave] = wave_least, most[wave] = wave_most;
+        __syncthreads();
+        end = most[0], all_least = least[0];
+#pragma unroll
+        for (int w = 1; w < kRowWaves; w++) end = max(end, most[w]), all_least = min(all_least, least[w]);
+        end = __builtin_amdgcn_readfirstlane(end);
+        all_least = __builtin_amdgcn_readfirstlane(all_least);
     }
-    wave_most = __builtin_amdgcn_readfirstlane(wave_most);
-    wave_least = __builtin_amdgcn_readfirstlane(wave_least);
-    if (lane == 0) least[wave] = wave_least, most[wave] = wave_most;
-    if (tid < 2) odd_tile[tid] = -1;
-    __syncthreads();
-    int32_t end = most[0], all_least = least[0];
-#pragma unroll
-    for (int w = 1; w < kRowWaves; w++) end = max(end, most[w]), all_least = min(all_least, least[w]);
-    end = __builtin_amdgcn_readfirstlane(end);
-    all_least = __builtin_amdgcn_readfirstlane(all_least);
+    const bool real = lim >= 0;
     if (seq < 0 || split + 1 < p.splits) end = min(end, begin + p.chunk);
     const int nt = end > begin ? (end - begin + kTileTokens - 1) / kTileTokens : 0;
-    const int parts = a.common.splits + a.own.splits;
     if (nt == 0 && parts > 1) return;
+    if (tid < 2) odd_tile[tid] = -1;
+    __syncthreads();  // (before the first store may set it)
 
     u4 q[D / 16];
     {
@@ -276,8 +297,8 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
     constexpr int kIds = R::KP + (kSame ? 0 : R::VP) + 1;
     int32_t id[kIds];
     auto run_at = [&](int i) {
-        return i < R::KP ? (512 / R::KT * i + (64 / R::KT) * wave) / 16
-               : i < kIds - 1 ? (512 / R::VT * (i - R::KP) + (64 / R::VT) * wave) / 16 : wave;
+        return i < R::KP ? (kThreads / R::KT * i + (64 / R::KT) * wave) / 16
+               : i < kIds - 1 ? (kThreads / R::VT * (i - R::KP) + (64 / R::VT) * wave) / 16 : wave;
     };
     auto fetch = [&](int32_t tok) {
 #pragma unroll
@@ -339,13 +360,13 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
     // ... and into the LDS, in 16 bits.
     auto store = [&](int32_t tok, int t, int buf) {
         if (!whole) blank();
-        char* keys = tiles + buf * 2 * RowsLds<D>::kTileBytes;
-        char* values = keys + RowsLds<D>::kTileBytes;
+        char* keys = tiles + buf * 2 * RowsLds<D, NW>::kTileBytes;
+        char* values = keys + RowsLds<D, NW>::kTileBytes;
         const bool look = tok + kTileTokens > all_least;  // (tokens that not all rows attend to)
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < R::KP; i++) {
-            const int r = (512 / R::KT) * i + tid / R::KT, ch = tid % R::KT;
+            const int r = (kThreads / R::KT) * i + tid / R::KT, ch = tid % R::KT;
             const u4 x = st.k[i];
             if (R::k16) {
                 *(u4*)(keys + key_place<D>(r, ch)) = x;
@@ -358,7 +379,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
         }
 #pragma unroll
         for (int i = 0; i < R::VP; i++) {
-            const int r = (512 / R::VT) * i + tid / R::VT, ch = tid % R::VT;
+            const int r = (kThreads / R::VT) * i + tid / R::VT, ch = tid % R::VT;
             const u4 x = st.v[i];
             if (R::k16) {
                 *(u4*)(values + value_place<D>(r, ch)) = x;
@@ -377,13 +398,13 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
             } else {
                 // code - 8 in place of the code and min + 8 scale in place of min: both
                 // are then of the values' size, and so is what rounding a weight costs
-                constexpr int NW = R::VB == 32 ? 2 : 4;  // dwords of eight codes: a chunk each
+                constexpr int kWords = R::VB == 32 ? 2 : 4;  // dwords of eight codes: a chunk each
 #pragma unroll
-                for (int j = 0; j < NW; j++) {
+                for (int j = 0; j < kWords; j++) {
                     const uint32_t even = less_eight(x[j] & 0x0F0F0F0Fu), other = less_eight((x[j] >> 4) & 0x0F0F0F0Fu);
                     const uint32_t lo = __builtin_amdgcn_perm(other, even, 0x05010400u);
                     const uint32_t hi = __builtin_amdgcn_perm(other, even, 0x07030602u);
-                    *(u4*)(values + value_place<D>(r, NW * ch + j)) =
+                    *(u4*)(values + value_place<D>(r, kWords * ch + j)) =
                         u4{cvt_codes<true, false>(lo, 512.0f), cvt_codes<true, true>(lo, 512.0f),
                            cvt_codes<true, false>(hi, 512.0f), cvt_codes<true, true>(hi, 512.0f)};
                 }
@@ -412,7 +433,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
     // Lane constants of the LDS reads.  Keys: 16-byte chunk 2 i + hf of token c,
     // the chunk's upper bit a constant offset; values: of each 32 dims the rows and
     // bytes of a transposing read (tokens 8 and 16 further lie a constant further).
-    constexpr int kKeys = 4, kRow = RowsLds<D>::kRow;
+    constexpr int kKeys = 4, kRow = RowsLds<D, NW>::kRow;
     uint32_t key_lane[kKeys], value_lane[DT];
     {
         const uint32_t tr_row = 4 * hf + ((lane & 15) >> 2), tr_byte = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
@@ -431,7 +452,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
     auto key_of = [&](const char* keys, int i) { return *(const u4*)(keys + key_lane[i % kKeys] + i / kKeys * 128); };
     // Scores (not scaled) of the tile's 32 tokens `sub`; the lane's are 8 (i / 4) + 4 hf + i % 4.
     auto score = [&](int buf, int sub) {
-        const char* keys = tiles + buf * 2 * RowsLds<D>::kTileBytes + 32 * sub * kRow;
+        const char* keys = tiles + buf * 2 * RowsLds<D, NW>::kTileBytes + 32 * sub * kRow;
         f16v s;
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = 0.0f;
@@ -492,8 +513,8 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
     // scores of the tokens `next` of the tile in next_buf, whose largest is returned
     // (of whatever lies there where these were the last ones).
     auto step = [&](f16v& s, int32_t tok, int buf, int sub, int next_buf, int next) {
-        const char* values = tiles + (buf * 2 + 1) * RowsLds<D>::kTileBytes + 32 * sub * kRow;
-        const char* keys = tiles + next_buf * 2 * RowsLds<D>::kTileBytes + 32 * next * kRow;
+        const char* values = tiles + (buf * 2 + 1) * RowsLds<D, NW>::kTileBytes + 32 * sub * kRow;
+        const char* keys = tiles + next_buf * 2 * RowsLds<D, NW>::kTileBytes + 32 * next * kRow;
         const float by = wide ? 1.0f : a.scale, off = wide ? 0.0f : m;
         float w[16], part_sum = 0.0f;
         u4 part_of[2][kParts];  // [16 tokens][part]
@@ -598,7 +619,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
     // 0 would carry them into every row.  So they join the rows that attend to them
     // here, and the products find zeros in their place.
     auto settle = [&](int32_t tok, int buf) {
-        char* values = tiles + (buf * 2 + 1) * RowsLds<D>::kTileBytes;
+        char* values = tiles + (buf * 2 + 1) * RowsLds<D, NW>::kTileBytes;
         if (tg < wt)
             for (int r = 0; r < kTileTokens; r++) {
                 if (((r >> 5) & (wt - 1)) != tg) continue;
@@ -624,7 +645,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
         if (FMT == FKV_PAGES_FP8_INT4) {
             if (tid < kTileTokens && !(fabsf(value_min[buf][tid]) < INFINITY)) value_scale[buf][tid] = value_min[buf][tid] = 0.0f;
         } else {
-            for (int i = tid; i < RowsLds<D>::kTileBytes / 8; i += 64 * kRowWaves) {
+            for (int i = tid; i < RowsLds<D, NW>::kTileBytes / 8; i += 64 * kRowWaves) {
                 const u2 w = *(const u2*)(values + 8 * i);
                 *(u2*)(values + 8 * i) = u2{finite_or_zero<kVB>(w.x), finite_or_zero<kVB>(w.y)};
             }
@@ -657,8 +678,8 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
         const int32_t tok = begin + t * kTileTokens;
         const int buf = t & 1;
         if (__builtin_amdgcn_readfirstlane(odd_tile[buf]) == t) settle(tok, buf);
-        for (int j = wt; j <= 4; j += wt) {
-            const bool last = j == 4;
+        for (int j = wt; j <= kSubs; j += wt) {
+            const bool last = j == kSubs;
             if (last && t + 1 < nt) {
                 __syncthreads();
                 store(tok + kTileTokens, t + 1, buf ^ 1);
@@ -689,13 +710,13 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) paged_rows_kernel(RowsArgs 
     }
     __syncthreads();
     constexpr int N = D / 16;
-    for (int i = 0; i < wr; i++) {
-        const int rr = tid >> 4, d0 = (tid & 15) * N;
+    for (int r = tid >> 4; r < 32 * wr; r += kThreads / 16) {
+        const int i = r >> 5, rr = r & 31, d0 = (tid & 15) * N;
         int b, l, hq;
-        const int32_t lim = place(row0 + 32 * i + rr, b, l, hq);
+        const int32_t lim = place(row0 + r, b, l, hq);
         const int64_t at = ((int64_t)b * a.Hq + hq) * a.L + l;
         if (lim < 0) {
-            if (parts == 1 && a.lse && (tid & 15) == 0 && row0 + 32 * i + rr < rows) a.lse[at] = -INFINITY;
+            if (parts == 1 && a.lse && (tid & 15) == 0 && row0 + r < rows) a.lse[at] = -INFINITY;
             continue;
         }
         float top = kLowest, all = 0.0f, low = 0.0f, x[N] = {};
@@ -801,34 +822,65 @@ __global__ void __launch_bounds__(256) paged_rows_join_kernel(RowsArgs a, int64_
 
 struct RowsPlan {
     RowParts common, own;
+    int32_t shared;
+    int waves;  // of a workgroup
     int64_t blocks, bytes;
 };
 
-static int waves_for(int64_t rows) { return rows > 128 ? 8 : rows > 64 ? 4 : rows > 32 ? 2 : 1; }
-
-// Workgroups and workspace of a call (a function of sizes alone).
+// Workgroups and workspace of a call (a function of sizes alone).  How many parts
+// the tokens are cut into is what a model of the time finds best: a workgroup
+// takes kBegin for its beginning and end and a time per tile of tokens that grows
+// with its rows (the cache's bytes, then the products), the chip has `slots` of
+// them at once, and parts cost their join.
 static RowsPlan plan_rows(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, int64_t shared, int64_t max_len) {
     RowsPlan r;
+    if (B == 1) shared = 0;  // (with nobody)
+    r.shared = (int32_t)shared;
     const int64_t G = Hq / p->H, own_rows = L * G, all_rows = B * own_rows;
-    const int64_t own_tokens = std::max<int64_t>(1, max_len - shared);
-    r.own.wr = waves_for(own_rows);
-    r.own.tiles = (int32_t)cdiv(own_rows, 32 * r.own.wr);
-    r.common.wr = waves_for(all_rows);
-    r.common.tiles = shared ? (int32_t)cdiv(all_rows, 32 * r.common.wr) : 0;
-    // tiles of 128 tokens in all, dealt to 512 workgroups of two tiles at least
-    const int64_t tiles = p->H * (r.common.tiles * cdiv(shared, kTileTokens) + B * r.own.tiles * cdiv(own_tokens, kTileTokens));
-    const int64_t per = std::max<int64_t>(2, cdiv(tiles, 512));
-    auto cut = [&](RowParts& part, int64_t tokens, int64_t groups) {
-        // (workgroups enough without parts: none)
-        const int64_t n = groups >= 256 ? 1 : cdiv(cdiv(tokens, kTileTokens), per);
-        part.chunk = (int32_t)(cdiv(cdiv(tokens, kTileTokens), std::max<int64_t>(n, 1)) * kTileTokens);
-        part.splits = (int32_t)cdiv(tokens, part.chunk);
+    r.waves = (shared ? all_rows : own_rows) > kFewRows ? 8 : 4;
+    const int64_t tile = 16 * r.waves, slots = r.waves == 8 ? 256 : 512;
+    auto part = [&](int64_t rows) {
+        RowParts q;
+        q.wr = rows > 128 && r.waves == 8 ? 8 : rows > 64 ? 4 : rows > 32 ? 2 : 1;
+        q.tiles = (int32_t)cdiv(rows, 32 * q.wr);
+        return q;
     };
-    r.common.chunk = kTileTokens;
-    r.common.splits = 0;
-    if (shared) cut(r.common, shared, p->H * r.common.tiles);
-    cut(r.own, own_tokens, p->H * B * r.own.tiles);
-    r.blocks = p->H * ((int64_t)r.common.tiles * r.common.splits + (int64_t)B * r.own.tiles * r.own.splits);
+    // us for a tile
+    auto time = [&](const RowParts& q) { return q.wr == 8 ? 4.9f : q.wr == 4 ? (r.waves == 8 ? 3.7f : 4.3f) : 2.8f; };
+    r.own = part(own_rows);
+    r.common = part(all_rows);
+    if (!shared) r.common.tiles = 0;
+    const int64_t own_tiles = cdiv(std::max<int64_t>(1, max_len - shared), tile), common_tiles = cdiv(shared, tile);
+    const int64_t own_pieces = (int64_t)B * p->H * r.own.tiles, common_pieces = (int64_t)p->H * r.common.tiles;
+    const float join = (float)((double)all_rows * p->H * (p->D + 4) * 8 / 4e6);  // a record of each row, written and read
+    float best = INFINITY;
+    const int64_t most = std::min<int64_t>(shared ? common_tiles : own_tiles, 64);
+    for (int64_t n = 1; n <= most; n++) {
+        int64_t own_parts = n, common_parts = 0;
+        float t, longest = 0;
+        double work = 0;
+        if (shared) {
+            common_parts = cdiv(common_tiles, cdiv(common_tiles, n));
+            longest = kBegin + cdiv(common_tiles, n) * time(r.common);
+            work = common_pieces * common_parts * longest;
+            own_parts = std::max<int64_t>(1, (int64_t)(own_tiles * time(r.own) / longest + 0.999f));
+        }
+        own_parts = cdiv(own_tiles, cdiv(own_tiles, own_parts));
+        const float own_time = kBegin + cdiv(own_tiles, own_parts) * time(r.own);
+        longest = std::max(longest, own_time);
+        // (many sequences have lengths of their own: three quarters of max_len, say)
+        if (B <= 4 && !shared) t = cdiv(own_pieces * own_parts, slots) * own_time;
+        else t = (float)(work + 0.75 * own_pieces * own_parts * own_time) / slots + 0.75f * longest;
+        if (common_parts + own_parts > 1) t += kJoin + (common_parts + own_parts) * join;
+        if (t < best) {
+            best = t;
+            r.common.splits = (int32_t)common_parts;
+            r.own.splits = (int32_t)own_parts;
+        }
+    }
+    r.common.chunk = (int32_t)(shared ? cdiv(common_tiles, r.common.splits) * tile : tile);
+    r.own.chunk = (int32_t)(cdiv(own_tiles, r.own.splits) * tile);
+    r.blocks = common_pieces * r.common.splits + own_pieces * r.own.splits;
     const int64_t parts = r.common.splits + r.own.splits;
     r.bytes = parts > 1 ? (int64_t)B * Hq * L * parts * (p->D + 4) * 4 : 0;
     return r;
@@ -849,7 +901,8 @@ static int check_rows(const char* who, const fkv_pages* p, int32_t Hq, int32_t B
 template <int D, int FMT, bool BF>
 static int launch_rows(const RowsArgs& a, const RowsPlan& p, hipStream_t s) {
     const char* w = "fkv_paged_attn_rows";
-    if (int e = start_kernel(w, paged_rows_kernel<D, FMT, BF>, (uint32_t)p.blocks, 64 * kRowWaves, s, a)) return e;
+    if (int e = p.waves == 8 ? start_kernel(w, paged_rows_kernel<D, FMT, BF, 8>, (uint32_t)p.blocks, 512, s, a)
+                             : start_kernel(w, paged_rows_kernel<D, FMT, BF, 4>, (uint32_t)p.blocks, 256, s, a)) return e;
     if (p.bytes == 0) return FKV_OK;
     const int64_t rows = (int64_t)a.B * a.Hq * a.L;
     return start_kernel(w, paged_rows_join_kernel<D, BF>, (uint32_t)cdiv(rows, 4), 256, s, a, rows);
@@ -921,7 +974,7 @@ int fkv_paged_attn_rows(const fkv_pages* pages, const fkv_rows* query, int32_t q
     a.Hq = Hq;
     a.G = Hq / pages->H;
     a.L = L;
-    a.shared = (int32_t)shared;
+    a.shared = p.shared;
     a.scale = std::fabs(scale) * 1.4426950408889634f;
     a.q_sign = std::signbit(scale) ? 0x80008000u : 0;
     a.q_mask = ~0u;
