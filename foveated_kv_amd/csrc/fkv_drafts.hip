@@ -22,8 +22,11 @@ namespace fkv {
 
 constexpr int kDraftThreads = 256;
 constexpr int kMaxDrafts = 63;      // a lane each, and one for the end
-constexpr int64_t kChunk = 4096;    // tokens of a vocabulary's chunk, or more
+constexpr int kChunkGroups = 4;     // groups of 256 tokens a wave has of a chunk
+constexpr int64_t kChunk = 256 * kChunkGroups * (kDraftThreads / 64);  // tokens of a chunk (4096), or a multiple of it
 constexpr int kMaxChunks = 512;
+constexpr int kSmallGroups = 8;     // ... and of a small vocabulary
+constexpr int64_t kSmall = 256 * kSmallGroups * 16;
 
 struct DraftArgs {
     const char* target;
@@ -84,87 +87,177 @@ struct Weights {
         const double d = q ? (double)pv - (double)qv : v == x ? 0.0 : (double)pv;
         return d > 0.0 ? d : 0.0;
     }
-    __device__ double at(int64_t v) const { return of(prob<DT>(p, v), q ? prob<DT>(q, v) : 0.0f, v); }
-    __device__ double plain(int64_t v) const {
-        const double d = prob<DT>(p, v);
-        return d > 0.0 ? d : 0.0;
-    }
 };
 
-__device__ inline double block_sum(double v, double* lds) {
+// A block's tokens: wave w has kGroups groups of 256 neighbouring ones from
+// first + 256 kGroups w on, four neighbouring ones a lane.
+template <int DT, bool VEC, int GROUPS>
+__device__ inline void load_weights(const Weights<DT>& w, int64_t first, int64_t last, bool plain, double (&x)[GROUPS][4],
+                                    double& whole) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    f4 p[GROUPS], q[GROUPS];
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++) {
+        const int64_t v = first + 256 * (GROUPS * wave + g) + 4 * lane;
+        p[g] = q[g] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        auto four = [&](const char* row) {
+            f4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (VEC) {  // (rows of a multiple of four tokens, aligned)
+                if (v < last) {
+                    if (DT == FKV_F32) {
+                        r = *(const f4*)(row + 4 * v);
+                    } else {
+                        const fkv_u2 u = *(const fkv_u2*)(row + 2 * v);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint16_t k = (uint16_t)(u[i / 2] >> (16 * (i & 1)));
+                            r[i] = DT == FKV_F16 ? h2f(k) : bf2f(k);
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (v + i < last) r[i] = prob<DT>(row, v + i);
+            }
+            return r;
+        };
+        p[g] = four(w.p);
+        if (w.q) q[g] = four(w.q);
+    }
+    whole = 0.0;
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const double own = p[g][i] > 0.0f ? (double)p[g][i] : 0.0;
+            whole += own;
+            x[g][i] = plain ? own : w.of(p[g][i], q[g][i], first + 256 * (GROUPS * wave + g) + 4 * lane + i);
+        }
+}
+
+__device__ inline double wave_total(double v) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) v += wave_xor(v, o);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.0;
+    return v;
+}
+template <int GROUPS>
+__device__ inline double lane_total(const double (&x)[GROUPS][4]) {
+    double v = 0.0;
 #pragma unroll
-    for (int w = 0; w < kDraftThreads / 64; w++) v += lds[w];
-    __syncthreads();
+    for (int g = 0; g < GROUPS; g++) v += (x[g][0] + x[g][1]) + (x[g][2] + x[g][3]);
     return v;
 }
 
-// Sums of one chunk.  VEC: rows are 16-byte aligned and of a multiple of 16 bytes.
+// Sums over a block of NT threads, of every thread's two numbers; `sums` keeps the
+// waves' of the first.
+template <int NT>
+__device__ inline void block_sums(double a, double b, double (&sums)[NT / 64], double (&other)[NT / 64], double& sa, double& sb) {
+    a = wave_total(a), b = wave_total(b);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = a, other[threadIdx.x >> 6] = b;
+    __syncthreads();
+    sa = sb = 0.0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) sa += sums[w], sb += other[w];
+}
+
+// The first token of the block at which the running sum, from `base` on, exceeds
+// goal, or the last one with a weight where rounding leaves none; by the waves'
+// sums, then a group's, then a lane's.  One thread writes it to *found.
+template <int NT, int GROUPS>
+__device__ inline void find_token(const double (&x)[GROUPS][4], const double (&sums)[NT / 64], double base, double goal,
+                                  int64_t first, int64_t* found) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int chosen = 0;
+    double run = base, at = base;
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) {
+        if (sums[w] > 0.0 && !(at > goal)) chosen = w, run = at;
+        at += sums[w];
+    }
+    if (wave != chosen) return;
+    int group = 0;
+    double in_group = run;
+    at = run;
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++) {
+        const double total = wave_total((x[g][0] + x[g][1]) + (x[g][2] + x[g][3]));
+        if (total > 0.0 && !(at > goal)) group = g, in_group = at;
+        at += total;
+    }
+    double y[4] = {};
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] = group == g ? x[g][i] : y[i];
+    const double mine = (y[0] + y[1]) + (y[2] + y[3]);
+    double before = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double z = __shfl_up(before, o, 64);
+        if (lane >= o) before += z;
+    }
+    double sum = in_group + (before - mine);
+    int past = 4, real = -1;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        sum += y[i];
+        if (y[i] > 0.0) {
+            real = i;
+            if (past == 4 && sum > goal) past = i;
+        }
+    }
+    const uint64_t hit = __ballot(past < 4), any = __ballot(real >= 0);
+    const int64_t v = first + 256 * (GROUPS * wave + group) + 4 * lane;
+    if (hit ? lane == __builtin_ctzll(hit) : lane == 63 - __builtin_clzll(any | 1)) *found = v + (hit ? past : max(real, 0));
+}
+
+__device__ inline void write_tokens(const DraftArgs& a, int b, int at, int64_t token) {
+    const int tid = threadIdx.x;
+    if (tid <= a.K) {
+        const int64_t x = tid < at ? drafted(a, b, tid) : tid == at ? token : -1;
+        const int64_t o = (int64_t)b * (a.K + 1) + tid;
+        if (a.is64) ((int64_t*)a.out)[o] = x;
+        else ((int32_t*)a.out)[o] = (int32_t)x;
+    }
+    if (tid == 0) a.accepted[b] = at;
+}
+
+// Sums of one chunk.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kDraftThreads) draft_sums_kernel(DraftArgs a) {
-    __shared__ double lds[kDraftThreads / 64];
+    __shared__ double sums[kDraftThreads / 64], other[kDraftThreads / 64];
     const int b = blockIdx.y;
     int n;
     const int at = standing<DT>(a, b, n);
     const Weights<DT> w(a, b, at, at < n);
     const int64_t first = (int64_t)blockIdx.x * a.chunk, last = min(first + a.chunk, (int64_t)a.V);
     double sum = 0.0, whole = 0.0;
-    if (VEC) {
-        constexpr int N = DT == FKV_F32 ? 4 : 8;  // of a load
-        constexpr int U = 4;
-        const fkv_u4 none = {0, 0, 0, 0};
-        for (int64_t v0 = first + N * threadIdx.x; v0 < last; v0 += U * N * kDraftThreads) {
-            fkv_u4 x[U], y[U];
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int64_t v = v0 + u * N * kDraftThreads;
-                const bool in = v < last;
-                x[u] = in ? *(const fkv_u4*)(w.p + v * (16 / N)) : none;
-                y[u] = in && w.q ? *(const fkv_u4*)(w.q + v * (16 / N)) : none;
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++)
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    auto value = [&](const fkv_u4& r) {
-                        if (DT == FKV_F32) return __uint_as_float(r[i % 4]);
-                        const uint16_t k = (uint16_t)(r[i / 2 % 4] >> (16 * (i & 1)));
-                        return DT == FKV_F16 ? h2f(k) : bf2f(k);
-                    };
-                    const float p = value(x[u]);
-                    sum += w.of(p, value(y[u]), v0 + u * N * kDraftThreads + i);
-                    whole += p > 0.0f ? (double)p : 0.0;
-                }
-        }
-    } else {
-        for (int64_t v = first + threadIdx.x; v < last; v += kDraftThreads) {
-            sum += w.at(v);
-            whole += w.plain(v);
-        }
+    for (int64_t v = first; v < last; v += kChunk) {
+        double x[kChunkGroups][4], y;
+        load_weights<DT, VEC, kChunkGroups>(w, v, last, false, x, y);
+        sum += lane_total(x);
+        whole += y;
     }
-    sum = block_sum(sum, lds);
-    whole = block_sum(whole, lds);
+    block_sums<kDraftThreads>(sum, whole, sums, other, sum, whole);
     if (threadIdx.x == 0) a.sums[(int64_t)b * a.chunks + blockIdx.x] = make_double2(sum, whole);
 }
 
-// The next token of one sequence, and its results.
-template <int DT>
+// The next token of one sequence from its chunks' sums, and its results.
+template <int DT, bool VEC>
 __global__ void __launch_bounds__(kDraftThreads) draft_choice_kernel(DraftArgs a) {
-    __shared__ double chunk_sum[2][kMaxChunks], before[kDraftThreads / 64];
-    __shared__ int64_t found, last_real;
-    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int n;
-    const int at = standing<DT>(a, b, n);
-    const Weights<DT> w(a, b, at, at < n);
+    __shared__ double chunk_sum[2][kMaxChunks], sums[kDraftThreads / 64], other[kDraftThreads / 64];
+    __shared__ int64_t found;
+    const int b = blockIdx.x, tid = threadIdx.x;
     for (int i = tid; i < a.chunks; i += kDraftThreads) {
         const double2 s = a.sums[(int64_t)b * a.chunks + i];
         chunk_sum[0][i] = s.x, chunk_sum[1][i] = s.y;
     }
-    if (tid == 0) found = last_real = -1;
+    int n;
+    const int at = standing<DT>(a, b, n);
+    const Weights<DT> w(a, b, at, at < n);
+    if (tid == 0) found = -1;
     __syncthreads();
     double total = 0.0, whole = 0.0;
     for (int i = 0; i < a.chunks; i++) total += chunk_sum[0][i], whole += chunk_sum[1][i];
@@ -172,7 +265,6 @@ __global__ void __launch_bounds__(kDraftThreads) draft_choice_kernel(DraftArgs a
     // probabilities.
     const bool plain = !(total > 0.0);
     if (plain) total = whole;
-    int64_t token = -1;
     if (total > 0.0 && total < (double)INFINITY) {
         const double goal = (double)a.uniforms[(int64_t)b * (a.K + 1) + a.K] * total;
         // the chunk in which the running sum passes it (rounding: or the last with any weight)
@@ -185,47 +277,45 @@ __global__ void __launch_bounds__(kDraftThreads) draft_choice_kernel(DraftArgs a
             if (sum > goal) break;
         }
         const int64_t first = (int64_t)c * a.chunk, last = min(first + a.chunk, (int64_t)a.V);
-        const int64_t per = (a.chunk + kDraftThreads - 1) / kDraftThreads;
-        const int64_t v0 = min(first + tid * per, last), v1 = min(v0 + per, last);
-        double mine = 0.0;
-        int64_t real = -1;
-        for (int64_t v = v0; v < v1; v++) {
-            const double x = plain ? w.plain(v) : w.at(v);
-            mine += x;
-            if (x > 0.0) real = v;
+        // (a chunk of several blocks, by a vocabulary of more than 2^21: one by one)
+        for (int64_t v = first; v < last; v += kChunk) {
+            double x[kChunkGroups][4], y, block;
+            load_weights<DT, VEC, kChunkGroups>(w, v, last, plain, x, y);
+            block_sums<kDraftThreads>(lane_total(x), 0.0, sums, other, block, y);
+            if (block > 0.0) find_token<kDraftThreads>(x, sums, base, goal, v, &found);
+            base += block;
+            __syncthreads();
+            if (base > goal) break;
         }
-        double sums = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double x = __shfl_up(sums, o, 64);
-            if (lane >= o) sums += x;
-        }
-        if (lane == 63) before[wave] = sums;
-        __syncthreads();
-        double run = base + (sums - mine);
-        for (int i = 0; i < wave; i++) run += before[i];
-        // the first token, over all threads, at which the running sum passes it
-        int64_t mine_at = -1;
-        for (int64_t v = v0; v < v1; v++) {
-            const double x = plain ? w.plain(v) : w.at(v);
-            run += x;
-            if (x > 0.0 && run > goal) {
-                mine_at = v;
-                break;
-            }
-        }
-        atomicMin((unsigned long long*)&found, (unsigned long long)mine_at);  // (-1: above all)
-        atomicMax((long long*)&last_real, (long long)real);
-        __syncthreads();
-        token = found >= 0 ? found : last_real;
     }
-    if (tid <= a.K) {
-        const int64_t x = tid < at ? drafted(a, b, tid) : tid == at ? token : -1;
-        const int64_t o = (int64_t)b * (a.K + 1) + tid;
-        if (a.is64) ((int64_t*)a.out)[o] = x;
-        else ((int32_t*)a.out)[o] = (int32_t)x;
+    __syncthreads();
+    write_tokens(a, b, at, found);
+}
+
+// Both in one for a small vocabulary, a workgroup a sequence: one launch, and each
+// probability read once.
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(1024) draft_small_kernel(DraftArgs a) {
+    __shared__ double sums[16], other[16];
+    __shared__ int64_t found;
+    const int b = blockIdx.x;
+    if (threadIdx.x == 0) found = -1;
+    int n;
+    const int at = standing<DT>(a, b, n);
+    const Weights<DT> w(a, b, at, at < n);
+    double x[kSmallGroups][4], whole, total;
+    load_weights<DT, VEC, kSmallGroups>(w, 0, a.V, false, x, whole);
+    block_sums<1024>(lane_total(x), whole, sums, other, total, whole);
+    const bool plain = !(total > 0.0);
+    if (plain) {  // (the same for the whole workgroup)
+        __syncthreads();
+        load_weights<DT, VEC, kSmallGroups>(w, 0, a.V, true, x, whole);
+        block_sums<1024>(lane_total(x), 0.0, sums, other, total, whole);
     }
-    if (tid == 0) a.accepted[b] = at;
+    if (total > 0.0 && total < (double)INFINITY)
+        find_token<1024>(x, sums, 0.0, (double)a.uniforms[(int64_t)b * (a.K + 1) + a.K] * total, 0, &found);
+    __syncthreads();
+    write_tokens(a, b, at, found);
 }
 
 struct DraftPlan {
@@ -287,14 +377,17 @@ int fkv_verify_drafts(const fkv_rows* target, const fkv_rows* draft, int32_t dty
     a.chunk = (int32_t)p.chunk;
     a.chunks = (int32_t)p.chunks;
     a.is64 = tokens64 != 0;
-    const bool vec = !(((uintptr_t)a.target | a.t_sb | a.t_sk | (uintptr_t)a.draft | a.d_sb | a.d_sk | V * es) & 15);
+    // (four tokens a load, which rows of a multiple of four allow)
+    const bool vec = !(((uintptr_t)a.target | a.t_sb | a.t_sk | (uintptr_t)a.draft | a.d_sb | a.d_sk | V * es) & (4 * es - 1));
     hipStream_t s = (hipStream_t)stream;
     auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
+        if (V <= kSmall)
+            return start_kernel(w, vec ? draft_small_kernel<DT, true> : draft_small_kernel<DT, false>, B, 1024, s, a);
         const dim3 grid((uint32_t)p.chunks, B);
         if (int e = start_kernel(w, vec ? draft_sums_kernel<DT, true> : draft_sums_kernel<DT, false>, grid, kDraftThreads, s, a))
             return e;
-        return start_kernel(w, draft_choice_kernel<DT>, B, kDraftThreads, s, a);
+        return start_kernel(w, vec ? draft_choice_kernel<DT, true> : draft_choice_kernel<DT, false>, B, kDraftThreads, s, a);
     };
     if (dtype == FKV_F16) return go(std::integral_constant<int, FKV_F16>{});
     if (dtype == FKV_BF16) return go(std::integral_constant<int, FKV_BF16>{});
