@@ -224,6 +224,52 @@ def test_scores_that_fp32_cannot_tell_apart(paged):
         assert layer.attend_sparse(q, table.cuda(), _i32([6 * page]), k, return_pages=True)[1].flatten().tolist() == want
 
 
+@pytest.mark.parametrize("qd", [torch.bfloat16, torch.float16])
+def test_long_contexts(paged, qd):
+    """More pages than the choice holds keys of (8192), scores of all kinds: far
+    apart, near one another, and equal."""
+    page, D, n = 16, 64, 9001
+    layer = _with_bounds(paged, paged.PagedLayer(600, 1, D, page, "fp8"))
+    k = _randn(50, 600, 1, page, D)
+    k[200:400] = k[200] + 1e-3 * _randn(51, 200, 1, page, D)
+    k[400:] *= 0.01
+    ids = torch.arange(600, dtype=torch.int32, device="cuda").view(600, 1)
+    layer.write(k.cuda(), _randn(52, 600, 1, page, D).cuda(), ids, 0)
+    table = torch.randint(0, 600, (1, n), generator=torch.Generator().manual_seed(53)).int()
+    q = _randn(54, 1, 3, 1, D).to(qd).cuda()
+    for k in (2, 40, 700, 3500):
+        _check(layer, q, table, [n * page - 3], k)
+    assert n > 8192
+
+
+def test_very_long_context(paged):
+    """More pages than the choice has marks for (2^18), of which many are equal."""
+    page, D, n = 16, 64, 2 ** 18 + 1000
+    layer = _with_bounds(paged, paged.PagedLayer(50, 1, D, page, "bf16"))
+    layer.k.copy_(_randn(55, 50, 1, page, D))
+    layer.v.copy_(_randn(56, 50, 1, page, D))
+    layer.bound(torch.arange(50, dtype=torch.int32, device="cuda").view(50, 1), 0, page)
+    table = torch.randint(0, 50, (1, n), generator=torch.Generator().manual_seed(57)).int()
+    q = _randn(58, 1, 1, 1, D).bfloat16().cuda()
+    for k in (3, 6000):
+        _check(layer, q, table, [n * page], k)
+
+
+def test_scores_that_overflow_fp32(paged):
+    """Bounds whose products pass the end of fp32's range, of either sign."""
+    page, D = 16, 64
+    layer = _with_bounds(paged, paged.PagedLayer(8, 1, D, page, "bf16"))
+    layer.k.fill_(1.0)
+    for i, x in enumerate([3e38, -3e38, 2e38, 1.0, -1e38, 2.5e38, 1e30]):
+        layer.k[i, ..., :3] = x
+    layer.bound(torch.arange(8, dtype=torch.int32, device="cuda").view(8, 1), 0, page)
+    table = torch.arange(8, dtype=torch.int32).view(1, 8)
+    q = torch.full((1, 2, 1, D), 4.0, dtype=torch.bfloat16, device="cuda")
+    for k, want in ((2, [0, 7]), (3, [0, 5, 7]), (4, [0, 2, 5, 7]), (6, [0, 2, 3, 5, 6, 7]), (7, [0, 2, 3, 4, 5, 6, 7])):
+        got = layer.attend_sparse(q, table.cuda(), _i32([8 * page]), k, return_pages=True, scale=0.0)[1]
+        assert got.flatten().tolist() == want
+
+
 def test_pages_outside_the_pool_and_bounds_not_finite(paged):
     page, H, G, D = 16, 2, 3, 64
     layer = _with_bounds(paged, _filled(paged, "bf16", 30, H, D, page, 40))
