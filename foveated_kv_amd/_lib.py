@@ -228,8 +228,14 @@ def calls():
         except ImportError as e:
             raise FkvLibraryError(f"cannot load {_HERE}/_fkv_calls.so: {e}; run `make -C foveated_kv_amd/csrc` "
                                   "or __graft_entry__.build()") from e
-        _fkv_calls.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
-            "fkv_rope_apply", "fkv_paged_write", "fkv_paged_read", "fkv_paged_attn_workspace", "fkv_paged_attn")), check)
+        def addresses(*names):
+            return [ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names]
+
+        _fkv_calls.bind(*addresses("fkv_rope_apply", "fkv_paged_write", "fkv_paged_read", "fkv_paged_attn_workspace",
+                                   "fkv_paged_attn"), check)
+        _fkv_calls.bind_drafting(*addresses("fkv_paged_attn_rows_workspace", "fkv_paged_attn_rows",
+                                            "fkv_paged_attn_sparse_workspace", "fkv_paged_attn_sparse",
+                                            "fkv_verify_drafts_workspace", "fkv_verify_drafts"))
         _calls = _fkv_calls
     return _calls
 

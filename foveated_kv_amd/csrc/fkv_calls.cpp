@@ -5,7 +5,9 @@
 // A decode step's kernels take 4 to 5 us and their launch 3, which the checks in
 // Python more than doubled.  Host time of a call, a step of 64 sequences with 32
 // query and 8 KV heads: rotation 8.1 us from Python, 4.6 so; write 10.9 and 5.1;
-// attention over 512 tokens of one 9.5 and 4.6.
+// attention over 512 tokens of one 9.5 and 4.6; of one sequence, five tokens over
+// 4000 15.1 and 9.3 (two launches), one over 8 of 63 pages 17.5 and 11.5 (four),
+// five drafts of 32000 entries verified 14.7 and 6.1.
 //
 // Each function returns NotImplemented for whatever is not plain -- a wrong
 // argument, a tensor to be copied first, one of another GPU than the current
@@ -38,6 +40,14 @@ struct {
     decltype(&fkv_paged_attn_workspace) workspace;
     decltype(&fkv_paged_attn) attn;
 } lib;
+struct {
+    decltype(&fkv_paged_attn_rows_workspace) rows_workspace;
+    decltype(&fkv_paged_attn_rows) rows;
+    decltype(&fkv_paged_attn_sparse_workspace) sparse_workspace;
+    decltype(&fkv_paged_attn_sparse) sparse;
+    decltype(&fkv_verify_drafts_workspace) verify_workspace;
+    decltype(&fkv_verify_drafts) verify;
+} drafting;
 PyObject* check = nullptr;  // _lib.check(code, name), which raises
 
 // What a call meets that paged.py has to look at.
@@ -293,6 +303,15 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// The default of attention's scale, or a number.
+float scale_of(PyObject* o, int64_t D) {
+    if (o == Py_None) return (float)(1.0 / std::sqrt((double)D));
+    need(PyFloat_Check(o) || PyLong_Check(o));
+    const double scale = PyFloat_AsDouble(o);
+    need(!PyErr_Occurred());
+    return (float)scale;
+}
+
 // attend(key, query, table, lens, max_len, lens_add, scale, out, return_lse)
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return plain(n, 9, [&](bool& begun) {
@@ -308,12 +327,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         int64_t most = (int64_t)t.n * pg->page_size;
         if (a[4] != Py_None) most = std::min(most, integer(a[4]));
         const int32_t lens_add = int32_of(integer(a[5]));
-        double scale = 1.0 / std::sqrt((double)pg->D);
-        if (a[6] != Py_None) {
-            need(PyFloat_Check(a[6]) || PyLong_Check(a[6]));
-            scale = PyFloat_AsDouble(a[6]);
-            need(!PyErr_Occurred());
-        }
+        const float scale = scale_of(a[6], pg->D);
         const fkv_rows rq = rows(q);
         at::Tensor out, lse, work;
         if (a[7] == Py_None) {
@@ -329,12 +343,141 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         need(bytes >= 0);
         if (bytes) work = at::empty({bytes}, q.options().dtype(at::kByte));
         launch(begun, "fkv_paged_attn", [&] {
-            return lib.attn(pg, &rq, dt, Hq, B, t.ids, t.n, t.stride, lens, lens_add, most, (float)scale, out.data_ptr(),
+            return lib.attn(pg, &rq, dt, Hq, B, t.ids, t.n, t.stride, lens, lens_add, most, scale, out.data_ptr(),
                             want_lse && lse.numel() ? (float*)lse.data_ptr() : nullptr, bytes ? work.data_ptr() : nullptr,
                             bytes, stream);
         });
         PyObject* o = THPVariable_Wrap(std::move(out));
         return want_lse ? Py_BuildValue("(NN)", o, THPVariable_Wrap(std::move(lse))) : o;
+    });
+}
+
+// attend_tokens(key, query, table, lens, max_len, lens_add, scale, out, return_lse, n_new, shared)
+PyObject* attend_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return plain(n, 11, [&](bool& begun) {
+        const PagesKey key(a[0]);
+        const fkv_pages* pg = key.pages;
+        void* stream = stream_of(key.index);
+        const at::Tensor& q = tensor(a[1], key.index);
+        need(q.dim() == 4 && q.size(3) == pg->D);
+        const int32_t dt = dtype_code(q.scalar_type()), B = int32_of(q.size(0)), Hq = int32_of(q.size(1)),
+                      L = int32_of(q.size(2));
+        const Table t = table(a[2], key.index);
+        need(t.B == B);
+        const int32_t* lens = lengths(a[3], key.index, B);
+        int64_t most = (int64_t)t.n * pg->page_size;
+        if (a[4] != Py_None) most = std::min(most, integer(a[4]));
+        const int32_t lens_add = int32_of(integer(a[5]));
+        const float scale = scale_of(a[6], pg->D);
+        const fkv_rows rq = rows(q);
+        need(PyBool_Check(a[8]));
+        const bool want_lse = a[8] == Py_True;
+        const int32_t* n_new = a[9] == Py_None ? nullptr : lengths(a[9], key.index, B);
+        const int64_t shared = integer(a[10]);
+        need(shared >= 0 && shared <= (int64_t)t.n * pg->page_size && shared % pg->page_size == 0);
+        at::Tensor out = result(a[7], key.index, q, n_new != nullptr), lse, work;
+        const fkv_rows ro = rows(out);
+        if (want_lse) lse = at::empty({B, Hq, L}, q.options().dtype(at::kFloat));
+        const int64_t bytes = drafting.rows_workspace(pg, Hq, B, L, shared, most);
+        need(bytes >= 0);
+        if (bytes) work = at::empty({bytes}, q.options().dtype(at::kByte));
+        launch(begun, "fkv_paged_attn_rows", [&] {
+            return drafting.rows(pg, &rq, dt, Hq, B, L, t.ids, t.n, t.stride, lens, lens_add, n_new, shared, most, scale,
+                                 &ro, want_lse && lse.numel() ? (float*)lse.data_ptr() : nullptr,
+                                 bytes ? work.data_ptr() : nullptr, bytes, stream);
+        });
+        PyObject* o = THPVariable_Wrap(std::move(out));
+        return want_lse ? Py_BuildValue("(NN)", o, THPVariable_Wrap(std::move(lse))) : o;
+    });
+}
+
+// attend_sparse(key, bounds, query, table, lens, n_select, max_len, lens_add, scale, out, return_lse, return_pages)
+PyObject* attend_sparse(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return plain(n, 12, [&](bool& begun) {
+        const PagesKey key(a[0]);
+        const fkv_pages* pg = key.pages;
+        void* stream = stream_of(key.index);
+        const at::Tensor &bounds = tensor(a[1], key.index), &q = tensor(a[2], key.index);
+        need(q.dim() == 4 && q.size(2) == 1 && q.size(3) == pg->D);
+        const int32_t dt = dtype_code(q.scalar_type()), B = int32_of(q.size(0)), Hq = int32_of(q.size(1));
+        need(B <= 1 || q.stride(0) == Hq * q.stride(1));
+        const Table t = table(a[3], key.index);
+        need(t.B == B);
+        const int32_t* lens = lengths(a[4], key.index, B);
+        const int32_t n_select = int32_of(integer(a[5]));
+        need(n_select >= 1);
+        int64_t most = (int64_t)t.n * pg->page_size;
+        if (a[6] != Py_None) most = std::min(most, integer(a[6]));
+        const int32_t lens_add = int32_of(integer(a[7]));
+        const float scale = scale_of(a[8], pg->D);
+        fkv_rows rq = rows(q);
+        at::Tensor out, lse, pages;
+        if (a[9] == Py_None) {
+            out = at::empty(q.sizes(), q.options());
+        } else {
+            out = result(a[9], key.index, q, false);
+            need(out.is_contiguous() && !((uintptr_t)out.data_ptr() & 15));
+        }
+        need(PyBool_Check(a[10]) && PyBool_Check(a[11]));
+        const bool want_lse = a[10] == Py_True, want_pages = a[11] == Py_True;
+        if (want_lse) lse = at::empty({B, Hq}, q.options().dtype(at::kFloat));
+        if (want_pages) pages = at::empty({B, pg->H, n_select}, q.options().dtype(at::kInt));
+        const int64_t bytes = drafting.sparse_workspace(pg, Hq, B, t.n, n_select, most);
+        need(bytes >= 0);
+        const at::Tensor work = at::empty({bytes}, q.options().dtype(at::kByte));
+        launch(begun, "fkv_paged_attn_sparse", [&] {
+            return drafting.sparse(pg, bounds.data_ptr(), &rq, dt, Hq, B, t.ids, t.n, t.stride, lens, lens_add, most,
+                                   n_select, scale, out.data_ptr(), want_lse && lse.numel() ? (float*)lse.data_ptr() : nullptr,
+                                   want_pages && pages.numel() ? (int32_t*)pages.data_ptr() : nullptr,
+                                   bytes ? work.data_ptr() : nullptr, bytes, stream);
+        });
+        PyObject* o = THPVariable_Wrap(std::move(out));
+        if (want_lse && want_pages)
+            return Py_BuildValue("(NNN)", o, THPVariable_Wrap(std::move(lse)), THPVariable_Wrap(std::move(pages)));
+        if (want_lse) return Py_BuildValue("(NN)", o, THPVariable_Wrap(std::move(lse)));
+        return want_pages ? Py_BuildValue("(NN)", o, THPVariable_Wrap(std::move(pages))) : o;
+    });
+}
+
+// (B, n, V) probabilities, n rows of them, that need no copy.
+fkv_rows probabilities(const at::Tensor& t, int64_t B, int64_t n, int64_t V) {
+    need(t.dim() == 3 && t.size(0) == B && t.size(1) == n && t.size(2) == V && (V == 1 || t.stride(2) == 1));
+    return fkv_rows{t.data_ptr(), t.stride(0), 0, t.stride(1)};
+}
+
+// verify(target, draft, tokens, uniforms, n_draft)
+PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return plain(n, 5, [&](bool& begun) {
+        const int64_t index = c10::hip::current_device();
+        void* stream = stream_of(index);
+        const at::Tensor& target = tensor(a[0], index);
+        need(target.dim() == 3 && target.size(1) >= 1 && target.size(2) >= 1);
+        const int32_t dt = dtype_code(target.scalar_type()), B = int32_of(target.size(0)), K = int32_of(target.size(1) - 1),
+                      V = int32_of(target.size(2));
+        const fkv_rows rt = probabilities(target, B, K + 1, V);
+        fkv_rows rd = {nullptr, 0, 0, 0};
+        if (a[1] != Py_None) {
+            const at::Tensor& draft = tensor(a[1], index);
+            need(draft.scalar_type() == target.scalar_type());
+            rd = probabilities(draft, B, K, V);
+        }
+        const at::Tensor &tokens = tensor(a[2], index), &uniforms = tensor(a[3], index);
+        need(tokens.dim() == 2 && tokens.size(0) == B && tokens.size(1) == K && tokens.is_contiguous() &&
+             (tokens.scalar_type() == at::kInt || tokens.scalar_type() == at::kLong));
+        need(uniforms.dim() == 2 && uniforms.size(0) == B && uniforms.size(1) == K + 1 && uniforms.is_contiguous() &&
+             uniforms.scalar_type() == at::kFloat);
+        const int32_t* n_draft = a[4] == Py_None ? nullptr : lengths(a[4], index, B);
+        at::Tensor out = at::empty({B, K + 1}, tokens.options()), accepted = at::empty({B}, target.options().dtype(at::kInt));
+        const int64_t bytes = drafting.verify_workspace(B, K, V);
+        need(bytes >= 0);
+        const at::Tensor work = at::empty({bytes}, target.options().dtype(at::kByte));
+        launch(begun, "fkv_verify_drafts", [&] {
+            return drafting.verify(&rt, a[1] == Py_None ? nullptr : &rd, dt, B, K, V, tokens.data_ptr(),
+                                   tokens.scalar_type() == at::kLong, (const float*)uniforms.data_ptr(), n_draft,
+                                   out.data_ptr(), (int32_t*)accepted.data_ptr(), bytes ? work.data_ptr() : nullptr, bytes,
+                                   stream);
+        });
+        return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(accepted)));
     });
 }
 
@@ -351,12 +494,27 @@ PyObject* bind(PyObject*, PyObject* args) {
     Py_RETURN_NONE;
 }
 
+// bind_drafting(addresses of fkv_paged_attn_rows_workspace, fkv_paged_attn_rows,
+// fkv_paged_attn_sparse_workspace, fkv_paged_attn_sparse, fkv_verify_drafts_workspace, fkv_verify_drafts)
+PyObject* bind_drafting(PyObject*, PyObject* args) {
+    unsigned long long p[6];
+    if (!PyArg_ParseTuple(args, "KKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5)) return nullptr;
+    drafting = {(decltype(drafting.rows_workspace))p[0],   (decltype(drafting.rows))p[1],
+                (decltype(drafting.sparse_workspace))p[2], (decltype(drafting.sparse))p[3],
+                (decltype(drafting.verify_workspace))p[4], (decltype(drafting.verify))p[5]};
+    Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, "addresses of libfkv's entry points, _lib.check"},
     {"rope", (PyCFunction)(void (*)())rope, METH_FASTCALL, "Rope.__call__"},
     {"write", (PyCFunction)(void (*)())write, METH_FASTCALL, "PagedLayer.write"},
     {"read", (PyCFunction)(void (*)())read, METH_FASTCALL, "PagedLayer.read"},
     {"attend", (PyCFunction)(void (*)())attend, METH_FASTCALL, "PagedLayer.attend"},
+    {"bind_drafting", bind_drafting, METH_VARARGS, "addresses of libfkv's entry points"},
+    {"attend_tokens", (PyCFunction)(void (*)())attend_tokens, METH_FASTCALL, "PagedLayer.attend_tokens"},
+    {"attend_sparse", (PyCFunction)(void (*)())attend_sparse, METH_FASTCALL, "PagedLayer.attend_sparse"},
+    {"verify", (PyCFunction)(void (*)())verify, METH_FASTCALL, "drafts.verify_drafts"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fkv_calls", "the paged cache's calls", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -43,6 +43,9 @@ def verify_drafts(target, draft, tokens, uniforms, n_draft=None):
     leaves nothing) and the target's after the last one: so tokens are distributed
     as the target's own.  It is -1 where the sum is not a positive number.
     Probabilities need not sum to one."""
+    done = _lib.calls().verify(target, draft, tokens, uniforms, n_draft)
+    if done is not NotImplemented:
+        return done
     if not isinstance(target, torch.Tensor):
         raise TypeError(f"target must be a tensor, got {type(target).__name__}")
     _require_device(target)

@@ -558,6 +558,10 @@ class PagedLayer(_Fixed):
         once for all.
 
         ``out`` may have any strides, and be the query."""
+        done = _lib.calls().attend_tokens(self._key, query, table, lens, max_len, lens_add, scale, out, return_lse, n_new,
+                                          shared)
+        if done is not NotImplemented:
+            return done
         index = self._index
         shape, dtype, table, P, stride, lens, most = self._attention(query, table, lens, max_len, lens_add, False)
         B, Hq, L, D = shape
@@ -595,6 +599,10 @@ class PagedLayer(_Fixed):
         then -1.  ``scale`` must not be negative."""
         if self.bounds is None:
             raise ValueError("the layer keeps no bounds (PagedLayer(bounds=True), or wrap(bounds=...))")
+        done = _lib.calls().attend_sparse(self._key, self.bounds, query, table, lens, n_select, max_len, lens_add, scale,
+                                          out, return_lse, return_pages)
+        if done is not NotImplemented:
+            return done
         index = self._index
         shape, dtype, table, P, stride, lens, most = self._attention(query, table, lens, max_len, lens_add, True)
         B, Hq, _, D = shape

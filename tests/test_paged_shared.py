@@ -278,3 +278,15 @@ def test_workspaces(c):  # noqa: F811
                     assert 0 <= size <= max(1 << 28, B * Hq * L * 40 * 4 * (D + 4))
             assert 0 < c.lib.fkv_paged_attn_sparse_workspace(pg, Hq, B, 512, 64, 8192) <= 1 << 28
     assert c.lib.fkv_verify_drafts_workspace(64, 5, 128000) > 0
+
+
+def test_compiled_calls_leave_what_is_not_plain():
+    """Without a device every call is left to Python, whatever its arguments are."""
+    calls = _lib.calls()
+    x, i = torch.zeros(2, 2, 3, 64), torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: calls.attend_tokens((0, 0), x, i[None], i, None, 0, None, None, False, None, 0),
+                 lambda: calls.attend_tokens(), lambda: calls.attend_tokens(*[x] * 11), lambda: calls.attend_tokens(*[None] * 11),
+                 lambda: calls.attend_sparse((0, 0), x, x, i[None], i, 3, None, 0, None, None, False, False),
+                 lambda: calls.attend_sparse(), lambda: calls.attend_sparse(*[i] * 12),
+                 lambda: calls.verify(x[0], None, i, x, None), lambda: calls.verify(), lambda: calls.verify(*[1] * 5)):
+        assert call() is NotImplemented
