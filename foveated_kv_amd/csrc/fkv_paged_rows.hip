@@ -141,6 +141,14 @@ __device__ inline uint32_t round_pair_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
+// Pages that a call reads once are not kept in the caches: 32 sequences to 8K tokens,
+// 540 MB, take 111 us so and 123 as other loads.  Where several workgroups read them
+// (a prompt's chunk 577 us and 597 so, shared tokens) the caches serve all but the first.
+template <bool ONCE, typename T>
+__device__ inline T read(const T* p) {
+    return ONCE ? __builtin_nontemporal_load(p) : *p;
+}
+
 // A tile's tokens as a thread loads them: 16 (INT4 of 64 dims: 8) bytes of a row
 // at a time, neighbouring threads a row.
 template <int D, int FMT>
@@ -188,7 +196,7 @@ __device__ inline uint32_t finite_or_zero(uint32_t w) {
     return ((w & e) == e ? 0 : w & 0xFFFFu) | (((w >> 16) & e) == e ? 0 : w & 0xFFFF0000u);
 }
 
-template <int D, int FMT, bool BF, int NW>
+template <int D, int FMT, bool BF, int NW, bool ONCE>
 __global__ void __launch_bounds__(64 * NW, 2) paged_rows_kernel(RowsArgs a) {
     using R = Rows<D, FMT>;
     constexpr int kRowWaves = NW, kTileTokens = 16 * NW, kSubs = NW / 2, kThreads = 64 * NW;
@@ -326,7 +334,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows_kernel(RowsArgs a) {
         if (tok + kTileTokens < end) fetch(tok + kTileTokens);
 #pragma unroll
         for (int i = 0; i < R::KP; i++) {
-            st.k[i] = *(const u4*)(a.pg.k + first[i] * R::KB + (uint32_t)(((tid / R::KT) & 15) * R::KB + 16 * (tid % R::KT)));
+            st.k[i] = read<ONCE>((const u4*)(a.pg.k + first[i] * R::KB + (uint32_t)(((tid / R::KT) & 15) * R::KB + 16 * (tid % R::KT))));
             if (FMT >= FKV_PAGES_FP8 && !kFactors) st.kx[i] = (a.pg.k_exp + first[i])[(tid / R::KT) & 15];
         }
 #pragma unroll
@@ -335,10 +343,10 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows_kernel(RowsArgs a) {
             const uint32_t r = (tid / R::VT) & 15;
             const char* at = a.pg.v + row * R::VB;
             if (R::VB == 32) {
-                const u2 x = *(const u2*)(at + r * R::VB + 8 * (tid % R::VT));
+                const u2 x = read<ONCE>((const u2*)(at + r * R::VB + 8 * (tid % R::VT)));
                 st.v[i] = u4{x.x, x.y, 0, 0};
             } else {
-                st.v[i] = *(const u4*)(at + r * R::VB + 16 * (tid % R::VT));
+                st.v[i] = read<ONCE>((const u4*)(at + r * R::VB + 16 * (tid % R::VT)));
             }
             if (FMT == FKV_PAGES_FP8) st.vx[i] = ((const uint8_t*)a.pg.v_scale)[row + r];
         }
@@ -901,8 +909,10 @@ static int check_rows(const char* who, const fkv_pages* p, int32_t Hq, int32_t B
 template <int D, int FMT, bool BF>
 static int launch_rows(const RowsArgs& a, const RowsPlan& p, hipStream_t s) {
     const char* w = "fkv_paged_attn_rows";
-    if (int e = p.waves == 8 ? start_kernel(w, paged_rows_kernel<D, FMT, BF, 8>, (uint32_t)p.blocks, 512, s, a)
-                             : start_kernel(w, paged_rows_kernel<D, FMT, BF, 4>, (uint32_t)p.blocks, 256, s, a)) return e;
+    const bool once = a.shared == 0 && a.own.tiles == 1;  // (each token is read by one workgroup)
+    if (int e = p.waves == 8 ? start_kernel(w, paged_rows_kernel<D, FMT, BF, 8, false>, (uint32_t)p.blocks, 512, s, a)
+                : once       ? start_kernel(w, paged_rows_kernel<D, FMT, BF, 4, true>, (uint32_t)p.blocks, 256, s, a)
+                             : start_kernel(w, paged_rows_kernel<D, FMT, BF, 4, false>, (uint32_t)p.blocks, 256, s, a)) return e;
     if (p.bytes == 0) return FKV_OK;
     const int64_t rows = (int64_t)a.B * a.Hq * a.L;
     return start_kernel(w, paged_rows_join_kernel<D, BF>, (uint32_t)cdiv(rows, 4), 256, s, a, rows);

