@@ -49,7 +49,8 @@ constexpr int kRowsMaxSeqs = 4096;
 // More rows than this on a KV head: workgroups of eight waves and 128 tokens a tile
 // in place of four and 64, of which a CU has two at once.
 constexpr int64_t kFewRows = 256;
-constexpr float kBegin = 6.0f, kJoin = 4.0f;  // us, see plan_rows()
+constexpr float kBegin = 6.0f, kJoin = 4.0f, kJoinPart = 0.12f;  // us, see plan_rows()
+constexpr int kEvenSeqs = 256;  // sequences whose lengths even parts are made from
 constexpr float kLowest = -3.402823466e38f;  // running maximum before the first token: no score lies below it
 // As in the one-token kernel: the running maximum follows a score that exceeds
 // it by more than 2^8, and stays 2^7 below the scores of fp16 pages, whose
@@ -80,6 +81,9 @@ struct RowsArgs {
     float* records;  // workspace: per row and part D numerators, maximum, sum
     RowParts common, own;
     int32_t lens_add, B, Hq, G, L, shared;
+    int32_t tile;     // tokens of a tile
+    int32_t even;     // != 0: as many parts of all sequences as this (see even_chunk()), of
+    int32_t least;    // this many tiles or more
     float scale;      // |scale| * log2(e)
     uint32_t q_sign, q_mask;  // its sign, for two 16-bit numbers; 0 where it is 0 (and |scale| 1)
 };
@@ -95,6 +99,50 @@ __device__ inline int32_t length_of(const RowsArgs& a, int32_t len) {
 __device__ inline int32_t limit_of(const RowsArgs& a, int b, int l) {
     const int32_t n = a.n_new ? min(max(a.n_new[b], 0), a.L) : a.L;
     return l >= n ? -1 : max(length_of(a, a.lens[b]) - n + l + 1, 0);
+}
+
+// Parts of the sequences' own tokens from their lengths, which only the device has:
+// the shortest parts of which there are `even` at most, that is, which the chip takes
+// all at once.  -> tokens of a part; the sequence and the part that are number `unit`
+// of all (seq -1: there are fewer).  Parts of max_len / n, whatever n, leave some of the
+// chip idle where lengths differ, and empty workgroups among the others: 16 sequences of
+// up to 32K tokens take 179 us and 183 to 313 so (n from 3 to 16), 32 of up to 8K 109 and
+// 114 to 136, 32 of 8K each 177 and 173 to 231.
+// Integers only: both kernels find the same.
+__device__ inline int32_t even_parts(const RowsArgs& a, int lane, uint32_t unit, int& seq, int& split) {
+    uint32_t tiles[kEvenSeqs / 64], total = 0, longest = 0;
+#pragma unroll
+    for (int j = 0; j < kEvenSeqs / 64; j++) {
+        const int b = 64 * j + lane;
+        const int32_t n = b < a.B ? length_of(a, a.lens[b]) : 0;
+        tiles[j] = ((uint32_t)n + a.tile - 1) / (uint32_t)a.tile;
+        total += tiles[j], longest = max(longest, tiles[j]);
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) longest = max(longest, wave_xor(longest, o));
+    auto of_lane = [](uint32_t v, int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i); };
+    const uint32_t even = a.even, splits = a.own.splits;
+    uint32_t chunk = max(max((of_lane(sum_up_to(total), 63) + even - 1) / even, (longest + splits - 1) / splits), (uint32_t)a.least);
+    chunk = __builtin_amdgcn_readfirstlane(max(chunk, 1u));
+    longest = __builtin_amdgcn_readfirstlane(longest);
+    for (;;) {
+        uint32_t before = 0;
+        seq = -1;
+#pragma unroll
+        for (int j = 0; j < kEvenSeqs / 64; j++) {
+            if (64 * j >= a.B) break;
+            const uint32_t parts = (tiles[j] + chunk - 1) / chunk, upto = before + sum_up_to(parts);
+            const uint64_t past = __ballot(upto > unit);
+            if (past && seq < 0) {
+                const int i = __builtin_ctzll(past);
+                seq = 64 * j + i, split = (int)(unit - (of_lane(upto, i) - of_lane(parts, i)));
+            }
+            before = of_lane(upto, 63);
+        }
+        if (before <= even || chunk >= longest) break;
+        chunk = min(chunk + chunk / 16 + 1, longest);
+    }
+    return (int32_t)(chunk * a.tile);
 }
 
 // 16-bit numbers that a weight enters the products as.  One, rounded, for results
@@ -225,10 +273,18 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows_kernel(RowsArgs a) {
         rest -= a.common.tiles * a.common.splits;
         p = a.own;
         // (the last rows attend to the most tokens: they come first)
-        const int per_tile = a.own.splits * a.B, t = rest / per_tile;
+        const int per_tile = a.own.splits * a.B, t = ONCE && a.even ? 0 : rest / per_tile;
         tile = a.own.tiles - 1 - t;
         rest -= t * per_tile;
-        seq = rest / a.own.splits, split = rest - seq * a.own.splits;
+        if (ONCE && a.even) {
+            p.chunk = even_parts(a, threadIdx.x & 63, rest, seq, split);
+            if (seq < 0) return;
+        } else {
+            // (The first tokens of all sequences, then the next.  Later parts are empty where
+            // sequences are short, and a sequence's long where it is: neither may come at a
+            // step that is a power of two, which would put them on the same few CUs.)
+            split = rest / a.B, seq = (rest + split * 5) % a.B;
+        }
     }
     const int rows = seq < 0 ? a.B * a.L * a.G : a.L * a.G;
     const int wr = p.wr, wt = min(kSubs, kRowWaves / wr), rg = wave & (wr - 1), tg = wave / wr;
@@ -241,7 +297,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows_kernel(RowsArgs a) {
         hq = h * a.G + r - token * a.G;
         return r < rows ? limit_of(a, b, l) : -1;
     };
-    const int32_t begin = (seq < 0 ? 0 : a.shared) + split * p.chunk;
+    // (even parts may begin beyond 2^31, where no tokens are)
+    const int32_t begin = (int32_t)min((seq < 0 ? 0 : a.shared) + (int64_t)split * p.chunk, (int64_t)0x7FFFFFFF);
     const int parts = a.common.splits + a.own.splits;
     // The ends of rows [first, last): the most tokens that one attends to (-1: none
     // is real) and the least that a real one does.  A sequence's own rows come by
@@ -282,7 +339,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows_kernel(RowsArgs a) {
         all_least = __builtin_amdgcn_readfirstlane(all_least);
     }
     const bool real = lim >= 0;
-    if (seq < 0 || split + 1 < p.splits) end = min(end, begin + p.chunk);
+    if (seq < 0 || split + 1 < p.splits) end = (int32_t)min((int64_t)end, (int64_t)begin + p.chunk);
     const int nt = end > begin ? (end - begin + kTileTokens - 1) / kTileTokens : 0;
     if (nt == 0 && parts > 1) return;
     if (tid < 2) odd_tile[tid] = -1;
@@ -778,9 +835,11 @@ __global__ void __launch_bounds__(256) paged_rows_join_kernel(RowsArgs a, int64_
         return;
     }
     const int parts = a.common.splits + a.own.splits;
+    int seq, split;
+    const uint32_t own_chunk = a.even ? even_parts(a, lane, 0, seq, split) : a.own.chunk, chunk = a.common.chunk;
     // (parts whose tokens begin below the row's end have a record)
-    const int n_common = a.common.splits ? min(a.common.splits, (min(lim, a.shared) + a.common.chunk - 1) / a.common.chunk) : 0;
-    const int n_own = lim > a.shared ? min(a.own.splits, (lim - a.shared + a.own.chunk - 1) / a.own.chunk) : 0;
+    const int n_common = a.common.splits ? (int)min((uint32_t)a.common.splits, ((uint32_t)min(lim, a.shared) + chunk - 1) / chunk) : 0;
+    const int n_own = lim > a.shared ? (int)min((uint32_t)a.own.splits, ((uint32_t)(lim - a.shared) + own_chunk - 1) / own_chunk) : 0;
     const int n = n_common + n_own;
     const float* rec = a.records + at * parts * (D + 4);
     float m = kLowest, sum = 0.0f, x[N] = {};
@@ -830,7 +889,7 @@ __global__ void __launch_bounds__(256) paged_rows_join_kernel(RowsArgs a, int64_
 
 struct RowsPlan {
     RowParts common, own;
-    int32_t shared;
+    int32_t shared, even, least;  // see even_parts()
     int waves;  // of a workgroup
     int64_t blocks, bytes;
 };
@@ -838,8 +897,9 @@ struct RowsPlan {
 // Workgroups and workspace of a call (a function of sizes alone).  How many parts
 // the tokens are cut into is what a model of the time finds best: a workgroup
 // takes kBegin for its beginning and end and a time per tile of tokens that grows
-// with its rows (the cache's bytes, then the products), the chip has `slots` of
-// them at once, and parts cost their join.
+// with its rows (the cache's bytes, then the products) and where two share a CU, the
+// chip has `slots` of them at once, and parts cost their join.  Against the best of 15
+// counts of parts it takes 0 to 13 % more (ten calls with shared tokens).
 static RowsPlan plan_rows(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, int64_t shared, int64_t max_len) {
     RowsPlan r;
     if (B == 1) shared = 0;  // (with nobody)
@@ -853,42 +913,65 @@ static RowsPlan plan_rows(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, 
         q.tiles = (int32_t)cdiv(rows, 32 * q.wr);
         return q;
     };
-    // us for a tile
-    auto time = [&](const RowParts& q) { return q.wr == 8 ? 4.9f : q.wr == 4 ? (r.waves == 8 ? 3.7f : 4.3f) : 2.8f; };
+    // us for a tile, of a workgroup of four waves as one of two on a CU or alone on it
+    auto time = [&](const RowParts& q) {
+        if (q.wr == 8) return 4.9f;
+        if (q.wr == 4) return r.waves == 8 ? 3.7f : p->format == FKV_PAGES_FP8_INT4 ? 3.5f : 4.3f;
+        return 2.8f;
+    };
+    auto time_alone = [&](const RowParts& q) {
+        if (r.waves == 8) return time(q);
+        if (q.wr == 4) return p->format == FKV_PAGES_FP8_INT4 ? 2.4f : 2.15f;
+        return 1.6f;
+    };
     r.own = part(own_rows);
     r.common = part(all_rows);
     if (!shared) r.common.tiles = 0;
     const int64_t own_tiles = cdiv(std::max<int64_t>(1, max_len - shared), tile), common_tiles = cdiv(shared, tile);
     const int64_t own_pieces = (int64_t)B * p->H * r.own.tiles, common_pieces = (int64_t)p->H * r.common.tiles;
-    const float join = (float)((double)all_rows * p->H * (p->D + 4) * 8 / 4e6);  // a record of each row, written and read
-    float best = INFINITY;
-    const int64_t most = std::min<int64_t>(shared ? common_tiles : own_tiles, 64);
-    for (int64_t n = 1; n <= most; n++) {
-        int64_t own_parts = n, common_parts = 0;
-        float t, longest = 0;
-        double work = 0;
-        if (shared) {
-            common_parts = cdiv(common_tiles, cdiv(common_tiles, n));
-            longest = kBegin + cdiv(common_tiles, n) * time(r.common);
-            work = common_pieces * common_parts * longest;
-            own_parts = std::max<int64_t>(1, (int64_t)(own_tiles * time(r.own) / longest + 0.999f));
-        }
-        own_parts = cdiv(own_tiles, cdiv(own_tiles, own_parts));
-        const float own_time = kBegin + cdiv(own_tiles, own_parts) * time(r.own);
-        longest = std::max(longest, own_time);
-        // (many sequences have lengths of their own: three quarters of max_len, say)
-        if (B <= 4 && !shared) t = cdiv(own_pieces * own_parts, slots) * own_time;
-        else t = (float)(work + 0.75 * own_pieces * own_parts * own_time) / slots + 0.75f * longest;
-        if (common_parts + own_parts > 1) t += kJoin + (common_parts + own_parts) * join;
-        if (t < best) {
-            best = t;
-            r.common.splits = (int32_t)common_parts;
-            r.own.splits = (int32_t)own_parts;
+    // a record of each row, written and read
+    const float join = (float)((double)all_rows * p->H * (p->D + 4) * 8 / 4e6) + kJoinPart;
+    r.common.splits = 0;
+    r.even = r.least = 0;
+    if (!shared && B > 4 && B <= kEvenSeqs && r.own.tiles == 1 && own_pieces * 4 <= slots * 3) {
+        // Few sequences, whose lengths differ: see even_parts().  Parts are not so short
+        // that their records cost more than they gain
+        r.even = (int32_t)(slots / p->H);
+        r.least = std::max(1, (int32_t)std::sqrt((float)own_tiles * join / time(r.own)));
+        r.own.splits = (int32_t)std::min<int64_t>(std::min(cdiv(own_tiles, r.least), cdiv(4 * r.even, B)), 64);
+        if (r.own.splits == 1) r.even = 0;
+    } else {
+        float best = INFINITY;
+        const int64_t most = std::min<int64_t>(shared ? common_tiles : own_tiles, 64);
+        for (int64_t n = 1; n <= most; n++) {
+            int64_t own_parts = n, common_parts = 0;
+            float t, longest = 0;
+            double work = 0;
+            if (shared) {
+                common_parts = cdiv(common_tiles, cdiv(common_tiles, n));
+                const int64_t of = cdiv(common_tiles, n), blocks = common_pieces * common_parts;
+                longest = kBegin + of * (blocks > 256 ? time(r.common) : time_alone(r.common));
+                work = blocks * (kBegin + of * time(r.common));
+                own_parts = std::max<int64_t>(1, (int64_t)(own_tiles * time(r.own) / longest + 0.999f));
+            }
+            own_parts = cdiv(own_tiles, cdiv(own_tiles, own_parts));
+            const float own_time = kBegin + cdiv(own_tiles, own_parts) * time(r.own);
+            // (many sequences have lengths of their own: six tenths of max_len, say)
+            work = (work + 0.6 * own_pieces * own_parts * own_time) / slots;
+            if (shared) t = std::max(longest, (float)work);
+            else if (B <= 4) t = cdiv(own_pieces * own_parts, slots) * own_time;
+            else t = std::max((float)work, kBegin + cdiv(own_tiles, own_parts) * time_alone(r.own));
+            if (common_parts + own_parts > 1) t += kJoin + (common_parts + own_parts) * join;
+            if (t < best) {
+                best = t;
+                r.common.splits = (int32_t)common_parts;
+                r.own.splits = (int32_t)own_parts;
+            }
         }
     }
     r.common.chunk = (int32_t)(shared ? cdiv(common_tiles, r.common.splits) * tile : tile);
     r.own.chunk = (int32_t)(cdiv(own_tiles, r.own.splits) * tile);
-    r.blocks = common_pieces * r.common.splits + own_pieces * r.own.splits;
+    r.blocks = common_pieces * r.common.splits + (r.even ? (int64_t)p->H * r.even : own_pieces * r.own.splits);
     const int64_t parts = r.common.splits + r.own.splits;
     r.bytes = parts > 1 ? (int64_t)B * Hq * L * parts * (p->D + 4) * 4 : 0;
     return r;
@@ -985,6 +1068,9 @@ int fkv_paged_attn_rows(const fkv_pages* pages, const fkv_rows* query, int32_t q
     a.G = Hq / pages->H;
     a.L = L;
     a.shared = p.shared;
+    a.tile = 16 * p.waves;
+    a.even = p.even;
+    a.least = p.least;
     a.scale = std::fabs(scale) * 1.4426950408889634f;
     a.q_sign = std::signbit(scale) ? 0x80008000u : 0;
     a.q_mask = ~0u;

@@ -299,19 +299,6 @@ struct ChoiceLds {
     int32_t digit, above, inside, counts[2][kWaves];
 };
 
-template <int CTRL, int ROWS = 15>
-__device__ inline uint32_t dpp_or_0(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 15, false);
-}
-// The sum over the lanes up to and with this one.
-__device__ inline uint32_t sum_up_to(uint32_t v) {
-    v += dpp_or_0<0x111>(v);  // row_shr:1, 2, 4, 8
-    v += dpp_or_0<0x112>(v);
-    v += dpp_or_0<0x114>(v);
-    v += dpp_or_0<0x118>(v);
-    v += dpp_or_0<0x142, 10>(v);  // row_bcast:15 into the second and fourth row
-    return v + dpp_or_0<0x143, 12>(v);  // row_bcast:31 into the upper half
-}
 // The sum over a row of 16 lanes, in all of them.
 __device__ inline uint32_t row_sum(uint32_t v) {
     v += dpp_or_0<kDppXor1>(v);

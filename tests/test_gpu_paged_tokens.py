@@ -131,6 +131,45 @@ def test_split_rows(paged, fmt, D, H, G, L, lens):
         _bits_equal(layer.attend_tokens(q, table.cuda(), _i32(lens), max(lens)), b, "again")
 
 
+UNEVEN = {
+    "one long": [2900] + [3] * 8,
+    "long last": [1] * 30 + [2500],
+    "falling": [1900 - 190 * i for i in range(11)],
+    "none": [0] * 7,
+    "some none": [0, 1100, 0, 0, 700, 0, 64, 65],
+    "many": [(97 * i * i) % 400 for i in range(130)],
+}
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "fp8"])
+@pytest.mark.parametrize("name", UNEVEN)
+@pytest.mark.parametrize("H", [1, 3])
+def test_parts_of_uneven_sequences(paged, fmt, name, H):
+    """Parts that the device makes of the lengths; a bound of the lengths that is
+    too small or too large; padded batches."""
+    lens = UNEVEN[name]
+    B, D, G, L, page = len(lens), 64, 2, 3, 16
+    _flush("uneven", fmt, name, H)
+    counts = [max(1, -(-n // page)) for n in lens]
+    layer = _filled(paged, fmt, sum(counts) + 2, H, D, page, 50)
+    table = _table(51, sum(counts) + 2, counts)
+    _spoil(layer, table, lens)
+    q = _randn(52, B, H * G, L, D).to(DTYPES["bf16"]).cuda()
+    for kw in ({}, {"max_len": max(lens)}, {"max_len": max(lens) // 3}, {"lens_add": -40}):
+        _check(layer, q, table, lens, **kw)
+    _check(layer, q, table, lens, [(2 * b) % (L + 1) for b in range(B)])
+    # a captured call follows the lengths of its replays
+    long, new = _i32(lens), torch.cuda.CUDAGraph()
+    on = table.cuda()
+    layer.attend_tokens(q, on, long)
+    with torch.cuda.graph(new):
+        out = layer.attend_tokens(q, on, long)
+    for shift in (1, 3, 5):
+        long.copy_(_i32([max(0, n - 170 * shift) for n in lens]))
+        new.replay()
+        _bits_equal(out.clone(), layer.attend_tokens(q, on, long), shift)
+
+
 @pytest.mark.parametrize("fmt,qd", KINDS)
 @pytest.mark.parametrize("D,H,G,L,B,shared", [(128, 2, 4, 1, 9, 256), (64, 1, 7, 3, 5, 48), (128, 1, 2, 2, 70, 1024),
                                               (64, 2, 1, 9, 2, 16)])
