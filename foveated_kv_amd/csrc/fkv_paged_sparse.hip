@@ -191,14 +191,14 @@ __device__ inline float row_max(float v) {
 // pages, columns heads.  An fp16 query is the sum of two bf16 numbers, of which the
 // second is in the column eight to the right: 8 heads at a time.
 // Bound by a wave's latencies: the length and ids, 8 KB of bounds, some 200 vector
-// instructions.  35 MB in 14 us (16 ragged sequences, 8 KV heads), 8 MB in 5 us.
+// instructions.  35 MB in 12 us (16 ragged sequences, 8 KV heads), 8 MB in 5 us.
 template <int D, bool BF>
 __global__ void __launch_bounds__(256) page_score_kernel(SparseArgs a) {
     constexpr int NJ = D / 32, NH = BF ? 16 : 8;
     const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = blockIdx.z, h = blockIdx.y;
-    int32_t p0 = ((int32_t)blockIdx.x * 4 + wave) * 16;
+    const int b = blockIdx.z, h = blockIdx.x;
+    int32_t p0 = ((int32_t)blockIdx.y * 4 + wave) * 16;
     const int32_t* ids = a.table.ids + b * a.table.stride;
     int32_t id = ids[min(p0 + c, a.table.n - 1)];        // (asked for together with the length)
     const int32_t n = pages_of(a, length_of(a, b)) - 1;  // (the newest page needs no score)
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(256) page_score_kernel(SparseArgs a) {
         }
     };
     if (a.G <= NH) queries(0);
-    for (const int32_t hop = (int32_t)gridDim.x * 64; p0 < n; p0 += hop) {
+    for (const int32_t hop = (int32_t)gridDim.y * 64; p0 < n; p0 += hop) {
         const bool held = (uint32_t)id < (uint32_t)a.pg.n_pages;
         const uint16_t* box = a.bounds + ((int64_t)(held ? id : 0) * a.pg.H + h) * 2 * D + 8 * kq;
         u4 mn[NJ], mx[NJ];
@@ -736,10 +736,11 @@ int fkv_paged_attn_sparse(const fkv_pages* pages, const void* bounds, const fkv_
     if (int e = check_apart(w, "out, which is not the query, and the query", &result, heads, query, heads, true)) return e;
     const int64_t most = std::min<int64_t>(max_len, (int64_t)n_table * pages->page_size);
     const int64_t scored = cdiv(most, pages->page_size) - 1;
-    // (about 512 workgroups, two a CU, of 64 pages at a time; for 16 sequences of up to 1024
-    // pages 256 take 18 us, 512 14, 1024 16)
-    const int64_t groups = std::max<int64_t>(1, std::min<int64_t>(cdiv(scored, 64), cdiv(512, rows)));
-    const dim3 grid((uint32_t)groups, pages->H, B);
+    // (about 768 workgroups, three a CU, of 64 pages at a time, neighbours of other heads,
+    // which have as many pages to score; for 16 sequences of up to 1024
+    // pages 512 take 0.9 us more, 1024 2)
+    const int64_t groups = std::max<int64_t>(1, std::min<int64_t>(cdiv(scored, 64), cdiv(768, rows)));
+    const dim3 grid(pages->H, (uint32_t)groups, B);
     auto choose = [&](auto score, auto choice) {
         if (n_table > n_select)  // (else all pages are taken)
             if (int e = start_kernel(w, score, grid, 256, s, a)) return e;
