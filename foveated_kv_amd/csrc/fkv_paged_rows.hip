@@ -79,6 +79,7 @@ struct RowsArgs {
     const int32_t* n_new;
     float* lse;
     float* records;  // workspace: per row and part D numerators, maximum, sum
+    int32_t* chunk;  // workspace, of even parts: how many tokens they have
     RowParts common, own;
     int32_t lens_add, B, Hq, G, L, shared;
     int32_t tile;     // tokens of a tile
@@ -108,7 +109,6 @@ __device__ inline int32_t limit_of(const RowsArgs& a, int b, int l) {
 // chip idle where lengths differ, and empty workgroups among the others: 16 sequences of
 // up to 32K tokens take 179 us and 183 to 313 so (n from 3 to 16), 32 of up to 8K 109 and
 // 114 to 136, 32 of 8K each 177 and 173 to 231.
-// Integers only: both kernels find the same.
 __device__ inline int32_t even_parts(const RowsArgs& a, int lane, uint32_t unit, int& seq, int& split) {
     uint32_t tiles[kEvenSeqs / 64], total = 0, longest = 0;
 #pragma unroll
@@ -277,7 +277,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows_kernel(RowsArgs a) {
         tile = a.own.tiles - 1 - t;
         rest -= t * per_tile;
         if (ONCE && a.even) {
-            p.chunk = even_parts(a, threadIdx.x & 63, rest, seq, split);
+            p.chunk = even_parts(a, lane, rest, seq, split);
+            if (blockIdx.x == 0 && tid == 0) *a.chunk = p.chunk;  // (for the join)
             if (seq < 0) return;
         } else {
             // (The first tokens of all sequences, then the next.  Later parts are empty where
@@ -835,8 +836,7 @@ __global__ void __launch_bounds__(256) paged_rows_join_kernel(RowsArgs a, int64_
         return;
     }
     const int parts = a.common.splits + a.own.splits;
-    int seq, split;
-    const uint32_t own_chunk = a.even ? even_parts(a, lane, 0, seq, split) : a.own.chunk, chunk = a.common.chunk;
+    const uint32_t own_chunk = a.even ? scalar_load(a.chunk, 0) : a.own.chunk, chunk = a.common.chunk;
     // (parts whose tokens begin below the row's end have a record)
     const int n_common = a.common.splits ? (int)min((uint32_t)a.common.splits, ((uint32_t)min(lim, a.shared) + chunk - 1) / chunk) : 0;
     const int n_own = lim > a.shared ? (int)min((uint32_t)a.own.splits, ((uint32_t)(lim - a.shared) + own_chunk - 1) / own_chunk) : 0;
@@ -973,7 +973,7 @@ static RowsPlan plan_rows(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, 
     r.own.chunk = (int32_t)(cdiv(own_tiles, r.own.splits) * tile);
     r.blocks = common_pieces * r.common.splits + (r.even ? (int64_t)p->H * r.even : own_pieces * r.own.splits);
     const int64_t parts = r.common.splits + r.own.splits;
-    r.bytes = parts > 1 ? (int64_t)B * Hq * L * parts * (p->D + 4) * 4 : 0;
+    r.bytes = parts > 1 ? (int64_t)B * Hq * L * parts * (p->D + 4) * 4 + 16 : 0;
     return r;
 }
 
@@ -1060,6 +1060,7 @@ int fkv_paged_attn_rows(const fkv_pages* pages, const fkv_rows* query, int32_t q
     a.n_new = n_new;
     a.lse = lse;
     a.records = (float*)workspace;
+    a.chunk = (int32_t*)((char*)workspace + p.bytes - 16);
     a.common = p.common;
     a.own = p.own;
     a.lens_add = lens_add;
