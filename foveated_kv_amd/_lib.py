@@ -235,7 +235,7 @@ def calls():
                                    "fkv_paged_attn"), check)
         _fkv_calls.bind_drafting(*addresses("fkv_paged_attn_rows_workspace", "fkv_paged_attn_rows",
                                             "fkv_paged_attn_sparse_workspace", "fkv_paged_attn_sparse",
-                                            "fkv_verify_drafts_workspace", "fkv_verify_drafts"))
+                                            "fkv_verify_drafts_workspace", "fkv_verify_drafts", "fkv_paged_bounds"))
         _calls = _fkv_calls
     return _calls
 

@@ -7,7 +7,7 @@
 // query and 8 KV heads: rotation 8.1 us from Python, 4.6 so; write 10.9 and 5.1;
 // attention over 512 tokens of one 9.5 and 4.6; of one sequence, five tokens over
 // 4000 15.1 and 9.3 (two launches), one over 8 of 63 pages 17.5 and 11.5 (four),
-// five drafts of 32000 entries verified 14.7 and 6.1.
+// five drafts of 32000 entries verified 14.7 and 6.1, bounds 5.6 and 3.7.
 //
 // Each function returns NotImplemented for whatever is not plain -- a wrong
 // argument, a tensor to be copied first, one of another GPU than the current
@@ -47,6 +47,7 @@ struct {
     decltype(&fkv_paged_attn_sparse) sparse;
     decltype(&fkv_verify_drafts_workspace) verify_workspace;
     decltype(&fkv_verify_drafts) verify;
+    decltype(&fkv_paged_bounds) bounds;
 } drafting;
 PyObject* check = nullptr;  // _lib.check(code, name), which raises
 
@@ -439,6 +440,23 @@ PyObject* attend_sparse(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// bound(key, bounds, table, start, n, n_new)
+PyObject* bound(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return plain(n, 6, [&](bool& begun) -> PyObject* {
+        const PagesKey key(a[0]);
+        void* stream = stream_of(key.index);
+        const at::Tensor& bounds = tensor(a[1], key.index);
+        const Table t = table(a[2], key.index);
+        const fkv_positions start = positions(a[3], key.index, t.B, 1, false);
+        const int32_t L = int32_of(integer(a[4]));
+        const int32_t* n_new = a[5] == Py_None ? nullptr : lengths(a[5], key.index, t.B);
+        launch(begun, "fkv_paged_bounds", [&] {
+            return drafting.bounds(key.pages, bounds.data_ptr(), t.B, L, t.ids, t.n, t.stride, &start, n_new, stream);
+        });
+        Py_RETURN_NONE;
+    });
+}
+
 // (B, n, V) probabilities, n rows of them, that need no copy.
 fkv_rows probabilities(const at::Tensor& t, int64_t B, int64_t n, int64_t V) {
     need(t.dim() == 3 && t.size(0) == B && t.size(1) == n && t.size(2) == V && (V == 1 || t.stride(2) == 1));
@@ -495,13 +513,15 @@ PyObject* bind(PyObject*, PyObject* args) {
 }
 
 // bind_drafting(addresses of fkv_paged_attn_rows_workspace, fkv_paged_attn_rows,
-// fkv_paged_attn_sparse_workspace, fkv_paged_attn_sparse, fkv_verify_drafts_workspace, fkv_verify_drafts)
+// fkv_paged_attn_sparse_workspace, fkv_paged_attn_sparse, fkv_verify_drafts_workspace, fkv_verify_drafts,
+// fkv_paged_bounds)
 PyObject* bind_drafting(PyObject*, PyObject* args) {
-    unsigned long long p[6];
-    if (!PyArg_ParseTuple(args, "KKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5)) return nullptr;
+    unsigned long long p[7];
+    if (!PyArg_ParseTuple(args, "KKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6)) return nullptr;
     drafting = {(decltype(drafting.rows_workspace))p[0],   (decltype(drafting.rows))p[1],
                 (decltype(drafting.sparse_workspace))p[2], (decltype(drafting.sparse))p[3],
-                (decltype(drafting.verify_workspace))p[4], (decltype(drafting.verify))p[5]};
+                (decltype(drafting.verify_workspace))p[4], (decltype(drafting.verify))p[5],
+                (decltype(drafting.bounds))p[6]};
     Py_RETURN_NONE;
 }
 
@@ -514,6 +534,7 @@ PyMethodDef methods[] = {
     {"bind_drafting", bind_drafting, METH_VARARGS, "addresses of libfkv's entry points"},
     {"attend_tokens", (PyCFunction)(void (*)())attend_tokens, METH_FASTCALL, "PagedLayer.attend_tokens"},
     {"attend_sparse", (PyCFunction)(void (*)())attend_sparse, METH_FASTCALL, "PagedLayer.attend_sparse"},
+    {"bound", (PyCFunction)(void (*)())bound, METH_FASTCALL, "PagedLayer.bound"},
     {"verify", (PyCFunction)(void (*)())verify, METH_FASTCALL, "drafts.verify_drafts"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fkv_calls", "the paged cache's calls", -1, methods,

@@ -453,6 +453,8 @@ class PagedLayer(_Fixed):
         were filled otherwise needs once."""
         if self.bounds is None:
             raise ValueError("the layer keeps no bounds (PagedLayer(bounds=True), or wrap(bounds=...))")
+        if _lib.calls().bound(self._key, self.bounds, table, start, n, n_new) is not NotImplemented:
+            return
         index = self._index
         table, B, P, stride = self._table(table)
         n = int(n)

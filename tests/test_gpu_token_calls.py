@@ -55,6 +55,28 @@ def test_selected_pages(paged, monkeypatch, fmt):  # noqa: F811
     _both(monkeypatch, lambda: layer.attend_sparse(q, table[:, ::2], lens, 3), False)
 
 
+@pytest.mark.parametrize("fmt", ["fp16", "fp8_int4"])
+def test_bounds(paged, monkeypatch, fmt):  # noqa: F811
+    layer, table, _ = _layer(paged, fmt, bounds=True)
+    want = layer.bounds.clone()
+    wide = torch.cat([table, table], 1)
+
+    def bound(*args):
+        layer.bounds.zero_()
+        layer.bound(*args)
+        return [layer.bounds]
+
+    for args, plain in (((table, 0, 120), True), ((table, 0, 0), True), ((table, _i(0, 3, 40), 9), True),
+                        ((table, _i(0, 3, 40), 9, _i(9, 0, 2)), True), ((wide[:, :8], 5, 70), True),
+                        ((table[:, ::2], 0, 60), False), ((table, 0, 9, _i(9, 1, 0, 1, 2, 1)[::2]), False)):
+        got = _both(monkeypatch, lambda: [t.clone() for t in bound(*args)], plain)
+        if args[2] == 120:
+            assert torch.equal(got[0], want)
+    for n in (-1, 2 ** 31):
+        with pytest.raises(ValueError, match="n must be"):
+            layer.bound(table, 0, n)
+
+
 def test_refusals_are_worded_in_python(paged):  # noqa: F811
     layer, table, dtype = _layer(paged, bounds=True)
     q, lens = _randn(5, B, H * G, 5, D), _i(120, 0, 37)

@@ -288,5 +288,6 @@ def test_compiled_calls_leave_what_is_not_plain():
                  lambda: calls.attend_tokens(), lambda: calls.attend_tokens(*[x] * 11), lambda: calls.attend_tokens(*[None] * 11),
                  lambda: calls.attend_sparse((0, 0), x, x, i[None], i, 3, None, 0, None, None, False, False),
                  lambda: calls.attend_sparse(), lambda: calls.attend_sparse(*[i] * 12),
+                 lambda: calls.bound((0, 0), x, i[None], 0, 3, None), lambda: calls.bound(*[i] * 6),
                  lambda: calls.verify(x[0], None, i, x, None), lambda: calls.verify(), lambda: calls.verify(*[1] * 5)):
         assert call() is NotImplemented
