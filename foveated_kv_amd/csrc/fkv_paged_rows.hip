@@ -60,6 +60,7 @@ constexpr int kRowsMaxSeqs = 4096;
 // in place of four and 64, of which a CU has two at once.
 constexpr int64_t kFewRows = 256;
 constexpr float kBegin = 6.0f, kJoin = 4.0f, kJoinPart = 0.12f;  // us, see plan_rows()
+constexpr int kManyParts = 16;   // see paged_rows_join_kernel()
 constexpr int kEvenSeqs = 256;  // sequences whose lengths even parts are made from
 constexpr float kLowest = -3.402823466e38f;  // running maximum before the first token: no score lies below it
 // As in the one-token kernel: the running maximum follows a score that exceeds
@@ -831,18 +832,20 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows_kernel(RowsArgs a) {
     }
 }
 
-// The records of a row, in order: a wave a row.
-template <int D, bool BF>
+// The records of a row, in order: a wave a row, or four waves, each every fourth eight
+// records, where there are more than kManyParts (65 records of 768 rows: 10 us and 7).
+template <int D, bool BF, int WAVES>
 __global__ void __launch_bounds__(256) paged_rows_join_kernel(RowsArgs a, int64_t n_rows) {
     constexpr int N = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ float part[WAVES][D + 2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t at = WAVES == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     if (at >= n_rows) return;
     const int64_t bh = at / a.L;
     const int l = (int)(at - bh * a.L), b = (int)(bh / a.Hq), hq = (int)(bh - (int64_t)b * a.Hq);
     const int32_t lim = limit_of(a, b, l);
     if (lim < 0) {
-        if (a.lse && lane == 0) a.lse[at] = -INFINITY;
+        if (a.lse && threadIdx.x % (64 * WAVES) == 0) a.lse[at] = -INFINITY;
         return;
     }
     const int parts = a.common.splits + a.own.splits;
@@ -854,7 +857,7 @@ __global__ void __launch_bounds__(256) paged_rows_join_kernel(RowsArgs a, int64_
     const float* rec = a.records + at * parts * (D + 4);
     float m = kLowest, sum = 0.0f, x[N] = {};
     constexpr int U = 8;  // records a step, their loads in flight together
-    for (int i = 0; i < n; i += U) {
+    for (int i = WAVES == 4 ? wave * U : 0; i < n; i += WAVES * U) {
         float2 st[U];
         float v[U][N];
 #pragma unroll
@@ -881,6 +884,26 @@ __global__ void __launch_bounds__(256) paged_rows_join_kernel(RowsArgs a, int64_
 #pragma unroll
                 for (int j = 0; j < N; j++) x[j] = fmaf(w, v[k][j], x[j]);
             }
+        }
+    }
+    if (WAVES == 4) {
+        float* mine = part[wave];
+        if (lane == 0) mine[D] = m, mine[D + 1] = sum;
+#pragma unroll
+        for (int j = 0; j < N; j++) mine[64 * j + lane] = x[j];
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) m = fmaxf(m, part[w][D]);
+        sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; j++) x[j] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float f = __builtin_amdgcn_exp2f(part[w][D] - m);
+            sum = fmaf(f, part[w][D + 1], sum);
+#pragma unroll
+            for (int j = 0; j < N; j++) x[j] = fmaf(f, part[w][64 * j + lane], x[j]);
         }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -1008,7 +1031,9 @@ static int launch_rows(const RowsArgs& a, const RowsPlan& p, hipStream_t s) {
                              : start_kernel(w, paged_rows_kernel<D, FMT, BF, 4, false>, (uint32_t)p.blocks, 256, s, a)) return e;
     if (p.bytes == 0) return FKV_OK;
     const int64_t rows = (int64_t)a.B * a.Hq * a.L;
-    return start_kernel(w, paged_rows_join_kernel<D, BF>, (uint32_t)cdiv(rows, 4), 256, s, a, rows);
+    if (a.common.splits + a.own.splits > kManyParts && rows < 1 << 24)  // (2^32 threads)
+        return start_kernel(w, paged_rows_join_kernel<D, BF, 4>, (uint32_t)rows, 256, s, a, rows);
+    return start_kernel(w, paged_rows_join_kernel<D, BF, 1>, (uint32_t)cdiv(rows, 4), 256, s, a, rows);
 }
 
 template <int D>
