@@ -97,14 +97,28 @@ template <int CTRL, int ROWS = 15>
 __device__ inline uint32_t dpp_or_0(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 15, false);
 }
+template <int CTRL, int ROWS = 15>
+__device__ inline double dpp_or_0(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)dpp_or_0<CTRL, ROWS>((uint32_t)(u >> 32)) << 32 | dpp_or_0<CTRL, ROWS>((uint32_t)u));
+}
 // The sum over the lanes up to and with this one.
-__device__ inline uint32_t sum_up_to(uint32_t v) {
+template <typename T>
+__device__ inline T sum_up_to(T v) {
     v += dpp_or_0<0x111>(v);  // row_shr:1, 2, 4, 8
     v += dpp_or_0<0x112>(v);
     v += dpp_or_0<0x114>(v);
     v += dpp_or_0<0x118>(v);
     v += dpp_or_0<0x142, 10>(v);  // row_bcast:15 into the second and fourth row
     return v + dpp_or_0<0x143, 12>(v);  // row_bcast:31 into the upper half
+}
+// The sum over a row of 16 lanes, in all of them.
+template <typename T>
+__device__ inline T row_sum(T v) {
+    v += dpp_or_0<kDppXor1>(v);
+    v += dpp_or_0<kDppXor2>(v);
+    v += dpp_or_0<0x141>(v);         // row_half_mirror
+    return v + dpp_or_0<0x140>(v);   // row_mirror
 }
 
 }  // namespace fkv

@@ -299,25 +299,6 @@ struct ChoiceLds {
     int32_t digit, above, inside, counts[2][kWaves];
 };
 
-// The sum over a row of 16 lanes, in all of them.
-__device__ inline uint32_t row_sum(uint32_t v) {
-    v += dpp_or_0<kDppXor1>(v);
-    v += dpp_or_0<kDppXor2>(v);
-    v += dpp_or_0<0x141>(v);
-    return v + dpp_or_0<0x140>(v);
-}
-template <int CTRL>
-__device__ inline double dpp_f64(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    return __builtin_bit_cast(double, (uint64_t)dpp_or_0<CTRL>((uint32_t)(u >> 32)) << 32 | dpp_or_0<CTRL>((uint32_t)u));
-}
-__device__ inline double row_sum(double v) {
-    v += dpp_f64<kDppXor1>(v);
-    v += dpp_f64<kDppXor2>(v);
-    v += dpp_f64<0x141>(v);
-    return v + dpp_f64<0x140>(v);
-}
-
 // Of 64 lanes, each with N counts that follow the ones of the lane below: the place
 // in whose count the need-th lies, by the lane that has it.
 template <int N, typename FOUND>

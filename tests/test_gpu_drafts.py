@@ -207,3 +207,20 @@ def test_captured(verify):
         for (g, s, bufs, out), d in zip(runs, data):
             want = _want(*d[i])
             assert np.array_equal(out[0].cpu().numpy(), want[0]) and np.array_equal(out[1].cpu().numpy(), want[1])
+
+
+@pytest.mark.parametrize("V", [300, 12000, 40000, 300000])
+def test_small_weights_before_large_ones(verify, V):
+    """A number of zero takes the first token with a weight, however small beside
+    those behind it: none is lost in a difference of sums."""
+    target = torch.zeros((6, 1, V))
+    first = [0, 1, V // 7, V // 2, V - 2, V - 1]
+    for b, t in enumerate(first):
+        target[b, 0, t] = 1e-30
+        for later in (t + 1, t + 70, t + 300, t + 5000, V - 1):
+            if later < V and later != t:
+                target[b, 0, later] = 1.0
+    none = torch.zeros((6, 0), dtype=torch.long)
+    _check(verify, target, None, none, torch.zeros((6, 1)))
+    got, _ = verify(target.cuda(), None, none.cuda(), torch.zeros((6, 1)).cuda())
+    assert got[:, 0].tolist() == first
