@@ -57,7 +57,7 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRowsMaxSeqs = 4096;
 // More rows than this on a KV head: workgroups of eight waves and 128 tokens a tile
-// in place of four and 64, of which a CU has two at once.
+// in place of four and 64, of which a CU has two at once (see plan_rows()).
 constexpr int64_t kFewRows = 256;
 constexpr float kBegin = 6.0f, kJoin = 4.0f, kJoinPart = 0.12f;  // us, see plan_rows()
 constexpr int kManyParts = 16;   // see paged_rows_join_kernel()
@@ -201,7 +201,7 @@ __device__ inline uint32_t round_pair_bf16(float a, float b) {
 }
 
 // Pages that a call reads once are not kept in the caches: 32 sequences to 8K tokens,
-// 540 MB, take 111 us so and 123 as other loads.  Where several workgroups read them
+// 540 MB, take 10 % less time so than by other loads.  Where several workgroups read them
 // (a prompt's chunk 577 us and 597 so, shared tokens) the caches serve all but the first.
 template <bool ONCE, typename T>
 __device__ inline T read(const T* p) {
@@ -833,7 +833,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows_kernel(RowsArgs a) {
 }
 
 // The records of a row, in order: a wave a row, or four waves, each every fourth eight
-// records, where there are more than kManyParts (65 records of 768 rows: 10 us and 7).
+// records, where there are more than kManyParts (65 records of 768 rows: 10.6 us and 7.6).
 template <int D, bool BF, int WAVES>
 __global__ void __launch_bounds__(256) paged_rows_join_kernel(RowsArgs a, int64_t n_rows) {
     constexpr int N = D / 64;
@@ -933,12 +933,13 @@ struct RowsPlan {
 // with its rows (the cache's bytes, then the products) and where two share a CU, the
 // chip has `slots` of them at once, and parts cost their join.  Against the best of 15
 // counts of parts it takes 0 to 13 % more (ten calls with shared tokens).
-static RowsPlan plan_rows(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, int64_t shared, int64_t max_len) {
+static RowsPlan plan_waves(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, int64_t shared, int64_t max_len, int waves,
+                           float& best) {
     RowsPlan r;
-    if (B == 1) shared = 0;  // (with nobody)
     r.shared = (int32_t)shared;
     const int64_t G = Hq / p->H, own_rows = L * G, all_rows = B * own_rows;
-    r.waves = (shared ? all_rows : own_rows) > kFewRows ? 8 : 4;
+    r.waves = waves;
+    best = INFINITY;
     const int64_t tile = 16 * r.waves, slots = r.waves == 8 ? 256 : 512;
     auto part = [&](int64_t rows) {
         RowParts q;
@@ -966,7 +967,7 @@ static RowsPlan plan_rows(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, 
     const float join = (float)((double)all_rows * p->H * (p->D + 4) * 8 / 4e6) + kJoinPart;
     r.common.splits = 0;
     r.even = r.least = 0;
-    if (!shared && B > 4 && B <= kEvenSeqs && r.own.tiles == 1 && own_pieces * 4 <= slots * 3) {
+    if (!shared && B > 4 && B <= kEvenSeqs && r.own.tiles == 1 && waves == 4 && own_pieces * 4 <= slots * 3) {
         // Few sequences, whose lengths differ: see even_parts().  Parts are not so short
         // that their records cost more than they gain
         r.even = (int32_t)(slots / p->H);
@@ -974,7 +975,6 @@ static RowsPlan plan_rows(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, 
         r.own.splits = (int32_t)std::min<int64_t>(std::min(cdiv(own_tiles, r.least), cdiv(4 * r.even, B)), 64);
         if (r.own.splits == 1) r.even = 0;
     } else {
-        float best = INFINITY;
         const int64_t most = std::min<int64_t>(shared ? common_tiles : own_tiles, 64);
         for (int64_t n = 1; n <= most; n++) {
             int64_t own_parts = n, common_parts = 0;
@@ -1008,6 +1008,22 @@ static RowsPlan plan_rows(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, 
     const int64_t parts = r.common.splits + r.own.splits;
     r.bytes = parts > 1 ? (int64_t)B * Hq * L * parts * (p->D + 4) * 4 + 16 : 0;
     return r;
+}
+
+// Many rows take workgroups of eight waves (100 new tokens of 4 heads over 16K: 59 us,
+// with four 65; 64 of them the same).  Where many rows share tokens and few have their
+// own, either may be better, and the model, which sees four waves 15 % slower than they
+// are, decides: 128 sequences of up to 1K tokens of their own take 90 us with four and
+// 110 with eight behind 4K shared tokens, 197 and 184 behind 32K.
+static RowsPlan plan_rows(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, int64_t shared, int64_t max_len) {
+    if (B == 1) shared = 0;  // (with nobody)
+    const int64_t own_rows = (int64_t)L * (Hq / p->H);
+    float four, eight;
+    if (own_rows > kFewRows) return plan_waves(p, Hq, B, L, shared, max_len, 8, eight);
+    const RowsPlan r = plan_waves(p, Hq, B, L, shared, max_len, 4, four);
+    if (!shared || B * own_rows <= kFewRows) return r;
+    const RowsPlan wide = plan_waves(p, Hq, B, L, shared, max_len, 8, eight);
+    return four <= 1.15f * eight ? r : wide;
 }
 
 static int check_rows(const char* who, const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, int64_t shared, int64_t max_len) {
