@@ -975,14 +975,17 @@ static RowsPlan plan_waves(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L,
         r.own.splits = (int32_t)std::min<int64_t>(std::min(cdiv(own_tiles, r.least), cdiv(4 * r.even, B)), 64);
         if (r.own.splits == 1) r.even = 0;
     } else {
-        const int64_t most = std::min<int64_t>(shared ? common_tiles : own_tiles, 64);
-        for (int64_t n = 1; n <= most; n++) {
+        const int64_t cut = shared ? common_tiles : own_tiles, most = std::min<int64_t>(cut, 64);
+        for (int64_t n = 1, last = 0; n <= most; n++) {
+            const int64_t of = cdiv(cut, n);  // tiles of a part
+            if (of == last) continue;         // (fewer parts are as long)
+            last = of;
             int64_t own_parts = n, common_parts = 0;
             float t, longest = 0;
             double work = 0;
             if (shared) {
-                common_parts = cdiv(common_tiles, cdiv(common_tiles, n));
-                const int64_t of = cdiv(common_tiles, n), blocks = common_pieces * common_parts;
+                common_parts = cdiv(common_tiles, of);
+                const int64_t blocks = common_pieces * common_parts;
                 longest = kBegin + of * (blocks > 256 ? time(r.common) : time_alone(r.common));
                 work = blocks * (kBegin + of * time(r.common));
                 own_parts = std::max<int64_t>(1, (int64_t)(own_tiles * time(r.own) / longest + 0.999f));
