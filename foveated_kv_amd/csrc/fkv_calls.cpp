@@ -6,7 +6,7 @@
 // Python more than doubled.  Host time of a call, a step of 64 sequences with 32
 // query and 8 KV heads: rotation 8.1 us from Python, 4.6 so; write 10.9 and 5.1;
 // attention over 512 tokens of one 9.5 and 4.6; of one sequence, five tokens over
-// 4000 15.1 and 9.3 (two launches), one over 8 of 63 pages 17.5 and 11.5 (four),
+// 4000 14.2 and 8.6 (two launches), one over 8 of 63 pages 17.5 and 11.5 (four),
 // five drafts of 32000 entries verified 14.7 and 6.1, bounds 5.6 and 3.7.
 //
 // Each function returns NotImplemented for whatever is not plain -- a wrong
