@@ -60,7 +60,7 @@ constexpr int kRowsMaxSeqs = 4096;
 // in place of four and 64, of which a CU has two at once (see plan_rows()).
 constexpr int64_t kFewRows = 256;
 constexpr float kBegin = 6.0f, kJoin = 4.0f, kJoinPart = 0.12f;  // us, see plan_rows()
-constexpr int kManyParts = 16;   // see paged_rows_join_kernel()
+constexpr int kManyParts = 16;  // see paged_rows_join_kernel()
 constexpr int kEvenSeqs = 256;  // sequences whose lengths even parts are made from
 constexpr float kLowest = -3.402823466e38f;  // running maximum before the first token: no score lies below it
 // As in the one-token kernel: the running maximum follows a score that exceeds
@@ -94,7 +94,7 @@ struct RowsArgs {
     RowParts common, own;
     int32_t lens_add, B, Hq, G, L, shared;
     int32_t tile;     // tokens of a tile
-    int32_t even;     // != 0: as many parts of all sequences as this (see even_chunk()), of
+    int32_t even;     // != 0: as many parts of all sequences as this (see even_parts()), of
     int32_t least;    // this many tiles or more
     float scale;      // |scale| * log2(e)
     uint32_t q_sign, q_mask;  // its sign, for two 16-bit numbers; 0 where it is 0 (and |scale| 1)
@@ -988,7 +988,9 @@ static RowsPlan plan_waves(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L,
                 const int64_t blocks = common_pieces * common_parts;
                 longest = kBegin + of * (blocks > 256 ? time(r.common) : time_alone(r.common));
                 work = blocks * (kBegin + of * time(r.common));
+                // (no longer than those; but no more than fill the chip, whose records cost more)
                 own_parts = std::max<int64_t>(1, (int64_t)(own_tiles * time(r.own) / longest + 0.999f));
+                own_parts = std::min(own_parts, std::max<int64_t>(16, cdiv(2 * slots, own_pieces)));
             }
             own_parts = cdiv(own_tiles, cdiv(own_tiles, own_parts));
             const float own_time = kBegin + cdiv(own_tiles, own_parts) * time(r.own);
@@ -1114,7 +1116,7 @@ int fkv_paged_attn_rows(const fkv_pages* pages, const fkv_rows* query, int32_t q
     a.n_new = n_new;
     a.lse = lse;
     a.records = (float*)workspace;
-    a.chunk = (int32_t*)((char*)workspace + p.bytes - 16);
+    a.chunk = p.even ? (int32_t*)((char*)workspace + p.bytes - 16) : nullptr;
     a.common = p.common;
     a.own = p.own;
     a.lens_add = lens_add;

@@ -172,7 +172,7 @@ def test_parts_of_uneven_sequences(paged, fmt, name, H):
 
 @pytest.mark.parametrize("fmt,qd", KINDS)
 @pytest.mark.parametrize("D,H,G,L,B,shared", [(128, 2, 4, 1, 9, 256), (64, 1, 7, 3, 5, 48), (128, 1, 2, 2, 70, 1024),
-                                              (64, 2, 1, 9, 2, 16)])
+                                              (64, 2, 1, 9, 2, 16), (64, 1, 4, 1, 150, 512), (64, 1, 4, 70, 4, 256)])
 def test_shared_beginning(paged, fmt, qd, D, H, G, L, B, shared):
     """A beginning that all sequences share, read from the first row alone;
     sequences that end before it does, and with it."""
