@@ -397,8 +397,10 @@ __global__ void __launch_bounds__(kThreads) page_choice_kernel(SparseArgs a) {
     if (!all && want > 0) {
         // a score or a size that is not finite says nothing of any page: all in 64 bits then
         float size = 0.0f, hi = -INFINITY, lo = INFINITY;
+        int32_t there = 0;  // pages that have a score (those that are not there have -inf; lane 0 counts the wave's)
         for (int32_t i = tid; i < n; i += kThreads) {
             const float2 s = i == tid ? score0 : scores[i];
+            there += __popcll(__ballot(s.x > -INFINITY));
             if (in_lds) held[i] = s.x, held_ids[i] = i == tid ? id0 : ids[i];
             size = fmaxf(size, s.x < INFINITY ? s.y : INFINITY);
             hi = fmaxf(hi, s.x);
@@ -408,13 +410,14 @@ __global__ void __launch_bounds__(kThreads) page_choice_kernel(SparseArgs a) {
 #pragma unroll
         for (int o = 16; o <= 32; o <<= 1)
             size = fmaxf(size, wave_xor(size, o)), hi = fmaxf(hi, wave_xor(hi, o)), lo = fminf(lo, wave_xor(lo, o));
-        if (lane == 0) lds.ends[0][wave] = size, lds.ends[1][wave] = hi, lds.ends[2][wave] = lo;
+        if (lane == 0) lds.ends[0][wave] = size, lds.ends[1][wave] = hi, lds.ends[2][wave] = lo, lds.counts[1][wave] = there;
         if (tid < kBins) lds.bins[tid] = 0;
         if (tid == 0) listed = 0;
         __syncthreads();
         {
             const int w = lane & 15;
             size = row_max(lds.ends[0][w]), hi = row_max(lds.ends[1][w]), lo = -row_max(-lds.ends[2][w]);
+            there = (int32_t)row_sum((uint32_t)lds.counts[1][w]);
         }
         if (size < INFINITY) {
             // A score in 32 bits is a sum of 4 D exact products at most: off by 2^-14 of
@@ -450,7 +453,9 @@ __global__ void __launch_bounds__(kThreads) page_choice_kernel(SparseArgs a) {
                 inside = lds.inside;
                 hi = top - (at - 1) * step + slack, lo = top - at * step - slack;
             }
-            if (over == INFINITY && under == -INFINITY) over = hi + 1.02f * off, under = hi > -INFINITY ? lo - 1.02f * off : -INFINITY;
+            // Few pages, or all within `off`: undecided, and with them those that are not there
+            // where the others are not enough.
+            if (over == INFINITY && under == -INFINITY) over = hi + 1.02f * off, under = there >= want ? lo - 1.02f * off : -INFINITY;
         }
         // how many are above, and the undecided ones
         int32_t up = 0, at = 0;
