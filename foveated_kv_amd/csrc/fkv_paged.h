@@ -27,6 +27,10 @@ struct TableView {
     int32_t n;  // entries per sequence
 };
 
+// Tokens that a table may hold for a sequence.  Launches are planned for no more,
+// whatever bound of the lengths a caller names.
+constexpr int64_t kMostTokens = 0x7FFFFFFF - 4096;
+
 // Rows (b, h, l) of an activation tensor, strides in elements.
 struct RowsView {
     char* data;

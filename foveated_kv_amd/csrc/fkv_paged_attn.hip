@@ -903,6 +903,7 @@ constexpr int64_t kManyRows = 96;
 static AttnPlan plan_of(const fkv_pages* p, int32_t Hq, int32_t B, int64_t max_len) {
     AttnPlan r;
     r.G = Hq / p->H;
+    max_len = std::min(max_len, kMostTokens);
     const int64_t rows16 = (int64_t)B * p->H * ((r.G + 15) / 16);
     r.split = max_len > (rows16 >= kManyRows ? 2 * kWholeRows : kWholeRows);
     // Groups of more than 16 heads: two tiles of heads a pass over the rows.  32
@@ -977,7 +978,7 @@ int fkv_paged_attn(const fkv_pages* pages, const fkv_rows* query, int32_t q_dtyp
     const char* w = "fkv_paged_attn";
     if (int e = check_attn(w, pages, Hq, B, max_len)) return e;
     if (int e = check_table(w, table, n_table, table_stride, B)) return e;
-    if ((int64_t)n_table * pages->page_size > 0x7FFFFFFF - 4096) return set_error(std::string(w) + ": more than 2^31 tokens a sequence");
+    if ((int64_t)n_table * pages->page_size > kMostTokens) return set_error(std::string(w) + ": more than 2^31 tokens a sequence");
     if (q_dtype != FKV_F16 && q_dtype != FKV_BF16) return set_error(std::string(w) + ": queries must be fp16 or bf16");
     if (pages->format <= FKV_PAGES_BF16 && (q_dtype == FKV_BF16) != (pages->format == FKV_PAGES_BF16))
         return set_error(std::string(w) + ": queries must have the 16-bit pages' type");

@@ -1024,6 +1024,7 @@ static RowsPlan plan_waves(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L,
 // 110 with eight behind 4K shared tokens, 197 and 184 behind 32K.
 static RowsPlan plan_rows(const fkv_pages* p, int32_t Hq, int32_t B, int32_t L, int64_t shared, int64_t max_len) {
     if (B == 1) shared = 0;  // (with nobody)
+    max_len = std::min(max_len, kMostTokens);
     const int64_t own_rows = (int64_t)L * (Hq / p->H);
     float four, eight;
     if (own_rows > kFewRows) return plan_waves(p, Hq, B, L, shared, max_len, 8, eight);
@@ -1040,7 +1041,7 @@ static int check_rows(const char* who, const fkv_pages* p, int32_t Hq, int32_t B
     if (Hq < 1 || Hq % p->H) return set_error(w + ": query heads must be a multiple of the KV heads");
     if (L < 0 || (int64_t)B * L * Hq >= 1 << 28) return set_error(w + ": at most 2^28 rows of queries");
     if (max_len < 0) return set_error(w + ": negative max_len");
-    if (shared < 0 || shared % p->page_size || shared > 0x7FFFFFFF - 4096)
+    if (shared < 0 || shared % p->page_size || shared > kMostTokens)
         return set_error(w + ": shared tokens must fill whole pages");
     return FKV_OK;
 }
@@ -1089,7 +1090,7 @@ int fkv_paged_attn_rows(const fkv_pages* pages, const fkv_rows* query, int32_t q
     if (int e = check_rows(w, pages, Hq, B, L, shared, max_len)) return e;
     if (int e = check_table(w, table, n_table, table_stride, B)) return e;
     const int64_t cap = (int64_t)n_table * pages->page_size;
-    if (cap > 0x7FFFFFFF - 4096) return set_error(std::string(w) + ": more than 2^31 tokens a sequence");
+    if (cap > kMostTokens) return set_error(std::string(w) + ": more than 2^31 tokens a sequence");
     if (shared > cap) return set_error(std::string(w) + ": more shared tokens than the table holds");
     if (q_dtype != FKV_F16 && q_dtype != FKV_BF16) return set_error(std::string(w) + ": queries must be fp16 or bf16");
     if (pages->format <= FKV_PAGES_BF16 && (q_dtype == FKV_BF16) != (pages->format == FKV_PAGES_BF16))

@@ -590,9 +590,9 @@ static int check_sparse(const char* who, const fkv_pages* p, int32_t Hq, int32_t
     if (int e = check_pages(who, p)) return e;
     if (B < 0 || (int64_t)B * p->H > 4096) return set_error(w + ": at most 4096 sequences times KV heads");
     if (Hq < 1 || Hq % p->H) return set_error(w + ": query heads must be a multiple of the KV heads");
-    if (n_table < 0 || (int64_t)n_table * p->page_size > 0x7FFFFFFF - 4096)
+    if (n_table < 0 || (int64_t)n_table * p->page_size > kMostTokens)
         return set_error(w + ": more than 2^31 tokens a sequence");
-    if (n_select < 1 || (int64_t)n_select * p->page_size > 0x7FFFFFFF - 4096)
+    if (n_select < 1 || (int64_t)n_select * p->page_size > kMostTokens)
         return set_error(w + ": at least one page must be selected, and less than 2^31 tokens");
     if ((int64_t)p->n_pages * p->H > 0x7FFFFFFF) return set_error(w + ": more than 2^31 pages times KV heads");
     // (the limits of the attention, whose tiles are 128 tokens of 16 heads)
