@@ -567,7 +567,10 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows_kernel(RowsArgs a) {
         top *= a.scale;  // (not negative: the queries carry its sign)
         if (__any(top > m + (kRowSlack + kRowBias<FMT>))) {
             top = fmaxf(top, wave_xor(top, 32));
-            const float up = fmaxf(m, top - kRowBias<FMT>), f = __builtin_amdgcn_exp2f(m - up);
+            // (Before a row's first weight that is not 0 the numerators are 0, or infinite values
+            // of this tile that settle() added: these stay.)
+            const float up = fmaxf(m, top - kRowBias<FMT>);
+            const float f = sum + wave_xor(sum, 32) == 0.0f ? 1.0f : __builtin_amdgcn_exp2f(m - up);
             m = up;
             wide = __any(fabsf(m) > kWide && m != kLowest);
             sum *= f;
