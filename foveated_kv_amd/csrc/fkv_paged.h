@@ -97,6 +97,23 @@ int check_pages(const char* who, const fkv_pages* p);
 int check_table(const char* who, const int32_t* table, int32_t n_table, int64_t stride, int32_t B);
 PageView page_view(const fkv_pages* p);
 
+// 16-bit numbers that the matrix products take two weights as, one after the other: the
+// upper half of each (bf16), or the fp16 number nearest towards 0 and, next, kUp times
+// what that leaves (see fkv_paged_attn.hip).
+constexpr float kUp = 1024.0f;
+__device__ inline uint32_t take_bf16(float& x, float& y) {
+    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+    x -= __uint_as_float(a & 0xFFFF0000u);
+    y -= __uint_as_float(b & 0xFFFF0000u);
+    return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+__device__ inline uint32_t take_fp16(float& x, float& y) {
+    const fkv_h2 h = __builtin_bit_cast(fkv_h2, __builtin_amdgcn_cvt_pkrtz(x, y));
+    x = fmaf(-kUp, (float)h.x, kUp * x);
+    y = fmaf(-kUp, (float)h.y, kUp * y);
+    return as_u32(h);
+}
+
 template <int CTRL, int ROWS = 15>
 __device__ inline uint32_t dpp_or_0(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 15, false);

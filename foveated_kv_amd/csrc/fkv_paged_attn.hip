@@ -358,19 +358,6 @@ __device__ inline void mask_values(Step<D, FMT>& st, const Place& p, int g) {
 // D = 64 85.8, 86.2; 13.2, 13.5; 5.7, 5.9.  Values taken apart into bf16, for which
 // weights are as above, cost 1 % and, 512 tokens of one sequence, 2.1 to 2.7 us.)
 constexpr int kParts = 3;
-constexpr float kUp = 1024.0f;
-__device__ inline uint32_t take_bf16(float& x, float& y) {
-    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
-    x -= __uint_as_float(a & 0xFFFF0000u);
-    y -= __uint_as_float(b & 0xFFFF0000u);
-    return __builtin_amdgcn_perm(b, a, 0x07060302u);
-}
-__device__ inline uint32_t take_fp16(float& x, float& y) {
-    const fkv_h2 h = __builtin_bit_cast(fkv_h2, __builtin_amdgcn_cvt_pkrtz(x, y));
-    x = fmaf(-kUp, (float)h.x, kUp * x);
-    y = fmaf(-kUp, (float)h.y, kUp * y);
-    return as_u32(h);
-}
 
 // A tile's running maximum and the step's weights.
 template <int D, int FMT>

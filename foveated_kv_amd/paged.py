@@ -559,6 +559,11 @@ class PagedLayer(_Fixed):
         table's first row for all sequences: they are read from that row alone,
         once for all.
 
+        Each softmax weight enters the matrix products as the sum of two 16-bit
+        numbers: within 2^-16 of it (bf16 pages), 2^-18 (quantised ones) or 2^-21
+        (fp16 ones), small parts of what rounding the result costs; ``attend``
+        keeps all 24 bits.
+
         ``out`` may have any strides, and be the query."""
         done = _lib.calls().attend_tokens(self._key, query, table, lens, max_len, lens_add, scale, out, return_lse, n_new,
                                           shared)
@@ -912,6 +917,10 @@ class PagedKVCache:
                                         q_out=q_out)
 
     def attend(self, layer, query, seqs=None, scale=None, out=None):
+        """Attention of one new token per sequence over all its tokens, or over
+        ``sparse_pages`` of its pages: ``PagedLayer.attend_sparse`` there,
+        ``attend_tokens`` where the sequences begin with the same pages, and
+        ``attend`` otherwise."""
         sl, table = self._batch(seqs)
         lens, most = self.pages._view(self.pages.lens, sl), max(self.pages._lens[sl], default=0)
         if self.sparse_pages:

@@ -694,8 +694,11 @@ int fkv_paged_attn(const fkv_pages* pages, const fkv_rows* query, int32_t q_dtyp
  * one is not written, its lse -inf.  The first `shared` tokens (whole pages, at
  * most the table's; 0: none) lie in the pages of the table's first row for every
  * sequence, and are read there alone, for as many of them as a sequence has.
- * Tokens that a query does not attend to take no part in it, whatever they are.
- * Types, max_len and workspace as for fkv_paged_attn.  Asynchronous,
+ * Tokens that a query does not attend to take no part in it, whatever they are; an
+ * infinite value among those that it does makes that dim of the result infinite (or
+ * NaN, where its weight is 0).  Softmax weights enter the products within 2^-16 of
+ * themselves (bf16 pages), 2^-18 (quantised ones), 2^-21 (fp16 ones, or 2^-46 of
+ * the row's largest).  Types, max_len and workspace as for fkv_paged_attn.  Asynchronous,
  * capturable. */
 int64_t fkv_paged_attn_rows_workspace(const fkv_pages* pages, int32_t Hq, int32_t B, int32_t L, int64_t shared,
                                       int64_t max_len);
