@@ -863,7 +863,13 @@ class PagedKVCache:
     what it is handed; without it keys and queries come rotated.  Pages that all
     sequences of a call begin with are attended to once for all of them.  With
     ``sparse_pages`` layers keep bounds of their pages, and ``attend`` takes that
-    many pages of each sequence (``PagedLayer.attend_sparse``)."""
+    many pages of each sequence (``PagedLayer.attend_sparse``).
+
+    A call that a HIP graph captures follows the page table's device tensors at each
+    replay, whatever sequences they hold then: it takes every sequence's tokens from
+    its own row of the table (nothing is read once for several) and the numbers of
+    new tokens from the device.  ``PagedLayer``'s calls take ``shared`` and ``n_new``
+    as they are told."""
 
     def __init__(self, n_layers, n_kv_heads, head_dim, n_pages, max_seqs=1, max_tokens=32768, page_size=64,
                  fmt="fp16", rope=None, device="cuda", sparse_pages=0):
@@ -905,6 +911,19 @@ class PagedKVCache:
         sl = self.pages._range(seqs)
         return sl, self.pages._view(self.pages.table, sl)
 
+    def _captured(self):
+        """Is the call captured?  What the host knows of the sequences now may then be
+        otherwise at a replay."""
+        return self.pages.table.is_cuda and torch.cuda.is_current_stream_capturing()
+
+    def _n_new(self, sl, new):
+        """The numbers of new tokens, where a call needs them: None, all are."""
+        return self.pages._view(self.pages.new, sl) if len(set(new)) > 1 or self._captured() else None
+
+    def _shared(self, sl):
+        n = self.pages.common_tokens(sl)
+        return 0 if n and self._captured() else n
+
     def write(self, layer, k, v, q=None, seqs=None, q_out=None):
         """The new tokens of the last ``extend`` of the same sequences; see
         ``PagedLayer.write``."""
@@ -912,9 +931,8 @@ class PagedKVCache:
         new = self.pages._new[sl]
         if new and max(new) != k.shape[2]:
             raise ValueError(f"k holds {k.shape[2]} tokens, the last extend made room for {max(new)}")
-        n_new = None if len(set(new)) <= 1 else self.pages._view(self.pages.new, sl)
-        return self.layers[layer].write(k, v, table, self.pages._view(self.pages.start, sl), n_new=n_new, q=q, rope=self.rope,
-                                        q_out=q_out)
+        return self.layers[layer].write(k, v, table, self.pages._view(self.pages.start, sl), n_new=self._n_new(sl, new), q=q,
+                                        rope=self.rope, q_out=q_out)
 
     def attend(self, layer, query, seqs=None, scale=None, out=None):
         """Attention of one new token per sequence over all its tokens, or over
@@ -925,7 +943,7 @@ class PagedKVCache:
         lens, most = self.pages._view(self.pages.lens, sl), max(self.pages._lens[sl], default=0)
         if self.sparse_pages:
             return self.layers[layer].attend_sparse(query, table, lens, self.sparse_pages, most, scale=scale, out=out)
-        shared = self.pages.common_tokens(sl)
+        shared = self._shared(sl)
         if shared:
             return self.layers[layer].attend_tokens(query, table, lens, most, scale=scale, out=out, shared=shared)
         return self.layers[layer].attend(query, table, lens, most, scale=scale, out=out)
@@ -938,10 +956,9 @@ class PagedKVCache:
         new = self.pages._new[sl]
         if new and max(new) != query.shape[2]:
             raise ValueError(f"query holds {query.shape[2]} tokens, the last extend made room for {max(new)}")
-        n_new = None if len(set(new)) <= 1 else self.pages._view(self.pages.new, sl)
         return self.layers[layer].attend_tokens(query, table, self.pages._view(self.pages.lens, sl),
-                                                max(self.pages._lens[sl], default=0), scale=scale, out=out, n_new=n_new,
-                                                shared=self.pages.common_tokens(sl))
+                                                max(self.pages._lens[sl], default=0), scale=scale, out=out,
+                                                n_new=self._n_new(sl, new), shared=self._shared(sl))
 
     def read(self, layer, seqs=None, dtype=None):
         """K, V (B, H, longest length, D); rows past a sequence's length are
