@@ -401,7 +401,7 @@ PyObject* attend_sparse(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor &bounds = tensor(a[1], key.index), &q = tensor(a[2], key.index);
         need(q.dim() == 4 && q.size(2) == 1 && q.size(3) == pg->D);
         const int32_t dt = dtype_code(q.scalar_type()), B = int32_of(q.size(0)), Hq = int32_of(q.size(1));
-        need(B <= 1 || q.stride(0) == Hq * q.stride(1));
+        need(B <= 1 || pg->H == 1 || q.stride(0) == Hq * q.stride(1));
         const Table t = table(a[3], key.index);
         need(t.B == B);
         const int32_t* lens = lengths(a[4], key.index, B);

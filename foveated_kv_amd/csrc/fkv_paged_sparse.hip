@@ -684,7 +684,8 @@ int fkv_paged_attn_sparse(const fkv_pages* pages, const void* bounds, const fkv_
     if (!bounds || (uintptr_t)bounds & 15) return set_error(std::string(w) + ": bounds must be 16-byte aligned device memory");
     if (((uintptr_t)query->data | (uintptr_t)out | (uintptr_t)workspace) & 15 || (query->stride_b | query->stride_h) & 7)
         return set_error(std::string(w) + ": query, out and workspace must be 16-byte aligned, query strides multiples of 8");
-    if (B > 1 && query->stride_b != Hq * query->stride_h)
+    // (the attention takes each KV head's queries as a sequence's, a stride apart)
+    if (B > 1 && pages->H > 1 && query->stride_b != Hq * query->stride_h)
         return set_error(std::string(w) + ": heads of neighbouring sequences must follow one another");
     const SparsePlan p = plan_sparse(pages, Hq, B, n_table, n_select, max_len);
     if (p.attn_bytes < 0) return FKV_EINVAL;
@@ -711,7 +712,7 @@ int fkv_paged_attn_sparse(const fkv_pages* pages, const void* bounds, const fkv_
     const fkv_pages one = by_head(pages);
     const int32_t rows = B * pages->H;
     fkv_rows q = *query;
-    q.stride_b = (int64_t)a.G * query->stride_h;
+    if (pages->H > 1) q.stride_b = (int64_t)a.G * query->stride_h;
     auto attend = [&](int32_t seqs) {
         return fkv_paged_attn(&one, &q, q_dtype, a.G, seqs, a.chosen, n_select, n_select, a.len, 0,
                               most_tokens(pages, n_select, max_len), scale, out, lse, (char*)workspace + p.attn_at,

@@ -617,7 +617,7 @@ class PagedLayer(_Fixed):
         if n_select < 1:
             raise ValueError(f"n_select must be positive, got {n_select}")
         n_select = min(n_select, 2 ** 31 - 1)
-        if B > 1 and query.stride(0) != Hq * query.stride(1):
+        if B > 1 and self.n_kv_heads > 1 and query.stride(0) != Hq * query.stride(1):
             query = query.contiguous()
         rows, held = _rows(query, shape)
         if out is None:

@@ -725,8 +725,9 @@ int fkv_paged_bounds(const fkv_pages* pages, void* bounds, int32_t B, int32_t L,
  * in 64 bits (equal ones: the lower page; a bound that is not finite: first; a
  * page id outside the pool: last); all pages where there are no more.  selected (B,
  * H, n_select) int32 or NULL: the pages, ascending, as entries of the sequence's
- * table row, then -1.  scale must not be negative; the query's rows of neighbouring
- * sequences follow one another (stride_b = Hq * stride_h).  Otherwise as
+ * table row, then -1.  scale must not be negative; with several KV heads and
+ * sequences, the query's rows of neighbouring sequences follow one another (stride_b =
+ * Hq * stride_h).  Otherwise as
  * fkv_paged_attn, over the selected pages' tokens.  At most 4096 sequences times
  * KV heads. */
 int64_t fkv_paged_attn_sparse_workspace(const fkv_pages* pages, int32_t Hq, int32_t B, int32_t n_table,
