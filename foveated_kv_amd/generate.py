@@ -337,9 +337,9 @@ class PagedCacheWrapper:
     at position start(b) + l of the rows handed back, of which those past the
     sequence's tokens are zeros or padding.  With one token it leaves the write
     to the attention call that follows, which rotates the query in the same
-    launch and attends to every stored token (``attn_mask`` is not looked at);
-    with ``in_place`` so it does with several, each of which sees the tokens up to
-    itself."""
+    launch and attends by ``PagedKVCache.attend`` (``attn_mask`` is not looked at).
+    With ``in_place`` so it does with any number of them, each of which sees all
+    tokens up to itself (``attend_tokens``)."""
 
     def __init__(self, cache, layer_idx, seqs=None, in_place=False):
         self.cache, self.layer_idx, self.seqs = cache, layer_idx, cache.pages._range(seqs)
@@ -376,7 +376,7 @@ class PagedCacheWrapper:
         layer = self.cache.layers[self.layer_idx]
         want = {"fp16": torch.float16, "bf16": torch.bfloat16}.get(
             layer.fmt, query.dtype if query.dtype != torch.float32 else torch.float16)
-        attend = self.cache.attend if self._n_new == 1 else self.cache.attend_tokens
+        attend = self.cache.attend_tokens if self.in_place else self.cache.attend
         return attend(self.layer_idx, q.to(want), seqs=self.seqs, scale=scale).to(query.dtype)
 
 
@@ -529,12 +529,15 @@ def generate_paged(model, tokenizer, prompts, cache, max_tokens: int = 100, temp
     need one length.
 
     ``share_prefix``: the whole pages that all prompts begin with alike are
-    prefilled once, held in common, and attended to once for all sequences.
+    prefilled once, held in common, and attended to once for all sequences.  The
+    rest of a prompt then attends to the pages (with quantised ones to what these
+    hold of the rows), where a prompt by itself attends to its rows as they came.
 
     ``draft_model`` with ``draft_cache``, a ``PagedKVCache`` of its own with the
     same room: it drafts ``n_draft`` tokens a round, which the model verifies in
     one call (``verify_drafts``).  Tokens are distributed as the model's own, and
-    with temp=0 they are its largest.  Both caches must rotate."""
+    with temp=0 they are its largest.  Both caches must rotate, and ``cache``
+    attend to all pages (no ``sparse_pages``)."""
     one = isinstance(prompts, str)
     dev = _model_device(model)
     ids = [tokenizer.encode(p) for p in ([prompts] if one else prompts)]
@@ -551,6 +554,9 @@ def generate_paged(model, tokenizer, prompts, cache, max_tokens: int = 100, temp
             raise ValueError("drafting needs two caches that rotate (PagedKVCache(rope=...))")
         if not 1 <= n_draft <= 63:
             raise ValueError(f"n_draft must be from 1 to 63, got {n_draft}")
+        if cache.sparse_pages:
+            raise ValueError("drafted tokens are verified by attention over all pages: no drafting for a cache with sparse_pages, "
+                             "whose one-token calls are another model (draft_cache may have them)")
         drafter = _Drafter(draft_model, draft_cache, n_draft)
     caches = [cache] + ([draft_cache] if drafter else [])
     if any(B > c.pages.max_seqs or any(c.pages.lengths(slice(0, B))) for c in caches):

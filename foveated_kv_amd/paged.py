@@ -950,8 +950,8 @@ class PagedKVCache:
 
     def attend_tokens(self, layer, query, seqs=None, scale=None, out=None):
         """Attention of all new tokens of the last ``extend`` of the same
-        sequences, each over those up to itself; see
-        ``PagedLayer.attend_tokens``."""
+        sequences, each over all those up to itself (also with ``sparse_pages``);
+        see ``PagedLayer.attend_tokens``."""
         sl, table = self._batch(seqs)
         new = self.pages._new[sl]
         if new and max(new) != query.shape[2]:
