@@ -461,8 +461,11 @@ class _Drafter:
     def draft(self, tok, counts, temp):
         """counts[b] tokens after tok (B,) for each sequence (-1: a finished one)
         -> tokens (B, most), and the probabilities that they were drawn from
-        (None where none were).  Stores tok and every drafted token."""
+        (None where none were).  Stores tok and every drafted token, unless there
+        are none to draft."""
         B, most = len(counts), max(counts)
+        if most == 0:  # (no sequence goes on behind this round)
+            return torch.zeros((B, 0), dtype=torch.long, device=tok.device), None
         wrappers = paged_wrappers(self.cache, slice(0, B))
         tokens, probs = [], []
         for i in range(most + 1):
@@ -472,8 +475,6 @@ class _Drafter:
                 tok = _next_token(logits, temp)
                 tokens.append(tok)
                 probs.append(_probabilities(logits, temp) if temp else None)
-        if not tokens:
-            return torch.zeros((B, 0), dtype=torch.long, device=tok.device), None
         return torch.stack(tokens, 1), torch.stack(probs, 1) if temp else None
 
 
@@ -486,8 +487,8 @@ def _decode_drafted(model, cache, drafter, tok, out, done, max_tokens, temp, eos
     calls = drafted = stood = 0
     done[:] = [d or len(o) >= max_tokens for d, o in zip(done, out)]
     while not all(done):
-        # (a sequence near its end drafts no more than it may still take)
-        counts = [-1 if d else min(drafter.n, max_tokens - len(o)) for d, o in zip(done, out)]
+        # (a sequence near its end drafts no more than it may still take beside the token that follows)
+        counts = [-1 if d else min(drafter.n, max_tokens - len(o) - 1) for d, o in zip(done, out)]
         tokens, probs = drafter.draft(tok, counts, temp)
         cache.extend([n + 1 for n in counts], batch)
         logits = model(torch.cat([tok.reshape(B, 1), tokens], 1), cache=wrappers)
