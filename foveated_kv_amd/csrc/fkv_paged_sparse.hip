@@ -152,8 +152,8 @@ struct SparseArgs {
     uint64_t* exact;    // workspace: (B, H, table.n) scores in 64 bits, as numbers of the same order
     int32_t* chosen;    // workspace: (B * H, n_select) pages of the table for the attention, id * H + h
     int32_t* len;       // workspace: (B * H) tokens in them
-    int32_t* selected;  // result (B, H, n_select) or NULL
-    int32_t lens_add, Hq, G, n_select;
+    int32_t* selected;  // result (B, H, n_result) or NULL
+    int32_t lens_add, Hq, G, n_select, n_result;
 };
 
 __device__ inline int32_t length_of(const SparseArgs& a, int b) {
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kThreads) page_choice_kernel(SparseArgs a) {
         }
     }
     int32_t* chosen = a.chosen + (int64_t)row * a.n_select;
-    int32_t* selected = a.selected ? a.selected + (int64_t)row * a.n_select : nullptr;
+    int32_t* selected = a.selected ? a.selected + (int64_t)row * a.n_result : nullptr;
     auto take = [&](int32_t slot, int32_t page) {
         const int32_t id = !all && in_lds && page < n ? held_ids[page] : ids[page];
         chosen[slot] = (uint32_t)id < (uint32_t)a.pg.n_pages ? id * a.pg.H + h : -1;
@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(kThreads) page_choice_kernel(SparseArgs a) {
         a.len[row] = pages > 0 ? want * a.pg.page_size + len - n * a.pg.page_size : 0;
     }
     if (selected)
-        for (int32_t i = (pages > 0 ? want + 1 : 0) + tid; i < a.n_select; i += kThreads) selected[i] = -1;
+        for (int32_t i = (pages > 0 ? want + 1 : 0) + tid; i < a.n_result; i += kThreads) selected[i] = -1;
 }
 
 // ---------------------------------------------------------------------------
@@ -607,8 +607,12 @@ static int64_t most_tokens(const fkv_pages* p, int32_t n_select, int64_t max_len
     return std::min<int64_t>((int64_t)n_select * p->page_size, max_len);
 }
 
+// A sequence has no more pages than its table's row.
+static int32_t pages_to_select(int32_t n_table, int32_t n_select) { return std::min(n_select, std::max(n_table, 1)); }
+
 static SparsePlan plan_sparse(const fkv_pages* p, int32_t Hq, int32_t B, int32_t n_table, int32_t n_select, int64_t max_len) {
     SparsePlan r;
+    n_select = pages_to_select(n_table, n_select);
     const fkv_pages one = by_head(p);
     const int64_t rows = (int64_t)B * p->H;
     r.exact_at = round_up(8 * rows * n_table, 256);
@@ -707,7 +711,8 @@ int fkv_paged_attn_sparse(const fkv_pages* pages, const void* bounds, const fkv_
     a.lens_add = lens_add;
     a.Hq = Hq;
     a.G = Hq / pages->H;
-    a.n_select = n_select;
+    a.n_result = n_select;
+    a.n_select = n_select = pages_to_select(n_table, n_select);
     hipStream_t s = (hipStream_t)stream;
     const fkv_pages one = by_head(pages);
     const int32_t rows = B * pages->H;

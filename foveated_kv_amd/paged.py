@@ -603,7 +603,8 @@ class PagedLayer(_Fixed):
         ``bounds``) promise the largest scores with any of the head's queries; all
         pages of a sequence that has no more.  ``return_pages``: also which,
         (B, H, n_select) int32, ascending, as entries of the sequence's table row,
-        then -1.  ``scale`` must not be negative."""
+        then -1.  ``scale`` must not be negative.  At most 4096 sequences times KV
+        heads a call."""
         if self.bounds is None:
             raise ValueError("the layer keeps no bounds (PagedLayer(bounds=True), or wrap(bounds=...))")
         done = _lib.calls().attend_sparse(self._key, self.bounds, query, table, lens, n_select, max_len, lens_add, scale,

@@ -28,3 +28,16 @@ def test_workspaces_of_lengths_beyond_the_most(H, Hq, B, L, shared, D, fmt):
         assert want >= 0
         for n in (MOST + 1, 2 ** 31, 2 ** 36, 2 ** 40, 2 ** 62, 2 ** 63 - 1):
             assert size(n) == want, n
+
+
+@pytest.mark.parametrize("n_table", [0, 1, 7, 500])
+def test_workspaces_of_more_pages_than_there_are(n_table):
+    """As many pages as a table holds are selected at most, and no more is kept for
+    them."""
+    lib, pg = _lib.load(), _pages(8)
+
+    def size(n_select):
+        return lib.fkv_paged_attn_sparse_workspace(R(pg), 32, 64, n_table, n_select, MOST)
+
+    for n in (n_table + 1, 1000, 100000):
+        assert size(n) == size(max(n_table, 1)) > 0
